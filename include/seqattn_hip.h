@@ -572,6 +572,119 @@ int32_t sa_run_resident_noalloc(const void* q, const void* k, const void* v, voi
                                 int32_t head_dim, int32_t dtype, int32_t kv_chunk_tokens,
                                 double softmax_scale, int32_t causal, void* stream);
 
+/*
+ * Rows of Q, K and V between a QKV projection and the attention: the norm of
+ * every head, the rotation by positions, and K and V into the pages of a cache.
+ *
+ *   q [tokens, q_heads, head_dim], k, v [tokens, kv_heads, head_dim]  bf16/fp16
+ *   q_out, k_out                     like q and k (either may be the input itself)
+ *   k_pages, v_pages [num_pages, page_tokens, kv_heads, head_dim]  as dtype, or int8 with
+ *   k_scales, v_scales [num_pages, page_tokens, kv_heads]          fp16 scales
+ *   slots [tokens] int64             token t's row is page slot / page_tokens, row slot % page_tokens;
+ *                                    a slot outside [0, num_pages * page_tokens) is not written
+ *   positions [axes, tokens]         int32 or int64, any value
+ *   frequencies [pairs] double       radians per position
+ *   q_weight, k_weight [head_dim]    as dtype or float32
+ *
+ * With a weight, a head's row x becomes x * rsqrt(mean(x^2) + eps) * weight (a
+ * tensor without one is not normalized).  Then pair i (i < pairs) of Q and K,
+ * elements (i, i + pairs) or, with `adjacent`, (2i, 2i + 1), is turned by
+ * frequencies[i] * position on the axis whose section holds i; elements past
+ * 2 * pairs stay.  All of it in FP32 (angles in FP64), one rounding to the
+ * output's type.  INT8: scale = fp16(amax / 127), values rint(x / (amax / 127)) of
+ * the unrounded row, 1 in place of a zero amax / 127; a row that is not finite
+ * gets scale NaN.
+ *
+ * q and q_out are NULL together; k goes to k_out or to k_pages (the other is
+ * NULL); v and v_pages come with k_pages.  Strides in elements, unit in the
+ * last dimension.  q, k, v, the outputs and 16-bit pages are 16-byte aligned
+ * with strides in multiples of 8; int8 pages 8-byte aligned, strides in
+ * multiples of 8.  head_dim is a multiple of 8 in [16, 256], axes at most 4,
+ * num_pages * page_tokens below 2^31.  The rows of one call have distinct
+ * slots.  Asynchronous on `stream`, a stream of `device`.
+ */
+#define SA_MAX_ROTARY_AXES 4
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    void *k_pages, *v_pages, *k_scales, *v_scales;
+    const int64_t* slots;
+    const void* positions;
+    const double* frequencies;
+    const void *q_weight, *k_weight;
+    int64_t stride_qt, stride_qh, stride_kt, stride_kh, stride_vt, stride_vh;
+    int64_t stride_qot, stride_qoh, stride_kot, stride_koh;
+    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
+    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t stride_pos_axis, stride_pos_token;
+    int64_t tokens, num_pages;
+    double eps;
+    int32_t q_heads, kv_heads, head_dim, page_tokens;
+    int32_t pairs, adjacent, axes, sections[SA_MAX_ROTARY_AXES];
+    int32_t positions_int64, q_weight_fp32, k_weight_fp32;
+    int32_t dtype, pages_int8;
+} sa_rows_args;
+
+int32_t sa_normalize_rotate_store(const sa_rows_args* args, int32_t device, void* stream);
+
+/*
+ * Rows of a page pool as packed K and V: k_out, v_out [tokens, kv_heads,
+ * head_dim] (bf16/fp16, contiguous) row t = the pages' row of slots[t], INT8
+ * values times their scale; zeros for a slot outside the pool.  16-bit pages
+ * have the outputs' type.  Limits as above.
+ */
+typedef struct {
+    const void *k_pages, *v_pages, *k_scales, *v_scales;
+    const int64_t* slots;
+    void *k_out, *v_out;
+    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
+    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t tokens, num_pages;
+    int32_t kv_heads, head_dim, page_tokens, dtype, pages_int8, reserved;
+} sa_read_args;
+
+int32_t sa_read_kv(const sa_read_args* args, int32_t device, void* stream);
+
+/*
+ * Attention of one new token per sequence over a paged K/V cache.
+ *
+ *   q, out [sequences, q_heads, head_dim]  bf16/fp16
+ *   pages, scales                          as above
+ *   page_table [sequences, max_pages]      int32, page of keys page_tokens * i .. of a sequence
+ *   lengths [sequences]                    int32, keys the sequence's token sees
+ *   lse [q_heads, sequences]               fp32, natural log; may be NULL
+ *
+ * Key j of sequence s is row j % page_tokens of page page_table[s, j /
+ * page_tokens].  A length below 0 counts as 0, one past the table's row as the
+ * row's keys; keys of a page outside [0, num_pages) are not seen.  A token
+ * that sees no key gets output 0 and LSE -inf.  Nothing in rows past a
+ * length is used, whatever they hold.
+ *
+ * `workspace` (sa_paged_decode_workspace_bytes, 16-byte aligned) is the call's
+ * own until it has run.
+ */
+typedef struct {
+    const void *q, *k_pages, *v_pages, *k_scales, *v_scales;
+    const int32_t *page_table, *lengths;
+    void* out;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t stride_qt, stride_qh, stride_ot, stride_oh;
+    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
+    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t stride_table, lse_stride_h;
+    int64_t num_pages;
+    double softmax_scale;
+    int32_t sequences, max_pages;
+    int32_t q_heads, kv_heads, head_dim, page_tokens, dtype, pages_int8;
+} sa_decode_args;
+
+int32_t sa_paged_decode(const sa_decode_args* args, int32_t device, void* stream);
+
+/* Workspace bytes of a call (its sizes only; pointers and strides are not read). */
+int32_t sa_paged_decode_workspace_bytes(const sa_decode_args* args, int32_t device, int64_t* bytes);
+
 /* hipStream_t of the pipeline's H2D (which == 0) or D2H (which == 1) copy stream. */
 void* sa_pipeline_stream(sa_pipeline* pipeline, int32_t which);
 

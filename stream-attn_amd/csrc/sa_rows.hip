@@ -1,0 +1,531 @@
+// Rows of Q, K and V between a QKV projection and the attention: the norm of
+// every head, the rotation by positions of one or several axes, and K and V
+// rows into and out of the pages of a device-resident cache.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w                (per head, where there is a weight)
+//   (a, b) -> (a cos t - b sin t, b cos t + a sin t)  t = frequency[i] * position[axis of i]
+//   INT8 pages: step = amax / 127, codes rint(y / step), scale fp16(step)
+//
+// Bytes bound: about ten operations per element that is read once and written
+// once.
+
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+
+#include "sa_common.h"
+#include "sa_types.h"
+
+namespace sa {
+namespace {
+
+struct PageRows {
+  char* base;       // row of slot s: base + page * stride_p + row * stride_t + head * stride_h, in elements
+  uint16_t* scale;  // fp16 scales, null for 16-bit pages
+  int64_t sp, st, sh, ss_p, ss_t, ss_h;
+};
+
+struct RowsParams {
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out, *k_out;
+  PageRows kp, vp;
+  const int64_t* slots;
+  const void* positions;
+  const double* frequencies;
+  const void *q_weight, *k_weight;
+  int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, sqo_t, sqo_h, sko_t, sko_h;
+  int64_t pos_axis, pos_token, token0;
+  float eps, inv_dim;
+  uint32_t num_slots, page_tokens;
+  int32_t q_heads, kv_heads, head_dim, pairs, axes;
+  int32_t end0, end1, end2;  // first pair past axis 0, 1, 2
+  int32_t heads;             // rows of a token: Q's, K's and V's
+  int32_t lane_log2;         // log2 of the lanes of a head
+  int32_t pos64, qw32, kw32;
+};
+
+// How a lane's W pairs lie in a row.  With halves, unit u holds pairs W u ..
+// W u + W - 1: their first elements are W consecutive ones, their second
+// elements W consecutive ones.  The elements past 2 * pairs go through as
+// pairs of their own that are not turned.  The scalar form takes any number
+// of pairs, element by element.
+enum Form { kHalves, kAdjacent, kScalar };
+
+template <Form F, int W>
+struct Unit {
+  int lo, hi;  // first elements of the two runs (halves), of the first pair (adjacent)
+  int first;   // first pair
+  int pairs, rest;
+
+  __device__ Unit(int u, int pairs_, int head_dim) : first(u * W), pairs(pairs_), rest((head_dim - 2 * pairs_) / 2) {
+    if (F == kAdjacent) {
+      lo = 2 * first, hi = lo + 1;
+    } else {
+      const bool turned = first < pairs;
+      lo = turned ? first : first + pairs;
+      hi = lo + (turned ? pairs : rest);
+    }
+  }
+  // Elements of pair i of the unit (scalar form).
+  __device__ int at_lo(int i) const { return first + i < pairs ? first + i : first + i + pairs; }
+  __device__ int at_hi(int i) const { return first + i < pairs ? first + i + pairs : first + i + pairs + rest; }
+};
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+template <int N>  // N dwords, 4 N bytes aligned up to 16
+__device__ inline Words<N> load_words(const void* p) {
+  Words<N> r;
+  if constexpr (N == 4) {
+    const u32x4 t = *static_cast<const u32x4*>(p);
+    for (int i = 0; i < 4; ++i) r.w[i] = t[i];
+  } else if constexpr (N == 2) {
+    const u32x2 t = *static_cast<const u32x2*>(p);
+    r.w[0] = t[0], r.w[1] = t[1];
+  } else {
+    r.w[0] = *static_cast<const uint32_t*>(p);
+  }
+  return r;
+}
+
+template <int N>
+__device__ inline void store_words(void* p, const Words<N>& r) {
+  if constexpr (N == 4)
+    *static_cast<u32x4*>(p) = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+  else if constexpr (N == 2)
+    *static_cast<u32x2*>(p) = u32x2{r.w[0], r.w[1]};
+  else
+    *static_cast<uint32_t*>(p) = r.w[0];
+}
+
+// The W pairs of a unit as floats.
+template <typename T, Form F, int W>
+__device__ inline void load_pairs(const uint16_t* row, const Unit<F, W>& u, float (&a)[W], float (&b)[W]) {
+  if constexpr (F == kScalar) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = T::lo(row[u.at_lo(i)]), b[i] = T::lo(row[u.at_hi(i)]);
+  } else if constexpr (F == kAdjacent) {
+    const Words<W> x = load_words<W>(row + u.lo);
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = T::lo(x.w[i]), b[i] = T::hi(x.w[i]);
+  } else {
+    const Words<W / 2> x = load_words<W / 2>(row + u.lo), y = load_words<W / 2>(row + u.hi);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      a[2 * i] = T::lo(x.w[i]), a[2 * i + 1] = T::hi(x.w[i]);
+      b[2 * i] = T::lo(y.w[i]), b[2 * i + 1] = T::hi(y.w[i]);
+    }
+  }
+}
+
+template <typename T, Form F, int W>
+__device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const float (&a)[W], const float (&b)[W]) {
+  if constexpr (F == kScalar) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      row[u.at_lo(i)] = (uint16_t)T::pack(a[i], 0.f);
+      row[u.at_hi(i)] = (uint16_t)T::pack(b[i], 0.f);
+    }
+  } else if constexpr (F == kAdjacent) {
+    Words<W> x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.w[i] = T::pack(a[i], b[i]);
+    store_words<W>(row + u.lo, x);
+  } else {
+    Words<W / 2> x, y;
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      x.w[i] = T::pack(a[2 * i], a[2 * i + 1]);
+      y.w[i] = T::pack(b[2 * i], b[2 * i + 1]);
+    }
+    store_words<W / 2>(row + u.lo, x);
+    store_words<W / 2>(row + u.hi, y);
+  }
+}
+
+__device__ inline uint32_t pack_codes(float a, float b, float c, float d) {
+  return ((uint32_t)(int32_t)a & 0xffu) | ((uint32_t)(int32_t)b & 0xffu) << 8 | ((uint32_t)(int32_t)c & 0xffu) << 16 |
+         (uint32_t)(int32_t)d << 24;
+}
+
+template <Form F, int W>
+__device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (&a)[W], const float (&b)[W]) {
+  if constexpr (F == kScalar) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      row[u.at_lo(i)] = (char)(int32_t)a[i];
+      row[u.at_hi(i)] = (char)(int32_t)b[i];
+    }
+  } else if constexpr (F == kAdjacent) {
+    static_assert(W == 4, "one 8-byte run");
+    store_words<2>(row + u.lo, Words<2>{{pack_codes(a[0], b[0], a[1], b[1]), pack_codes(a[2], b[2], a[3], b[3])}});
+  } else {
+    Words<W / 4> x, y;
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      x.w[i] = pack_codes(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
+      y.w[i] = pack_codes(b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]);
+    }
+    store_words<W / 4>(row + u.lo, x);
+    store_words<W / 4>(row + u.hi, y);
+  }
+}
+
+// A sum or maximum over the 2^n lanes of a head.
+__device__ inline float sum_lanes(float x, int lane_log2) {
+  for (int i = 0; i < lane_log2; ++i) x += __shfl_xor(x, 1 << i);
+  return x;
+}
+__device__ inline float max_lanes(float x, int lane_log2) {
+  for (int i = 0; i < lane_log2; ++i) x = fmaxf(x, __shfl_xor(x, 1 << i));
+  return x;
+}
+
+// One workgroup per token; its waves take the token's rows (Q's heads, then
+// K's, then V's) in turn, 64 >> lane_log2 rows at a time, so that the angles
+// are computed once per wave.
+template <typename T, Form F, int W, bool kInt8>
+__global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
+  const int64_t token = p.token0 + blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int unit_lane = lane & ((1 << p.lane_log2) - 1);
+  const int per_step = 64 >> p.lane_log2;
+  const bool live = unit_lane * 2 * W < p.head_dim;  // head_dim / 2W lanes of the 2^n hold a unit
+  const Unit<F, W> u(live ? unit_lane : 0, p.pairs, p.head_dim);
+
+  float cos_t[W], sin_t[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) cos_t[i] = 1.f, sin_t[i] = 0.f;
+  if (p.pairs > 0) {
+    double pos[SA_MAX_ROTARY_AXES];
+#pragma unroll
+    for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x) {
+      const int64_t at = (x < p.axes ? x : 0) * p.pos_axis + token * p.pos_token;
+      pos[x] = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[at]
+                       : (double)static_cast<const int32_t*>(p.positions)[at];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int pair = u.first + i;
+      if (pair < p.pairs) {
+        // Turns in FP64 (far positions have their fraction there), its
+        // fraction in FP32: the sine instruction takes turns.
+        const double at = pair < p.end0 ? pos[0] : pair < p.end1 ? pos[1] : pair < p.end2 ? pos[2] : pos[3];
+        const double turns = at * (p.frequencies[pair] * 0.15915494309189533577);
+        const float fraction = (float)(turns - rint(turns));
+        cos_t[i] = __builtin_amdgcn_cosf(fraction);
+        sin_t[i] = __builtin_amdgcn_sinf(fraction);
+      }
+    }
+  }
+
+  bool stored = false;
+  uint32_t page = 0, row_in_page = 0;
+  if (p.slots != nullptr) {
+    const int64_t slot = p.slots[token];
+    stored = slot >= 0 && slot < (int64_t)p.num_slots;
+    if (stored) page = (uint32_t)slot / p.page_tokens, row_in_page = (uint32_t)slot - page * p.page_tokens;
+  }
+
+  for (int first = wave * per_step; first < p.heads; first += 4 * per_step) {
+    const int row = first + (lane >> p.lane_log2);
+    const bool is_q = row < p.q_heads, is_v = row >= p.q_heads + p.kv_heads;
+    const int head = is_q ? row : is_v ? row - p.q_heads - p.kv_heads : row - p.q_heads;
+    const bool active = live && row < p.heads;
+    const uint16_t* in = is_q   ? p.q + token * p.sq_t + head * p.sq_h
+                         : is_v ? p.v + token * p.sv_t + head * p.sv_h
+                                : p.k + token * p.sk_t + head * p.sk_h;
+    float a[W], b[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = b[i] = 0.f;
+    if (active) load_pairs<T, F, W>(in, u, a, b);
+    const void* weight = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) squares += a[i] * a[i] + b[i] * b[i];
+    squares = sum_lanes(squares, p.lane_log2);
+    if (active && weight != nullptr) {
+      const float r = rsqrtf(squares * p.inv_dim + p.eps);
+      float wa[W], wb[W];
+      if (is_q ? p.qw32 : p.kw32) {
+        const float* w = static_cast<const float*>(weight);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          wa[i] = w[F == kAdjacent ? u.lo + 2 * i : F == kHalves ? u.lo + i : u.at_lo(i)];
+          wb[i] = w[F == kAdjacent ? u.lo + 2 * i + 1 : F == kHalves ? u.hi + i : u.at_hi(i)];
+        }
+      } else {
+        load_pairs<T, F, W>(static_cast<const uint16_t*>(weight), u, wa, wb);
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
+    }
+    if (!is_v) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float x = a[i] * cos_t[i] - b[i] * sin_t[i];
+        b[i] = b[i] * cos_t[i] + a[i] * sin_t[i];
+        a[i] = x;
+      }
+    }
+    if (is_q || p.slots == nullptr) {
+      uint16_t* out = is_q ? p.q_out + token * p.sqo_t + head * p.sqo_h : p.k_out + token * p.sko_t + head * p.sko_h;
+      if (active) store_pairs<T, F, W>(out, u, a, b);
+    }
+    if (p.slots == nullptr) continue;
+    const PageRows& pages = is_v ? p.vp : p.kp;
+    const int64_t at = page * pages.sp + row_in_page * pages.st + head * pages.sh;
+    if constexpr (kInt8) {
+      float amax = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(b[i])));
+        finite = finite && fabsf(a[i]) <= FLT_MAX && fabsf(b[i]) <= FLT_MAX;
+      }
+      amax = max_lanes(finite ? amax : INFINITY, p.lane_log2);
+      if (active && !is_q && stored) {
+        const float step = amax / 127.f;
+        const float div = step > 0.f ? step : 1.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          a[i] = fminf(fmaxf(rintf(a[i] / div), -127.f), 127.f);
+          b[i] = fminf(fmaxf(rintf(b[i] / div), -127.f), 127.f);
+        }
+        store_codes<F, W>(pages.base + at, u, a, b);
+        if (unit_lane == 0) {
+          const float scale = amax <= FLT_MAX ? div : NAN;
+          pages.scale[page * pages.ss_p + row_in_page * pages.ss_t + head * pages.ss_h] = (uint16_t)Fp16::pack(scale, 0.f);
+        }
+      }
+    } else if (active && !is_q && stored) {
+      store_pairs<T, F, W>(reinterpret_cast<uint16_t*>(pages.base) + at, u, a, b);
+    }
+  }
+}
+
+struct ReadParams {
+  PageRows kp, vp;
+  const int64_t* slots;
+  uint16_t *k_out, *v_out;
+  int64_t token0;
+  uint32_t num_slots, page_tokens;
+  int32_t kv_heads, head_dim;
+};
+
+// One workgroup per token: lane i of it moves granules (8 elements) i, i +
+// 256, ... of the token's K and V rows.
+template <typename T, bool kInt8>
+__global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
+  const int64_t token = p.token0 + blockIdx.x;
+  const int64_t slot = p.slots[token];
+  const bool held = slot >= 0 && slot < (int64_t)p.num_slots;
+  const uint32_t page = held ? (uint32_t)slot / p.page_tokens : 0;
+  const uint32_t row = held ? (uint32_t)slot - page * p.page_tokens : 0;
+  const int granules = p.head_dim / 8, each = p.kv_heads * granules;
+  for (int i = threadIdx.x; i < 2 * each; i += 256) {
+    const bool is_v = i >= each;
+    const int g = is_v ? i - each : i, head = g / granules, d = 8 * (g - head * granules);
+    const PageRows& pages = is_v ? p.vp : p.kp;
+    u32x4 w = {0, 0, 0, 0};
+    if (held) {
+      const int64_t at = page * pages.sp + row * pages.st + head * pages.sh + d;
+      if constexpr (kInt8) {
+        const u32x2 c = *reinterpret_cast<const u32x2*>(pages.base + at);
+        const float scale = Fp16::lo(pages.scale[page * pages.ss_p + row * pages.ss_t + head * pages.ss_h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = T::pack(byte_float(c[j / 2], 2 * (j & 1)) * scale, byte_float(c[j / 2], 2 * (j & 1) + 1) * scale);
+      } else {
+        w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(pages.base) + at);
+      }
+    }
+    *reinterpret_cast<u32x4*>((is_v ? p.v_out : p.k_out) + token * each * 8 + g * 8) = w;
+  }
+}
+
+bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+bool page_rows(PageRows& r, const void* base, const void* scale, int64_t sp, int64_t st, int64_t sh, int64_t ss_p,
+               int64_t ss_t, int64_t ss_h, bool int8) {
+  r = {static_cast<char*>(const_cast<void*>(base)), int8 ? static_cast<uint16_t*>(const_cast<void*>(scale)) : nullptr,
+       sp, st, sh, ss_p, ss_t, ss_h};
+  return base != nullptr && aligned(base, int8 ? 8 : 16) && sp % 8 == 0 && st % 8 == 0 && sh % 8 == 0 &&
+         (!int8 || (scale != nullptr && aligned(scale, 2)));
+}
+
+int32_t invalid(const char* entry, const char* what) {
+  set_error("%s: %s", entry, what);
+  return SA_ERR_INVALID_ARGUMENT;
+}
+
+int32_t check_sizes(const char* entry, int32_t dtype, int32_t head_dim, int32_t heads, int64_t tokens) {
+  if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_FP16) {
+    set_error("%s: unsupported dtype code %d", entry, dtype);
+    return SA_ERR_UNSUPPORTED_DTYPE;
+  }
+  if (head_dim < 16 || head_dim > 256 || head_dim % 8) {
+    set_error("%s: head_dim must be a multiple of 8 in [16, 256], got %d", entry, head_dim);
+    return SA_ERR_UNSUPPORTED_HEAD_DIM;
+  }
+  if (tokens < 0 || tokens > INT32_MAX || heads < 1 || heads > (1 << 20)) return invalid(entry, "tokens or heads out of range");
+  return 0;
+}
+
+int32_t check_pool(const char* entry, int64_t num_pages, int32_t page_tokens) {
+  if (page_tokens < 1 || num_pages < 0 || num_pages > INT32_MAX / page_tokens)
+    return invalid(entry, "num_pages * page_tokens must be below 2^31");
+  return 0;
+}
+
+// Launches of 2^32 threads and more go in parts.
+constexpr int64_t kTokensPerLaunch = 1 << 23;
+
+template <typename T, bool kInt8>
+int32_t launch_rows(RowsParams p, int64_t tokens, bool adjacent, hipStream_t stream) {
+  // Sixteen bytes per access wherever the pairs allow it, then 8, then single
+  // elements.
+  const int32_t rest = (p.head_dim - 2 * p.pairs) / 2;
+  const auto fits = [&](int w) { return p.pairs % w == 0 && rest % w == 0; };
+  const int form = adjacent || p.pairs == 0 ? 0 : fits(8) ? 1 : fits(4) ? 2 : 3;
+  const int units = p.head_dim / (form == 1 ? 16 : 8);
+  p.lane_log2 = 0;
+  while ((1 << p.lane_log2) < units) ++p.lane_log2;
+  for (p.token0 = 0; p.token0 < tokens; p.token0 += kTokensPerLaunch) {
+    const dim3 grid((uint32_t)(tokens - p.token0 < kTokensPerLaunch ? tokens - p.token0 : kTokensPerLaunch));
+    if (form == 0)
+      rows_kernel<T, kAdjacent, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+    else if (form == 1)
+      rows_kernel<T, kHalves, 8, kInt8><<<grid, 256, 0, stream>>>(p);
+    else if (form == 2)
+      rows_kernel<T, kHalves, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+    else
+      rows_kernel<T, kScalar, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+    SA_HIP_RETURN(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" {
+
+int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* stream) try {
+  using namespace sa;
+  const char* entry = "sa_normalize_rotate_store";
+  clear_error();
+  if (a == nullptr) return invalid(entry, "null arguments");
+  const bool pages = a->k_pages != nullptr;
+  int32_t rc = check_sizes(entry, a->dtype, a->head_dim, a->kv_heads, a->tokens);
+  if (rc != 0) return rc;
+  const bool has_q = a->q != nullptr;
+  if (has_q && (a->q_heads < 1 || a->q_heads > (1 << 20))) return invalid(entry, "q_heads out of range");
+  if (a->k == nullptr || has_q != (a->q_out != nullptr) || pages == (a->k_out != nullptr) ||
+      pages != (a->v_pages != nullptr) || pages != (a->v != nullptr) || pages != (a->slots != nullptr))
+    return invalid(entry, "q with q_out; k with k_out, or k and v with k_pages, v_pages and slots");
+  const int64_t strides[] = {a->stride_qt, a->stride_qh, a->stride_kt, a->stride_kh, a->stride_vt, a->stride_vh,
+                             a->stride_qot, a->stride_qoh, a->stride_kot, a->stride_koh};
+  for (int64_t s : strides)
+    if (s % 8) return invalid(entry, "strides must be multiples of 8 elements");
+  for (const void* x : {a->q, a->k, a->v, (const void*)a->q_out, (const void*)a->k_out, a->q_weight, a->k_weight})
+    if (!aligned(x, 16)) return invalid(entry, "rows and weights must be 16-byte aligned");
+  if (a->pairs < 0 || 2 * (int64_t)a->pairs > a->head_dim) return invalid(entry, "at most head_dim / 2 pairs");
+  int32_t ends[SA_MAX_ROTARY_AXES] = {};
+  if (a->pairs > 0) {
+    if (a->positions == nullptr || a->frequencies == nullptr || !aligned(a->positions, a->positions_int64 ? 8 : 4) ||
+        !aligned(a->frequencies, 8))
+      return invalid(entry, "a rotation needs positions and frequencies");
+    if (a->axes < 1 || a->axes > SA_MAX_ROTARY_AXES) return invalid(entry, "1 to 4 axes");
+    int32_t end = 0;
+    for (int32_t x = 0; x < a->axes; ++x) {
+      if (a->sections[x] < 1 || a->sections[x] > a->pairs - end) return invalid(entry, "the sections must add up to the pairs");
+      ends[x] = end += a->sections[x];
+    }
+    if (end != a->pairs) return invalid(entry, "the sections must add up to the pairs");
+    for (int32_t x = a->axes; x < SA_MAX_ROTARY_AXES; ++x) ends[x] = end;
+  }
+  RowsParams p{};
+  if (pages) {
+    rc = check_pool(entry, a->num_pages, a->page_tokens);
+    if (rc != 0) return rc;
+    if (!page_rows(p.kp, a->k_pages, a->k_scales, a->stride_kpp, a->stride_kpt, a->stride_kph, a->stride_ksp,
+                   a->stride_kst, a->stride_ksh, a->pages_int8) ||
+        !page_rows(p.vp, a->v_pages, a->v_scales, a->stride_vpp, a->stride_vpt, a->stride_vph, a->stride_vsp,
+                   a->stride_vst, a->stride_vsh, a->pages_int8) || !aligned(a->slots, 8))
+      return invalid(entry, "pages, scales or slots are missing or not aligned");
+    p.num_slots = (uint32_t)(a->num_pages * a->page_tokens);
+    p.page_tokens = (uint32_t)a->page_tokens;
+    p.slots = a->slots;
+  }
+  if (a->tokens == 0) return 0;
+  p.q = static_cast<const uint16_t*>(a->q), p.k = static_cast<const uint16_t*>(a->k), p.v = static_cast<const uint16_t*>(a->v);
+  p.q_out = static_cast<uint16_t*>(a->q_out), p.k_out = static_cast<uint16_t*>(a->k_out);
+  p.positions = a->positions, p.frequencies = a->frequencies;
+  p.q_weight = a->q_weight, p.k_weight = a->k_weight;
+  p.sq_t = a->stride_qt, p.sq_h = a->stride_qh, p.sk_t = a->stride_kt, p.sk_h = a->stride_kh;
+  p.sv_t = a->stride_vt, p.sv_h = a->stride_vh;
+  p.sqo_t = a->stride_qot, p.sqo_h = a->stride_qoh, p.sko_t = a->stride_kot, p.sko_h = a->stride_koh;
+  p.pos_axis = a->stride_pos_axis, p.pos_token = a->stride_pos_token;
+  p.eps = (float)a->eps, p.inv_dim = 1.f / (float)a->head_dim;
+  p.q_heads = has_q ? a->q_heads : 0, p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
+  p.heads = p.q_heads + p.kv_heads * (pages ? 2 : 1);
+  p.pairs = a->pairs, p.axes = a->axes;
+  p.end0 = ends[0], p.end1 = ends[1], p.end2 = ends[2];
+  p.pos64 = a->positions_int64, p.qw32 = a->q_weight_fp32, p.kw32 = a->k_weight_fp32;
+  DeviceGuard guard(device);
+  SA_HIP_RETURN(guard.status());
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  const bool bf16 = a->dtype == SA_DTYPE_BF16;
+  if (pages && a->pages_int8)
+    return bf16 ? launch_rows<Bf16, true>(p, a->tokens, a->adjacent, hs) : launch_rows<Fp16, true>(p, a->tokens, a->adjacent, hs);
+  return bf16 ? launch_rows<Bf16, false>(p, a->tokens, a->adjacent, hs) : launch_rows<Fp16, false>(p, a->tokens, a->adjacent, hs);
+} catch (const std::exception& error) {
+  return sa::exception_status("sa_normalize_rotate_store", error);
+}
+
+int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
+  using namespace sa;
+  const char* entry = "sa_read_kv";
+  clear_error();
+  if (a == nullptr) return invalid(entry, "null arguments");
+  int32_t rc = check_sizes(entry, a->dtype, a->head_dim, a->kv_heads, a->tokens);
+  if (rc == 0) rc = check_pool(entry, a->num_pages, a->page_tokens);
+  if (rc != 0) return rc;
+  ReadParams p{};
+  if (!page_rows(p.kp, a->k_pages, a->k_scales, a->stride_kpp, a->stride_kpt, a->stride_kph, a->stride_ksp, a->stride_kst,
+                 a->stride_ksh, a->pages_int8) ||
+      !page_rows(p.vp, a->v_pages, a->v_scales, a->stride_vpp, a->stride_vpt, a->stride_vph, a->stride_vsp, a->stride_vst,
+                 a->stride_vsh, a->pages_int8))
+    return invalid(entry, "pages or scales are missing or not aligned");
+  if (a->slots == nullptr || !aligned(a->slots, 8) || a->k_out == nullptr || a->v_out == nullptr ||
+      !aligned(a->k_out, 16) || !aligned(a->v_out, 16))
+    return invalid(entry, "slots or outputs are missing or not aligned");
+  if (a->tokens == 0) return 0;
+  p.k_out = static_cast<uint16_t*>(a->k_out), p.v_out = static_cast<uint16_t*>(a->v_out);
+  p.slots = a->slots;
+  p.num_slots = (uint32_t)(a->num_pages * a->page_tokens), p.page_tokens = (uint32_t)a->page_tokens;
+  p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
+  DeviceGuard guard(device);
+  SA_HIP_RETURN(guard.status());
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  const bool bf16 = a->dtype == SA_DTYPE_BF16;
+  for (p.token0 = 0; p.token0 < a->tokens; p.token0 += kTokensPerLaunch) {
+    const dim3 grid((uint32_t)(a->tokens - p.token0 < kTokensPerLaunch ? a->tokens - p.token0 : kTokensPerLaunch));
+    if (a->pages_int8)
+      bf16 ? read_kernel<Bf16, true><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, true><<<grid, 256, 0, hs>>>(p);
+    else
+      bf16 ? read_kernel<Bf16, false><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, false><<<grid, 256, 0, hs>>>(p);
+    SA_HIP_RETURN(hipGetLastError());
+  }
+  return 0;
+} catch (const std::exception& error) {
+  return sa::exception_status("sa_read_kv", error);
+}
+
+}  // extern "C"

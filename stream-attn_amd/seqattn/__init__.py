@@ -12,6 +12,7 @@ caller's QKV and output projections around the streamed attention.
 
 from .api import StreamingAttentionRunner, clear_runner_cache, streaming_attn_func, streaming_attn_varlen_func
 from .config import PagedAttentionConfig, ProjectionPipelineConfig, StreamingAttentionConfig
+from .device_cache import DeviceKVCache
 from .paged import (
     CallbackOutputSink,
     HostMemoryPlan,
@@ -32,12 +33,14 @@ from .projection import (
     QKVProjector,
     streaming_projected_self_attention,
 )
+from .rotary import rotary_frequencies
 from .stats import PagedAttentionStats, ProjectedAttentionStats, StreamingAttentionStats
 from .storage import NvmeOutputSink, NvmeQKVStore, NvmeQKVWriter, ephemeral_nvme_directory, load_nvme_output
 
 __all__ = [
     "AttentionPlan",
     "CallbackOutputSink",
+    "DeviceKVCache",
     "HostMemoryPlan",
     "HostMemorySnapshot",
     "KVLayout",
@@ -64,6 +67,7 @@ __all__ = [
     "build_plan",
     "ephemeral_nvme_directory",
     "load_nvme_output",
+    "rotary_frequencies",
     "clear_runner_cache",
     "streaming_attn_func",
     "streaming_attn_varlen_func",

@@ -159,6 +159,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sa_pipeline_kernel_busy": (
         c_int32, [c_void_p, ctypes.POINTER(c_double), ctypes.POINTER(c_double), ctypes.POINTER(c_int64)]
     ),
+    # Their argument structs are packed bytes (seqattn.kernels.rows, .decode).
+    "sa_normalize_rotate_store": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
+    "sa_read_kv": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
+    "sa_paged_decode": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
+    "sa_paged_decode_workspace_bytes": (c_int32, [ctypes.c_char_p, c_int32, ctypes.POINTER(c_int64)]),
     "sa_pipeline_stream": (c_void_p, [c_void_p, c_int32]),
     "sa_pipeline_output_slot": (c_void_p, [c_void_p, c_int32]),
     "sa_pipeline_q_buffer": (c_void_p, [c_void_p]),

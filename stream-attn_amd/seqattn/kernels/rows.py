@@ -1,0 +1,354 @@
+"""Rows between a QKV projection and the attention: norms, rotations, cache pages.
+
+``normalize_rotate_qk`` normalizes every head of Q and K and rotates it by its
+token's position on one or several axes, in one pass.  ``append_kv`` writes K
+and V rows into the pages of a device-resident cache, ``normalize_rotate_append``
+does both in one launch (K goes straight from the projection's output to its
+page), and ``read_kv`` returns pages as packed rows.  None of them has a
+counterpart in the reference.
+
+Pages are ``[num_pages, page_tokens, kv_heads, head_dim]`` tensors of any page,
+token and head strides, 16-bit or INT8.  INT8 pages hold the storage format of
+:mod:`seqattn.quantization` with one token per group: ``[num_pages,
+page_tokens, kv_heads]`` float16 scales.  Slot ``page * page_tokens + row``
+names a row of them.  :class:`seqattn.DeviceKVCache` keeps such pages.
+
+Every launch is asynchronous on torch's current stream of the operands' device
+and allocates nothing but the outputs that are not given, so it can be captured
+into a graph.
+"""
+
+from __future__ import annotations
+
+import struct
+from collections.abc import Sequence
+
+import torch
+
+from .. import _native
+
+MAX_ROTARY_AXES = 4
+# sa_rows_args: 14 pointers, 26 strides and counts, eps, 16 int32.
+_ROWS_ARGS = struct.Struct("=14Q26qd16i")
+# sa_read_args: 7 pointers, 14 strides and counts, 6 int32.
+_READ_ARGS = struct.Struct("=7Q14q6i")
+_NO_STRIDES = (0, 0, 0)
+
+
+def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, *, output: bool = False) -> None:
+    """[tokens, heads, head_dim] rows that the kernels can address."""
+    if rows.ndim != 3:
+        raise ValueError(f"{name} must use packed [tokens, heads, head_dim] layout")
+    if rows.device.type != "cuda":
+        raise ValueError("kernel operands must be device tensors")
+    st, sh, sd = rows.stride()
+    if sd != 1:
+        raise ValueError("kernel operands must have a unit stride in the last dimension")
+    if st % 8 or sh % 8 or rows.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned, with token and head strides in multiples of 8 elements")
+    if like is None:
+        _native.dtype_code(rows.dtype)
+        if rows.shape[2] % 8 or not 16 <= rows.shape[2] <= 256:
+            raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {rows.shape[2]}")
+        if rows.shape[1] < 1:
+            raise ValueError(f"{name} has no heads")
+    elif rows.device != like.device or rows.dtype != like.dtype:
+        raise ValueError(f"{name} must have the device and dtype of the other rows")
+    if output:
+        tokens, heads, dim = rows.shape
+        if (tokens > 1 and st < dim) or (heads > 1 and sh < dim) or (
+                tokens > 1 and heads > 1 and st < heads * sh and sh < tokens * st):
+            raise ValueError(f"{name} has rows that overlap")
+    elif rows.requires_grad and torch.is_grad_enabled():
+        raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+
+
+def check_pages(name: str, pages: torch.Tensor, scales: torch.Tensor | None, like: torch.Tensor) -> None:
+    """A page pool, and its scales, on ``like``'s device."""
+    if pages.ndim != 4:
+        raise ValueError(f"{name} must use [num_pages, page_tokens, kv_heads, head_dim] layout")
+    sp, st, sh, sd = pages.stride()
+    int8 = pages.dtype == torch.int8
+    if sd != 1 or sp % 8 or st % 8 or sh % 8 or pages.data_ptr() % (8 if int8 else 16):
+        raise ValueError(f"{name} must be aligned, with a unit stride in head_dim and the others in multiples of 8 elements")
+    if pages.device != like.device:
+        raise ValueError(f"{name} must live on the device of the rows")
+    if not pages.numel():
+        raise ValueError(f"{name} has no pages")
+    if pages.shape[0] * pages.shape[1] > 2**31 - 1:
+        raise ValueError(f"{name} has 2^31 rows or more")
+    if not int8:
+        if scales is not None:
+            raise ValueError("only INT8 pages have scales")
+        return
+    if scales is None:
+        raise ValueError("INT8 pages need their scales")
+    if scales.dtype != torch.float16 or scales.shape != pages.shape[:3] or scales.device != pages.device:
+        raise ValueError("INT8 scales must be float16 [num_pages, page_tokens, kv_heads] on the pages' device")
+
+
+def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype) -> bool:
+    """Both pools of a cache; whether they hold INT8."""
+    check_pages("k_pages", k_pages, k_scales, like)
+    check_pages("v_pages", v_pages, v_scales, like)
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must have the same shape and dtype")
+    if k_pages.dtype == torch.int8:
+        return True
+    if k_pages.dtype != dtype:
+        raise ValueError(f"pages of {k_pages.dtype} do not match rows of {dtype}")
+    return False
+
+
+def _check_slots(slots: torch.Tensor, tokens: int, device: torch.device) -> None:
+    if slots.dtype != torch.int64 or slots.ndim != 1 or slots.device != device:
+        raise ValueError("slots must be a one-dimensional int64 tensor on the rows' device")
+    if slots.shape[0] != tokens or (tokens > 1 and slots.stride(0) != 1):
+        raise ValueError("slots must hold one slot per token, contiguously")
+
+
+def _scale_strides(scales: torch.Tensor | None) -> tuple[int, ...]:
+    return _NO_STRIDES if scales is None else scales.stride()
+
+
+def _weight(name: str, weight: torch.Tensor | None, rows: torch.Tensor) -> int:
+    if weight is None:
+        return 0
+    if weight.shape != rows.shape[2:] or weight.device != rows.device or weight.stride(0) != 1:
+        raise ValueError(f"{name} must be a contiguous [head_dim] tensor on the rows' device")
+    if weight.dtype not in (rows.dtype, torch.float32):
+        raise ValueError(f"{name} must have the rows' dtype or float32")
+    if weight.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    if weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+    return weight.data_ptr()
+
+
+def _rotation(positions, frequencies, sections, pairing, rows: torch.Tensor):
+    """(positions, frequencies) pointers, position strides, pairs, axes, sections, int64 positions."""
+    if pairing not in ("halves", "adjacent"):
+        raise ValueError("pairing must be 'halves' or 'adjacent'")
+    if frequencies is None:
+        if positions is not None or sections is not None:
+            raise ValueError("a rotation needs both positions and frequencies")
+        return 0, 0, 0, 0, 0, 0, (0, 0, 0, 0), 0
+    if positions is None:
+        raise ValueError("a rotation needs both positions and frequencies")
+    tokens, _, dim = rows.shape
+    device = rows.device
+    if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or frequencies.device != device:
+        raise ValueError("frequencies must be a float64 [pairs] tensor on the rows' device")
+    pairs = frequencies.shape[0]
+    if not 1 <= pairs <= dim // 2 or (pairs > 1 and frequencies.stride(0) != 1):
+        raise ValueError("frequencies must be contiguous, for 1 to head_dim / 2 pairs")
+    if positions.dtype not in (torch.int64, torch.int32) or positions.device != device:
+        raise ValueError("positions must be an int32 or int64 tensor on the rows' device")
+    sections = (pairs,) if sections is None else tuple(sections)
+    axes = len(sections)
+    if not 1 <= axes <= MAX_ROTARY_AXES or sum(sections) != pairs or min(sections) < 1:
+        raise ValueError(f"sections must be 1 to {MAX_ROTARY_AXES} positive counts that add up to the pairs")
+    if positions.ndim == 1 and axes == 1:
+        axis_stride, token_stride = 0, positions.stride(0)
+    elif positions.ndim == 2 and positions.shape[0] == axes:
+        axis_stride, token_stride = positions.stride()
+    else:
+        raise ValueError(f"positions must be [{axes}, tokens]" + (" or [tokens]" if axes == 1 else ""))
+    if positions.shape[-1] != tokens:
+        raise ValueError("positions must hold one position per token and axis")
+    return (positions.data_ptr(), frequencies.data_ptr(), axis_stride, token_stride, pairs, axes,
+            (*sections, *(0,) * (MAX_ROTARY_AXES - axes)), positions.dtype == torch.int64)
+
+
+def _run_rows(q, k, v, q_out, k_out, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps):
+    """Launch sa_normalize_rotate_store on checked rows; ``pools`` = (k_pages, v_pages, k_scales, v_scales, int8) or None."""
+    tokens, kv_heads, dim = k.shape
+    where, freq, axis_stride, token_stride, pairs, axes, counts, wide = _rotation(positions, frequencies, sections, pairing, k)
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("eps must be finite and non-negative")
+    weights = _weight("q_weight", q_weight, k), _weight("k_weight", k_weight, k)
+    if tokens == 0:
+        return
+    if pools is None:
+        pages, page_strides, scale_strides, num_pages, page_tokens, int8 = (0, 0, 0, 0), _NO_STRIDES * 2, _NO_STRIDES * 2, 0, 0, 0
+    else:
+        k_pages, v_pages, k_scales, v_scales, int8 = pools
+        pages = (k_pages.data_ptr(), v_pages.data_ptr(), _native.ptr(k_scales) or 0, _native.ptr(v_scales) or 0)
+        page_strides = (*k_pages.stride()[:3], *v_pages.stride()[:3])
+        scale_strides = (*_scale_strides(k_scales), *_scale_strides(v_scales))
+        num_pages, page_tokens = k_pages.shape[:2]
+    args = _ROWS_ARGS.pack(
+        0 if q is None else q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
+        0 if q_out is None else q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
+        *pages, 0 if slots is None else slots.data_ptr(), where, freq, *weights,
+        *((0, 0) if q is None else q.stride()[:2]), *k.stride()[:2], *((0, 0) if v is None else v.stride()[:2]),
+        *((0, 0) if q_out is None else q_out.stride()[:2]), *((0, 0) if k_out is None else k_out.stride()[:2]),
+        *page_strides, *scale_strides, axis_stride, token_stride, tokens, num_pages, eps,
+        0 if q is None else q.shape[1], kv_heads, dim, page_tokens, pairs, pairing == "adjacent", axes, *counts, wide,
+        q_weight is not None and q_weight.dtype == torch.float32,
+        k_weight is not None and k_weight.dtype == torch.float32, _native.dtype_code(k.dtype), int8)
+    device = k.device
+    status = _native.lib().sa_normalize_rotate_store(args, device.index, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        _native.check(status, "sa_normalize_rotate_store")
+
+
+def _check_qk(q: torch.Tensor, k: torch.Tensor) -> None:
+    check_rows("q", q)
+    check_rows("k", k, q)
+    if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("q and k must have the same tokens and head_dim")
+
+
+def _output(name: str, out: torch.Tensor | None, rows: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+    check_rows(name, out, rows, output=True)
+    if out.shape != rows.shape:
+        raise ValueError(f"{name} must have the shape of its input")
+    return out
+
+
+def normalize_rotate_qk(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    frequencies: torch.Tensor | None = None,
+    *,
+    sections: Sequence[int] | None = None,
+    pairing: str = "halves",
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm and rotation of every head of ``q [tokens, q_heads, head_dim]`` and ``k [tokens, kv_heads, head_dim]``.
+
+    With ``q_weight`` (``[head_dim]``, the rows' dtype or float32) each head of
+    Q becomes ``x * rsqrt(mean(x^2) + eps) * q_weight``; likewise K.  Then pair
+    ``i`` of ``frequencies`` (float64 ``[pairs]``, radians per position, at most
+    ``head_dim / 2``), elements ``(i, i + pairs)`` with ``pairing="halves"`` or
+    ``(2i, 2i + 1)`` with ``"adjacent"``, is rotated by ``frequencies[i] *
+    position``; elements past ``2 * pairs`` are not.  ``positions`` is ``[tokens]``, or
+    ``[axes, tokens]`` for up to 4 axes of which axis ``a`` turns ``sections[a]``
+    consecutive pairs (:func:`seqattn.rotary_frequencies` makes the usual
+    frequencies).  Without positions and frequencies nothing is rotated.
+
+    Returns ``(q_out, k_out)``, new tensors unless given.  An output may be
+    its input itself, but must not otherwise share memory with an input.
+    """
+    _check_qk(q, k)
+    if positions is None and frequencies is None and q_weight is None and k_weight is None:
+        raise ValueError("normalize_rotate_qk needs a weight or a rotation")
+    q_out, k_out = _output("q_out", q_out, q), _output("k_out", k_out, k)
+    _run_rows(q, k, None, q_out, k_out, None, None, positions, frequencies, sections, pairing, q_weight, k_weight, eps)
+    return q_out, k_out
+
+
+def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots):
+    check_rows("v", v, k)
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have identical shapes, got {k.shape} and {v.shape}")
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype)
+    if k_pages.shape[2:] != k.shape[1:]:
+        raise ValueError("the pages' kv_heads and head_dim must be the rows'")
+    _check_slots(slots, k.shape[0], k.device)
+    return k_pages, v_pages, k_scales, v_scales, int8
+
+
+def append_kv(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+) -> None:
+    """Write rows ``k, v [tokens, kv_heads, head_dim]`` to the pages' ``slots`` (int64 ``[tokens]``).
+
+    A row whose slot is negative (padding) or past the pool is not written.
+    The slots of a call are distinct: of two rows with one slot either may
+    stay, in parts.  INT8 pages: a row that is not finite reads back as NaN.
+    """
+    check_rows("k", k)
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    _run_rows(None, k, v, None, None, pools, slots, None, None, None, "adjacent", None, None, 0.0)
+
+
+def normalize_rotate_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    slots: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    frequencies: torch.Tensor | None = None,
+    *,
+    sections: Sequence[int] | None = None,
+    pairing: str = "halves",
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+    q_out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`normalize_rotate_qk` and :func:`append_kv` of its K and of V, in one launch.
+
+    Returns the normalized and rotated Q.  INT8 pages take K before it is
+    rounded to 16 bits.  Q is written for every token, also where a row's slot
+    is negative.
+    """
+    _check_qk(q, k)
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    q_out = _output("q_out", q_out, q)
+    _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps)
+    return q_out
+
+
+def read_kv(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The pages' rows at ``slots`` as packed ``(k, v) [tokens, kv_heads, head_dim]``, the runners' layout.
+
+    INT8 rows come as ``value * scale`` in ``dtype`` (default bfloat16), others
+    in the pages' own dtype.  A slot outside the pool gives zeros.
+    """
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype == torch.int8 else k_pages.dtype
+    code = _native.dtype_code(dtype)
+    if slots.ndim != 1:
+        raise ValueError("slots must be a one-dimensional int64 tensor on the rows' device")
+    if slots.device.type != "cuda":
+        raise ValueError("kernel operands must be device tensors")
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, slots, dtype)
+    tokens, (num_pages, page_tokens, heads, dim) = slots.shape[0], k_pages.shape
+    _check_slots(slots, tokens, k_pages.device)
+    if dim % 8 or not 16 <= dim <= 256:
+        raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {dim}")
+    k_out = torch.empty((tokens, heads, dim), dtype=dtype, device=k_pages.device)
+    v_out = torch.empty_like(k_out)
+    if tokens == 0:
+        return k_out, v_out
+    args = _READ_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), _native.ptr(k_scales) or 0, _native.ptr(v_scales) or 0,
+        slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+        *k_pages.stride()[:3], *v_pages.stride()[:3], *_scale_strides(k_scales), *_scale_strides(v_scales),
+        tokens, num_pages, heads, dim, page_tokens, code, int8, 0)
+    device = k_pages.device
+    _native.check(_native.lib().sa_read_kv(args, device.index, torch.cuda.current_stream(device).cuda_stream), "sa_read_kv")
+    return k_out, v_out
+
+
+__all__ = ["append_kv", "normalize_rotate_append", "normalize_rotate_qk", "read_kv"]

@@ -1,0 +1,333 @@
+"""GPU tests of the norm, rotation and cache rows (``seqattn.kernels.rows``) against 64 bits.
+
+Bounds.  A 16-bit result is rounded once: half a step of its value.  Before
+that it is FP32: the norm's sum of at most 256 squares (a tree of FP32
+additions), the reciprocal root, two products and the rotation's two come to
+under 16 roundings of 2^-24 of the pair's size; the sine and cosine
+instructions are within 2^-20 (their input is the FP64 angle's fraction of a
+turn, rounded to 2^-26).  So 2^-18 of the pair's size covers both.  INT8 adds
+half a step of the row's code, the scale's FP16 rounding (2^-11) and the
+rounding of the value read back.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from seqattn import DeviceKVCache, rotary_frequencies
+from seqattn.kernels import append_kv, normalize_rotate_append, normalize_rotate_qk, read_kv
+from paged_reference import HALF_STEP, normalized, quantized, rotated
+
+pytestmark = pytest.mark.gpu
+
+FP32 = 2.0**-18
+
+
+def rows(gen, *shape, dtype):
+    return torch.randn(shape, generator=gen).to(dtype)
+
+
+def close(got, ref, size, dtype):
+    error = (got.double().cpu() - ref).abs()
+    bound = HALF_STEP[dtype] * (ref.abs() + FP32 * size) + FP32 * size + 2.0**-24
+    assert bool((error <= bound).all()), float((error / bound).max())
+
+
+CASES = [
+    # tokens, q_heads, kv_heads, head_dim, sections, pairing, dtype
+    (1, 1, 1, 16, (8,), "halves", torch.bfloat16),
+    (3, 4, 2, 128, (16, 24, 24), "halves", torch.bfloat16),
+    (7, 5, 1, 128, (64,), "adjacent", torch.float16),
+    (2, 8, 2, 80, (20,), "halves", torch.float16),       # partial, runs of 4 pairs
+    (5, 3, 3, 96, (11, 6), "halves", torch.bfloat16),    # 17 pairs: element by element
+    (4, 2, 2, 72, (36,), "halves", torch.bfloat16),      # runs of 4
+    (4, 2, 1, 24, (5,), "adjacent", torch.bfloat16),     # partial, an odd number of pairs
+    (3, 6, 2, 256, (32, 48, 48), "halves", torch.float16),
+    (2, 2, 2, 256, (127,), "halves", torch.bfloat16),    # element by element, 64 lanes
+    (9, 40, 8, 64, (8, 8, 8, 8), "adjacent", torch.bfloat16),
+    (300, 33, 11, 40, (16,), "halves", torch.bfloat16),
+    (2, 3, 1, 248, (62,), "halves", torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,sections,pairing,dtype", CASES)
+@pytest.mark.parametrize("weights", ["both", "q", "none"])
+def test_normalize_rotate_matches_64_bits(tokens, q_heads, kv_heads, dim, sections, pairing, dtype, weights):
+    gen = torch.Generator().manual_seed(tokens * 1000 + dim)
+    # Views of one projection's output.
+    fused = rows(gen, tokens, q_heads + 2 * kv_heads, dim, dtype=dtype)
+    wq = (1 + 0.2 * torch.randn(dim, generator=gen)).to(dtype) if weights != "none" else None
+    wk = 1 + 0.2 * torch.randn(dim, generator=gen) if weights == "both" else None  # float32
+    positions = torch.randint(-5000, 2**31 - 1, (len(sections), tokens), generator=gen)
+    freq = rotary_frequencies(sections, shared=len(sections) == 2, device="cpu")
+    dev = fused.cuda()
+    q, k, _ = dev.split([q_heads, kv_heads, kv_heads], dim=1)
+    qo, ko = normalize_rotate_qk(q, k, positions.cuda(), freq.cuda(), sections=sections, pairing=pairing,
+                                 q_weight=None if wq is None else wq.cuda(), k_weight=None if wk is None else wk.cuda(),
+                                 eps=1e-5)
+    for got, start, heads, w in ((qo, 0, q_heads, wq), (ko, q_heads, kv_heads, wk)):
+        ref, size = rotated(normalized(fused[:, start : start + heads], w, 1e-5), positions, freq, sections, pairing)
+        close(got, ref, size, dtype)
+
+
+def test_far_positions_and_int32_positions():
+    gen = torch.Generator().manual_seed(5)
+    x = rows(gen, 6, 2, 64, dtype=torch.float16)
+    freq = rotary_frequencies(32, device="cpu")
+    far = torch.tensor([0, 1, -1, 2**31 - 1, 2**40 + 3, -(2**38) - 7])
+    q, _ = normalize_rotate_qk(x.cuda(), x.cuda(), far.cuda(), freq.cuda())
+    # The angle in 64 bits is off by 2^-53 of 2^40 radians, 2^-13; both sides
+    # have the same products.  Positions below 2^31 hold the tight bound.
+    ref, size = rotated(x.double(), far[None], freq, (32,), "halves")
+    error = (q.double().cpu() - ref).abs()
+    assert bool((error[:4] <= HALF_STEP[x.dtype] * (ref[:4].abs() + FP32 * size[:4]) + FP32 * size[:4]).all())
+    assert bool((error[4:] <= HALF_STEP[x.dtype] * ref[4:].abs() + 2.0**-11 * size[4:]).all())
+    near = far[:4].to(torch.int32)
+    same, _ = normalize_rotate_qk(x[:4].cuda(), x[:4].cuda(), near.cuda(), freq.cuda())
+    assert torch.equal(same, q[:4])
+
+
+def test_in_place_strided_outputs_and_no_tokens():
+    gen = torch.Generator().manual_seed(7)
+    fused = rows(gen, 10, 8, 96, dtype=torch.bfloat16).cuda()
+    freq, pos = rotary_frequencies(48), torch.arange(10, device="cuda")
+    w = torch.ones(96, device="cuda")
+    q, k = fused[:, :6], fused[:, 6:]
+    want = normalize_rotate_qk(q, k, pos, freq, q_weight=w, k_weight=w)
+    by_head = torch.zeros((6, 10, 96), dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    got = normalize_rotate_qk(q, k, pos, freq, q_weight=w, k_weight=w, q_out=by_head, k_out=k)
+    assert got[0] is by_head and torch.equal(by_head, want[0]) and torch.equal(k, want[1])
+    empty = normalize_rotate_qk(fused[:0, :6], fused[:0, 6:], pos[:0], freq)
+    assert empty[0].shape == (0, 6, 96)
+    # Norm alone.
+    q2, k2 = normalize_rotate_qk(want[0], want[1], q_weight=w)
+    assert torch.equal(k2, want[1])
+    ref = normalized(want[0].cpu(), w.cpu(), 1e-6)
+    close(q2, ref, ref.abs(), torch.bfloat16)
+
+
+def test_zero_rows_and_non_finite_rows_stay_in_their_head():
+    x = torch.zeros((4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    x[1, 0] = float("inf")
+    x[2, 1] = float("nan")
+    x[3] = 1.0
+    freq, pos = rotary_frequencies(32), torch.arange(4, device="cuda")
+    w = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    q, k = normalize_rotate_qk(x, x, pos, freq, q_weight=w, k_weight=w, eps=1e-6)
+    assert torch.equal(q.nan_to_num(7.0), k.nan_to_num(7.0))
+    assert bool((q[0] == 0).all()) and bool((q[1, 1] == 0).all()) and bool((q[2, 0] == 0).all())
+    assert not bool(torch.isfinite(q[1, 0]).any()) and bool(torch.isnan(q[2, 1]).all())
+    assert bool(torch.isfinite(q[3]).all())
+
+
+def pools(pages, page, heads, dim, dtype, layout, int8):
+    if layout == "heads":
+        make = lambda *s, t: torch.full((s[0], s[2], s[1], *s[3:]), 3, dtype=t, device="cuda").transpose(1, 2)  # noqa: E731
+    else:
+        make = lambda *s, t: torch.full(s, 3, dtype=t, device="cuda")  # noqa: E731
+    stored = torch.int8 if int8 else dtype
+    k, v = make(pages, page, heads, dim, t=stored), make(pages, page, heads, dim, t=stored)
+    if not int8:
+        return k, v, None, None
+    return k, v, make(pages, page, heads, t=torch.float16), make(pages, page, heads, t=torch.float16)
+
+
+def int8_close(got, rows_, size, dtype):
+    """Values read back from INT8 pages against the rows that went in."""
+    codes, _, step = quantized(rows_)
+    error = (got.double().cpu() - rows_).abs()
+    row_size = size.amax(-1, keepdim=True)
+    bound = (0.5 + 127 * 2.0**-11) * step[..., None] * (1 + 2.0**-7) + 2 * FP32 * row_size + HALF_STEP[dtype] * got.double().cpu().abs() + 2.0**-24
+    assert bool((error <= bound).all()), float((error / bound).max())
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("layout", ["heads", "tokens"])
+@pytest.mark.parametrize("tokens,heads,dim,page,dtype", [
+    (1, 1, 16, 1, torch.bfloat16), (37, 3, 80, 5, torch.float16), (200, 8, 128, 64, torch.bfloat16),
+    (11, 2, 256, 16, torch.bfloat16), (19, 5, 24, 7, torch.float16)])
+def test_append_and_read(tokens, heads, dim, page, dtype, layout, int8):
+    gen = torch.Generator().manual_seed(tokens)
+    k, v = rows(gen, tokens, heads, dim, dtype=dtype), rows(gen, tokens, heads, dim, dtype=dtype)
+    k[0, 0] = 0  # a row of zeros
+    pages = -(-tokens // page) + 2
+    kp, vp, ks, vs = pools(pages, page, heads, dim, dtype, layout, int8)
+    slots = torch.randperm(pages * page, generator=gen)[:tokens]
+    before = [t.clone() for t in (kp, vp)]
+    append_kv(k.cuda(), v.cuda(), kp, vp, slots.cuda(), k_scales=ks, v_scales=vs)
+    ko, vo = read_kv(kp, vp, slots.cuda(), k_scales=ks, v_scales=vs, dtype=dtype)
+    for got, x, pool, scale in ((ko, k, kp, ks), (vo, v, vp, vs)):
+        if not int8:
+            assert torch.equal(got.cpu(), x)
+            assert torch.equal(pool.cpu()[slots // page, slots % page], x)
+            continue
+        # Rows that are not rotated are quantized from the same floats as the
+        # storage format's, with the same operations.
+        step = x.float().abs().amax(-1) / 127.0
+        step = torch.where(step > 0, step, torch.ones_like(step))
+        codes = torch.round(x.float() / step[..., None]).clamp(-127, 127)
+        assert torch.equal(pool.cpu()[slots // page, slots % page].float(), codes)
+        assert torch.equal(scale.cpu()[slots // page, slots % page], step.half())
+        assert torch.equal(got.cpu(), (codes * step.half().float()[..., None]).to(dtype))
+    # Rows of no slot of this call keep what they held.
+    untouched = torch.ones(pages * page, dtype=torch.bool)
+    untouched[slots] = False
+    at = untouched.nonzero().squeeze(1)
+    for pool, old in zip((kp, vp), before):
+        assert torch.equal(pool[at // page, at % page], old[at // page, at % page])
+
+
+def test_slots_outside_the_pool_are_skipped_and_read_as_zeros():
+    k = torch.ones((6, 2, 32), dtype=torch.bfloat16, device="cuda")
+    kp, vp, _, _ = pools(2, 4, 2, 32, torch.bfloat16, "heads", False)
+    slots = torch.tensor([-1, 8, 5, 2**40, -(2**40), 2**31], device="cuda")
+    append_kv(k, k, kp, vp, slots)
+    held = torch.zeros((2, 4), dtype=torch.bool)
+    held[1, 1] = True
+    assert bool((kp.cpu()[held] == 1).all()) and bool((kp.cpu()[~held] == 3).all())
+    ko, vo = read_kv(kp, vp, slots)
+    assert bool((ko[2] == 1).all()) and bool((vo[2] == 1).all())
+    assert bool((ko[[0, 1, 3, 4, 5]] == 0).all())
+
+
+def test_int8_rows_that_are_not_finite_read_back_as_nan():
+    k = torch.ones((3, 2, 32), dtype=torch.bfloat16, device="cuda")
+    k[0, 0, 3] = float("inf")
+    k[1, 1, 31] = float("nan")
+    kp, vp, ks, vs = pools(1, 4, 2, 32, torch.bfloat16, "heads", True)
+    slots = torch.arange(3, device="cuda")
+    append_kv(k, k, kp, vp, slots, k_scales=ks, v_scales=vs)
+    got, _ = read_kv(kp, vp, slots, k_scales=ks, v_scales=vs)
+    assert bool(torch.isnan(got[0, 0]).all()) and bool(torch.isnan(got[1, 1]).all())
+    assert bool((got[0, 1] - 1).abs().max() < 2**-7) and bool((got[2] - 1).abs().max() < 2**-7)
+
+
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,sections,pairing,dtype", CASES)
+@pytest.mark.parametrize("int8", [False, True])
+def test_fused_append_matches_the_parts(tokens, q_heads, kv_heads, dim, sections, pairing, dtype, int8):
+    gen = torch.Generator().manual_seed(dim + tokens)
+    fused = rows(gen, tokens, q_heads + 2 * kv_heads, dim, dtype=dtype)
+    positions = torch.randint(0, 10**6, (len(sections), tokens), generator=gen)
+    freq = rotary_frequencies(sections, device="cpu")
+    wq, wk = ((1 + 0.2 * torch.randn(dim, generator=gen)).to(dtype) for _ in range(2))
+    q, k, v = fused.cuda().split([q_heads, kv_heads, kv_heads], dim=1)
+    options = dict(sections=sections, pairing=pairing, q_weight=wq.cuda(), k_weight=wk.cuda())
+    q_ref, k_ref = normalize_rotate_qk(q, k, positions.cuda(), freq.cuda(), **options)
+    cache = DeviceKVCache(tokens // 4 + 2, 4, kv_heads, dim, dtype=dtype, storage_dtype="int8" if int8 else None)
+    slots = torch.randperm(cache.num_pages * 4, generator=gen)[:tokens].cuda()
+    q_out = cache.normalize_rotate_append(q, k, v, slots, positions.cuda(), freq.cuda(), **options)
+    assert torch.equal(q_out, q_ref)
+    ko, vo = cache.read(slots)
+    if not int8:
+        assert torch.equal(ko, k_ref) and torch.equal(vo, v)
+        return
+    ref, size = rotated(normalized(fused[:, q_heads : q_heads + kv_heads], wk, 1e-6), positions, freq, sections, pairing)
+    int8_close(ko, ref, size, dtype)
+    int8_close(vo, fused[:, q_heads + kv_heads :].double(), fused[:, q_heads + kv_heads :].double().abs(), dtype)
+
+
+def test_pools_past_32_bit_offsets():
+    # The last pages of a pool of 2^32 elements and more: one buffer serves as
+    # K and, 64 rows of one head further, as V.
+    pages, page, heads, dim = 32800, 64, 16, 128
+    pool = torch.zeros((pages, heads, page, dim), dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    assert pool.numel() > 2**32
+    k = torch.randn((3, heads, dim), device="cuda").to(torch.bfloat16)
+    k_pool, v_pool = pool[: pages // 2 + 16385], pool
+    slots = torch.tensor([pages * page - 1, pages * page - 64, 5], device="cuda")
+    append_kv(k, k, v_pool, v_pool, slots)
+    ko, vo = read_kv(v_pool, v_pool, slots)
+    assert torch.equal(ko, k) and torch.equal(vo, k)
+    assert torch.equal(pool[pages - 1, page - 1], k[0]) and torch.equal(pool[0, 5], k[2])
+    assert k_pool.shape[0] < pages
+    del pool, k_pool, v_pool
+    torch.cuda.empty_cache()
+
+
+def test_replayed_graph_and_other_stream():
+    gen = torch.Generator().manual_seed(11)
+    fused = rows(gen, 5, 8, 64, dtype=torch.bfloat16).cuda()
+    q, k, v = fused.split([4, 2, 2], dim=1)
+    freq, pos = rotary_frequencies(32), torch.arange(5, device="cuda")
+    cache = DeviceKVCache(4, 4, 2, 64)
+    slots = torch.arange(5, device="cuda")
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        cache.normalize_rotate_append(q, k, v, slots, pos, freq)
+        cache.read(slots)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        q_out = cache.normalize_rotate_append(q, k, v, slots, pos, freq)
+        ko, vo = cache.read(slots)
+    for step in range(4):
+        fused.copy_(rows(gen, 5, 8, 64, dtype=torch.bfloat16))
+        pos.add_(17 * step)
+        slots.copy_(torch.randperm(16, generator=gen)[:5])
+        graph.replay()
+        torch.cuda.synchronize()
+        want_q, want_k = normalize_rotate_qk(q, k, pos, freq)
+        assert torch.equal(q_out, want_q) and torch.equal(ko, want_k) and torch.equal(vo, v)
+
+
+def test_refusals():
+    q = torch.zeros((4, 4, 64), dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros((4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    freq, pos = rotary_frequencies(32), torch.arange(4, device="cuda")
+    w = torch.ones(64, device="cuda")
+
+    def refused(match, *args, **options):
+        with pytest.raises(ValueError, match=match):
+            normalize_rotate_qk(*args, **options)
+
+    refused("needs a weight or a rotation", q, k)
+    refused("both positions and frequencies", q, k, pos)
+    refused("both positions and frequencies", q, k, None, freq)
+    refused("same tokens and head_dim", q, k[:3], pos, freq)
+    refused("device and dtype", q, k.half(), pos, freq)
+    refused("float16 or bfloat16", q.float(), k.float(), pos, freq)
+    refused("multiple of 8", q[..., :12], k[..., :12], pos, freq[:6])
+    refused("unit stride", q.transpose(1, 2), k, pos, freq)
+    refused("aligned", torch.zeros(4 * 4 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 4, 64), k, pos, freq)
+    refused("float64", q, k, pos, freq.float())
+    refused("head_dim / 2 pairs", q, k, pos, rotary_frequencies(33))
+    refused("positions must be", q, k, pos, freq, sections=(16, 16))
+    refused("add up to the pairs", q, k, pos, freq, sections=(16, 15))
+    refused("add up to the pairs", q, k, pos.expand(5, 4), freq, sections=(8, 8, 8, 4, 4))
+    refused("one position per token", q, k, pos[:3], freq)
+    refused("int32 or int64", q, k, pos.float(), freq)
+    refused("pairing", q, k, pos, freq, pairing="pairs")
+    refused("q_weight", q, k, pos, freq, q_weight=w[:32])
+    refused("dtype or float32", q, k, pos, freq, k_weight=w.half())
+    refused("eps", q, k, pos, freq, q_weight=w, eps=-1.0)
+    refused("eps", q, k, pos, freq, q_weight=w, eps=float("nan"))
+    refused("shape of its input", q, k, pos, freq, q_out=k.clone())
+    refused("overlap", q, k, pos, freq, q_out=q[:1].expand(4, 4, 64))
+    refused("inference-only", q.clone().requires_grad_(), k, pos, freq)
+    with torch.no_grad():
+        normalize_rotate_qk(q.clone().requires_grad_(), k, pos, freq)
+
+    kp, vp, _, _ = pools(2, 4, 2, 64, torch.bfloat16, "heads", False)
+    k8, v8, s8, t8 = pools(2, 4, 2, 64, torch.bfloat16, "heads", True)
+    slots = torch.arange(4, device="cuda")
+
+    def no_append(match, *args, **options):
+        with pytest.raises(ValueError, match=match):
+            append_kv(*args, **options)
+
+    no_append("identical shapes", k, k[:3], kp, vp, slots)
+    no_append("one slot per token", k, k, kp, vp, slots[:3])
+    no_append("int64", k, k, kp, vp, slots.int())
+    no_append("same shape and dtype", k, k, kp, vp[:1], slots)
+    no_append("need their scales", k, k, k8, v8, slots)
+    no_append("only INT8", k, k, kp, vp, slots, k_scales=s8)
+    no_append("float16", k, k, k8, v8, slots, k_scales=s8.float(), v_scales=t8)
+    no_append("do not match", k.half(), k.half(), kp, vp, slots)
+    no_append("kv_heads and head_dim", k[:, :1], k[:, :1], kp, vp, slots)
+    with pytest.raises(ValueError, match="do not match"):
+        read_kv(kp, vp, slots, dtype=torch.float16)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        read_kv(k8, v8, slots, k_scales=s8, v_scales=t8, dtype=torch.float32)
+    with pytest.raises(ValueError, match="needs a weight|both positions"):
+        normalize_rotate_append(q, k, k, kp, vp, slots, pos)
