@@ -25,8 +25,9 @@ LIB_PATH = LIB_DIR / "libseqattn_hip.so"
 PROBE_LIB_PATH = LIB_DIR / "libseqattn_probe.so"
 ARCH = "gfx950"
 
-SOURCES = ("sa_kernels.hip", "sa_rows.hip", "sa_decode.hip", "sa_update_d32.hip", "sa_update_d64.hip",
-           "sa_update_d128.hip", "sa_update_d256.hip", "sa_pipeline.cpp")
+SOURCES = ("sa_kernels.hip", "sa_rows.hip", "sa_decode.hip", "sa_decode_d64.hip", "sa_decode_d128.hip",
+           "sa_decode_d256.hip", "sa_update_d32.hip", "sa_update_d64.hip", "sa_update_d128.hip",
+           "sa_update_d256.hip", "sa_pipeline.cpp")
 PROBE_SOURCES = ("sa_probe.hip",)
 
 # Device-side flags.  Packed FP32 VALU instructions are disabled for all

@@ -1,0 +1,49 @@
+// The decoding attention's launch, shared by the sources that compile one head
+// size's kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sa_types.h"
+
+namespace sa {
+
+constexpr int kDecodeWaves = 4;  // wavefronts of a workgroup
+constexpr int kDecodeTile = 32;  // keys of a wave's step
+
+// A sequence's keys of one K/V head, for up to 8 NB of its query heads, are an
+// item.  The tiles of all items, sequence by sequence and head by head, are
+// dealt to the workgroups in equal contiguous ranges, so an item is in one
+// workgroup's range or split over neighbouring ones.
+struct DecodeParams {
+  const uint16_t* q;
+  const char *k, *v;
+  const uint16_t *ks, *vs;
+  const int32_t *table, *lengths;
+  uint16_t* out;
+  float* lse;
+  float* parts;    // two per workgroup: 8 NB rows of head_dim padded, then maximum and sum of each row
+  int32_t* owned;  // per workgroup: (sequence, head item, last workgroup) of an item that starts in its range and ends in another's; sequence -1: none
+  int64_t sq_t, sq_h, so_t, so_h, kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh, s_table, lse_h;
+  float scale_log2;
+  int32_t sequences, num_pages, max_pages, head_dim, page_tokens, room;  // room: keys of a table row
+  int32_t kv_heads, group, blocks;  // blocks: items of a K/V head
+  int32_t step_pages, step_rows;    // kDecodeWaves tiles in pages and rows
+  uint32_t page_magic, page_shift;  // key / page_tokens = key * magic >> shift
+};
+
+struct DecodeLaunch {
+  DecodeParams p;
+  int32_t workgroups;
+  bool bf16, int8, wide, any_page;  // wide: 16 query heads per item instead of 8; any_page: pages that end inside 16 keys
+  hipStream_t stream;
+};
+
+// One padded head_dim each.
+void launch_decode_d64(const DecodeLaunch& l);
+void launch_decode_d128(const DecodeLaunch& l);
+void launch_decode_d256(const DecodeLaunch& l);
+
+}  // namespace sa

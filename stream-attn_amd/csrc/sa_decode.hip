@@ -1,8 +1,4 @@
-// Attention of one new token per sequence over a paged K/V cache.
-//
-//   s_j = scale * q . k_j,  out = sum_j e^(s_j) v_j / sum_j e^(s_j),  lse = log sum_j e^(s_j)
-//
-// The plainest form: a wave per (sequence, query head), one key at a time.
+// Entry points of the decoding attention (sa_decode.h, sa_decode_kernel.h).
 
 #include <hip/hip_runtime.h>
 
@@ -10,71 +6,10 @@
 #include <cstdint>
 
 #include "sa_common.h"
-#include "sa_types.h"
+#include "sa_decode.h"
 
 namespace sa {
 namespace {
-
-struct DecodeParams {
-  const uint16_t* q;
-  const char *k, *v;
-  const uint16_t *ks, *vs;
-  const int32_t *table, *lengths;
-  uint16_t* out;
-  float* lse;
-  int64_t sq_t, sq_h, so_t, so_h, kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh, s_table, lse_h;
-  float scale_log2;
-  int32_t num_pages, max_pages, group, head_dim, page_tokens;
-};
-
-template <typename T, bool kInt8>
-__device__ inline float element(const char* base, int64_t at) {
-  if constexpr (kInt8) return (float)base[at];
-  return T::lo(reinterpret_cast<const uint16_t*>(base)[at]);
-}
-
-template <typename T, bool kInt8>
-__global__ __launch_bounds__(64) void decode_kernel(const DecodeParams p) {
-  const int s = blockIdx.x, h = blockIdx.y, kvh = h / p.group, lane = threadIdx.x;
-  const int64_t room = (int64_t)p.max_pages * p.page_tokens;
-  const int64_t len = p.lengths[s] < room ? p.lengths[s] : room;
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    q[i] = d < p.head_dim ? T::lo(p.q[s * p.sq_t + h * p.sq_h + d]) : 0.f;
-  }
-  for (int64_t j = 0; j < len; ++j) {
-    const int32_t page = p.table[s * p.s_table + j / p.page_tokens];
-    const int64_t row = j % p.page_tokens;
-    if (page < 0 || page >= p.num_pages) continue;
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < p.head_dim) dot += q[i] * element<T, kInt8>(p.k, page * p.kp + row * p.kt + kvh * p.kh + d);
-    }
-    for (int i = 1; i < 64; i <<= 1) dot += __shfl_xor(dot, i);
-    if (kInt8) dot *= Fp16::lo(p.ks[page * p.ksp + row * p.kst + kvh * p.ksh]);
-    if (dot * p.scale_log2 == -INFINITY) continue;
-    const float x = dot * p.scale_log2, top = fmaxf(m, x);
-    const float keep = exp2f(m - top), w = exp2f(x - top);
-    m = top;
-    l = l * keep + w;
-    const float vw = kInt8 ? w * Fp16::lo(p.vs[page * p.vsp + row * p.vst + kvh * p.vsh]) : w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < p.head_dim) acc[i] = acc[i] * keep + vw * element<T, kInt8>(p.v, page * p.vp + row * p.vt + kvh * p.vh + d);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < p.head_dim) p.out[s * p.so_t + h * p.so_h + d] = (uint16_t)T::pack(l == 0.f ? 0.f : acc[i] / l, 0.f);
-  }
-  if (p.lse != nullptr && lane == 0) p.lse[h * p.lse_h + s] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-}
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
@@ -100,6 +35,23 @@ int32_t check(const sa_decode_args* a) {
   return 0;
 }
 
+constexpr int kCUs = 256;
+
+int padded(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Workgroups of a launch: what the chip holds at once (four waves each; two to
+// a CU, one with the registers of head sizes past 128).  A launch over fewer
+// tiles leaves some without work.
+int workgroups(const sa_decode_args* a) { return kCUs * (padded(a->head_dim) == 256 ? 1 : 2); }
+
+bool wide(const sa_decode_args* a) { return a->q_heads / a->kv_heads > 8; }
+
+// owned, then parts.
+int64_t owned_bytes(const sa_decode_args* a) { return (int64_t)workgroups(a) * 16; }
+int64_t workspace_bytes(const sa_decode_args* a) {
+  return owned_bytes(a) + (int64_t)workgroups(a) * 2 * (wide(a) ? 16 : 8) * (padded(a->head_dim) + 2) * 4;
+}
+
 }  // namespace
 }  // namespace sa
 
@@ -110,7 +62,7 @@ int32_t sa_paged_decode_workspace_bytes(const sa_decode_args* a, int32_t device,
   sa::clear_error();
   if (a == nullptr || bytes == nullptr) return sa::invalid("null arguments");
   const int32_t rc = sa::check(a);
-  *bytes = 0;
+  *bytes = rc == 0 && a->sequences > 0 ? sa::workspace_bytes(a) : 0;
   return rc;
 }
 
@@ -131,7 +83,12 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
       !aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->k_pages, page_align) || !aligned(a->v_pages, page_align) ||
       !aligned(a->page_table, 4) || !aligned(a->lengths, 4))
     return invalid("an operand is missing or not aligned");
-  DecodeParams p{};
+  if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
+    return invalid("the workspace is missing, too small or not aligned");
+  for (int64_t s : {a->stride_kpt, a->stride_vpt})
+    if (s < 0 || s >= (1 << 26)) return invalid("token strides of the pages must be below 2^26 elements");
+  DecodeLaunch launch{};
+  DecodeParams& p = launch.p;
   p.q = static_cast<const uint16_t*>(a->q), p.out = static_cast<uint16_t*>(a->out), p.lse = a->lse;
   p.k = static_cast<const char*>(a->k_pages), p.v = static_cast<const char*>(a->v_pages);
   p.ks = static_cast<const uint16_t*>(a->k_scales), p.vs = static_cast<const uint16_t*>(a->v_scales);
@@ -141,17 +98,29 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   p.ksp = a->stride_ksp, p.kst = a->stride_kst, p.ksh = a->stride_ksh, p.vsp = a->stride_vsp, p.vst = a->stride_vst, p.vsh = a->stride_vsh;
   p.s_table = a->stride_table, p.lse_h = a->lse_stride_h;
   p.scale_log2 = (float)(a->softmax_scale * 1.4426950408889634074);
-  p.num_pages = (int32_t)a->num_pages, p.max_pages = a->max_pages;
-  p.group = a->q_heads / a->kv_heads, p.head_dim = a->head_dim, p.page_tokens = a->page_tokens;
+  p.sequences = a->sequences, p.num_pages = (int32_t)a->num_pages, p.max_pages = a->max_pages;
+  p.head_dim = a->head_dim, p.page_tokens = a->page_tokens, p.room = a->max_pages * a->page_tokens;
+  launch.wide = wide(a);
+  p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads;
+  const int32_t item_heads = launch.wide ? 16 : 8;
+  p.blocks = (p.group + item_heads - 1) / item_heads;
+  p.step_pages = kDecodeWaves * kDecodeTile / p.page_tokens, p.step_rows = kDecodeWaves * kDecodeTile % p.page_tokens;
+  // Exact for keys below 2^31: magic = floor(2^(31 + n) / page_tokens) + 1 with
+  // 2^n >= page_tokens is off by less than 2^-31 of a page per key.
+  uint32_t n = 0;
+  while ((1u << n) < (uint32_t)p.page_tokens) ++n;
+  p.page_shift = 31 + n;
+  p.page_magic = (uint32_t)(((uint64_t)1 << p.page_shift) / (uint32_t)p.page_tokens + 1);
+  p.owned = static_cast<int32_t*>(a->workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + owned_bytes(a));
+  launch.workgroups = workgroups(a);
+  launch.bf16 = a->dtype == SA_DTYPE_BF16, launch.int8 = a->pages_int8 != 0;
+  launch.any_page = a->page_tokens % 16 != 0;
+  launch.stream = static_cast<hipStream_t>(stream);
   DeviceGuard guard(device);
   SA_HIP_RETURN(guard.status());
-  const dim3 grid(a->sequences, a->q_heads);
-  hipStream_t hs = static_cast<hipStream_t>(stream);
-  const bool bf16 = a->dtype == SA_DTYPE_BF16;
-  if (a->pages_int8)
-    bf16 ? decode_kernel<Bf16, true><<<grid, 64, 0, hs>>>(p) : decode_kernel<Fp16, true><<<grid, 64, 0, hs>>>(p);
-  else
-    bf16 ? decode_kernel<Bf16, false><<<grid, 64, 0, hs>>>(p) : decode_kernel<Fp16, false><<<grid, 64, 0, hs>>>(p);
+  const int width = padded(a->head_dim);
+  (width == 64 ? launch_decode_d64 : width == 128 ? launch_decode_d128 : launch_decode_d256)(launch);
   SA_HIP_RETURN(hipGetLastError());
   return 0;
 } catch (const std::exception& error) {
