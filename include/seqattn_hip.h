@@ -595,7 +595,8 @@ int32_t sa_run_resident_noalloc(const void* q, const void* k, const void* v, voi
  * the unrounded row, 1 in place of a zero amax / 127; a row that is not finite
  * gets scale NaN.
  *
- * q and q_out are NULL together; k goes to k_out or to k_pages (the other is
+ * K's and V's pages have the same strides, and so have their scales.  q and
+ * q_out are NULL together; k goes to k_out or to k_pages (the other is
  * NULL); v and v_pages come with k_pages.  Strides in elements, unit in the
  * last dimension.  q, k, v, the outputs and 16-bit pages are 16-byte aligned
  * with strides in multiples of 8; int8 pages 8-byte aligned, strides in
@@ -614,8 +615,8 @@ typedef struct {
     const void *q_weight, *k_weight;
     int64_t stride_qt, stride_qh, stride_kt, stride_kh, stride_vt, stride_vh;
     int64_t stride_qot, stride_qoh, stride_kot, stride_koh;
-    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
-    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
+    int64_t stride_sp, stride_st, stride_sh; /* of their scales */
     int64_t stride_pos_axis, stride_pos_token;
     int64_t tokens, num_pages;
     double eps;
@@ -637,8 +638,8 @@ typedef struct {
     const void *k_pages, *v_pages, *k_scales, *v_scales;
     const int64_t* slots;
     void *k_out, *v_out;
-    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
-    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
+    int64_t stride_sp, stride_st, stride_sh; /* of their scales */
     int64_t tokens, num_pages;
     int32_t kv_heads, head_dim, page_tokens, dtype, pages_int8, reserved;
 } sa_read_args;
@@ -661,7 +662,7 @@ int32_t sa_read_kv(const sa_read_args* args, int32_t device, void* stream);
  * length is used, whatever they hold.
  *
  * `workspace` (sa_paged_decode_workspace_bytes, 16-byte aligned) is the call's
- * own until it has run.
+ * own until it has run.  Token strides of the pages are in [0, 2^26).
  */
 typedef struct {
     const void *q, *k_pages, *v_pages, *k_scales, *v_scales;
@@ -671,8 +672,8 @@ typedef struct {
     void* workspace;
     int64_t workspace_bytes;
     int64_t stride_qt, stride_qh, stride_ot, stride_oh;
-    int64_t stride_kpp, stride_kpt, stride_kph, stride_vpp, stride_vpt, stride_vph;
-    int64_t stride_ksp, stride_kst, stride_ksh, stride_vsp, stride_vst, stride_vsh;
+    int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
+    int64_t stride_sp, stride_st, stride_sh; /* of their scales */
     int64_t stride_table, lse_stride_h;
     int64_t num_pages;
     double softmax_scale;

@@ -12,11 +12,12 @@ namespace sa {
 
 constexpr int kDecodeWaves = 4;  // wavefronts of a workgroup
 constexpr int kDecodeTile = 32;  // keys of a wave's step
+constexpr int kMaxWorkgroups = 512;
 
 // A sequence's keys of one K/V head, for up to 8 NB of its query heads, are an
 // item.  The tiles of all items, sequence by sequence and head by head, are
-// dealt to the workgroups in equal contiguous ranges, so an item is in one
-// workgroup's range or split over neighbouring ones.
+// dealt to the waves in equal contiguous runs, so an item is in one wave's run
+// or split over neighbouring ones.
 struct DecodeParams {
   const uint16_t* q;
   const char *k, *v;
@@ -25,12 +26,16 @@ struct DecodeParams {
   uint16_t* out;
   float* lse;
   float* parts;    // two per workgroup: 8 NB rows of head_dim padded, then maximum and sum of each row
-  int32_t* owned;  // per workgroup: (sequence, head item, last workgroup) of an item that starts in its range and ends in another's; sequence -1: none
-  int64_t sq_t, sq_h, so_t, so_h, kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh, s_table, lse_h;
+  // The items that are split: (sequence or -1, item of the sequence, first and
+  // last workgroup).  By item where there are no more items than workgroups
+  // (by_item), else by the first workgroup, whose run ends in it.
+  int32_t* owned;
+  int64_t sq_t, sq_h, so_t, so_h, sp, st, sh, ssp, sst, ssh, s_table, lse_h;  // sp .. ssh: of the pages and their scales
   float scale_log2;
   int32_t sequences, num_pages, max_pages, head_dim, page_tokens, room;  // room: keys of a table row
+  int32_t by_item;
   int32_t kv_heads, group, blocks;  // blocks: items of a K/V head
-  int32_t step_pages, step_rows;    // kDecodeWaves tiles in pages and rows
+  int32_t step_pages, step_rows;    // a tile in pages and rows
   uint32_t page_magic, page_shift;  // key / page_tokens = key * magic >> shift
 };
 

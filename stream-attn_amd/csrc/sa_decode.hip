@@ -40,11 +40,11 @@ constexpr int kCUs = 256;
 int padded(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 // Workgroups of a launch: what the chip holds at once (four waves each; two to
-// a CU, one with the registers of head sizes past 128).  A launch over fewer
-// tiles leaves some without work.
-int workgroups(const sa_decode_args* a) { return kCUs * (padded(a->head_dim) == 256 ? 1 : 2); }
-
+// a CU, one with the registers of head sizes past 128 or 16 query heads).  A
+// launch over fewer tiles leaves some without work.
 bool wide(const sa_decode_args* a) { return a->q_heads / a->kv_heads > 8; }
+int workgroups(const sa_decode_args* a) { return kCUs * (padded(a->head_dim) == 256 || wide(a) ? 1 : 2); }
+static_assert(kMaxWorkgroups == 2 * kCUs, "the join holds a factor per part");
 
 // owned, then parts.
 int64_t owned_bytes(const sa_decode_args* a) { return (int64_t)workgroups(a) * 16; }
@@ -73,8 +73,8 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   const int32_t rc = check(a);
   if (rc != 0) return rc;
   if (a->sequences == 0) return 0;
-  const int64_t strides[] = {a->stride_qt, a->stride_qh, a->stride_ot, a->stride_oh, a->stride_kpp, a->stride_kpt,
-                             a->stride_kph, a->stride_vpp, a->stride_vpt, a->stride_vph};
+  const int64_t strides[] = {a->stride_qt, a->stride_qh, a->stride_ot, a->stride_oh, a->stride_pp, a->stride_pt,
+                             a->stride_ph};
   for (int64_t s : strides)
     if (s % 8) return invalid("strides must be multiples of 8 elements");
   const int64_t page_align = a->pages_int8 ? 8 : 16;
@@ -85,8 +85,7 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
     return invalid("an operand is missing or not aligned");
   if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
     return invalid("the workspace is missing, too small or not aligned");
-  for (int64_t s : {a->stride_kpt, a->stride_vpt})
-    if (s < 0 || s >= (1 << 26)) return invalid("token strides of the pages must be below 2^26 elements");
+  if (a->stride_pt < 0 || a->stride_pt >= (1 << 26)) return invalid("the pages' token stride must be below 2^26 elements");
   DecodeLaunch launch{};
   DecodeParams& p = launch.p;
   p.q = static_cast<const uint16_t*>(a->q), p.out = static_cast<uint16_t*>(a->out), p.lse = a->lse;
@@ -94,8 +93,8 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   p.ks = static_cast<const uint16_t*>(a->k_scales), p.vs = static_cast<const uint16_t*>(a->v_scales);
   p.table = a->page_table, p.lengths = a->lengths;
   p.sq_t = a->stride_qt, p.sq_h = a->stride_qh, p.so_t = a->stride_ot, p.so_h = a->stride_oh;
-  p.kp = a->stride_kpp, p.kt = a->stride_kpt, p.kh = a->stride_kph, p.vp = a->stride_vpp, p.vt = a->stride_vpt, p.vh = a->stride_vph;
-  p.ksp = a->stride_ksp, p.kst = a->stride_kst, p.ksh = a->stride_ksh, p.vsp = a->stride_vsp, p.vst = a->stride_vst, p.vsh = a->stride_vsh;
+  p.sp = a->stride_pp, p.st = a->stride_pt, p.sh = a->stride_ph;
+  p.ssp = a->stride_sp, p.sst = a->stride_st, p.ssh = a->stride_sh;
   p.s_table = a->stride_table, p.lse_h = a->lse_stride_h;
   p.scale_log2 = (float)(a->softmax_scale * 1.4426950408889634074);
   p.sequences = a->sequences, p.num_pages = (int32_t)a->num_pages, p.max_pages = a->max_pages;
@@ -104,7 +103,7 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads;
   const int32_t item_heads = launch.wide ? 16 : 8;
   p.blocks = (p.group + item_heads - 1) / item_heads;
-  p.step_pages = kDecodeWaves * kDecodeTile / p.page_tokens, p.step_rows = kDecodeWaves * kDecodeTile % p.page_tokens;
+  p.step_pages = kDecodeTile / p.page_tokens, p.step_rows = kDecodeTile % p.page_tokens;
   // Exact for keys below 2^31: magic = floor(2^(31 + n) / page_tokens) + 1 with
   // 2^n >= page_tokens is off by less than 2^-31 of a page per key.
   uint32_t n = 0;
@@ -114,6 +113,7 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   p.owned = static_cast<int32_t*>(a->workspace);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + owned_bytes(a));
   launch.workgroups = workgroups(a);
+  p.by_item = (int64_t)a->sequences * p.kv_heads * p.blocks <= launch.workgroups;
   launch.bf16 = a->dtype == SA_DTYPE_BF16, launch.int8 = a->pages_int8 != 0;
   launch.any_page = a->page_tokens % 16 != 0;
   launch.stream = static_cast<hipStream_t>(stream);

@@ -94,6 +94,30 @@ __device__ inline float other_half(float x) {
 // 2^x of a running maximum's change: 0 from -inf, 1 where nothing changes.
 __device__ inline float ratio(float from, float to) { return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to); }
 
+// A wave's share of one item: tiles first .. last - 1 of the item's `tiles`.
+struct Piece {
+  int64_t start;  // the launch's tile that is the item's first
+  const int32_t* table;
+  int32_t s, length, tiles, first, last;
+  int32_t kv_head, block;  // query heads 8 NB block .. of the K/V head's group
+};
+
+// The kernel's arguments, read again where they are used: what only a piece's
+// ends need would otherwise sit in scalar registers, and those that do not fit
+// in lanes of vector registers, all through the loop over the keys.
+typedef const DecodeParams __attribute__((address_space(4)))* Arguments;
+__device__ inline Arguments arguments() {
+  Arguments a = (Arguments)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+
+__device__ inline int32_t length_of(Arguments a, int s) {
+  const int32_t n = a->lengths[s];
+  return n < a->room ? n : a->room;
+}
+__device__ inline int32_t tiles_of(int32_t length) { return length > 0 ? (length - 1) / kDecodeTile + 1 : 0; }
+
 // A wave's loads of one step, in flight while the step before is computed.
 template <bool kInt8, int DP, bool kAnyPage>
 struct Step {
@@ -104,45 +128,54 @@ struct Step {
   uint32_t scale;  // INT8: lane g's of K (g < 8) or V, key 4 (g % 8) + j
   uint32_t seen;   // bit t: key 4t + j has weight
   bool full;       // all 32 keys have
+  // Page numbers first_id + lane of the sequence, for the steps to come.
+  int32_t ids, first_id;
 
-  // Keys key0 .. key0 + 31 of a sequence with `length` keys.  key0 is in row
-  // `row` of page number `page` of the sequence.
-  __device__ __attribute__((always_inline)) void load(const DecodeParams& p, const int32_t* table, int head, int32_t key0,
-                                                      int32_t length, int32_t page, int32_t row, int j, int g) {
+  __device__ inline int32_t id_of(const DecodeParams& p, const Piece& x, int32_t n, int lane) {
+    if (n - first_id >= 64) {
+      first_id = n;
+      ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
+    }
+    return __builtin_amdgcn_readlane(ids, n - first_id);
+  }
+
+  // Keys key0 .. key0 + 31 of the piece's sequence; key0 is in row `row` of its
+  // page number `page`.
+  __device__ __attribute__((always_inline)) void load(const DecodeParams& p, const Piece& x, int32_t key0, int32_t page,
+                                                      int32_t row, int lane) {
+    const int j = lane >> 4, g = lane & 15;
+    const char *kh = p.k + x.kv_head * p.sh * ES, *vh = p.v + x.kv_head * p.sh * ES;
     uint32_t at[NP];
 #pragma unroll
     for (int c = 0; c < NP; ++c) at[c] = (128 * c + EL * g < p.head_dim ? 128 * c + EL * g : 0) * ES;
     const bool second = g >= 8;
     if constexpr (!kAnyPage) {
       // Two runs of 16 keys, each in one page.
-      bool held = true;
+      full = x.length - key0 >= kDecodeTile;
+      const uint32_t rows = j * (uint32_t)p.st * ES;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int32_t n = page, r = row + 16 * h;
-        if (r >= p.page_tokens) ++n, r -= p.page_tokens;
-        int32_t id = n < p.max_pages ? uniform(table[n]) : -1;
-        const bool ok = id >= 0 && id < p.num_pages;
+        if (h == 1 && (row += 16) >= p.page_tokens) ++page, row -= p.page_tokens;
+        int32_t id = id_of(p, x, page, lane);
+        const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
         if (!ok) id = 0;  // rows of a page that exists, read and not used
-        held = held && ok;
-        const char* kb = p.k + (id * p.kp + r * p.kt + head * p.kh) * ES;
-        const char* vb = p.v + (id * p.vp + r * p.vt + head * p.vh) * ES;
-        const uint32_t kr = j * (uint32_t)p.kt * ES, vr = j * (uint32_t)p.vt * ES;
+        full = full && ok;
+        const int64_t base = (id * p.sp + row * p.st) * ES;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int c = 0; c < NP; ++c) k[4 * h + u][c] = load_dwords<RW>(kb + 4 * u * p.kt * ES, kr + at[c]);
+          for (int c = 0; c < NP; ++c) k[4 * h + u][c] = load_dwords<RW>(kh + base + 4 * u * p.st * ES, rows + at[c]);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int c = 0; c < NP; ++c) v[4 * h + u][c] = load_dwords<RW>(vb + 4 * u * p.vt * ES, vr + at[c]);
+          for (int c = 0; c < NP; ++c) v[4 * h + u][c] = load_dwords<RW>(vh + base + 4 * u * p.st * ES, rows + at[c]);
         if constexpr (kInt8) {
-          const uint16_t* s = second ? p.vs + id * p.vsp + r * p.vst + head * p.vsh : p.ks + id * p.ksp + r * p.kst + head * p.ksh;
-          if ((g >> 2 & 1) == h) scale = s[(4 * (g & 3) + j) * (second ? p.vst : p.kst)];
+          const uint16_t* s = (second ? p.vs : p.ks) + id * p.ssp + row * p.sst + x.kv_head * p.ssh;
+          if ((g >> 2 & 1) == h) scale = s[(4 * (g & 3) + j) * p.sst];
         }
         const uint32_t mask = ok ? 15u : 0u;
         seen = h == 0 ? mask : seen | mask << 4;
       }
-      full = held && key0 + kDecodeTile <= length;
     } else {
       seen = 0;
 #pragma unroll
@@ -150,129 +183,159 @@ struct Step {
         const int32_t key = key0 + 4 * t + j;
         const int32_t n = (int32_t)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift);
         const int32_t r = key - n * p.page_tokens;
-        int32_t id = n < p.max_pages ? table[n] : -1;
-        const bool ok = id >= 0 && id < p.num_pages;
+        int32_t id = n < p.max_pages ? x.table[n] : -1;
+        const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
         if (!ok) id = 0;
         seen |= (uint32_t)ok << t;
-        const char* kb = p.k + (id * p.kp + r * p.kt + head * p.kh) * ES;
-        const char* vb = p.v + (id * p.vp + r * p.vt + head * p.vh) * ES;
+        const int64_t base = (id * p.sp + r * p.st) * ES;
 #pragma unroll
-        for (int c = 0; c < NP; ++c) k[t][c] = load_dwords<RW>(kb, at[c]), v[t][c] = load_dwords<RW>(vb, at[c]);
+        for (int c = 0; c < NP; ++c) k[t][c] = load_dwords<RW>(kh + base, at[c]), v[t][c] = load_dwords<RW>(vh + base, at[c]);
         if constexpr (kInt8)
-          if ((g & 7) == t) scale = second ? p.vs[id * p.vsp + r * p.vst + head * p.vsh] : p.ks[id * p.ksp + r * p.kst + head * p.ksh];
+          if ((g & 7) == t) scale = (second ? p.vs : p.ks)[id * p.ssp + r * p.sst + x.kv_head * p.ssh];
       }
-      full = __all(seen == 255u) && key0 + kDecodeTile <= length;
+      full = __all(seen == 255u) && x.length - key0 >= kDecodeTile;
     }
-    if (key0 + kDecodeTile > length) {
+    if (x.length - key0 < kDecodeTile) {
 #pragma unroll
       for (int t = 0; t < 8; ++t)
-        if (key0 + 4 * t + j >= length) seen &= ~(1u << t);
+        if (key0 + 4 * t + j >= x.length) seen &= ~(1u << t);
     }
   }
 };
 
-// Part of a sequence's keys, for one item: maximum, sum and O^T per query head.
+// What a wave leaves of an item that it does not have whole: the item's head
+// (it started in an earlier range) or tail (it ends in a later one).
+struct PartInfo {
+  int64_t end;  // the launch's tile behind the item
+  int32_t s, kv_head, block;
+  int32_t state;  // 0: none, 1: goes on in the next wave, 2: ends here
+};
+
+// Every wave has an equal run of the launch's tiles.  Items that lie whole in
+// it are done there; the others' parts meet in LDS, and those of items that
+// leave the workgroup's run in the workspace.
 template <typename T, bool kInt8, int DP, int NB, bool kAnyPage>
-__global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) void decode_kernel(const DecodeParams p) {
   using S = Shape<DP>;
   using PT = std::conditional_t<kInt8, Bf16, T>;  // INT8: weights times V's scales, beyond float16's range
   constexpr int EL = S::EL, NP = S::NP, NI = S::NI, NC = S::NC;
   constexpr float bias = kBias<PT>;
   constexpr int kRow = 2 * DP;  // bytes of a key in LDS
-  __shared__ __attribute__((aligned(16))) char lds[kDecodeWaves][kDecodeTile * kRow + (kInt8 ? 256 : 0)];
-  __shared__ float stats[kDecodeWaves][8 * NB][2];
-  __shared__ int64_t found[3];
+  constexpr int kPart = 8 * NB * DP;  // floats of a part
+  __shared__ __attribute__((aligned(16))) char lds[kDecodeWaves][kDecodeTile * kRow + (kInt8 ? 256 : 0)];  // K, then the tail
+  __shared__ __attribute__((aligned(16))) float heads_lds[kDecodeWaves][kPart];
+  __shared__ float stats[kDecodeWaves][2][8 * NB][2];  // maximum and sum of the head's, the tail's rows
+  __shared__ PartInfo info[kDecodeWaves][2];
+  __shared__ int64_t found[kDecodeWaves][2];
+  static_assert(kPart * 4 <= kDecodeTile * kRow, "the tail's place");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int j = lane >> 4, g = lane & 15;
-  const int items = p.kv_heads * p.blocks;
-  const int w = blockIdx.x, workgroups = gridDim.x;
-  const auto length_of = [&](int s) {
-    const int32_t n = p.lengths[s];
-    return n < p.room ? n : p.room;
-  };
-  const auto tiles_of = [&](int s) {
-    const int32_t n = length_of(s);
-    return n > 0 ? (n + kDecodeTile - 1) / kDecodeTile : 0;
-  };
-
-  // Tiles before every thread's run of sequences; the workgroup's range.
-  int64_t* sums = reinterpret_cast<int64_t*>(&lds[0][0]);
-  const int run = (p.sequences + 64 * kDecodeWaves - 1) / (64 * kDecodeWaves);
-  const int s_first = tid * run, s_last = s_first + run < p.sequences ? s_first + run : p.sequences;
-  int64_t own = 0;
-  for (int s = s_first; s < s_last; ++s) own += tiles_of(s);
-  int64_t upto = own;  // inclusive
-  for (int i = 1; i < 64; i <<= 1) {
-    const int64_t x = __shfl_up(upto, i);
-    if (lane >= i) upto += x;
-  }
-  if (lane == 63) sums[wave] = upto;
-  __syncthreads();
-  int64_t total = 0;
-  for (int i = 0; i < kDecodeWaves; ++i) {
-    if (i < wave) upto += sums[i];
-    total += sums[i];
-  }
-  total *= items;
-  // At least a tile for each of its waves.
-  int64_t share = (total + workgroups - 1) / workgroups;
-  if (share < kDecodeWaves) share = kDecodeWaves;
-  const int64_t begin = w * share, end = begin + share < total ? begin + share : total;
-  if (begin < end && (upto - own) * items <= begin && begin < upto * items) {
-    int64_t before = upto - own;
-    int s = s_first;
-    for (; s < s_last; ++s) {
-      const int64_t n = tiles_of(s);
-      if (begin < (before + n) * items) break;
-      before += n;
+  int64_t share, total;  // tiles of a wave's run
+  int64_t begin, end;
+  {
+    const Arguments a = arguments();
+    const int items = a->kv_heads * a->blocks, w = blockIdx.x, workgroups = gridDim.x;
+    // Tiles before every thread's run of sequences.
+    int64_t* sums = reinterpret_cast<int64_t*>(&lds[0][0]);
+    const int run = (a->sequences + 64 * kDecodeWaves - 1) / (64 * kDecodeWaves);
+    const int s_first = tid * run, s_last = s_first + run < a->sequences ? s_first + run : a->sequences;
+    int64_t own = 0;
+    for (int s = s_first; s < s_last; ++s) own += tiles_of(length_of(a, s));
+    int64_t upto = own;  // inclusive
+    for (int i = 1; i < 64; i <<= 1) {
+      const int64_t x = __shfl_up(upto, i);
+      if (lane >= i) upto += x;
     }
-    found[0] = s, found[1] = before * items;
-  }
-  // Sequences without keys have no tiles.
-  for (int s = w; s < p.sequences; s += workgroups) {
-    if (length_of(s) > 0) continue;
-    for (int i = tid; i < p.kv_heads * p.group * (p.head_dim / 8); i += 64 * kDecodeWaves) {
-      const int h = i / (p.head_dim / 8), d = 8 * (i - h * (p.head_dim / 8));
-      *reinterpret_cast<u32x4*>(p.out + s * p.so_t + h * p.so_h + d) = u32x4{0, 0, 0, 0};
-      if (d == 0 && p.lse != nullptr) p.lse[h * p.lse_h + s] = -INFINITY;
+    if (lane == 63) sums[wave] = upto;
+    if (tid < 2 * kDecodeWaves) info[tid >> 1][tid & 1].state = 0;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < kDecodeWaves; ++i) {
+      if (i < wave) upto += sums[i];
+      total += sums[i];
     }
+    total *= items;
+    const int64_t waves = (int64_t)workgroups * kDecodeWaves;
+    share = (total + waves - 1) / waves;
+    for (int i = 0; i < kDecodeWaves; ++i) {
+      const int64_t at = (w * kDecodeWaves + i) * share;
+      if (at >= total || at < (upto - own) * items || at >= upto * items) continue;
+      int64_t before = upto - own;
+      int s = s_first;
+      for (; s < s_last; ++s) {
+        const int64_t n = tiles_of(length_of(a, s));
+        if (at < (before + n) * items) break;
+        before += n;
+      }
+      found[i][0] = s, found[i][1] = before * items;
+    }
+    // Sequences without keys have no tiles.
+    for (int s = w; s < a->sequences; s += workgroups) {
+      if (length_of(a, s) > 0) continue;
+      const int granules = a->head_dim / 8;
+      for (int i = tid; i < a->kv_heads * a->group * granules; i += 64 * kDecodeWaves) {
+        const int h = i / granules, d = 8 * (i - h * granules);
+        *reinterpret_cast<u32x4*>(a->out + s * a->so_t + h * a->so_h + d) = u32x4{0, 0, 0, 0};
+        if (d == 0 && a->lse != nullptr) a->lse[h * a->lse_h + s] = -INFINITY;
+      }
+      for (int i = tid; a->by_item && i < items; i += 64 * kDecodeWaves) a->owned[4 * (s * items + i)] = -1;
+    }
+    if (tid == 0 && !a->by_item) a->owned[4 * w] = -1;
+    __syncthreads();
+    begin = (w * kDecodeWaves + wave) * share, end = begin + share < total ? begin + share : total;
   }
-  __syncthreads();
-  if (tid == 0) p.owned[4 * w] = -1;
-  if (begin >= end) return;
+  if ((int64_t)blockIdx.x * kDecodeWaves * share >= total) return;
 
   char* mine = &lds[wave][0];
   float* scales = reinterpret_cast<float*>(mine + kDecodeTile * kRow);
-  int s = uniform((int)found[0]);
-  int64_t at = begin;        // the next tile
-  int64_t s_start = found[1];  // the sequence's first
-  while (at < end) {
-    int32_t tiles = uniform(tiles_of(s));
-    while (at >= s_start + (int64_t)tiles * items) {
-      s_start += (int64_t)tiles * items;
-      tiles = uniform(tiles_of(++s));
-    }
-    const int32_t length = uniform(length_of(s));
-    const int item = uniform((int)((at - s_start) / tiles));
-    const int64_t item_start = s_start + (int64_t)item * tiles, item_end = item_start + tiles;
-    const int32_t first = uniform((int32_t)(at - item_start));
-    const int32_t last = uniform((int32_t)((item_end < end ? item_end : end) - item_start));
-    const int kv_head = item / p.blocks;
-    const int h0 = (item - kv_head * p.blocks) * 8 * NB;                  // of the group
-    const int heads = p.group - h0 < 8 * NB ? p.group - h0 : 8 * NB;
-    const int32_t* table = p.table + s * p.s_table;
-
+  Piece cur, next;
+  // The loads run ahead of the products by a step, also from a piece to the
+  // next: `tile` is the one in `step`.
+  Step<kInt8, DP, kAnyPage> step;
+  int32_t tile, page = 0, row = 0;
+  const auto enter = [&](const Piece& x) {
+    tile = x.first;
+    step.first_id = -64;
+    page = uniform((int32_t)((uint64_t)(uint32_t)(tile * kDecodeTile) * p.page_magic >> p.page_shift));
+    row = tile * kDecodeTile - page * p.page_tokens;
+    if constexpr (!kAnyPage) step.first_id = page - 64;
+  };
+  // The rest of a piece whose item starts at x.start, as far as the run goes.
+  const auto bound = [&](Piece& x) {
+    const int64_t left = end - x.start;
+    x.last = left < x.tiles ? (int32_t)left : x.tiles;
+  };
+  if (begin < end) {
+    const Arguments a = arguments();
+    cur.s = uniform((int)found[wave][0]);
+    cur.length = uniform(length_of(a, cur.s));
+    cur.tiles = tiles_of(cur.length);
+    const int64_t into = begin - found[wave][1];
+    const int item = uniform((int)(into / cur.tiles));
+    cur.start = found[wave][1] + (int64_t)item * cur.tiles;
+    cur.first = uniform((int32_t)(begin - cur.start));
+    cur.kv_head = item / a->blocks, cur.block = item - cur.kv_head * a->blocks;
+    cur.table = a->table + cur.s * a->s_table;
+    bound(cur);
+    next = cur;
+    enter(cur);
+    step.load(p, cur, tile * kDecodeTile, page, row, lane);
+  }
+  while (begin < end) {
     // Q^T: chunk c of column g's head, elements 32c + 8j .. + 7.
     u32x4 q[NB][NC];
+    {
+      const Arguments a = arguments();
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int h = 8 * n + (g & 7);
-      const uint16_t* row = p.q + s * p.sq_t + (kv_head * p.group + h0 + (h < heads ? h : 0)) * p.sq_h;
+      for (int n = 0; n < NB; ++n) {
+        const int h = 8 * (NB * cur.block + n) + (g & 7);  // of the group
+        const uint16_t* at = a->q + cur.s * a->sq_t + (cur.kv_head * a->group + (h < a->group ? h : 0)) * a->sq_h;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = 32 * c + 8 * j;
-        q[n][c] = h < heads && d < p.head_dim ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
+        for (int c = 0; c < NC; ++c) {
+          const int d = 32 * c + 8 * j;
+          q[n][c] = h < a->group && d < a->head_dim ? *reinterpret_cast<const u32x4*>(at + d) : u32x4{0, 0, 0, 0};
+        }
       }
     }
     // K's elements past head_dim are zeros that no step writes.
@@ -290,12 +353,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
       for (int i = 0; i < NI; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    Step<kInt8, DP, kAnyPage> step;
-    int32_t tile = first + wave;
-    int32_t page = uniform((int32_t)((uint64_t)(uint32_t)(tile * kDecodeTile) * p.page_magic >> p.page_shift));
-    int32_t row = tile * kDecodeTile - page * p.page_tokens;
-    if (tile < last) step.load(p, table, kv_head, tile * kDecodeTile, length, page, row, j, g);
-    while (tile < last) {
+    for (bool more = true; more;) {
       // K to LDS, 16-byte granules of row r exchanged by r so that the reads
       // below meet every bank once.
 #pragma unroll
@@ -327,12 +385,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
       if (!full) {
 #pragma unroll
         for (int t = 0; t < 8; ++t)
-          if (!(seen >> t & 1)) {
 #pragma unroll
-            for (int c = 0; c < NP; ++c)
+          for (int c = 0; c < NP; ++c)
 #pragma unroll
-              for (int i = 0; i < step.RW; ++i) step.v[t][c].w[i] = 0;
-          }
+            for (int i = 0; i < step.RW; ++i) step.v[t][c].w[i] = seen >> t & 1 ? step.v[t][c].w[i] : 0;
       }
       // V^T: product i's keys, a pair of loads per dword.
       u32x4 vt[NI];
@@ -348,11 +404,29 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
               vt[EL * c + i][u] = __builtin_amdgcn_perm(step.v[2 * u + 1][c].w[i / 2], step.v[2 * u][c].w[i / 2],
                                                         i & 1 ? 0x07060302u : 0x05040100u);
           }
-      tile += kDecodeWaves;
-      if (tile < last) {
+      if (++tile < cur.last) {
         page += p.step_pages, row += p.step_rows;
         if (row >= p.page_tokens) ++page, row -= p.page_tokens;
-        step.load(p, table, kv_head, tile * kDecodeTile, length, page, row, j, g);
+        step.load(p, next, tile * kDecodeTile, page, row, lane);
+      } else {
+        more = false;
+        if (cur.start + cur.last < end) {
+          // The next item: the sequence's next, or the first of the next
+          // sequence that has keys.
+          const Arguments a = arguments();
+          next.start += next.tiles, next.first = 0;
+          if (++next.block == a->blocks) next.block = 0, ++next.kv_head;
+          if (next.kv_head == a->kv_heads) {
+            next.kv_head = 0;
+            do next.length = uniform(length_of(a, ++next.s));
+            while (next.length <= 0);
+            next.tiles = tiles_of(next.length);
+            next.table = a->table + next.s * a->s_table;
+          }
+          bound(next);
+          enter(next);
+          step.load(p, next, tile * kDecodeTile, page, row, lane);
+        }
       }
       wave_lds_order();
 
@@ -365,9 +439,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
         for (int b = 0; b < 2; ++b) {
           const int r = 16 * b + 4 * (g & 3) + (g >> 2);
           const int turn = DP == 64 ? r >> 1 & 7 : r & 15;
-          const u32x4 a = *reinterpret_cast<const u32x4*>(mine + r * kRow + 16 * ((4 * c + j) ^ turn));
+          const u32x4 x = *reinterpret_cast<const u32x4*>(mine + r * kRow + 16 * ((4 * c + j) ^ turn));
 #pragma unroll
-          for (int n = 0; n < NB; ++n) st[n][b] = T::mma(a, q[n][c], st[n][b]);
+          for (int n = 0; n < NB; ++n) st[n][b] = T::mma(x, q[n][c], st[n][b]);
         }
       float ks[8], vs[8];
       if constexpr (kInt8) {
@@ -375,7 +449,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
         for (int t = 0; t < 8; t += 4) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(scales + 16 * j + t), y = *reinterpret_cast<const f32x4*>(scales + 16 * j + 8 + t);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ks[t + i] = x[i], vs[t + i] = seen >> (t + i) & 1 ? y[i] : 0.f;
+          for (int i = 0; i < 4; ++i) ks[t + i] = x[i], vs[t + i] = full || seen >> (t + i) & 1 ? y[i] : 0.f;
         }
       }
       wave_lds_order();
@@ -386,14 +460,18 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
         for (int t = 0; t < 8; ++t) {
           y[t] = st[n][t / 4][t & 3] * p.scale_log2;
           if constexpr (kInt8) y[t] *= ks[t];
-          if (!full && !(seen >> t & 1)) y[t] = -INFINITY;
-          top = fmaxf(top, y[t]);
         }
+        if (!full) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) y[t] = seen >> t & 1 ? y[t] : -INFINITY;
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) top = fmaxf(top, y[t]);
         if (__any(top > m[n] + (bias + kSlack))) {
           top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32)) - bias;
-          const float next = fmaxf(m[n], top), keep = ratio(m[n], next);
-          m[n] = next;
+          const float to = fmaxf(m[n], top), keep = ratio(m[n], to);
+          m[n] = to;
           l[n] *= keep;
 #pragma unroll
           for (int i = 0; i < NI; ++i) acc[n][i] *= keep;
@@ -414,28 +492,41 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
       }
     }
 
-    // The waves' parts: maxima and sums first, then O^T at the common maximum.
+    // The piece's end: high and low parts together, the lanes' sums together.
+    const Arguments a = arguments();
+    const bool starts = cur.first == 0, ends = cur.last == cur.tiles;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       l[n] += __shfl_xor(l[n], 16);
       l[n] += __shfl_xor(l[n], 32);
-      if (lane < 8) stats[wave][8 * n + lane][0] = m[n], stats[wave][8 * n + lane][1] = l[n];
-    }
-    __syncthreads();
-    float* part = reinterpret_cast<float*>(mine);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float top = -INFINITY;
-      for (int i = 0; i < kDecodeWaves; ++i) top = fmaxf(top, stats[i][8 * n + (g & 7)][0]);
-      const float f = ratio(m[n], top);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = acc[n][i][e] * f;
-          acc[n][i][e] = x + other_half(x);
-        }
-      if (g < 8) {
+        for (int e = 0; e < 4; ++e) acc[n][i][e] += other_half(acc[n][i][e]);
+      const int h = 8 * (NB * cur.block + n) + (g & 7);
+      if (g >= 8 || h >= a->group) continue;
+      if (starts && ends) {
+        const int head = cur.kv_head * a->group + h;
+        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+        uint16_t* out = a->out + cur.s * a->so_t + head * a->so_h;
+#pragma unroll
+        for (int c = 0; c < NP; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 128 * c + EL * (4 * j + e);
+            uint32_t o[EL / 2];
+#pragma unroll
+            for (int i = 0; i < EL; i += 2) o[i / 2] = T::pack(acc[n][EL * c + i][e] * inv, acc[n][EL * c + i + 1][e] * inv);
+            if (d >= a->head_dim) continue;
+            if constexpr (EL == 8)
+              *reinterpret_cast<u32x4*>(out + d) = u32x4{o[0], o[1], o[2], o[3]};
+            else
+              *reinterpret_cast<u32x2*>(out + d) = u32x2{o[0], o[1]};
+          }
+        if (j == 0 && a->lse != nullptr)
+          a->lse[head * a->lse_h + cur.s] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+      } else {
+        float* part = starts ? reinterpret_cast<float*>(mine) : heads_lds[wave];
 #pragma unroll
         for (int c = 0; c < NP; ++c)
 #pragma unroll
@@ -444,79 +535,126 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 ? 1 : 2) void decode_k
             for (int i = 0; i < EL; i += 4)
               *reinterpret_cast<f32x4*>(part + (8 * n + g) * DP + 128 * c + EL * (4 * j + e) + i) =
                   f32x4{acc[n][EL * c + i][e], acc[n][EL * c + i + 1][e], acc[n][EL * c + i + 2][e], acc[n][EL * c + i + 3][e]};
+        if (j == 0) stats[wave][starts][8 * n + g][0] = m[n], stats[wave][starts][8 * n + g][1] = l[n];
       }
     }
-    __syncthreads();
-    const bool starts = first == 0, ends = last == tiles;
-    float* slot = p.parts + ((int64_t)w * 2 + (starts ? 1 : 0)) * (8 * NB * (DP + 2));
+    if (lane == 0) {
+      if (starts && ends) {
+        if (a->by_item) a->owned[4 * ((cur.s * a->kv_heads + cur.kv_head) * a->blocks + cur.block)] = -1;
+      } else {
+        info[wave][starts] = {cur.start + cur.tiles, cur.s, cur.kv_head, cur.block, ends ? 2 : 1};
+      }
+    }
+    if (cur.start + cur.last >= end) break;
+    cur = next;
+  }
+
+  // The parts: wave 0's head, and the tails, each with the heads that go on from
+  // it in the waves behind.
+  __syncthreads();
+  const Arguments a = arguments();
+  const int w = blockIdx.x;
+  for (int from = -1; from < kDecodeWaves; ++from) {
+    const PartInfo part = info[from < 0 ? 0 : from][from < 0 ? 0 : 1];
+    if (part.state == 0) continue;
+    // Parts: (from, tail) or (0, head), then the heads of waves after .. upto - 1.
+    const int after = from < 0 ? 1 : from + 1;
+    int upto = after, state = part.state;
+    while (state == 1 && upto < kDecodeWaves && info[upto][0].state != 0) state = info[upto++][0].state;
+    const bool whole = from >= 0 && state == 2;
+    float* slot = a->parts + ((int64_t)w * 2 + (from < 0 ? 0 : 1)) * (8 * NB * (DP + 2));
+    const int h0 = 8 * NB * part.block, heads = a->group - h0 < 8 * NB ? a->group - h0 : 8 * NB;
     for (int i = tid; i < heads * (DP / 4); i += 64 * kDecodeWaves) {
       const int h = i / (DP / 4), d = 4 * (i % (DP / 4));
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-      float top = -INFINITY, weight = 0.f;
-#pragma unroll
-      for (int x = 0; x < kDecodeWaves; ++x) {
-        sum += *reinterpret_cast<const f32x4*>(&lds[x][0] + (h * DP + d) * 4);
-        top = fmaxf(top, stats[x][h][0]);
+      const float* x = from < 0 ? heads_lds[0] : reinterpret_cast<const float*>(&lds[from][0]);
+      const float* x_stats = stats[from < 0 ? 0 : from][from < 0 ? 0 : 1][h];
+      float top = x_stats[0];
+      for (int y = after; y < upto; ++y) top = fmaxf(top, stats[y][0][h][0]);
+      const float f = ratio(x_stats[0], top);
+      float weight = x_stats[1] * f;
+      f32x4 sum = *reinterpret_cast<const f32x4*>(x + h * DP + d) * f;
+      for (int y = after; y < upto; ++y) {
+        const float r = ratio(stats[y][0][h][0], top);
+        weight += stats[y][0][h][1] * r;
+        sum += *reinterpret_cast<const f32x4*>(heads_lds[y] + h * DP + d) * r;
       }
-#pragma unroll
-      for (int x = 0; x < kDecodeWaves; ++x) weight += stats[x][h][1] * ratio(stats[x][h][0], top);
-      if (starts && ends) {
-        const int head = kv_head * p.group + h0 + h;
+      if (whole) {
+        const int head = part.kv_head * a->group + h0 + h;
         const float inv = weight == 0.f ? 0.f : 1.f / weight;
-        if (d < p.head_dim) {
-          const u32x2 o = {T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
-          *reinterpret_cast<u32x2*>(p.out + s * p.so_t + head * p.so_h + d) = o;
-        }
-        if (d == 0 && p.lse != nullptr) p.lse[head * p.lse_h + s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
+        if (d < a->head_dim)
+          *reinterpret_cast<u32x2*>(a->out + part.s * a->so_t + head * a->so_h + d) =
+              u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
+        if (d == 0 && a->lse != nullptr) a->lse[head * a->lse_h + part.s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
       } else {
         *reinterpret_cast<f32x4*>(slot + h * DP + d) = sum;
         if (d == 0) slot[8 * NB * DP + 2 * h] = top, slot[8 * NB * DP + 2 * h + 1] = weight;
       }
     }
-    if (starts && !ends && tid == 0) {
-      p.owned[4 * w] = s, p.owned[4 * w + 1] = item;
-      p.owned[4 * w + 2] = (int32_t)((item_end - 1) / share);
+    if (tid == 0 && from >= 0 && (a->by_item || !whole)) {
+      const int item = part.kv_head * a->blocks + part.block;
+      int32_t* entry = a->owned + 4 * (a->by_item ? part.s * a->kv_heads * a->blocks + item : w);
+      entry[0] = whole ? -1 : part.s, entry[1] = item, entry[2] = w;
+      entry[3] = (int32_t)((part.end - 1) / (kDecodeWaves * share));
     }
-    __syncthreads();
-    at = item_start + last;
   }
 }
 
-// An item split over workgroups w .. last: its parts joined, one workgroup per
-// query head, a lane per four elements, the parts dealt to groups of lanes.
+// The parts of a split item joined: a workgroup per query head, a lane per four
+// elements, the parts dealt to groups of lanes.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int DP, int NB>
-__global__ __launch_bounds__(128) void join_kernel(const DecodeParams p) {
-  constexpr int kLanes = DP / 4, kGroups = 128 / kLanes, kSlot = 8 * NB * (DP + 2);
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const DecodeParams p) {
+  constexpr int kLanes = DP / 4, kGroups = kJoinThreads / kLanes, kSlot = 8 * NB * (DP + 2);
   __shared__ f32x4 sums[kGroups][kLanes];
-  __shared__ float stats[kGroups][2];
-  const int w = blockIdx.x, h = blockIdx.y;
-  const int s = p.owned[4 * w];
+  __shared__ float factors[kMaxWorkgroups], wave_stats[2][kJoinThreads / 64];
+  const int32_t* entry = p.owned + 4 * blockIdx.x;
+  const int s = entry[0], h = blockIdx.y, tid = threadIdx.x;
   if (s < 0) return;
-  const int item = p.owned[4 * w + 1], last = p.owned[4 * w + 2];
+  const int item = entry[1], w = entry[2], count = entry[3] - w + 1;
   const int kv_head = item / p.blocks, h0 = (item - kv_head * p.blocks) * 8 * NB;
   if (h0 + h >= p.group) return;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const auto slot = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == w ? 1 : 0)) * kSlot; };
-  float top = -INFINITY, weight = 0.f;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = w + group; i <= last; i += kGroups) top = fmaxf(top, slot(i)[8 * NB * DP + 2 * h]);
-  for (int i = w + group; i <= last; i += kGroups) {
-    const float* part = slot(i);
-    const float f = ratio(part[8 * NB * DP + 2 * h], top);
-    weight += part[8 * NB * DP + 2 * h + 1] * f;
-    sum += *reinterpret_cast<const f32x4*>(part + h * DP + 4 * lane) * f;
+  const float* parts = p.parts + (int64_t)w * 2 * kSlot;
+  const auto part = [&](int i) { return parts + (i == 0 ? kSlot : (int64_t)i * 2 * kSlot); };
+
+  // At most kMaxWorkgroups parts, two per thread.
+  float m[2], l[2], top = -INFINITY, weight = 0.f;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = tid + x * kJoinThreads;
+    m[x] = i < count ? part(i)[8 * NB * DP + 2 * h] : -INFINITY;
+    l[x] = i < count ? part(i)[8 * NB * DP + 2 * h + 1] : 0.f;
+    top = fmaxf(top, m[x]);
   }
+  for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+  if ((tid & 63) == 0) wave_stats[0][tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 64; ++i) top = fmaxf(top, wave_stats[0][i]);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = tid + x * kJoinThreads;
+    const float f = ratio(m[x], top);
+    weight += l[x] * f;
+    if (i < count) factors[i] = f;
+  }
+  for (int i = 1; i < 64; i <<= 1) weight += __shfl_xor(weight, i);
+  if ((tid & 63) == 0) wave_stats[1][tid >> 6] = weight;
+  __syncthreads();
+  weight = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 64; ++i) weight += wave_stats[1][i];
+
+  const int lane = tid % kLanes, group = tid / kLanes;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = group; i < count; i += kGroups)
+    sum += *reinterpret_cast<const f32x4*>(part(i) + h * DP + 4 * lane) * factors[i];
   sums[group][lane] = sum;
-  if (lane == 0) stats[group][0] = top, stats[group][1] = weight;
   __syncthreads();
   if (group != 0) return;
-  for (int i = 1; i < kGroups; ++i) top = fmaxf(top, stats[i][0]);
-  sum = f32x4{0.f, 0.f, 0.f, 0.f}, weight = 0.f;
-  for (int i = 0; i < kGroups; ++i) {
-    const float f = ratio(stats[i][0], top);
-    weight += stats[i][1] * f;
-    sum += sums[i][lane] * f;
-  }
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) sum += sums[i][lane];
   const int head = kv_head * p.group + h0 + h, d = 4 * lane;
   const float inv = weight == 0.f ? 0.f : 1.f / weight;
   if (d < p.head_dim)
@@ -532,7 +670,8 @@ void launch_decode(const DecodeLaunch& l) {
   else
     decode_kernel<T, kInt8, DP, NB, false><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
   const int heads = l.p.group < 8 * NB ? l.p.group : 8 * NB;
-  join_kernel<T, DP, NB><<<dim3(l.workgroups, heads), 128, 0, l.stream>>>(l.p);
+  const int entries = l.p.by_item ? l.p.sequences * l.p.kv_heads * l.p.blocks : l.workgroups;
+  join_kernel<T, DP, NB><<<dim3(entries, heads), kJoinThreads, 0, l.stream>>>(l.p);
 }
 
 template <typename T, int DP>

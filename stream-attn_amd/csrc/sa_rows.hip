@@ -351,11 +351,12 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-bool page_rows(PageRows& r, const void* base, const void* scale, int64_t sp, int64_t st, int64_t sh, int64_t ss_p,
-               int64_t ss_t, int64_t ss_h, bool int8) {
+template <typename Args>
+bool page_rows(PageRows& r, const void* base, const void* scale, const Args* a) {
+  const bool int8 = a->pages_int8;
   r = {static_cast<char*>(const_cast<void*>(base)), int8 ? static_cast<uint16_t*>(const_cast<void*>(scale)) : nullptr,
-       sp, st, sh, ss_p, ss_t, ss_h};
-  return base != nullptr && aligned(base, int8 ? 8 : 16) && sp % 8 == 0 && st % 8 == 0 && sh % 8 == 0 &&
+       a->stride_pp, a->stride_pt, a->stride_ph, a->stride_sp, a->stride_st, a->stride_sh};
+  return base != nullptr && aligned(base, int8 ? 8 : 16) && r.sp % 8 == 0 && r.st % 8 == 0 && r.sh % 8 == 0 &&
          (!int8 || (scale != nullptr && aligned(scale, 2)));
 }
 
@@ -454,10 +455,7 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* s
   if (pages) {
     rc = check_pool(entry, a->num_pages, a->page_tokens);
     if (rc != 0) return rc;
-    if (!page_rows(p.kp, a->k_pages, a->k_scales, a->stride_kpp, a->stride_kpt, a->stride_kph, a->stride_ksp,
-                   a->stride_kst, a->stride_ksh, a->pages_int8) ||
-        !page_rows(p.vp, a->v_pages, a->v_scales, a->stride_vpp, a->stride_vpt, a->stride_vph, a->stride_vsp,
-                   a->stride_vst, a->stride_vsh, a->pages_int8) || !aligned(a->slots, 8))
+    if (!page_rows(p.kp, a->k_pages, a->k_scales, a) || !page_rows(p.vp, a->v_pages, a->v_scales, a) || !aligned(a->slots, 8))
       return invalid(entry, "pages, scales or slots are missing or not aligned");
     p.num_slots = (uint32_t)(a->num_pages * a->page_tokens);
     p.page_tokens = (uint32_t)a->page_tokens;
@@ -498,10 +496,7 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
   if (rc == 0) rc = check_pool(entry, a->num_pages, a->page_tokens);
   if (rc != 0) return rc;
   ReadParams p{};
-  if (!page_rows(p.kp, a->k_pages, a->k_scales, a->stride_kpp, a->stride_kpt, a->stride_kph, a->stride_ksp, a->stride_kst,
-                 a->stride_ksh, a->pages_int8) ||
-      !page_rows(p.vp, a->v_pages, a->v_scales, a->stride_vpp, a->stride_vpt, a->stride_vph, a->stride_vsp, a->stride_vst,
-                 a->stride_vsh, a->pages_int8))
+  if (!page_rows(p.kp, a->k_pages, a->k_scales, a) || !page_rows(p.vp, a->v_pages, a->v_scales, a))
     return invalid(entry, "pages or scales are missing or not aligned");
   if (a->slots == nullptr || !aligned(a->slots, 8) || a->k_out == nullptr || a->v_out == nullptr ||
       !aligned(a->k_out, 16) || !aligned(a->v_out, 16))

@@ -9,15 +9,26 @@ captured graphs, each have their own.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
 
 from .. import _native
-from .rows import _scale_strides, check_pools, check_rows
+from .rows import NO_STRIDES, check_pools, check_rows
 
-# sa_decode_args: 10 pointers, 20 sizes and strides, the scale, 8 int32.
-_DECODE_ARGS = struct.Struct("=10Q20qd8i")
+# sa_decode_args: 10 pointers, 14 sizes and strides, the scale, 8 int32.
+_DECODE_ARGS = struct.Struct("=10Q14qd8i")
+
+
+@functools.lru_cache
+def _workspace_bytes(device_index: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace of a call, which depends on its head counts and head_dim alone."""
+    args = _DECODE_ARGS.pack(*(0,) * 24, 0.0, 1, 0, q_heads, kv_heads, head_dim, 1, 0, 0)
+    needed = ctypes.c_int64()
+    status = _native.lib().sa_paged_decode_workspace_bytes(args, device_index, ctypes.byref(needed))
+    _native.check(status, "sa_paged_decode_workspace_bytes")
+    return needed.value
 
 
 def paged_decode_attention(
@@ -38,7 +49,7 @@ def paged_decode_attention(
     ``q [sequences, q_heads, head_dim]`` attends to keys ``0 .. lengths[s] - 1``
     of its sequence: key ``j`` is row ``j % page_tokens`` of page
     ``page_table[s, j // page_tokens]`` (int32 ``[sequences, max_pages]``;
-    entries past a sequence's last page are not read).  ``lengths`` is int32
+    entries past a sequence's last page may be anything).  ``lengths`` is int32
     ``[sequences]``, on the device like the rest; a length past the table's row
     stands for the row's keys, one below zero for none.  Query head ``h`` reads
     K/V head ``h // (q_heads // kv_heads)``.  Keys of a page outside the pool are
@@ -49,8 +60,8 @@ def paged_decode_attention(
     Returns ``out`` (like ``q``), and with ``return_lse`` also the natural-log
     LSE ``[q_heads, sequences]``.
     """
-    check_rows("q", q)
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
+    code = check_rows("q", q)
+    check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
     sequences, q_heads, dim = q.shape
     num_pages, page_tokens, kv_heads, _ = k_pages.shape
     device = q.device
@@ -75,23 +86,18 @@ def paged_decode_attention(
             raise ValueError("out must have the shape of q")
     lse = torch.empty((q_heads, sequences), dtype=torch.float32, device=device) if return_lse else None
     if sequences:
-        scale = dim**-0.5 if softmax_scale is None else float(softmax_scale)
-
-        def pack(workspace: int, workspace_bytes: int) -> bytes:
-            return _DECODE_ARGS.pack(
-                q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _native.ptr(k_scales) or 0,
-                _native.ptr(v_scales) or 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-                0 if lse is None else lse.data_ptr(), workspace, workspace_bytes, *q.stride()[:2], *out.stride()[:2],
-                *k_pages.stride()[:3], *v_pages.stride()[:3], *_scale_strides(k_scales), *_scale_strides(v_scales),
-                page_table.stride(0), sequences, num_pages, scale, sequences, max_pages, q_heads, kv_heads, dim,
-                page_tokens, _native.dtype_code(q.dtype), int8)
-
-        lib = _native.lib()
-        needed = ctypes.c_int64()
-        _native.check(lib.sa_paged_decode_workspace_bytes(pack(0, 0), device.index, ctypes.byref(needed)), "sa_paged_decode")
-        workspace = torch.empty(needed.value, dtype=torch.uint8, device=device) if needed.value else None
-        status = lib.sa_paged_decode(pack(_native.ptr(workspace) or 0, needed.value), device.index,
-                                     torch.cuda.current_stream(device).cuda_stream)
+        index = device.index
+        needed = _workspace_bytes(index, q_heads, kv_heads, dim)
+        workspace = torch.empty(needed, dtype=torch.uint8, device=device)
+        int8 = k_scales is not None
+        args = _DECODE_ARGS.pack(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0,
+            v_scales.data_ptr() if int8 else 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+            0 if lse is None else lse.data_ptr(), workspace.data_ptr(), needed, *q.stride()[:2], *out.stride()[:2],
+            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0), sequences, num_pages,
+            dim**-0.5 if softmax_scale is None else float(softmax_scale), sequences, max_pages, q_heads, kv_heads, dim,
+            page_tokens, code, int8)
+        status = _native.lib().sa_paged_decode(args, index, _native.current_stream_handle(device))
         if status:
             _native.check(status, "sa_paged_decode")
     return (out, lse) if return_lse else out

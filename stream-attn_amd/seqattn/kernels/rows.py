@@ -8,7 +8,7 @@ page), and ``read_kv`` returns pages as packed rows.  None of them has a
 counterpart in the reference.
 
 Pages are ``[num_pages, page_tokens, kv_heads, head_dim]`` tensors of any page,
-token and head strides, 16-bit or INT8.  INT8 pages hold the storage format of
+token and head strides (K's and V's the same), 16-bit or INT8.  INT8 pages hold the storage format of
 :mod:`seqattn.quantization` with one token per group: ``[num_pages,
 page_tokens, kv_heads]`` float16 scales.  Slot ``page * page_tokens + row``
 names a row of them.  :class:`seqattn.DeviceKVCache` keeps such pages.
@@ -28,39 +28,41 @@ import torch
 from .. import _native
 
 MAX_ROTARY_AXES = 4
-# sa_rows_args: 14 pointers, 26 strides and counts, eps, 16 int32.
-_ROWS_ARGS = struct.Struct("=14Q26qd16i")
-# sa_read_args: 7 pointers, 14 strides and counts, 6 int32.
-_READ_ARGS = struct.Struct("=7Q14q6i")
-_NO_STRIDES = (0, 0, 0)
+# sa_rows_args: 14 pointers, 20 strides and counts, eps, 16 int32.
+_ROWS_ARGS = struct.Struct("=14Q20qd16i")
+# sa_read_args: 7 pointers, 8 strides and counts, 6 int32.
+_READ_ARGS = struct.Struct("=7Q8q6i")
+NO_STRIDES = (0, 0, 0)
 
 
-def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, *, output: bool = False) -> None:
-    """[tokens, heads, head_dim] rows that the kernels can address."""
+def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, *, output: bool = False) -> int:
+    """[tokens, heads, head_dim] rows that the kernels can address; their dtype code (0 where ``like`` has it)."""
     if rows.ndim != 3:
         raise ValueError(f"{name} must use packed [tokens, heads, head_dim] layout")
-    if rows.device.type != "cuda":
+    if not rows.is_cuda:
         raise ValueError("kernel operands must be device tensors")
     st, sh, sd = rows.stride()
     if sd != 1:
         raise ValueError("kernel operands must have a unit stride in the last dimension")
     if st % 8 or sh % 8 or rows.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned, with token and head strides in multiples of 8 elements")
+    code = 0
+    tokens, heads, dim = rows.shape
     if like is None:
-        _native.dtype_code(rows.dtype)
-        if rows.shape[2] % 8 or not 16 <= rows.shape[2] <= 256:
-            raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {rows.shape[2]}")
-        if rows.shape[1] < 1:
+        code = _native.dtype_code(rows.dtype)
+        if dim % 8 or not 16 <= dim <= 256:
+            raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {dim}")
+        if heads < 1:
             raise ValueError(f"{name} has no heads")
     elif rows.device != like.device or rows.dtype != like.dtype:
         raise ValueError(f"{name} must have the device and dtype of the other rows")
     if output:
-        tokens, heads, dim = rows.shape
         if (tokens > 1 and st < dim) or (heads > 1 and sh < dim) or (
                 tokens > 1 and heads > 1 and st < heads * sh and sh < tokens * st):
             raise ValueError(f"{name} has rows that overlap")
     elif rows.requires_grad and torch.is_grad_enabled():
         raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+    return code
 
 
 def check_pages(name: str, pages: torch.Tensor, scales: torch.Tensor | None, like: torch.Tensor) -> None:
@@ -75,7 +77,8 @@ def check_pages(name: str, pages: torch.Tensor, scales: torch.Tensor | None, lik
         raise ValueError(f"{name} must live on the device of the rows")
     if not pages.numel():
         raise ValueError(f"{name} has no pages")
-    if pages.shape[0] * pages.shape[1] > 2**31 - 1:
+    shape = pages.shape
+    if shape[0] * shape[1] > 2**31 - 1:
         raise ValueError(f"{name} has 2^31 rows or more")
     if not int8:
         if scales is not None:
@@ -91,9 +94,11 @@ def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype:
     """Both pools of a cache; whether they hold INT8."""
     check_pages("k_pages", k_pages, k_scales, like)
     check_pages("v_pages", v_pages, v_scales, like)
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        raise ValueError("k_pages and v_pages must have the same shape and dtype")
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+        raise ValueError("k_pages and v_pages must have the same shape and dtype, and the same strides")
     if k_pages.dtype == torch.int8:
+        if k_scales.stride() != v_scales.stride():
+            raise ValueError("k_scales and v_scales must have the same strides")
         return True
     if k_pages.dtype != dtype:
         raise ValueError(f"pages of {k_pages.dtype} do not match rows of {dtype}")
@@ -105,10 +110,6 @@ def _check_slots(slots: torch.Tensor, tokens: int, device: torch.device) -> None
         raise ValueError("slots must be a one-dimensional int64 tensor on the rows' device")
     if slots.shape[0] != tokens or (tokens > 1 and slots.stride(0) != 1):
         raise ValueError("slots must hold one slot per token, contiguously")
-
-
-def _scale_strides(scales: torch.Tensor | None) -> tuple[int, ...]:
-    return _NO_STRIDES if scales is None else scales.stride()
 
 
 def _weight(name: str, weight: torch.Tensor | None, rows: torch.Tensor) -> int:
@@ -160,7 +161,7 @@ def _rotation(positions, frequencies, sections, pairing, rows: torch.Tensor):
             (*sections, *(0,) * (MAX_ROTARY_AXES - axes)), positions.dtype == torch.int64)
 
 
-def _run_rows(q, k, v, q_out, k_out, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps):
+def _run_rows(q, k, v, q_out, k_out, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code):
     """Launch sa_normalize_rotate_store on checked rows; ``pools`` = (k_pages, v_pages, k_scales, v_scales, int8) or None."""
     tokens, kv_heads, dim = k.shape
     where, freq, axis_stride, token_stride, pairs, axes, counts, wide = _rotation(positions, frequencies, sections, pairing, k)
@@ -171,34 +172,39 @@ def _run_rows(q, k, v, q_out, k_out, pools, slots, positions, frequencies, secti
     if tokens == 0:
         return
     if pools is None:
-        pages, page_strides, scale_strides, num_pages, page_tokens, int8 = (0, 0, 0, 0), _NO_STRIDES * 2, _NO_STRIDES * 2, 0, 0, 0
+        pages, strides, num_pages, page_tokens, int8 = (0, 0, 0, 0), NO_STRIDES * 2, 0, 0, False
     else:
         k_pages, v_pages, k_scales, v_scales, int8 = pools
-        pages = (k_pages.data_ptr(), v_pages.data_ptr(), _native.ptr(k_scales) or 0, _native.ptr(v_scales) or 0)
-        page_strides = (*k_pages.stride()[:3], *v_pages.stride()[:3])
-        scale_strides = (*_scale_strides(k_scales), *_scale_strides(v_scales))
         num_pages, page_tokens = k_pages.shape[:2]
+        if int8:
+            pages = k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr()
+            strides = *k_pages.stride()[:3], *k_scales.stride()
+        else:
+            pages = k_pages.data_ptr(), v_pages.data_ptr(), 0, 0
+            strides = *k_pages.stride()[:3], *NO_STRIDES
+    none = 0, 0
     args = _ROWS_ARGS.pack(
         0 if q is None else q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
         0 if q_out is None else q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
         *pages, 0 if slots is None else slots.data_ptr(), where, freq, *weights,
-        *((0, 0) if q is None else q.stride()[:2]), *k.stride()[:2], *((0, 0) if v is None else v.stride()[:2]),
-        *((0, 0) if q_out is None else q_out.stride()[:2]), *((0, 0) if k_out is None else k_out.stride()[:2]),
-        *page_strides, *scale_strides, axis_stride, token_stride, tokens, num_pages, eps,
+        *(none if q is None else q.stride()[:2]), *k.stride()[:2], *(none if v is None else v.stride()[:2]),
+        *(none if q_out is None else q_out.stride()[:2]), *(none if k_out is None else k_out.stride()[:2]),
+        *strides, axis_stride, token_stride, tokens, num_pages, eps,
         0 if q is None else q.shape[1], kv_heads, dim, page_tokens, pairs, pairing == "adjacent", axes, *counts, wide,
         q_weight is not None and q_weight.dtype == torch.float32,
-        k_weight is not None and k_weight.dtype == torch.float32, _native.dtype_code(k.dtype), int8)
+        k_weight is not None and k_weight.dtype == torch.float32, code, int8)
     device = k.device
-    status = _native.lib().sa_normalize_rotate_store(args, device.index, torch.cuda.current_stream(device).cuda_stream)
+    status = _native.lib().sa_normalize_rotate_store(args, device.index, _native.current_stream_handle(device))
     if status:
         _native.check(status, "sa_normalize_rotate_store")
 
 
-def _check_qk(q: torch.Tensor, k: torch.Tensor) -> None:
-    check_rows("q", q)
+def _check_qk(q: torch.Tensor, k: torch.Tensor) -> int:
+    code = check_rows("q", q)
     check_rows("k", k, q)
     if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("q and k must have the same tokens and head_dim")
+    return code
 
 
 def _output(name: str, out: torch.Tensor | None, rows: torch.Tensor) -> torch.Tensor:
@@ -239,11 +245,11 @@ def normalize_rotate_qk(
     Returns ``(q_out, k_out)``, new tensors unless given.  An output may be
     its input itself, but must not otherwise share memory with an input.
     """
-    _check_qk(q, k)
+    code = _check_qk(q, k)
     if positions is None and frequencies is None and q_weight is None and k_weight is None:
         raise ValueError("normalize_rotate_qk needs a weight or a rotation")
     q_out, k_out = _output("q_out", q_out, q), _output("k_out", k_out, k)
-    _run_rows(q, k, None, q_out, k_out, None, None, positions, frequencies, sections, pairing, q_weight, k_weight, eps)
+    _run_rows(q, k, None, q_out, k_out, None, None, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out, k_out
 
 
@@ -274,9 +280,9 @@ def append_kv(
     The slots of a call are distinct: of two rows with one slot either may
     stay, in parts.  INT8 pages: a row that is not finite reads back as NaN.
     """
-    check_rows("k", k)
+    code = check_rows("k", k)
     pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
-    _run_rows(None, k, v, None, None, pools, slots, None, None, None, "adjacent", None, None, 0.0)
+    _run_rows(None, k, v, None, None, pools, slots, None, None, None, "adjacent", None, None, 0.0, code)
 
 
 def normalize_rotate_append(
@@ -304,10 +310,10 @@ def normalize_rotate_append(
     rounded to 16 bits.  Q is written for every token, also where a row's slot
     is negative.
     """
-    _check_qk(q, k)
+    code = _check_qk(q, k)
     pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
     q_out = _output("q_out", q_out, q)
-    _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps)
+    _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out
 
 
@@ -342,12 +348,14 @@ def read_kv(
     if tokens == 0:
         return k_out, v_out
     args = _READ_ARGS.pack(
-        k_pages.data_ptr(), v_pages.data_ptr(), _native.ptr(k_scales) or 0, _native.ptr(v_scales) or 0,
-        slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-        *k_pages.stride()[:3], *v_pages.stride()[:3], *_scale_strides(k_scales), *_scale_strides(v_scales),
+        k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0, v_scales.data_ptr() if int8 else 0,
+        slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *k_pages.stride()[:3],
+        *(k_scales.stride() if int8 else NO_STRIDES),
         tokens, num_pages, heads, dim, page_tokens, code, int8, 0)
     device = k_pages.device
-    _native.check(_native.lib().sa_read_kv(args, device.index, torch.cuda.current_stream(device).cuda_stream), "sa_read_kv")
+    status = _native.lib().sa_read_kv(args, device.index, _native.current_stream_handle(device))
+    if status:
+        _native.check(status, "sa_read_kv")
     return k_out, v_out
 
 

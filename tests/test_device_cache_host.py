@@ -63,7 +63,7 @@ def test_host_tensors_are_refused():
 
 ROWS_FIELDS = (
     "q k v q_out k_out k_pages v_pages k_scales v_scales slots positions frequencies q_weight k_weight "
-    "qt qh kt kh vt vh qot qoh kot koh kpp kpt kph vpp vpt vph ksp kst ksh vsp vst vsh pos_axis pos_token "
+    "qt qh kt kh vt vh qot qoh kot koh pp pt ph sp st sh pos_axis pos_token "
     "tokens num_pages eps q_heads kv_heads head_dim page_tokens pairs adjacent axes s0 s1 s2 s3 pos64 qw32 kw32 "
     "dtype int8").split()
 
@@ -90,7 +90,7 @@ def test_rows_entry_point_rejects_bad_arguments_without_a_gpu():
         (dict(turned, s0=31), -1, b"add up"), (dict(turned, s0=33), -1, b"add up"), (dict(turned, axes=2), -1, b"add up"),
         (dict(turned, frequencies=4), -1, b"positions"),
         (dict(paged, page_tokens=0), -1, b"2^31"), (dict(paged, num_pages=2**30), -1, b"2^31"),
-        (dict(paged, int8=1), -1, b"scales"), (dict(paged, kpp=4), -1, b"aligned"), (dict(paged, slots=4), -1, b"aligned"),
+        (dict(paged, int8=1), -1, b"scales"), (dict(paged, pp=4), -1, b"aligned"), (dict(paged, slots=4), -1, b"aligned"),
     ):
         assert lib.sa_normalize_rotate_store(rows_args(**fields), 0, None) == status, fields
         assert word in lib.sa_last_error(), (fields, lib.sa_last_error())
@@ -101,7 +101,7 @@ def test_rows_entry_point_rejects_bad_arguments_without_a_gpu():
 @built
 def test_read_entry_point_rejects_bad_arguments_without_a_gpu():
     lib = _native.lib()
-    names = "k v ks vs slots ko vo kpp kpt kph vpp vpt vph ksp kst ksh vsp vst vsh tokens pages heads dim page dtype int8 _".split()
+    names = "k v ks vs slots ko vo pp pt ph sp st sh tokens pages heads dim page dtype int8 _".split()
 
     def call(**fields):
         values = dict.fromkeys(names, 0)
@@ -110,7 +110,7 @@ def test_read_entry_point_rejects_bad_arguments_without_a_gpu():
         return lib.sa_read_kv(_READ_ARGS.pack(*(values[n] for n in names)), 0, None)
 
     assert call(dtype=3) == -2 and call(dim=20) == -3
-    for fields in (dict(k=0), dict(v=8), dict(slots=0), dict(ko=0), dict(vo=8), dict(kpt=4), dict(int8=1), dict(page=0),
+    for fields in (dict(k=0), dict(v=8), dict(slots=0), dict(ko=0), dict(vo=8), dict(pt=4), dict(int8=1), dict(page=0),
                    dict(pages=2**30), dict(tokens=2**31), dict(heads=0)):
         assert call(**fields) == -1, fields
         assert b"sa_read_kv" in lib.sa_last_error()
@@ -120,9 +120,8 @@ def test_read_entry_point_rejects_bad_arguments_without_a_gpu():
 @built
 def test_decode_entry_point_rejects_bad_arguments_without_a_gpu():
     lib = _native.lib()
-    names = ("q k v ks vs table lengths out lse workspace workspace_bytes qt qh ot oh kpp kpt kph vpp vpt vph ksp kst ksh "
-             "vsp vst vsh table_stride lse_stride num_pages scale sequences max_pages q_heads kv_heads dim page dtype "
-             "int8").split()
+    names = ("q k v ks vs table lengths out lse workspace workspace_bytes qt qh ot oh pp pt ph sp st sh "
+             "table_stride lse_stride num_pages scale sequences max_pages q_heads kv_heads dim page dtype int8").split()
 
     def args(**fields):
         values = dict.fromkeys(names, 0)
@@ -134,7 +133,7 @@ def test_decode_entry_point_rejects_bad_arguments_without_a_gpu():
     for fields, status in ((dict(dtype=2), -2), (dict(dim=12), -3), (dict(dim=264), -3), (dict(q_heads=3), -1),
                            (dict(kv_heads=0), -1), (dict(sequences=-1), -1), (dict(page=0), -1), (dict(num_pages=2**30), -1),
                            (dict(max_pages=2**30), -1), (dict(q=0), -1), (dict(out=8), -1), (dict(qt=4), -1),
-                           (dict(kpt=4), -1), (dict(int8=1), -1), (dict(table=0), -1), (dict(lengths=2), -1)):
+                           (dict(pt=4), -1), (dict(int8=1), -1), (dict(table=0), -1), (dict(lengths=2), -1)):
         assert lib.sa_paged_decode(args(**fields), 0, None) == status, fields
         assert b"sa_paged_decode" in lib.sa_last_error()
     assert lib.sa_paged_decode(args(sequences=0), 0, None) == 0
