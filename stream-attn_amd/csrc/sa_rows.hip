@@ -11,6 +11,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -36,7 +37,7 @@ struct RowsParams {
   const double* frequencies;
   const void *q_weight, *k_weight;
   int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, sqo_t, sqo_h, sko_t, sko_h;
-  int64_t pos_axis, pos_token, token0;
+  int64_t pos_axis, pos_token, token0, tokens;
   float eps, inv_dim;
   uint32_t num_slots, page_tokens;
   int32_t q_heads, kv_heads, head_dim, pairs, axes;
@@ -103,23 +104,59 @@ __device__ inline void store_words(void* p, const Words<N>& r) {
     *static_cast<uint32_t*>(p) = r.w[0];
 }
 
-// The W pairs of a unit as floats.
-template <typename T, Form F, int W>
-__device__ inline void load_pairs(const uint16_t* row, const Unit<F, W>& u, float (&a)[W], float (&b)[W]) {
+// The 2 W elements of a unit as they lie in memory.
+template <Form F, int W>
+struct Raw {
+  uint32_t w[W];  // kScalar: element pairs (lo, hi), halves and adjacent: the runs
+};
+
+template <Form F, int W>
+__device__ inline __attribute__((always_inline)) Raw<F, W> load_raw(const uint16_t* row, const Unit<F, W>& u) {
+  Raw<F, W> r;
   if constexpr (F == kScalar) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) a[i] = T::lo(row[u.at_lo(i)]), b[i] = T::lo(row[u.at_hi(i)]);
+    for (int i = 0; i < W; ++i) r.w[i] = row[u.at_lo(i)] | (uint32_t)row[u.at_hi(i)] << 16;
   } else if constexpr (F == kAdjacent) {
     const Words<W> x = load_words<W>(row + u.lo);
 #pragma unroll
-    for (int i = 0; i < W; ++i) a[i] = T::lo(x.w[i]), b[i] = T::hi(x.w[i]);
+    for (int i = 0; i < W; ++i) r.w[i] = x.w[i];
   } else {
     const Words<W / 2> x = load_words<W / 2>(row + u.lo), y = load_words<W / 2>(row + u.hi);
 #pragma unroll
+    for (int i = 0; i < W / 2; ++i) r.w[i] = x.w[i], r.w[W / 2 + i] = y.w[i];
+  }
+  return r;
+}
+
+// Its W pairs as floats.
+template <typename T, Form F, int W>
+__device__ inline __attribute__((always_inline)) void pairs_of(const Raw<F, W>& r, float (&a)[W], float (&b)[W]) {
+  if constexpr (F == kHalves) {
+#pragma unroll
     for (int i = 0; i < W / 2; ++i) {
-      a[2 * i] = T::lo(x.w[i]), a[2 * i + 1] = T::hi(x.w[i]);
-      b[2 * i] = T::lo(y.w[i]), b[2 * i + 1] = T::hi(y.w[i]);
+      a[2 * i] = T::lo(r.w[i]), a[2 * i + 1] = T::hi(r.w[i]);
+      b[2 * i] = T::lo(r.w[W / 2 + i]), b[2 * i + 1] = T::hi(r.w[W / 2 + i]);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = T::lo(r.w[i]), b[i] = T::hi(r.w[i]);
+  }
+}
+
+template <typename T, Form F, int W>
+__device__ inline __attribute__((always_inline)) void load_weight(const void* weight, bool fp32, const Unit<F, W>& u, float (&a)[W], float (&b)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) a[i] = b[i] = 1.f;
+  if (weight == nullptr) return;
+  if (fp32) {
+    const float* w = static_cast<const float*>(weight);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a[i] = w[F == kAdjacent ? u.lo + 2 * i : F == kHalves ? u.lo + i : u.at_lo(i)];
+      b[i] = w[F == kAdjacent ? u.lo + 2 * i + 1 : F == kHalves ? u.hi + i : u.at_hi(i)];
+    }
+  } else {
+    pairs_of<T, F, W>(load_raw<F, W>(static_cast<const uint16_t*>(weight), u), a, b);
   }
 }
 
@@ -176,53 +213,83 @@ __device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (
   }
 }
 
-// A sum or maximum over the 2^n lanes of a head.
-__device__ inline float sum_lanes(float x, int lane_log2) {
-  for (int i = 0; i < lane_log2; ++i) x += __shfl_xor(x, 1 << i);
-  return x;
+// A sum or maximum over the 2^n lanes of a head: exchanges within 4 lanes, then
+// mirrored halves of 8 and 16 (whose quarters hold one value by then).
+template <int kControl>
+__device__ inline float exchanged(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xf, 0xf, true));
 }
-__device__ inline float max_lanes(float x, int lane_log2) {
-  for (int i = 0; i < lane_log2; ++i) x = fmaxf(x, __shfl_xor(x, 1 << i));
+template <typename Join>
+__device__ inline float over_lanes(float x, int lane_log2, Join join) {
+  if (lane_log2 > 0) x = join(x, exchanged<0xb1>(x));
+  if (lane_log2 > 1) x = join(x, exchanged<0x4e>(x));
+  if (lane_log2 > 2) x = join(x, exchanged<0x141>(x));
+  if (lane_log2 > 3) x = join(x, exchanged<0x140>(x));
+  if (lane_log2 > 4) x = join(x, __shfl_xor(x, 16));
+  if (lane_log2 > 5) x = join(x, __shfl_xor(x, 32));
   return x;
 }
 
-// One workgroup per token; its waves take the token's rows (Q's heads, then
-// K's, then V's) in turn, 64 >> lane_log2 rows at a time, so that the angles
-// are computed once per wave.
+// Without a branch or a memory operand, which a conditional expression over
+// arrays can become.
+__device__ inline float choose(uint32_t mask, float x, float y) {
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & mask) | (__builtin_bit_cast(uint32_t, y) & ~mask));
+}
+__device__ inline int64_t choose(uint32_t mask, int64_t x, int64_t y) {
+  const int64_t m = (int64_t)(int32_t)mask;
+  return (x & m) | (y & ~m);
+}
+
+// rint(x / step), with the quotient rounded as a division rounds it: only next to
+// a half do the quotient and the product with the reciprocal (off by less than
+// 127 * 2^-22) round apart.
+template <int N>
+__device__ inline void codes(float (&x)[N], float step, float reciprocal) {
+  float q[N];
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = x[i] * reciprocal;
+    q[i] = rintf(y);
+    near = near || fabsf(y - q[i]) > 0.5f - 1.f / 16384;
+  }
+  if (__any(near)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = rintf(x[i] / step);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = fminf(fmaxf(q[i], -127.f), 127.f);
+}
+
+// A wave takes rows of one token (Q's heads, then K's, then V's), 64 >>
+// lane_log2 at a time, and loads the next ones before it works on these.  The
+// angles and weights are its own once per token, so with many tokens a wave
+// has all rows of one; with few, the rows are dealt to gridDim.y waves, which
+// is less time on the way through one.
 template <typename T, Form F, int W, bool kInt8>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
-  const int64_t token = p.token0 + blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t token = p.token0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (token >= p.tokens) return;
+  const int lane = threadIdx.x & 63;
   const int unit_lane = lane & ((1 << p.lane_log2) - 1);
   const int per_step = 64 >> p.lane_log2;
   const bool live = unit_lane * 2 * W < p.head_dim;  // head_dim / 2W lanes of the 2^n hold a unit
   const Unit<F, W> u(live ? unit_lane : 0, p.pairs, p.head_dim);
-
-  float cos_t[W], sin_t[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) cos_t[i] = 1.f, sin_t[i] = 0.f;
-  if (p.pairs > 0) {
-    double pos[SA_MAX_ROTARY_AXES];
-#pragma unroll
-    for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x) {
-      const int64_t at = (x < p.axes ? x : 0) * p.pos_axis + token * p.pos_token;
-      pos[x] = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[at]
-                       : (double)static_cast<const int32_t*>(p.positions)[at];
-    }
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const int pair = u.first + i;
-      if (pair < p.pairs) {
-        // Turns in FP64 (far positions have their fraction there), its
-        // fraction in FP32: the sine instruction takes turns.
-        const double at = pair < p.end0 ? pos[0] : pair < p.end1 ? pos[1] : pair < p.end2 ? pos[2] : pos[3];
-        const double turns = at * (p.frequencies[pair] * 0.15915494309189533577);
-        const float fraction = (float)(turns - rint(turns));
-        cos_t[i] = __builtin_amdgcn_cosf(fraction);
-        sin_t[i] = __builtin_amdgcn_sinf(fraction);
-      }
-    }
-  }
+  // Where the token's Q, K and V start, and their heads' strides.
+  const int64_t in_q = (int64_t)(p.q + token * p.sq_t), in_k = (int64_t)(p.k + token * p.sk_t), in_v = (int64_t)(p.v + token * p.sv_t);
+  const int64_t sq_h = p.sq_h, sk_h = p.sk_h, sv_h = p.sv_h;
+  const int v_row = p.q_heads + p.kv_heads;
+  // Every lane loads something: what no row or unit needs is a repetition.
+  const auto load = [&](int first) {
+    const int row = min(first + (lane >> p.lane_log2), p.heads - 1);
+    const uint32_t is_q = row < p.q_heads ? ~0u : 0u, is_v = row >= v_row ? ~0u : 0u;
+    const int head = row - (~is_q & p.q_heads) - (is_v & p.kv_heads);
+    const int64_t base = choose(is_q, in_q, choose(is_v, in_v, in_k)), stride = choose(is_q, sq_h, choose(is_v, sv_h, sk_h));
+    return load_raw<F, W>(reinterpret_cast<const uint16_t*>(base) + head * stride, u);
+  };
+  const int stride = gridDim.y * per_step;
+  int first = blockIdx.y * per_step;
+  Raw<F, W> raw = load(first);
 
   bool stored = false;
   uint32_t page = 0, row_in_page = 0;
@@ -231,41 +298,73 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     stored = slot >= 0 && slot < (int64_t)p.num_slots;
     if (stored) page = (uint32_t)slot / p.page_tokens, row_in_page = (uint32_t)slot - page * p.page_tokens;
   }
+  const int64_t at = page * p.kp.sp + row_in_page * p.kp.st;
+  const int64_t k_base = (int64_t)p.kp.base, v_base = (int64_t)p.vp.base;
+  const int64_t k_scales = (int64_t)p.kp.scale, v_scales = (int64_t)p.vp.scale;
+  const int64_t scale_at = page * p.kp.ss_p + row_in_page * p.kp.ss_t;
 
-  for (int first = wave * per_step; first < p.heads; first += 4 * per_step) {
-    const int row = first + (lane >> p.lane_log2);
-    const bool is_q = row < p.q_heads, is_v = row >= p.q_heads + p.kv_heads;
-    const int head = is_q ? row : is_v ? row - p.q_heads - p.kv_heads : row - p.q_heads;
-    const bool active = live && row < p.heads;
-    const uint16_t* in = is_q   ? p.q + token * p.sq_t + head * p.sq_h
-                         : is_v ? p.v + token * p.sv_t + head * p.sv_h
-                                : p.k + token * p.sk_t + head * p.sk_h;
-    float a[W], b[W];
+  float cos_t[W], sin_t[W], wqa[W], wqb[W], wka[W], wkb[W];
+  const bool normalizes = p.q_weight != nullptr || p.k_weight != nullptr;
+  if (normalizes) {
+    load_weight<T, F, W>(p.q_weight, p.qw32, u, wqa, wqb);
+    load_weight<T, F, W>(p.k_weight, p.kw32, u, wka, wkb);
+  }
+  if (p.pairs > 0) {
+    // Loads without branches around each, so that they are under way together.
+    int64_t pos[SA_MAX_ROTARY_AXES];
+    double frequency[W];
+    const int64_t axis = p.pos_axis, where = token * p.pos_token;
+    if (p.pos64) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) a[i] = b[i] = 0.f;
-    if (active) load_pairs<T, F, W>(in, u, a, b);
-    const void* weight = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
-    float squares = 0.f;
+      for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x)
+        pos[x] = static_cast<const int64_t*>(p.positions)[where + (x < p.axes ? x : 0) * axis];
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) squares += a[i] * a[i] + b[i] * b[i];
-    squares = sum_lanes(squares, p.lane_log2);
-    if (active && weight != nullptr) {
-      const float r = rsqrtf(squares * p.inv_dim + p.eps);
-      float wa[W], wb[W];
-      if (is_q ? p.qw32 : p.kw32) {
-        const float* w = static_cast<const float*>(weight);
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          wa[i] = w[F == kAdjacent ? u.lo + 2 * i : F == kHalves ? u.lo + i : u.at_lo(i)];
-          wb[i] = w[F == kAdjacent ? u.lo + 2 * i + 1 : F == kHalves ? u.hi + i : u.at_hi(i)];
-        }
-      } else {
-        load_pairs<T, F, W>(static_cast<const uint16_t*>(weight), u, wa, wb);
-      }
-#pragma unroll
-      for (int i = 0; i < W; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
+      for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x)
+        pos[x] = static_cast<const int32_t*>(p.positions)[where + (x < p.axes ? x : 0) * axis];
     }
-    if (!is_v) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) frequency[i] = p.frequencies[u.first + i < p.pairs ? u.first + i : 0];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int pair = u.first + i;
+      // Turns in FP64 (far positions have their fraction there), its fraction
+      // in FP32: the sine instruction takes turns.
+      const double at = (double)(pair < p.end0 ? pos[0] : pair < p.end1 ? pos[1] : pair < p.end2 ? pos[2] : pos[3]);
+      const double turns = pair < p.pairs ? at * (frequency[i] * 0.15915494309189533577) : 0.0;
+      const float fraction = (float)(turns - rint(turns));
+      cos_t[i] = __builtin_amdgcn_cosf(fraction);
+      sin_t[i] = __builtin_amdgcn_sinf(fraction);
+    }
+  }
+
+  const int64_t out_q = (int64_t)(p.q_out + token * p.sqo_t), out_k = (int64_t)(p.k_out + token * p.sko_t);
+  const int64_t sqo_h = p.sqo_h, sko_h = p.sko_h;
+  const bool weight_q = p.q_weight != nullptr, weight_k = p.k_weight != nullptr;
+  while (first < p.heads) {
+    const int row = first + (lane >> p.lane_log2);
+    const bool is_q = row < p.q_heads, is_v = row >= v_row;
+    const uint32_t mask_q = is_q ? ~0u : 0u, mask_v = is_v ? ~0u : 0u;
+    const int head = row - (~mask_q & p.q_heads) - (mask_v & p.kv_heads);
+    const bool active = live && row < p.heads;
+    float a[W], b[W];
+    pairs_of<T, F, W>(raw, a, b);
+    first += stride;
+    if (first < p.heads) raw = load(first);
+    if (normalizes) {
+      float squares = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) squares += a[i] * a[i] + b[i] * b[i];
+      squares = over_lanes(live ? squares : 0.f, p.lane_log2, [](float x, float y) { return x + y; });
+      const bool weighted = is_q ? weight_q : !is_v && weight_k;
+      const float r = weighted ? rsqrtf(squares * p.inv_dim + p.eps) : 1.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        a[i] *= r * choose(mask_q, wqa[i], choose(mask_v, 1.f, wka[i]));
+        b[i] *= r * choose(mask_q, wqb[i], choose(mask_v, 1.f, wkb[i]));
+      }
+    }
+    if (p.pairs > 0 && !is_v) {
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float x = a[i] * cos_t[i] - b[i] * sin_t[i];
@@ -274,12 +373,11 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
       }
     }
     if (is_q || p.slots == nullptr) {
-      uint16_t* out = is_q ? p.q_out + token * p.sqo_t + head * p.sqo_h : p.k_out + token * p.sko_t + head * p.sko_h;
+      uint16_t* out = reinterpret_cast<uint16_t*>(choose(mask_q, out_q, out_k)) + head * choose(mask_q, sqo_h, sko_h);
       if (active) store_pairs<T, F, W>(out, u, a, b);
     }
     if (p.slots == nullptr) continue;
-    const PageRows& pages = is_v ? p.vp : p.kp;
-    const int64_t at = page * pages.sp + row_in_page * pages.st + head * pages.sh;
+    char* pages = reinterpret_cast<char*>(choose(mask_v, v_base, k_base));
     if constexpr (kInt8) {
       float amax = 0.f;
       bool finite = true;
@@ -288,23 +386,18 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
         amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(b[i])));
         finite = finite && fabsf(a[i]) <= FLT_MAX && fabsf(b[i]) <= FLT_MAX;
       }
-      amax = max_lanes(finite ? amax : INFINITY, p.lane_log2);
+      amax = over_lanes(finite ? amax : INFINITY, p.lane_log2, [](float x, float y) { return fmaxf(x, y); });
       if (active && !is_q && stored) {
-        const float step = amax / 127.f;
-        const float div = step > 0.f ? step : 1.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          a[i] = fminf(fmaxf(rintf(a[i] / div), -127.f), 127.f);
-          b[i] = fminf(fmaxf(rintf(b[i] / div), -127.f), 127.f);
-        }
-        store_codes<F, W>(pages.base + at, u, a, b);
-        if (unit_lane == 0) {
-          const float scale = amax <= FLT_MAX ? div : NAN;
-          pages.scale[page * pages.ss_p + row_in_page * pages.ss_t + head * pages.ss_h] = (uint16_t)Fp16::pack(scale, 0.f);
-        }
+        const float step = amax / 127.f > 0.f ? amax / 127.f : 1.f;
+        const float reciprocal = 1.f / step;
+        codes(a, step, reciprocal);
+        codes(b, step, reciprocal);
+        store_codes<F, W>(pages + at + head * p.kp.sh, u, a, b);
+        if (unit_lane == 0)
+          reinterpret_cast<uint16_t*>(choose(mask_v, v_scales, k_scales))[scale_at + head * p.kp.ss_h] = (uint16_t)Fp16::pack(amax <= FLT_MAX ? step : NAN, 0.f);
       }
     } else if (active && !is_q && stored) {
-      store_pairs<T, F, W>(reinterpret_cast<uint16_t*>(pages.base) + at, u, a, b);
+      store_pairs<T, F, W>(reinterpret_cast<uint16_t*>(pages) + at + head * p.kp.sh, u, a, b);
     }
   }
 }
@@ -313,39 +406,59 @@ struct ReadParams {
   PageRows kp, vp;
   const int64_t* slots;
   uint16_t *k_out, *v_out;
-  int64_t token0;
+  int64_t token0, tokens;
   uint32_t num_slots, page_tokens;
   int32_t kv_heads, head_dim;
 };
 
-// One workgroup per token: lane i of it moves granules (8 elements) i, i +
-// 256, ... of the token's K and V rows.
+// Thread i of a workgroup moves granule (8 elements) i, i + 256, ... of K and
+// V rows of kReadTokens tokens, whose loads are under way together.
+constexpr int kReadTokens = 4;
+
 template <typename T, bool kInt8>
 __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
-  const int64_t token = p.token0 + blockIdx.x;
-  const int64_t slot = p.slots[token];
-  const bool held = slot >= 0 && slot < (int64_t)p.num_slots;
-  const uint32_t page = held ? (uint32_t)slot / p.page_tokens : 0;
-  const uint32_t row = held ? (uint32_t)slot - page * p.page_tokens : 0;
+  const int64_t token = p.token0 + (int64_t)blockIdx.x * kReadTokens;
+  int64_t at[kReadTokens], scale_at[kReadTokens];
+  bool held[kReadTokens];
+#pragma unroll
+  for (int t = 0; t < kReadTokens; ++t) {
+    const int64_t slot = token + t < p.tokens ? p.slots[token + t] : -1;
+    held[t] = slot >= 0 && slot < (int64_t)p.num_slots;
+    const uint32_t page = held[t] ? (uint32_t)slot / p.page_tokens : 0;
+    const uint32_t row = held[t] ? (uint32_t)slot - page * p.page_tokens : 0;  // row 0 is there to be read
+    at[t] = page * p.kp.sp + row * p.kp.st;
+    scale_at[t] = page * p.kp.ss_p + row * p.kp.ss_t;
+  }
   const int granules = p.head_dim / 8, each = p.kv_heads * granules;
   for (int i = threadIdx.x; i < 2 * each; i += 256) {
     const bool is_v = i >= each;
     const int g = is_v ? i - each : i, head = g / granules, d = 8 * (g - head * granules);
-    const PageRows& pages = is_v ? p.vp : p.kp;
-    u32x4 w = {0, 0, 0, 0};
-    if (held) {
-      const int64_t at = page * pages.sp + row * pages.st + head * pages.sh + d;
-      if constexpr (kInt8) {
-        const u32x2 c = *reinterpret_cast<const u32x2*>(pages.base + at);
-        const float scale = Fp16::lo(pages.scale[page * pages.ss_p + row * pages.ss_t + head * pages.ss_h]);
+    const char* base = is_v ? p.vp.base : p.kp.base;
+    u32x4 w[kReadTokens];
+    if constexpr (kInt8) {
+      const uint16_t* scales = is_v ? p.vp.scale : p.kp.scale;
+      u32x2 c[kReadTokens];
+      uint16_t scale[kReadTokens];
+#pragma unroll
+      for (int t = 0; t < kReadTokens; ++t) {
+        c[t] = *reinterpret_cast<const u32x2*>(base + at[t] + head * p.kp.sh + d);
+        scale[t] = scales[scale_at[t] + head * p.kp.ss_h];
+      }
+#pragma unroll
+      for (int t = 0; t < kReadTokens; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          w[j] = T::pack(byte_float(c[j / 2], 2 * (j & 1)) * scale, byte_float(c[j / 2], 2 * (j & 1) + 1) * scale);
-      } else {
-        w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(pages.base) + at);
-      }
+          w[t][j] = T::pack(byte_float(c[t][j / 2], 2 * (j & 1)) * Fp16::lo(scale[t]),
+                            byte_float(c[t][j / 2], 2 * (j & 1) + 1) * Fp16::lo(scale[t]));
+    } else {
+#pragma unroll
+      for (int t = 0; t < kReadTokens; ++t)
+        w[t] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(base) + at[t] + head * p.kp.sh + d);
     }
-    *reinterpret_cast<u32x4*>((is_v ? p.v_out : p.k_out) + token * each * 8 + g * 8) = w;
+#pragma unroll
+    for (int t = 0; t < kReadTokens; ++t)
+      if (token + t < p.tokens)
+        *reinterpret_cast<u32x4*>((is_v ? p.v_out : p.k_out) + (token + t) * each * 8 + g * 8) = held[t] ? w[t] : u32x4{0, 0, 0, 0};
   }
 }
 
@@ -386,6 +499,9 @@ int32_t check_pool(const char* entry, int64_t num_pages, int32_t page_tokens) {
 
 // Launches of 2^32 threads and more go in parts.
 constexpr int64_t kTokensPerLaunch = 1 << 23;
+// Waves that fill the chip: a token's rows are dealt to several waves where
+// there are fewer tokens.
+constexpr int64_t kWavesToFill = 16384;
 
 template <typename T, bool kInt8>
 int32_t launch_rows(RowsParams p, int64_t tokens, bool adjacent, hipStream_t stream) {
@@ -397,8 +513,12 @@ int32_t launch_rows(RowsParams p, int64_t tokens, bool adjacent, hipStream_t str
   const int units = p.head_dim / (form == 1 ? 16 : 8);
   p.lane_log2 = 0;
   while ((1 << p.lane_log2) < units) ++p.lane_log2;
+  p.tokens = tokens;
+  const int32_t per_step = 64 >> p.lane_log2, steps = (p.heads + per_step - 1) / per_step;
+  const int64_t waves = std::min<int64_t>(steps, (kWavesToFill + tokens - 1) / tokens);
   for (p.token0 = 0; p.token0 < tokens; p.token0 += kTokensPerLaunch) {
-    const dim3 grid((uint32_t)(tokens - p.token0 < kTokensPerLaunch ? tokens - p.token0 : kTokensPerLaunch));
+    const int64_t count = std::min(tokens - p.token0, kTokensPerLaunch);
+    const dim3 grid((uint32_t)((count + 3) / 4), (uint32_t)waves);
     if (form == 0)
       rows_kernel<T, kAdjacent, 4, kInt8><<<grid, 256, 0, stream>>>(p);
     else if (form == 1)
@@ -503,7 +623,7 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
     return invalid(entry, "slots or outputs are missing or not aligned");
   if (a->tokens == 0) return 0;
   p.k_out = static_cast<uint16_t*>(a->k_out), p.v_out = static_cast<uint16_t*>(a->v_out);
-  p.slots = a->slots;
+  p.slots = a->slots, p.tokens = a->tokens;
   p.num_slots = (uint32_t)(a->num_pages * a->page_tokens), p.page_tokens = (uint32_t)a->page_tokens;
   p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
   DeviceGuard guard(device);
@@ -511,7 +631,7 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
   hipStream_t hs = static_cast<hipStream_t>(stream);
   const bool bf16 = a->dtype == SA_DTYPE_BF16;
   for (p.token0 = 0; p.token0 < a->tokens; p.token0 += kTokensPerLaunch) {
-    const dim3 grid((uint32_t)(a->tokens - p.token0 < kTokensPerLaunch ? a->tokens - p.token0 : kTokensPerLaunch));
+    const dim3 grid((uint32_t)((std::min(a->tokens - p.token0, kTokensPerLaunch) + kReadTokens - 1) / kReadTokens));
     if (a->pages_int8)
       bf16 ? read_kernel<Bf16, true><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, true><<<grid, 256, 0, hs>>>(p);
     else
