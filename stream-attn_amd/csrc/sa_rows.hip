@@ -79,14 +79,16 @@ struct Words {
   uint32_t w[N];
 };
 
-template <int N>  // N dwords, 4 N bytes aligned up to 16
-__device__ inline Words<N> load_words(const void* p) {
+// N dwords, aligned to 4 N bytes up to 16.  With kOnce past the caches (a
+// launch over more than they hold reads and writes everything once).
+template <int N, bool kOnce>
+__device__ inline __attribute__((always_inline)) Words<N> load_words(const void* p) {
   Words<N> r;
   if constexpr (N == 4) {
-    const u32x4 t = *static_cast<const u32x4*>(p);
+    const u32x4 t = kOnce ? __builtin_nontemporal_load(static_cast<const u32x4*>(p)) : *static_cast<const u32x4*>(p);
     for (int i = 0; i < 4; ++i) r.w[i] = t[i];
   } else if constexpr (N == 2) {
-    const u32x2 t = *static_cast<const u32x2*>(p);
+    const u32x2 t = kOnce ? __builtin_nontemporal_load(static_cast<const u32x2*>(p)) : *static_cast<const u32x2*>(p);
     r.w[0] = t[0], r.w[1] = t[1];
   } else {
     r.w[0] = *static_cast<const uint32_t*>(p);
@@ -94,14 +96,23 @@ __device__ inline Words<N> load_words(const void* p) {
   return r;
 }
 
-template <int N>
-__device__ inline void store_words(void* p, const Words<N>& r) {
-  if constexpr (N == 4)
-    *static_cast<u32x4*>(p) = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
-  else if constexpr (N == 2)
-    *static_cast<u32x2*>(p) = u32x2{r.w[0], r.w[1]};
-  else
+template <int N, bool kOnce>
+__device__ inline __attribute__((always_inline)) void store_words(void* p, const Words<N>& r) {
+  if constexpr (N == 4) {
+    const u32x4 t = {r.w[0], r.w[1], r.w[2], r.w[3]};
+    if constexpr (kOnce)
+      __builtin_nontemporal_store(t, static_cast<u32x4*>(p));
+    else
+      *static_cast<u32x4*>(p) = t;
+  } else if constexpr (N == 2) {
+    const u32x2 t = {r.w[0], r.w[1]};
+    if constexpr (kOnce)
+      __builtin_nontemporal_store(t, static_cast<u32x2*>(p));
+    else
+      *static_cast<u32x2*>(p) = t;
+  } else {
     *static_cast<uint32_t*>(p) = r.w[0];
+  }
 }
 
 // The 2 W elements of a unit as they lie in memory.
@@ -110,18 +121,18 @@ struct Raw {
   uint32_t w[W];  // kScalar: element pairs (lo, hi), halves and adjacent: the runs
 };
 
-template <Form F, int W>
+template <Form F, int W, bool kOnce>
 __device__ inline __attribute__((always_inline)) Raw<F, W> load_raw(const uint16_t* row, const Unit<F, W>& u) {
   Raw<F, W> r;
   if constexpr (F == kScalar) {
 #pragma unroll
     for (int i = 0; i < W; ++i) r.w[i] = row[u.at_lo(i)] | (uint32_t)row[u.at_hi(i)] << 16;
   } else if constexpr (F == kAdjacent) {
-    const Words<W> x = load_words<W>(row + u.lo);
+    const Words<W> x = load_words<W, kOnce>(row + u.lo);
 #pragma unroll
     for (int i = 0; i < W; ++i) r.w[i] = x.w[i];
   } else {
-    const Words<W / 2> x = load_words<W / 2>(row + u.lo), y = load_words<W / 2>(row + u.hi);
+    const Words<W / 2> x = load_words<W / 2, kOnce>(row + u.lo), y = load_words<W / 2, kOnce>(row + u.hi);
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) r.w[i] = x.w[i], r.w[W / 2 + i] = y.w[i];
   }
@@ -156,11 +167,11 @@ __device__ inline __attribute__((always_inline)) void load_weight(const void* we
       b[i] = w[F == kAdjacent ? u.lo + 2 * i + 1 : F == kHalves ? u.hi + i : u.at_hi(i)];
     }
   } else {
-    pairs_of<T, F, W>(load_raw<F, W>(static_cast<const uint16_t*>(weight), u), a, b);
+    pairs_of<T, F, W>(load_raw<F, W, false>(static_cast<const uint16_t*>(weight), u), a, b);
   }
 }
 
-template <typename T, Form F, int W>
+template <typename T, Form F, int W, bool kOnce>
 __device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const float (&a)[W], const float (&b)[W]) {
   if constexpr (F == kScalar) {
 #pragma unroll
@@ -172,7 +183,7 @@ __device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const flo
     Words<W> x;
 #pragma unroll
     for (int i = 0; i < W; ++i) x.w[i] = T::pack(a[i], b[i]);
-    store_words<W>(row + u.lo, x);
+    store_words<W, kOnce>(row + u.lo, x);
   } else {
     Words<W / 2> x, y;
 #pragma unroll
@@ -180,8 +191,8 @@ __device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const flo
       x.w[i] = T::pack(a[2 * i], a[2 * i + 1]);
       y.w[i] = T::pack(b[2 * i], b[2 * i + 1]);
     }
-    store_words<W / 2>(row + u.lo, x);
-    store_words<W / 2>(row + u.hi, y);
+    store_words<W / 2, kOnce>(row + u.lo, x);
+    store_words<W / 2, kOnce>(row + u.hi, y);
   }
 }
 
@@ -190,7 +201,7 @@ __device__ inline uint32_t pack_codes(float a, float b, float c, float d) {
          (uint32_t)(int32_t)d << 24;
 }
 
-template <Form F, int W>
+template <Form F, int W, bool kOnce>
 __device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (&a)[W], const float (&b)[W]) {
   if constexpr (F == kScalar) {
 #pragma unroll
@@ -200,7 +211,7 @@ __device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (
     }
   } else if constexpr (F == kAdjacent) {
     static_assert(W == 4, "one 8-byte run");
-    store_words<2>(row + u.lo, Words<2>{{pack_codes(a[0], b[0], a[1], b[1]), pack_codes(a[2], b[2], a[3], b[3])}});
+    store_words<2, kOnce>(row + u.lo, Words<2>{{pack_codes(a[0], b[0], a[1], b[1]), pack_codes(a[2], b[2], a[3], b[3])}});
   } else {
     Words<W / 4> x, y;
 #pragma unroll
@@ -208,8 +219,8 @@ __device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (
       x.w[i] = pack_codes(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
       y.w[i] = pack_codes(b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]);
     }
-    store_words<W / 4>(row + u.lo, x);
-    store_words<W / 4>(row + u.hi, y);
+    store_words<W / 4, kOnce>(row + u.lo, x);
+    store_words<W / 4, kOnce>(row + u.hi, y);
   }
 }
 
@@ -266,7 +277,7 @@ __device__ inline void codes(float (&x)[N], float step, float reciprocal) {
 // angles and weights are its own once per token, so with many tokens a wave
 // has all rows of one; with few, the rows are dealt to gridDim.y waves, which
 // is less time on the way through one.
-template <typename T, Form F, int W, bool kInt8>
+template <typename T, Form F, int W, bool kInt8, bool kOnce>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
   const int64_t token = p.token0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (token >= p.tokens) return;
@@ -285,7 +296,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     const uint32_t is_q = row < p.q_heads ? ~0u : 0u, is_v = row >= v_row ? ~0u : 0u;
     const int head = row - (~is_q & p.q_heads) - (is_v & p.kv_heads);
     const int64_t base = choose(is_q, in_q, choose(is_v, in_v, in_k)), stride = choose(is_q, sq_h, choose(is_v, sv_h, sk_h));
-    return load_raw<F, W>(reinterpret_cast<const uint16_t*>(base) + head * stride, u);
+    return load_raw<F, W, kOnce>(reinterpret_cast<const uint16_t*>(base) + head * stride, u);
   };
   const int stride = gridDim.y * per_step;
   int first = blockIdx.y * per_step;
@@ -374,7 +385,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     }
     if (is_q || p.slots == nullptr) {
       uint16_t* out = reinterpret_cast<uint16_t*>(choose(mask_q, out_q, out_k)) + head * choose(mask_q, sqo_h, sko_h);
-      if (active) store_pairs<T, F, W>(out, u, a, b);
+      if (active) store_pairs<T, F, W, kOnce>(out, u, a, b);
     }
     if (p.slots == nullptr) continue;
     char* pages = reinterpret_cast<char*>(choose(mask_v, v_base, k_base));
@@ -392,12 +403,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
         const float reciprocal = 1.f / step;
         codes(a, step, reciprocal);
         codes(b, step, reciprocal);
-        store_codes<F, W>(pages + at + head * p.kp.sh, u, a, b);
+        store_codes<F, W, kOnce>(pages + at + head * p.kp.sh, u, a, b);
         if (unit_lane == 0)
           reinterpret_cast<uint16_t*>(choose(mask_v, v_scales, k_scales))[scale_at + head * p.kp.ss_h] = (uint16_t)Fp16::pack(amax <= FLT_MAX ? step : NAN, 0.f);
       }
     } else if (active && !is_q && stored) {
-      store_pairs<T, F, W>(reinterpret_cast<uint16_t*>(pages) + at + head * p.kp.sh, u, a, b);
+      store_pairs<T, F, W, kOnce>(reinterpret_cast<uint16_t*>(pages) + at + head * p.kp.sh, u, a, b);
     }
   }
 }
@@ -500,11 +511,17 @@ int32_t check_pool(const char* entry, int64_t num_pages, int32_t page_tokens) {
 // Launches of 2^32 threads and more go in parts.
 constexpr int64_t kTokensPerLaunch = 1 << 23;
 // Waves that fill the chip: a token's rows are dealt to several waves where
-// there are fewer tokens.
-constexpr int64_t kWavesToFill = 16384;
+// there are fewer tokens.  With 40 heads of 128: 4,099 tokens 18.3 us with 4,096,
+// 23 with 16,384; 6,000 tokens 25.4 and 28.6.
+constexpr int64_t kWavesToFill = 4096;
+// Bytes read and written from which a launch passes the caches by, those that
+// the Infinity Cache holds.  61,312 x 112 heads of 128 (3.5 GB) 677 -> 633 us,
+// 20,011 tokens with the append (492 MB) 98 -> 92; 8,190 x 32 heads of 80 (84 MB),
+// read again from the cache, 23 -> 26.
+constexpr int64_t kCacheBytes = 256 << 20;
 
-template <typename T, bool kInt8>
-int32_t launch_rows(RowsParams p, int64_t tokens, bool adjacent, hipStream_t stream) {
+template <typename T, bool kInt8, bool kOnce>
+int32_t launch_rows(RowsParams p, bool adjacent, hipStream_t stream) {
   // Sixteen bytes per access wherever the pairs allow it, then 8, then single
   // elements.
   const int32_t rest = (p.head_dim - 2 * p.pairs) / 2;
@@ -513,23 +530,29 @@ int32_t launch_rows(RowsParams p, int64_t tokens, bool adjacent, hipStream_t str
   const int units = p.head_dim / (form == 1 ? 16 : 8);
   p.lane_log2 = 0;
   while ((1 << p.lane_log2) < units) ++p.lane_log2;
-  p.tokens = tokens;
   const int32_t per_step = 64 >> p.lane_log2, steps = (p.heads + per_step - 1) / per_step;
-  const int64_t waves = std::min<int64_t>(steps, (kWavesToFill + tokens - 1) / tokens);
-  for (p.token0 = 0; p.token0 < tokens; p.token0 += kTokensPerLaunch) {
-    const int64_t count = std::min(tokens - p.token0, kTokensPerLaunch);
+  const int64_t waves = std::min<int64_t>(steps, (kWavesToFill + p.tokens - 1) / p.tokens);
+  for (p.token0 = 0; p.token0 < p.tokens; p.token0 += kTokensPerLaunch) {
+    const int64_t count = std::min(p.tokens - p.token0, kTokensPerLaunch);
     const dim3 grid((uint32_t)((count + 3) / 4), (uint32_t)waves);
     if (form == 0)
-      rows_kernel<T, kAdjacent, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+      rows_kernel<T, kAdjacent, 4, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else if (form == 1)
-      rows_kernel<T, kHalves, 8, kInt8><<<grid, 256, 0, stream>>>(p);
+      rows_kernel<T, kHalves, 8, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else if (form == 2)
-      rows_kernel<T, kHalves, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+      rows_kernel<T, kHalves, 4, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else
-      rows_kernel<T, kScalar, 4, kInt8><<<grid, 256, 0, stream>>>(p);
+      rows_kernel<T, kScalar, 4, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     SA_HIP_RETURN(hipGetLastError());
   }
   return 0;
+}
+
+template <typename T>
+int32_t launch_rows(const RowsParams& p, bool int8, bool adjacent, hipStream_t stream) {
+  const bool once = p.tokens * p.heads * p.head_dim * 4 >= kCacheBytes;
+  if (int8) return once ? launch_rows<T, true, true>(p, adjacent, stream) : launch_rows<T, true, false>(p, adjacent, stream);
+  return once ? launch_rows<T, false, true>(p, adjacent, stream) : launch_rows<T, false, false>(p, adjacent, stream);
 }
 
 }  // namespace
@@ -600,9 +623,9 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* s
   SA_HIP_RETURN(guard.status());
   hipStream_t hs = static_cast<hipStream_t>(stream);
   const bool bf16 = a->dtype == SA_DTYPE_BF16;
-  if (pages && a->pages_int8)
-    return bf16 ? launch_rows<Bf16, true>(p, a->tokens, a->adjacent, hs) : launch_rows<Fp16, true>(p, a->tokens, a->adjacent, hs);
-  return bf16 ? launch_rows<Bf16, false>(p, a->tokens, a->adjacent, hs) : launch_rows<Fp16, false>(p, a->tokens, a->adjacent, hs);
+  p.tokens = a->tokens;
+  const bool int8 = pages && a->pages_int8;
+  return bf16 ? launch_rows<Bf16>(p, int8, a->adjacent, hs) : launch_rows<Fp16>(p, int8, a->adjacent, hs);
 } catch (const std::exception& error) {
   return sa::exception_status("sa_normalize_rotate_store", error);
 }
