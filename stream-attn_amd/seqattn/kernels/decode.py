@@ -15,7 +15,7 @@ import struct
 import torch
 
 from .. import _native
-from .rows import NO_STRIDES, check_pools, check_rows
+from .rows import NO_STRIDES, check_pools, check_rows, new_rows
 
 # sa_decode_args: 10 pointers, 14 sizes and strides, the scale, 8 int32.
 _DECODE_ARGS = struct.Struct("=10Q14qd8i")
@@ -61,7 +61,7 @@ def paged_decode_attention(
     LSE ``[q_heads, sequences]``.
     """
     code = check_rows("q", q)
-    check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
     sequences, q_heads, dim = q.shape
     num_pages, page_tokens, kv_heads, _ = k_pages.shape
     device = q.device
@@ -79,22 +79,23 @@ def paged_decode_attention(
     if max_pages * page_tokens > 2**31 - 1:
         raise ValueError("page_table rows must hold fewer than 2^31 keys")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = new_rows(sequences, q_heads, dim, q.dtype, device)
     else:
         check_rows("out", out, q, output=True)
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
-    lse = torch.empty((q_heads, sequences), dtype=torch.float32, device=device) if return_lse else None
+    lse = None
+    if return_lse:
+        lse = torch.empty_strided((q_heads, sequences), (sequences, 1), dtype=torch.float32, device=device)
     if sequences:
         index = device.index
         needed = _workspace_bytes(index, q_heads, kv_heads, dim)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=device)
-        int8 = k_scales is not None
+        workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=device)
         args = _DECODE_ARGS.pack(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0,
             v_scales.data_ptr() if int8 else 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
             0 if lse is None else lse.data_ptr(), workspace.data_ptr(), needed, *q.stride()[:2], *out.stride()[:2],
-            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0), sequences, num_pages,
+            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0), max(sequences, 1), num_pages,
             dim**-0.5 if softmax_scale is None else float(softmax_scale), sequences, max_pages, q_heads, kv_heads, dim,
             page_tokens, code, int8)
         status = _native.lib().sa_paged_decode(args, index, _native.current_stream_handle(device))

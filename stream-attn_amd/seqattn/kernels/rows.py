@@ -65,44 +65,44 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
     return code
 
 
-def check_pages(name: str, pages: torch.Tensor, scales: torch.Tensor | None, like: torch.Tensor) -> None:
-    """A page pool, and its scales, on ``like``'s device."""
-    if pages.ndim != 4:
-        raise ValueError(f"{name} must use [num_pages, page_tokens, kv_heads, head_dim] layout")
-    sp, st, sh, sd = pages.stride()
-    int8 = pages.dtype == torch.int8
-    if sd != 1 or sp % 8 or st % 8 or sh % 8 or pages.data_ptr() % (8 if int8 else 16):
-        raise ValueError(f"{name} must be aligned, with a unit stride in head_dim and the others in multiples of 8 elements")
-    if pages.device != like.device:
-        raise ValueError(f"{name} must live on the device of the rows")
-    if not pages.numel():
-        raise ValueError(f"{name} has no pages")
-    shape = pages.shape
-    if shape[0] * shape[1] > 2**31 - 1:
-        raise ValueError(f"{name} has 2^31 rows or more")
-    if not int8:
-        if scales is not None:
-            raise ValueError("only INT8 pages have scales")
-        return
-    if scales is None:
-        raise ValueError("INT8 pages need their scales")
-    if scales.dtype != torch.float16 or scales.shape != pages.shape[:3] or scales.device != pages.device:
-        raise ValueError("INT8 scales must be float16 [num_pages, page_tokens, kv_heads] on the pages' device")
-
-
 def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype) -> bool:
-    """Both pools of a cache; whether they hold INT8."""
-    check_pages("k_pages", k_pages, k_scales, like)
-    check_pages("v_pages", v_pages, v_scales, like)
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+    """Both pools of a cache, on ``like``'s device; whether they hold INT8."""
+    shape, strides, stored = k_pages.shape, k_pages.stride(), k_pages.dtype
+    if len(shape) != 4:
+        raise ValueError("k_pages must use [num_pages, page_tokens, kv_heads, head_dim] layout")
+    if strides[3] != 1:
+        raise ValueError("pages must have a unit stride in head_dim")
+    if v_pages.shape != shape or v_pages.dtype != stored or v_pages.stride() != strides:
         raise ValueError("k_pages and v_pages must have the same shape and dtype, and the same strides")
-    if k_pages.dtype == torch.int8:
-        if k_scales.stride() != v_scales.stride():
-            raise ValueError("k_scales and v_scales must have the same strides")
-        return True
-    if k_pages.dtype != dtype:
-        raise ValueError(f"pages of {k_pages.dtype} do not match rows of {dtype}")
-    return False
+    int8 = stored == torch.int8
+    align = 8 if int8 else 16
+    if strides[0] % 8 or strides[1] % 8 or strides[2] % 8 or k_pages.data_ptr() % align or v_pages.data_ptr() % align:
+        raise ValueError("pages must be aligned, with their other strides in multiples of 8 elements")
+    if k_pages.device != like.device or v_pages.device != like.device:
+        raise ValueError("pages must live on the device of the rows")
+    if not k_pages.numel():
+        raise ValueError("the cache has no pages")
+    if shape[0] * shape[1] > 2**31 - 1:
+        raise ValueError("the cache has 2^31 rows or more")
+    if not int8:
+        if k_scales is not None or v_scales is not None:
+            raise ValueError("only INT8 pages have scales")
+        if stored != dtype:
+            raise ValueError(f"pages of {stored} do not match rows of {dtype}")
+        return False
+    if k_scales is None or v_scales is None:
+        raise ValueError("INT8 pages need their scales")
+    for scales in (k_scales, v_scales):
+        if scales.dtype != torch.float16 or scales.shape != shape[:3] or scales.device != like.device:
+            raise ValueError("INT8 scales must be float16 [num_pages, page_tokens, kv_heads] on the pages' device")
+    if k_scales.stride() != v_scales.stride():
+        raise ValueError("k_scales and v_scales must have the same strides")
+    return True
+
+
+def new_rows(tokens: int, heads: int, dim: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """Contiguous [tokens, heads, head_dim] memory (the strided form of torch.empty, which takes less host time)."""
+    return torch.empty_strided((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=device)
 
 
 def _check_slots(slots: torch.Tensor, tokens: int, device: torch.device) -> None:
@@ -209,7 +209,7 @@ def _check_qk(q: torch.Tensor, k: torch.Tensor) -> int:
 
 def _output(name: str, out: torch.Tensor | None, rows: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        return new_rows(*rows.shape, rows.dtype, rows.device)
     check_rows(name, out, rows, output=True)
     if out.shape != rows.shape:
         raise ValueError(f"{name} must have the shape of its input")
@@ -343,8 +343,7 @@ def read_kv(
     _check_slots(slots, tokens, k_pages.device)
     if dim % 8 or not 16 <= dim <= 256:
         raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {dim}")
-    k_out = torch.empty((tokens, heads, dim), dtype=dtype, device=k_pages.device)
-    v_out = torch.empty_like(k_out)
+    k_out, v_out = (new_rows(tokens, heads, dim, dtype, k_pages.device) for _ in range(2))
     if tokens == 0:
         return k_out, v_out
     args = _READ_ARGS.pack(
