@@ -35,16 +35,14 @@ int32_t check(const sa_decode_args* a) {
   return 0;
 }
 
-constexpr int kCUs = 256;
-
 int padded(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-// Workgroups of a launch: what the chip holds at once (four waves each; two to
-// a CU, one with the registers of head sizes past 128 or 16 query heads).  A
-// launch over fewer tiles leaves some without work.
+// Workgroups of a launch: what the chip holds at once.  A launch over fewer
+// tiles leaves some without work.
 bool wide(const sa_decode_args* a) { return a->q_heads / a->kv_heads > 8; }
-int workgroups(const sa_decode_args* a) { return kCUs * (padded(a->head_dim) == 256 || wide(a) ? 1 : 2); }
-static_assert(kMaxWorkgroups == 2 * kCUs, "the join holds a factor per part");
+int workgroups(const sa_decode_args* a) {
+  return kDecodeCUs * decode_occupancy(padded(a->head_dim), wide(a) ? 2 : 1, a->pages_int8 != 0);
+}
 
 // owned, then parts.
 int64_t owned_bytes(const sa_decode_args* a) { return (int64_t)workgroups(a) * 16; }

@@ -88,7 +88,7 @@ __device__ inline Dwords<N> load_dwords(const char* base, uint32_t offset) {
   return r;
 }
 
-__device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline __attribute__((always_inline)) int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // The value on the lane whose column is 8 further, of the same 16.
 __device__ inline float other_half(float x) {
@@ -104,6 +104,11 @@ struct Piece {
   const int32_t* table;
   int32_t s, length, tiles, first, last;
   int32_t kv_head, block;  // query heads 8 NB block .. of the K/V head's group
+
+  __device__ inline void bound(int64_t end) {  // as far as a run up to `end` goes
+    const int64_t left = end - start;
+    last = left < tiles ? (int32_t)left : tiles;
+  }
 };
 
 // The kernel's arguments, read again where they are used: what only a piece's
@@ -122,6 +127,52 @@ __device__ inline int32_t length_of(Arguments a, int s) {
 }
 __device__ inline int32_t tiles_of(int32_t length) { return length > 0 ? (length - 1) / kDecodeTile + 1 : 0; }
 
+// Where a wave's next load is: a tile of a piece, in row `row` of the
+// sequence's page number `page`.
+struct Reader {
+  Piece x;
+  int32_t tile, page, row;
+  int32_t ids, first_id;  // page numbers first_id + lane of the sequence
+
+  __device__ inline int32_t id_of(const DecodeParams& p, int32_t n, int lane) {
+    if (n - first_id >= 64) {
+      first_id = n;
+      ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
+    }
+    return __builtin_amdgcn_readlane(ids, n - first_id);
+  }
+
+  __device__ inline void enter(const DecodeParams& p) {  // at the piece's first tile
+    tile = x.first;
+    page = uniform((int32_t)((uint64_t)(uint32_t)(tile * kDecodeTile) * p.page_magic >> p.page_shift));
+    row = tile * kDecodeTile - page * p.page_tokens;
+    first_id = page - 64;
+  }
+
+  // To the next tile of a run up to tile `end` of the launch, which has one.
+  __device__ inline void advance(const DecodeParams& p, int64_t end) {
+    if (++tile < x.last) {
+      page += p.step_pages, row += p.step_rows;
+      if (row >= p.page_tokens) ++page, row -= p.page_tokens;
+      return;
+    }
+    // The next item: the sequence's next, or the first of the next sequence
+    // that has keys.
+    const Arguments a = arguments();
+    x.start += x.tiles, x.first = 0;
+    if (++x.block == a->blocks) x.block = 0, ++x.kv_head;
+    if (x.kv_head == a->kv_heads) {
+      x.kv_head = 0;
+      do x.length = uniform(length_of(a, ++x.s));
+      while (x.length <= 0);
+      x.tiles = tiles_of(x.length);
+      x.table = a->table + x.s * a->s_table;
+    }
+    x.bound(end);
+    enter(p);
+  }
+};
+
 // A wave's loads of one step, in flight while the step before is computed.
 template <bool kInt8, int DP, bool kAnyPage>
 struct Step {
@@ -132,22 +183,14 @@ struct Step {
   uint32_t scale;  // INT8: lane g's of K (g < 8) or V, key 4 (g % 8) + j
   uint32_t seen;   // bit t: key 4t + j has weight
   bool full;       // all 32 keys have
-  // Page numbers first_id + lane of the sequence, for the steps to come.
-  int32_t ids, first_id;
+  Piece x;       // whose keys they are
+  int32_t tile;  // 32 tile .. of the sequence
 
-  __device__ inline int32_t id_of(const DecodeParams& p, const Piece& x, int32_t n, int lane) {
-    if (n - first_id >= 64) {
-      first_id = n;
-      ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
-    }
-    return __builtin_amdgcn_readlane(ids, n - first_id);
-  }
-
-  // Keys key0 .. key0 + 31 of the piece's sequence; key0 is in row `row` of its
-  // page number `page`.
-  __device__ __attribute__((always_inline)) void load(const DecodeParams& p, const Piece& x, int32_t key0, int32_t page,
-                                                      int32_t row, int lane) {
+  __device__ __attribute__((always_inline)) void load(const DecodeParams& p, Reader& from, int lane) {
+    x = from.x, tile = from.tile;
     const int j = lane >> 4, g = lane & 15;
+    const int32_t key0 = tile * kDecodeTile;
+    int32_t page = from.page, row = from.row;
     const char *kh = p.k + x.kv_head * p.sh * ES, *vh = p.v + x.kv_head * p.sh * ES;
     uint32_t at[NP];
 #pragma unroll
@@ -160,7 +203,7 @@ struct Step {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (h == 1 && (row += 16) >= p.page_tokens) ++page, row -= p.page_tokens;
-        int32_t id = id_of(p, x, page, lane);
+        int32_t id = from.id_of(p, page, lane);
         const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
         if (!ok) id = 0;  // rows of a page that exists, read and not used
         full = full && ok;
@@ -219,7 +262,7 @@ struct PartInfo {
 // it are done there; the others' parts meet in LDS, and those of items that
 // leave the workgroup's run in the workspace.
 template <typename T, bool kInt8, int DP, int NB, bool kAnyPage>
-__global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) void decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8)) void decode_kernel(const DecodeParams p) {
   using S = Shape<DP>;
   using PT = std::conditional_t<kInt8, Bf16, T>;  // INT8: weights times V's scales, beyond float16's range
   constexpr int EL = S::EL, NP = S::NP, NI = S::NI, NC = S::NC;
@@ -293,71 +336,59 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
 
   char* mine = &lds[wave][0];
   float* scales = reinterpret_cast<float*>(mine + kDecodeTile * kRow);
-  Piece cur, next;
-  // The loads run ahead of the products by a step, also from a piece to the
-  // next: `tile` is the one in `step`.
-  Step<kInt8, DP, kAnyPage> step;
-  int32_t tile, page = 0, row = 0;
-  const auto enter = [&](const Piece& x) {
-    tile = x.first;
-    step.first_id = -64;
-    page = uniform((int32_t)((uint64_t)(uint32_t)(tile * kDecodeTile) * p.page_magic >> p.page_shift));
-    row = tile * kDecodeTile - page * p.page_tokens;
-    if constexpr (!kAnyPage) step.first_id = page - 64;
-  };
-  // The rest of a piece whose item starts at x.start, as far as the run goes.
-  const auto bound = [&](Piece& x) {
-    const int64_t left = end - x.start;
-    x.last = left < x.tiles ? (int32_t)left : x.tiles;
-  };
   if (begin < end) {
-    const Arguments a = arguments();
-    cur.s = uniform((int)found[wave][0]);
-    cur.length = uniform(length_of(a, cur.s));
-    cur.tiles = tiles_of(cur.length);
-    const int64_t into = begin - found[wave][1];
-    const int item = uniform((int)(into / cur.tiles));
-    cur.start = found[wave][1] + (int64_t)item * cur.tiles;
-    cur.first = uniform((int32_t)(begin - cur.start));
-    cur.kv_head = item / a->blocks, cur.block = item - cur.kv_head * a->blocks;
-    cur.table = a->table + cur.s * a->s_table;
-    bound(cur);
-    next = cur;
-    enter(cur);
-    step.load(p, cur, tile * kDecodeTile, page, row, lane);
-  }
-  while (begin < end) {
-    // Q^T: chunk c of column g's head, elements 32c + 8j .. + 7.
-    u32x4 q[NB][NC];
+    Reader reader;
+    Step<kInt8, DP, kAnyPage> step;
     {
       const Arguments a = arguments();
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int h = 8 * (NB * cur.block + n) + (g & 7);  // of the group
-        const uint16_t* at = a->q + cur.s * a->sq_t + (cur.kv_head * a->group + (h < a->group ? h : 0)) * a->sq_h;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int d = 32 * c + 8 * j;
-          q[n][c] = h < a->group && d < a->head_dim ? *reinterpret_cast<const u32x4*>(at + d) : u32x4{0, 0, 0, 0};
-        }
-      }
+      Piece& x = reader.x;
+      x.s = uniform((int)found[wave][0]);
+      x.length = uniform(length_of(a, x.s));
+      x.tiles = tiles_of(x.length);
+      const int64_t into = begin - found[wave][1];
+      const int item = uniform((int)(into / x.tiles));
+      x.start = found[wave][1] + (int64_t)item * x.tiles;
+      x.first = uniform((int32_t)(begin - x.start));
+      x.kv_head = item / a->blocks, x.block = item - x.kv_head * a->blocks;
+      x.table = a->table + x.s * a->s_table;
+      x.bound(end);
+      reader.enter(p);
     }
-    // K's elements past head_dim are zeros that no step writes.
-    if (p.head_dim < DP) {
-      for (int i = lane; i < kDecodeTile * kRow / 16; i += 64) reinterpret_cast<u32x4*>(mine)[i] = u32x4{0, 0, 0, 0};
-      wave_lds_order();
-    }
+    step.load(p, reader, lane);
 
+    u32x4 q[NB][NC];
     f32x4 acc[NB][NI];
     float m[NB], l[NB];
+    const auto start_piece = [&](const Piece& cur) __attribute__((always_inline)) {
+      // Q^T: chunk c of column g's head, elements 32c + 8j .. + 7.
+      {
+        const Arguments a = arguments();
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      m[n] = -INFINITY, l[n] = 0.f;
+        for (int n = 0; n < NB; ++n) {
+          const int h = 8 * (NB * cur.block + n) + (g & 7);  // of the group
+          const uint16_t* at = a->q + cur.s * a->sq_t + (cur.kv_head * a->group + (h < a->group ? h : 0)) * a->sq_h;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+          for (int c = 0; c < NC; ++c) {
+            const int d = 32 * c + 8 * j;
+            q[n][c] = h < a->group && d < a->head_dim ? *reinterpret_cast<const u32x4*>(at + d) : u32x4{0, 0, 0, 0};
+          }
+        }
+      }
+      // K's elements past head_dim are zeros that no step writes.
+      if (p.head_dim < DP) {
+        for (int i = lane; i < kDecodeTile * kRow / 16; i += 64) reinterpret_cast<u32x4*>(mine)[i] = u32x4{0, 0, 0, 0};
+        wave_lds_order();
+      }
 
-    for (bool more = true; more;) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    // A tile's products; its step takes the next load.
+    const auto work = [&](bool more) __attribute__((always_inline)) {
       // K to LDS, 16-byte granules of row r exchanged by r so that the reads
       // below meet every bank once.
 #pragma unroll
@@ -382,7 +413,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
             *reinterpret_cast<u32x2*>(mine + r * kRow + 16 * ((g >> 1) ^ turn) + 8 * (g & 1)) = u32x2{x[0], x[1]};
         }
       }
-      if constexpr (kInt8) scales[16 * j + g] = Fp16::lo(step.scale);
+      // K's scales with the softmax's.
+      if constexpr (kInt8) scales[16 * j + g] = Fp16::lo(step.scale) * (g < 8 ? p.scale_log2 : 1.f);
       const bool full = step.full;
       const uint32_t seen = step.seen;
       // Rows without weight may hold anything: 0 * NaN is not 0.
@@ -408,29 +440,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
               vt[EL * c + i][u] = __builtin_amdgcn_perm(step.v[2 * u + 1][c].w[i / 2], step.v[2 * u][c].w[i / 2],
                                                         i & 1 ? 0x07060302u : 0x05040100u);
           }
-      if (++tile < cur.last) {
-        page += p.step_pages, row += p.step_rows;
-        if (row >= p.page_tokens) ++page, row -= p.page_tokens;
-        step.load(p, next, tile * kDecodeTile, page, row, lane);
-      } else {
-        more = false;
-        if (cur.start + cur.last < end) {
-          // The next item: the sequence's next, or the first of the next
-          // sequence that has keys.
-          const Arguments a = arguments();
-          next.start += next.tiles, next.first = 0;
-          if (++next.block == a->blocks) next.block = 0, ++next.kv_head;
-          if (next.kv_head == a->kv_heads) {
-            next.kv_head = 0;
-            do next.length = uniform(length_of(a, ++next.s));
-            while (next.length <= 0);
-            next.tiles = tiles_of(next.length);
-            next.table = a->table + next.s * a->s_table;
-          }
-          bound(next);
-          enter(next);
-          step.load(p, next, tile * kDecodeTile, page, row, lane);
-        }
+      if (more) {
+        reader.advance(p, end);
+        step.load(p, reader, lane);
       }
       wave_lds_order();
 
@@ -447,23 +459,17 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
 #pragma unroll
           for (int n = 0; n < NB; ++n) st[n][b] = T::mma(x, q[n][c], st[n][b]);
         }
-      float ks[8], vs[8];
+      f32x4 factors[2] = {f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2}, factors[0]};
       if constexpr (kInt8) {
-#pragma unroll
-        for (int t = 0; t < 8; t += 4) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(scales + 16 * j + t), y = *reinterpret_cast<const f32x4*>(scales + 16 * j + 8 + t);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ks[t + i] = x[i], vs[t + i] = full || seen >> (t + i) & 1 ? y[i] : 0.f;
-        }
+        factors[0] = *reinterpret_cast<const f32x4*>(scales + 16 * j);
+        factors[1] = *reinterpret_cast<const f32x4*>(scales + 16 * j + 4);
       }
-      wave_lds_order();
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float y[8], top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          y[t] = st[n][t / 4][t & 3] * p.scale_log2;
-          if constexpr (kInt8) y[t] *= ks[t];
+          y[t] = st[n][t / 4][t & 3] * factors[t / 4][t & 3];
         }
         if (!full) {
 #pragma unroll
@@ -480,6 +486,16 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
 #pragma unroll
           for (int i = 0; i < NI; ++i) acc[n][i] *= keep;
         }
+        f32x4 vs[2];
+        if constexpr (kInt8) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            vs[b] = *reinterpret_cast<const f32x4*>(scales + 16 * j + 8 + 4 * b);
+            if (!full)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vs[b][e] = seen >> (4 * b + e) & 1 ? vs[b][e] : 0.f;
+          }
+        }
         const float base = m[n] == -INFINITY ? 0.f : m[n];
         const float low = g >= 8 ? 1.f : 0.f;
         u32x4 weights;
@@ -487,70 +503,77 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP == 256 || NB == 2 ? 1 : 2) vo
         for (int u = 0; u < 4; ++u) {
           float a = __builtin_amdgcn_exp2f(y[2 * u] - base), b = __builtin_amdgcn_exp2f(y[2 * u + 1] - base);
           l[n] += a + b;
-          if constexpr (kInt8) a *= vs[2 * u], b *= vs[2 * u + 1];
+          if constexpr (kInt8) a *= vs[u / 2][2 * (u & 1)], b *= vs[u / 2][2 * (u & 1) + 1];
           const uint32_t high = PT::pack(a, b);
           weights[u] = PT::pack(a - low * PT::lo(high), b - low * PT::hi(high));
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) acc[n][i] = PT::mma(vt[i], weights, acc[n][i]);
       }
-    }
-
-    // The piece's end: high and low parts together, the lanes' sums together.
-    const Arguments a = arguments();
-    const bool starts = cur.first == 0, ends = cur.last == cur.tiles;
+      wave_lds_order();
+    };
+    // A piece's end: high and low parts together, the lanes' sums together.
+    const auto end_piece = [&](const Piece& cur) __attribute__((always_inline)) {
+      const Arguments a = arguments();
+      const bool starts = cur.first == 0, ends = cur.last == cur.tiles;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      l[n] += __shfl_xor(l[n], 16);
-      l[n] += __shfl_xor(l[n], 32);
+      for (int n = 0; n < NB; ++n) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][i][e] += other_half(acc[n][i][e]);
-      const int h = 8 * (NB * cur.block + n) + (g & 7);
-      if (g >= 8 || h >= a->group) continue;
-      if (starts && ends) {
-        const int head = cur.kv_head * a->group + h;
-        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-        uint16_t* out = a->out + cur.s * a->so_t + head * a->so_h;
+          for (int e = 0; e < 4; ++e) acc[n][i][e] += other_half(acc[n][i][e]);
+        const int h = 8 * (NB * cur.block + n) + (g & 7);
+        if (g >= 8 || h >= a->group) continue;
+        if (starts && ends) {
+          const int head = cur.kv_head * a->group + h;
+          const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+          uint16_t* out = a->out + cur.s * a->so_t + head * a->so_h;
 #pragma unroll
-        for (int c = 0; c < NP; ++c)
+          for (int c = 0; c < NP; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 128 * c + EL * (4 * j + e);
-            uint32_t o[EL / 2];
+            for (int e = 0; e < 4; ++e) {
+              const int d = 128 * c + EL * (4 * j + e);
+              uint32_t o[EL / 2];
 #pragma unroll
-            for (int i = 0; i < EL; i += 2) o[i / 2] = T::pack(acc[n][EL * c + i][e] * inv, acc[n][EL * c + i + 1][e] * inv);
-            if (d >= a->head_dim) continue;
-            if constexpr (EL == 8)
-              *reinterpret_cast<u32x4*>(out + d) = u32x4{o[0], o[1], o[2], o[3]};
-            else
-              *reinterpret_cast<u32x2*>(out + d) = u32x2{o[0], o[1]};
-          }
-        if (j == 0 && a->lse != nullptr)
-          a->lse[head * a->lse_h + cur.s] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
-      } else {
-        float* part = starts ? reinterpret_cast<float*>(mine) : heads_lds[wave];
+              for (int i = 0; i < EL; i += 2) o[i / 2] = T::pack(acc[n][EL * c + i][e] * inv, acc[n][EL * c + i + 1][e] * inv);
+              if (d >= a->head_dim) continue;
+              if constexpr (EL == 8)
+                *reinterpret_cast<u32x4*>(out + d) = u32x4{o[0], o[1], o[2], o[3]};
+              else
+                *reinterpret_cast<u32x2*>(out + d) = u32x2{o[0], o[1]};
+            }
+          if (j == 0 && a->lse != nullptr)
+            a->lse[head * a->lse_h + cur.s] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+        } else {
+          float* part = starts ? reinterpret_cast<float*>(mine) : heads_lds[wave];
 #pragma unroll
-        for (int c = 0; c < NP; ++c)
+          for (int c = 0; c < NP; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int i = 0; i < EL; i += 4)
-              *reinterpret_cast<f32x4*>(part + (8 * n + g) * DP + 128 * c + EL * (4 * j + e) + i) =
-                  f32x4{acc[n][EL * c + i][e], acc[n][EL * c + i + 1][e], acc[n][EL * c + i + 2][e], acc[n][EL * c + i + 3][e]};
-        if (j == 0) stats[wave][starts][8 * n + g][0] = m[n], stats[wave][starts][8 * n + g][1] = l[n];
+              for (int i = 0; i < EL; i += 4)
+                *reinterpret_cast<f32x4*>(part + (8 * n + g) * DP + 128 * c + EL * (4 * j + e) + i) =
+                    f32x4{acc[n][EL * c + i][e], acc[n][EL * c + i + 1][e], acc[n][EL * c + i + 2][e], acc[n][EL * c + i + 3][e]};
+          if (j == 0) stats[wave][starts][8 * n + g][0] = m[n], stats[wave][starts][8 * n + g][1] = l[n];
+        }
       }
-    }
-    if (lane == 0) {
-      if (starts && ends) {
-        if (a->by_item) a->owned[4 * ((cur.s * a->kv_heads + cur.kv_head) * a->blocks + cur.block)] = -1;
-      } else {
-        info[wave][starts] = {cur.start + cur.tiles, cur.s, cur.kv_head, cur.block, ends ? 2 : 1};
+      if (lane == 0) {
+        if (starts && ends) {
+          if (a->by_item) a->owned[4 * ((cur.s * a->kv_heads + cur.kv_head) * a->blocks + cur.block)] = -1;
+        } else {
+          info[wave][starts] = {cur.start + cur.tiles, cur.s, cur.kv_head, cur.block, ends ? 2 : 1};
+        }
       }
+    };
+    for (int64_t left = end - begin; left > 0; --left) {
+      const Piece cur = step.x;
+      const int32_t tile = step.tile;
+      if (tile == cur.first) start_piece(cur);
+      work(left > 1);
+      if (tile + 1 == cur.last) end_piece(cur);
     }
-    if (cur.start + cur.last >= end) break;
-    cur = next;
   }
 
   // The parts: wave 0's head, and the tails, each with the heads that go on from
@@ -621,10 +644,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const DecodeParams p
   const float* parts = p.parts + (int64_t)w * 2 * kSlot;
   const auto part = [&](int i) { return parts + (i == 0 ? kSlot : (int64_t)i * 2 * kSlot); };
 
-  // At most kMaxWorkgroups parts, two per thread.
-  float m[2], l[2], top = -INFINITY, weight = 0.f;
+  // At most kMaxWorkgroups parts, kEach per thread.
+  constexpr int kEach = kMaxWorkgroups / kJoinThreads;
+  float m[kEach], l[kEach], top = -INFINITY, weight = 0.f;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
+  for (int x = 0; x < kEach; ++x) {
     const int i = tid + x * kJoinThreads;
     m[x] = i < count ? part(i)[8 * NB * DP + 2 * h] : -INFINITY;
     l[x] = i < count ? part(i)[8 * NB * DP + 2 * h + 1] : 0.f;
@@ -636,7 +660,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const DecodeParams p
 #pragma unroll
   for (int i = 0; i < kJoinThreads / 64; ++i) top = fmaxf(top, wave_stats[0][i]);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
+  for (int x = 0; x < kEach; ++x) {
     const int i = tid + x * kJoinThreads;
     const float f = ratio(m[x], top);
     weight += l[x] * f;

@@ -22,9 +22,9 @@ _DECODE_ARGS = struct.Struct("=10Q14qd8i")
 
 
 @functools.lru_cache
-def _workspace_bytes(device_index: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
-    """Workspace of a call, which depends on its head counts and head_dim alone."""
-    args = _DECODE_ARGS.pack(*(0,) * 24, 0.0, 1, 0, q_heads, kv_heads, head_dim, 1, 0, 0)
+def _workspace_bytes(device_index: int, q_heads: int, kv_heads: int, head_dim: int, int8: bool) -> int:
+    """Workspace of a call, which depends on its head counts, head_dim and kind of pages alone."""
+    args = _DECODE_ARGS.pack(*(0,) * 24, 0.0, 1, 0, q_heads, kv_heads, head_dim, 1, 0, int8)
     needed = ctypes.c_int64()
     status = _native.lib().sa_paged_decode_workspace_bytes(args, device_index, ctypes.byref(needed))
     _native.check(status, "sa_paged_decode_workspace_bytes")
@@ -89,15 +89,15 @@ def paged_decode_attention(
         lse = torch.empty_strided((q_heads, sequences), (sequences, 1), dtype=torch.float32, device=device)
     if sequences:
         index = device.index
-        needed = _workspace_bytes(index, q_heads, kv_heads, dim)
+        needed = _workspace_bytes(index, q_heads, kv_heads, dim, int8)
         workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=device)
         args = _DECODE_ARGS.pack(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0,
             v_scales.data_ptr() if int8 else 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
             0 if lse is None else lse.data_ptr(), workspace.data_ptr(), needed, *q.stride()[:2], *out.stride()[:2],
-            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0), max(sequences, 1), num_pages,
-            dim**-0.5 if softmax_scale is None else float(softmax_scale), sequences, max_pages, q_heads, kv_heads, dim,
-            page_tokens, code, int8)
+            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0),
+            max(sequences, 1), num_pages, dim**-0.5 if softmax_scale is None else float(softmax_scale), sequences, max_pages,
+            q_heads, kv_heads, dim, page_tokens, code, int8)
         status = _native.lib().sa_paged_decode(args, index, _native.current_stream_handle(device))
         if status:
             _native.check(status, "sa_paged_decode")
