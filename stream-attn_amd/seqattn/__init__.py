@@ -30,6 +30,7 @@ from .planner import AttentionPlan, build_plan
 from .projection import (
     OutputProjector,
     ProjectedAttentionRunner,
+    QKRotation,
     QKVProjector,
     streaming_projected_self_attention,
 )
@@ -59,6 +60,7 @@ __all__ = [
     "ProjectedAttentionRunner",
     "ProjectedAttentionStats",
     "ProjectionPipelineConfig",
+    "QKRotation",
     "QKVProjector",
     "StreamingAttentionConfig",
     "StreamingAttentionRunner",

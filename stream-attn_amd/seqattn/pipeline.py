@@ -4,6 +4,7 @@ src/seqattn/pipeline.py)."""
 from .projection import (
     OutputProjector,
     ProjectedAttentionRunner,
+    QKRotation,
     QKVProjector,
     streaming_projected_self_attention,
 )
@@ -11,6 +12,7 @@ from .projection import (
 __all__ = [
     "OutputProjector",
     "ProjectedAttentionRunner",
+    "QKRotation",
     "QKVProjector",
     "streaming_projected_self_attention",
 ]

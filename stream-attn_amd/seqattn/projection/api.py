@@ -9,7 +9,7 @@ from ..config import ProjectionPipelineConfig, StreamingAttentionConfig
 from ..planner import build_plan
 from ..stats import ProjectedAttentionStats
 from .runner import ProjectedAttentionRunner
-from .types import OutputProjector, QKVProjector
+from .types import OutputProjector, QKRotation, QKVProjector
 
 
 def streaming_projected_self_attention(
@@ -28,6 +28,7 @@ def streaming_projected_self_attention(
     causal: bool = False,
     stats: ProjectedAttentionStats | None = None,
     device: torch.device | str = "cuda",
+    qk_rotation: QKRotation | None = None,
 ) -> torch.Tensor:
     """One projected self-attention call: plan, runner, run."""
     attention_config = StreamingAttentionConfig() if attention_config is None else attention_config
@@ -51,6 +52,7 @@ def streaming_projected_self_attention(
         softmax_scale=softmax_scale,
         causal=causal,
         stats=stats,
+        qk_rotation=qk_rotation,
     )
 
 

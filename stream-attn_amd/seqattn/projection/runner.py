@@ -38,7 +38,7 @@ from ..config import ProjectionPipelineConfig, StreamingAttentionConfig
 from ..planner import AttentionPlan, build_plan
 from ..stats import ProjectedAttentionStats
 from ..streaming import StreamingAttentionRunner
-from .types import OutputProjector, QKVProjector
+from .types import OutputProjector, QKRotation, QKVProjector
 from .workspace import ProjectionWorkspace
 
 
@@ -187,22 +187,25 @@ class ProjectedAttentionRunner:
 
     # -- phase 1: projection producer ------------------------------------------
 
-    def _project(self, hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst) -> None:
+    def _project(self, hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst, rotation) -> None:
         """Chunked hidden H2D -> project_qkv -> copy into ``q/k/v_dst`` rows.
 
         Host destinations are written on the D2H stream; device destinations
-        on the compute stream right behind the projection.
+        on the compute stream right behind the projection, Q and K by the norm
+        and rotation itself where there is one.
         """
         workspace = self._workspace_for(hidden_cpu.shape[1])
         to_host = q_dst.device.type == "cpu"
         try:
-            self._project_chunks(hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst, workspace, to_host)
+            self._project_chunks(hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst, rotation, workspace, to_host)
         finally:
             # Also on a failed callback: no copy or projection of this call
             # may still touch the hidden slots when the next call refills them.
             workspace.drain()
 
-    def _project_chunks(self, hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst, workspace, to_host) -> None:
+    def _project_chunks(
+        self, hidden_cpu, project_qkv, stats, q_dst, k_dst, v_dst, rotation, workspace, to_host
+    ) -> None:
         tokens, hidden_features = hidden_cpu.shape
         chunk = self.pipeline_config.projection_chunk_tokens
         pinned_hidden = hidden_cpu.is_pinned()
@@ -220,10 +223,17 @@ class ProjectedAttentionRunner:
                 with self._range("seqattn:qkv_projection"):
                     q, k, v = project_qkv(workspace.hidden[slot][:n], start, stop)
                     self._validate_projected_tile(q, k, v, n)
+                    projected = (q, k, v)
+                    if rotation is not None:
+                        q, k = rotation.apply(
+                            q, k, start, stop,
+                            q_out=None if to_host else q_dst[start:stop], k_out=None if to_host else k_dst[start:stop],
+                        )
                 workspace.projected_ready[slot].record(workspace.compute_stream)
                 if not to_host:
-                    q_dst[start:stop].copy_(q)
-                    k_dst[start:stop].copy_(k)
+                    if rotation is None:
+                        q_dst[start:stop].copy_(q)
+                        k_dst[start:stop].copy_(k)
                     v_dst[start:stop].copy_(v)
                     workspace.copy_done[slot].record(workspace.compute_stream)
             if to_host:
@@ -234,7 +244,7 @@ class ProjectedAttentionRunner:
                     v_dst[start:stop].copy_(v, non_blocking=v_dst.is_pinned())
                     workspace.copy_done[slot].record(workspace.d2h_stream)
                 stats.projection_qkv_d2h_bytes += sum(t.numel() * t.element_size() for t in (q, k, v))
-            workspace.keepalive[slot] = (q, k, v)
+            workspace.keepalive[slot] = (*projected, q, k)
             workspace.busy[slot] = True
             stats.projection_chunks += 1
             stats.projection_hidden_h2d_bytes += n * hidden_features * element
@@ -244,17 +254,20 @@ class ProjectedAttentionRunner:
         hidden_cpu: torch.Tensor,
         project_qkv: QKVProjector,
         stats: ProjectedAttentionStats | None = None,
+        qk_rotation: QKRotation | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Run the chunked projection producer and return CPU-backed Q/K/V views."""
         stats = ProjectedAttentionStats() if stats is None else stats
         self._validate_hidden(hidden_cpu)
+        if qk_rotation is not None:
+            qk_rotation.validate(hidden_cpu.shape[0])
         stats.backend = self.attention.backend
         if self.q_cpu is None:
             self._allocate_host_qkv()
         tokens = hidden_cpu.shape[0]
         torch.cuda.synchronize(self.plan.device)
         started = time.perf_counter()
-        self._project(hidden_cpu, project_qkv, stats, self.q_cpu, self.k_cpu, self.v_cpu)
+        self._project(hidden_cpu, project_qkv, stats, self.q_cpu, self.k_cpu, self.v_cpu, qk_rotation)
         stats.projection_seconds += time.perf_counter() - started
         views = (self.q_cpu[:tokens], self.k_cpu[:tokens], self.v_cpu[:tokens])
         stats.qkv_host_bytes = sum(t.numel() * t.element_size() for t in views)
@@ -265,6 +278,7 @@ class ProjectedAttentionRunner:
         hidden_cpu: torch.Tensor,
         project_qkv: QKVProjector,
         stats: ProjectedAttentionStats | None = None,
+        qk_rotation: QKRotation | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The producer phase with device-resident results (additive).
 
@@ -273,13 +287,15 @@ class ProjectedAttentionRunner:
         """
         stats = ProjectedAttentionStats() if stats is None else stats
         self._validate_hidden(hidden_cpu)
+        if qk_rotation is not None:
+            qk_rotation.validate(hidden_cpu.shape[0])
         stats.backend = self.attention.backend
         if self.q_device is None:
             self._allocate_device_qkv()
         tokens = hidden_cpu.shape[0]
         torch.cuda.synchronize(self.plan.device)
         started = time.perf_counter()
-        self._project(hidden_cpu, project_qkv, stats, self.q_device, self.k_device, self.v_device)
+        self._project(hidden_cpu, project_qkv, stats, self.q_device, self.k_device, self.v_device, qk_rotation)
         stats.projection_seconds += time.perf_counter() - started
         return self.q_device[:tokens], self.k_device[:tokens], self.v_device[:tokens]
 
@@ -298,7 +314,9 @@ class ProjectedAttentionRunner:
         softmax_scale: float | None = None,
         causal: bool = False,
         stats: ProjectedAttentionStats | None = None,
+        qk_rotation: QKRotation | None = None,
     ) -> torch.Tensor:
+        """``qk_rotation`` (additive) normalizes and rotates the projected Q and K before the attention."""
         self._validate_hidden(hidden_cpu)
         tokens = hidden_cpu.shape[0]
         out = self._validate_out(out, tokens, output_features)
@@ -307,12 +325,12 @@ class ProjectedAttentionRunner:
         started = time.perf_counter()
         raw_output_bytes = tokens * self.plan.q_heads * self.plan.head_dim * out.element_size()
         if self.hbm_resident:
-            q, k, v = self.project_qkv_to_device(hidden_cpu, project_qkv, stats)
+            q, k, v = self.project_qkv_to_device(hidden_cpu, project_qkv, stats, qk_rotation)
             stats.raw_attention_roundtrip_bytes_avoided += 2 * raw_output_bytes
             attention_started = time.perf_counter()
             self._attend_resident(q, k, v, cu_seqlens, output_projector, out, softmax_scale, causal, stats)
         else:
-            q, k, v = self.project_qkv_to_host(hidden_cpu, project_qkv, stats)
+            q, k, v = self.project_qkv_to_host(hidden_cpu, project_qkv, stats, qk_rotation)
             stats.raw_attention_roundtrip_bytes_avoided += 2 * raw_output_bytes
             attention_started = time.perf_counter()
             self.attention.run_with_device_output(
