@@ -22,6 +22,9 @@
 namespace sa {
 namespace {
 
+// Launches of 2^32 threads and more go in parts.
+constexpr int64_t kTokensPerLaunch = 1 << 23;
+
 struct PageRows {
   char* base;       // row of slot s: base + page * stride_p + row * stride_t + head * stride_h, in elements
   uint16_t* scale;  // fp16 scales, null for 16-bit pages
@@ -44,8 +47,11 @@ struct RowsParams {
   int32_t end0, end1, end2;  // first pair past axis 0, 1, 2
   int32_t heads;             // rows of a token: Q's, K's and V's
   int32_t lane_log2;         // log2 of the lanes of a head
+  int32_t beside;            // log2 of a token's waves in a workgroup
   int32_t pos64, qw32, kw32;
 };
+
+constexpr int kMostPairs = 128;  // of a head
 
 // How a lane's W pairs lie in a row.  With halves, unit u holds pairs W u ..
 // W u + W - 1: their first elements are W consecutive ones, their second
@@ -262,7 +268,7 @@ __device__ inline void codes(float (&x)[N], float step, float reciprocal) {
   for (int i = 0; i < N; ++i) {
     const float y = x[i] * reciprocal;
     q[i] = rintf(y);
-    near = near || fabsf(y - q[i]) > 0.5f - 1.f / 16384;
+    near = near || fabsf(y - q[i]) > 0.5f - 1.f / 32768;
   }
   if (__any(near)) {
 #pragma unroll
@@ -279,9 +285,10 @@ __device__ inline void codes(float (&x)[N], float step, float reciprocal) {
 // is less time on the way through one.
 template <typename T, Form F, int W, bool kInt8, bool kOnce>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
-  const int64_t token = p.token0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  // A token's waves: 2^beside in the workgroup, in gridDim.y workgroups.
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t token = p.token0 + (int64_t)blockIdx.x * (4 >> p.beside) + (wave >> p.beside);
   if (token >= p.tokens) return;
-  const int lane = threadIdx.x & 63;
   const int unit_lane = lane & ((1 << p.lane_log2) - 1);
   const int per_step = 64 >> p.lane_log2;
   const bool live = unit_lane * 2 * W < p.head_dim;  // head_dim / 2W lanes of the 2^n hold a unit
@@ -298,8 +305,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     const int64_t base = choose(is_q, in_q, choose(is_v, in_v, in_k)), stride = choose(is_q, sq_h, choose(is_v, sv_h, sk_h));
     return load_raw<F, W, kOnce>(reinterpret_cast<const uint16_t*>(base) + head * stride, u);
   };
-  const int stride = gridDim.y * per_step;
-  int first = blockIdx.y * per_step;
+  const int stride = (gridDim.y << p.beside) * per_step;
+  int first = ((blockIdx.y << p.beside) + (wave & ((1 << p.beside) - 1))) * per_step;
   Raw<F, W> raw = load(first);
 
   bool stored = false;
@@ -321,31 +328,29 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     load_weight<T, F, W>(p.k_weight, p.kw32, u, wka, wkb);
   }
   if (p.pairs > 0) {
-    // Loads without branches around each, so that they are under way together.
-    int64_t pos[SA_MAX_ROTARY_AXES];
-    double frequency[W];
-    const int64_t axis = p.pos_axis, where = token * p.pos_token;
-    if (p.pos64) {
-#pragma unroll
-      for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x)
-        pos[x] = static_cast<const int64_t*>(p.positions)[where + (x < p.axes ? x : 0) * axis];
-    } else {
-#pragma unroll
-      for (int x = 0; x < SA_MAX_ROTARY_AXES; ++x)
-        pos[x] = static_cast<const int32_t*>(p.positions)[where + (x < p.axes ? x : 0) * axis];
+    // A pair per lane, then every lane's own from LDS (the wave's part of it:
+    // no barrier).
+    __shared__ float angles[4][2][kMostPairs];
+    for (int pair = lane; pair < p.pairs; pair += 64) {
+      const int axis = (pair >= p.end0) + (pair >= p.end1) + (pair >= p.end2);
+      const int64_t at = axis * p.pos_axis + token * p.pos_token;
+      const double position = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[at]
+                                      : (double)static_cast<const int32_t*>(p.positions)[at];
+      // Turns in FP64 (far positions have their fraction there), its fraction
+      // in FP32: the sine instruction takes turns.
+      const double turns = position * (p.frequencies[pair] * 0.15915494309189533577);
+      const float fraction = (float)(turns - rint(turns));
+      angles[wave][0][pair] = __builtin_amdgcn_cosf(fraction);
+      angles[wave][1][pair] = __builtin_amdgcn_sinf(fraction);
     }
-#pragma unroll
-    for (int i = 0; i < W; ++i) frequency[i] = p.frequencies[u.first + i < p.pairs ? u.first + i : 0];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const int pair = u.first + i;
-      // Turns in FP64 (far positions have their fraction there), its fraction
-      // in FP32: the sine instruction takes turns.
-      const double at = (double)(pair < p.end0 ? pos[0] : pair < p.end1 ? pos[1] : pair < p.end2 ? pos[2] : pos[3]);
-      const double turns = pair < p.pairs ? at * (frequency[i] * 0.15915494309189533577) : 0.0;
-      const float fraction = (float)(turns - rint(turns));
-      cos_t[i] = __builtin_amdgcn_cosf(fraction);
-      sin_t[i] = __builtin_amdgcn_sinf(fraction);
+      const float c = angles[wave][0][min(pair, p.pairs - 1)], s = angles[wave][1][min(pair, p.pairs - 1)];
+      cos_t[i] = pair < p.pairs ? c : 1.f;
+      sin_t[i] = pair < p.pairs ? s : 0.f;
     }
   }
 
@@ -390,14 +395,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     if (p.slots == nullptr) continue;
     char* pages = reinterpret_cast<char*>(choose(mask_v, v_base, k_base));
     if constexpr (kInt8) {
-      float amax = 0.f;
-      bool finite = true;
+      // The largest magnitude; as integers infinities and NaN are larger still.
+      uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(b[i])));
-        finite = finite && fabsf(a[i]) <= FLT_MAX && fabsf(b[i]) <= FLT_MAX;
-      }
-      amax = over_lanes(finite ? amax : INFINITY, p.lane_log2, [](float x, float y) { return fmaxf(x, y); });
+      for (int i = 0; i < W; ++i)
+        top = max(top, max(__builtin_bit_cast(uint32_t, a[i]) & 0x7fffffffu, __builtin_bit_cast(uint32_t, b[i]) & 0x7fffffffu));
+      const float amax = over_lanes(__builtin_bit_cast(float, min(top, 0x7f800000u)), p.lane_log2,
+                                    [](float x, float y) { return fmaxf(x, y); });
       if (active && !is_q && stored) {
         const float step = amax / 127.f > 0.f ? amax / 127.f : 1.f;
         const float reciprocal = 1.f / step;
@@ -411,6 +415,103 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
       store_pairs<T, F, W, kOnce>(reinterpret_cast<uint16_t*>(pages) + at + head * p.kp.sh, u, a, b);
     }
   }
+}
+
+// log2 of the lanes of a head with `elements` on each, and the heads of a wave.
+int32_t lanes_log2(int32_t head_dim, int32_t elements) {
+  int32_t n = 0;
+  while ((elements << n) < head_dim) ++n;
+  return n;
+}
+int32_t rows_per_step(int32_t lane_log2) { return 64 >> lane_log2; }
+
+struct StoreParams {
+  const uint16_t *k, *v;
+  PageRows kp, vp;
+  const int64_t* slots;
+  int64_t sk_t, sk_h, sv_t, sv_h, token0, tokens;
+  uint32_t num_slots, page_tokens;
+  int32_t kv_heads, head_dim, lane_log2;
+  int32_t each;  // tokens of a workgroup
+};
+
+// K and V rows to their pages as they are, few per token: where a token's would
+// leave lanes of a wave without one (rows_kernel), a workgroup has the rows of
+// `each` tokens, four of a thread under way together.  A row's granules (8
+// elements) are on 2^lane_log2 lanes.  60,000 rows of 128, with one K/V head
+// 44 -> 30 us (INT8 66 -> 40), two 28 -> 24; four and more as fast in rows_kernel,
+// 56 slower here (186 and 177).
+template <typename T, bool kInt8>
+__global__ __launch_bounds__(256) void store_kernel(const StoreParams p) {
+  constexpr int kTogether = 4;
+  const int64_t token0 = p.token0 + (int64_t)blockIdx.x * p.each;
+  const int count = (int)std::min<int64_t>(p.each, p.tokens - token0), per_token = 2 * p.kv_heads;
+  const int g = threadIdx.x & ((1 << p.lane_log2) - 1), d = 8 * g;
+  const bool live = d < p.head_dim;
+  const int groups = 256 >> p.lane_log2;
+  for (int first = threadIdx.x >> p.lane_log2; first - (int)(threadIdx.x >> p.lane_log2) < count * per_token;
+       first += kTogether * groups) {
+    u32x4 x[kTogether];
+    int64_t slot[kTogether];
+    int head[kTogether];
+    uint32_t is_v[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int row = first + i * groups;
+      const bool has = live && row < count * per_token;
+      const int t = has ? row / per_token : 0, h = has ? row - t * per_token : 0;
+      is_v[i] = h >= p.kv_heads ? ~0u : 0u;
+      head[i] = h - (is_v[i] & p.kv_heads);
+      const int64_t base = choose(is_v[i], (int64_t)p.v, (int64_t)p.k);
+      const int64_t at = (token0 + t) * choose(is_v[i], p.sv_t, p.sk_t) + head[i] * choose(is_v[i], p.sv_h, p.sk_h);
+      x[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(base) + at + (live ? d : 0));
+      slot[i] = p.slots[token0 + t];
+      if (!has || slot[i] >= (int64_t)p.num_slots) slot[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const bool stored = slot[i] >= 0;
+      const uint32_t page = stored ? (uint32_t)slot[i] / p.page_tokens : 0, row = stored ? (uint32_t)slot[i] - page * p.page_tokens : 0;
+      const int64_t at = page * p.kp.sp + row * p.kp.st + head[i] * p.kp.sh + d;
+      char* pages = reinterpret_cast<char*>(choose(is_v[i], (int64_t)p.vp.base, (int64_t)p.kp.base));
+      if constexpr (kInt8) {
+        float y[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = T::lo(x[i][e]), y[2 * e + 1] = T::hi(x[i][e]);
+          top = max(top, max(__builtin_bit_cast(uint32_t, y[2 * e]) & 0x7fffffffu, __builtin_bit_cast(uint32_t, y[2 * e + 1]) & 0x7fffffffu));
+        }
+        const float amax = over_lanes(live ? __builtin_bit_cast(float, min(top, 0x7f800000u)) : 0.f, p.lane_log2,
+                                      [](float a, float b) { return fmaxf(a, b); });
+        const float step = amax / 127.f > 0.f ? amax / 127.f : 1.f;
+        codes(y, step, 1.f / step);
+        if (!stored) continue;
+        *reinterpret_cast<u32x2*>(pages + at) = u32x2{pack_codes(y[0], y[1], y[2], y[3]), pack_codes(y[4], y[5], y[6], y[7])};
+        if (g == 0)
+          reinterpret_cast<uint16_t*>(choose(is_v[i], (int64_t)p.vp.scale, (int64_t)p.kp.scale))[page * p.kp.ss_p + row * p.kp.ss_t + head[i] * p.kp.ss_h] =
+              (uint16_t)Fp16::pack(amax <= FLT_MAX ? step : NAN, 0.f);
+      } else if (stored) {
+        *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(pages) + at) = x[i];
+      }
+    }
+  }
+}
+
+template <typename T>
+int32_t launch_store(StoreParams p, bool int8, hipStream_t stream) {
+  p.lane_log2 = lanes_log2(p.head_dim, 8);
+  p.each = std::max(1, (1024 >> p.lane_log2) / (2 * p.kv_heads));
+  const int64_t most = kTokensPerLaunch / p.each * p.each;
+  for (p.token0 = 0; p.token0 < p.tokens; p.token0 += most) {
+    const uint32_t grid = (uint32_t)((std::min(p.tokens - p.token0, most) + p.each - 1) / p.each);
+    if (int8)
+      store_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+    else
+      store_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    SA_HIP_RETURN(hipGetLastError());
+  }
+  return 0;
 }
 
 struct ReadParams {
@@ -508,8 +609,6 @@ int32_t check_pool(const char* entry, int64_t num_pages, int32_t page_tokens) {
   return 0;
 }
 
-// Launches of 2^32 threads and more go in parts.
-constexpr int64_t kTokensPerLaunch = 1 << 23;
 // Waves that fill the chip: a token's rows are dealt to several waves where
 // there are fewer tokens.  With 40 heads of 128: 4,099 tokens 18.3 us with 4,096,
 // 23 with 16,384; 6,000 tokens 25.4 and 28.6.
@@ -519,6 +618,11 @@ constexpr int64_t kWavesToFill = 4096;
 // 20,011 tokens with the append (492 MB) 98 -> 92; 8,190 x 32 heads of 80 (84 MB),
 // read again from the cache, 23 -> 26.
 constexpr int64_t kCacheBytes = 256 << 20;
+// A token's steps (64 >> lane_log2 rows each) from which two or four waves of
+// a workgroup take them in turn, so that rows that lie together are read
+// together: 14 steps, 61,312 tokens 647 us with one wave, 606 with two, 586 (6.0 TB/s)
+// with four; 6 steps, 20,011 tokens 88.7, 87.2 and 99.
+constexpr int32_t kTwoBeside = 6, kFourBeside = 12;
 
 template <typename T, bool kInt8, bool kOnce>
 int32_t launch_rows(RowsParams p, bool adjacent, hipStream_t stream) {
@@ -526,15 +630,15 @@ int32_t launch_rows(RowsParams p, bool adjacent, hipStream_t stream) {
   // elements.
   const int32_t rest = (p.head_dim - 2 * p.pairs) / 2;
   const auto fits = [&](int w) { return p.pairs % w == 0 && rest % w == 0; };
-  const int form = adjacent || p.pairs == 0 ? 0 : fits(8) ? 1 : fits(4) ? 2 : 3;
-  const int units = p.head_dim / (form == 1 ? 16 : 8);
-  p.lane_log2 = 0;
-  while ((1 << p.lane_log2) < units) ++p.lane_log2;
-  const int32_t per_step = 64 >> p.lane_log2, steps = (p.heads + per_step - 1) / per_step;
+  const int form = p.pairs > 0 ? (adjacent ? 0 : fits(8) ? 1 : fits(4) ? 2 : 3) : fits(8) ? 1 : 0;
+  p.lane_log2 = lanes_log2(p.head_dim, form == 1 ? 16 : 8);
+  const int32_t per_step = rows_per_step(p.lane_log2), steps = (p.heads + per_step - 1) / per_step;
   const int64_t waves = std::min<int64_t>(steps, (kWavesToFill + p.tokens - 1) / p.tokens);
+  p.beside = steps >= kFourBeside ? 2 : steps >= kTwoBeside ? 1 : 0;
   for (p.token0 = 0; p.token0 < p.tokens; p.token0 += kTokensPerLaunch) {
     const int64_t count = std::min(p.tokens - p.token0, kTokensPerLaunch);
-    const dim3 grid((uint32_t)((count + 3) / 4), (uint32_t)waves);
+    const int64_t tokens = 4 >> p.beside;  // of a workgroup
+    const dim3 grid((uint32_t)((count + tokens - 1) / tokens), (uint32_t)((waves + (1 << p.beside) - 1) >> p.beside));
     if (form == 0)
       rows_kernel<T, kAdjacent, 4, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else if (form == 1)
@@ -625,6 +729,13 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* s
   const bool bf16 = a->dtype == SA_DTYPE_BF16;
   p.tokens = a->tokens;
   const bool int8 = pages && a->pages_int8;
+  if (!has_q && pages && p.pairs == 0 && p.k_weight == nullptr && p.heads <= rows_per_step(lanes_log2(p.head_dim, 16))) {
+    StoreParams s{};
+    s.k = p.k, s.v = p.v, s.kp = p.kp, s.vp = p.vp, s.slots = p.slots;
+    s.sk_t = p.sk_t, s.sk_h = p.sk_h, s.sv_t = p.sv_t, s.sv_h = p.sv_h, s.tokens = p.tokens;
+    s.num_slots = p.num_slots, s.page_tokens = p.page_tokens, s.kv_heads = p.kv_heads, s.head_dim = p.head_dim;
+    return bf16 ? launch_store<Bf16>(s, int8, hs) : launch_store<Fp16>(s, int8, hs);
+  }
   return bf16 ? launch_rows<Bf16>(p, int8, a->adjacent, hs) : launch_rows<Fp16>(p, int8, a->adjacent, hs);
 } catch (const std::exception& error) {
   return sa::exception_status("sa_normalize_rotate_store", error);

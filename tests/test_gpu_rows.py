@@ -245,6 +245,47 @@ def test_pools_past_32_bit_offsets():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_launch_past_the_caches_equals_its_parts(int8):
+    """From 256 MB on a launch reads and writes past the caches: the same rows as in small launches."""
+    tokens, q_heads, kv_heads, dim = 9001, 48, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    fused = torch.randn((tokens, q_heads + 2 * kv_heads, dim), generator=gen, device="cuda").to(torch.bfloat16)
+    assert fused.numel() * 4 >= 256 << 20
+    q, k, v = fused.split([q_heads, kv_heads, kv_heads], dim=1)
+    freq, pos = rotary_frequencies((16, 24, 24)), torch.arange(3 * tokens, device="cuda").view(3, tokens)
+    options = dict(sections=(16, 24, 24), q_weight=torch.ones(dim, device="cuda"), k_weight=torch.ones(dim, device="cuda"))
+    slots = torch.randperm(9024, generator=gen, device="cuda")[:tokens]
+    caches = [DeviceKVCache(141, 64, kv_heads, dim, storage_dtype="int8" if int8 else None) for _ in range(2)]
+    whole = caches[0].normalize_rotate_append(q, k, v, slots, pos, freq, **options)
+    parts = [caches[1].normalize_rotate_append(q[i : i + 1000], k[i : i + 1000], v[i : i + 1000], slots[i : i + 1000],
+                                               pos[:, i : i + 1000], freq, **options) for i in range(0, tokens, 1000)]
+    assert torch.equal(whole, torch.cat(parts))
+    for a, b in zip(caches[0].read(slots), caches[1].read(slots)):
+        assert torch.equal(a, b)
+    # All of Q and K turned in place.
+    want = normalize_rotate_qk(q, k, pos, freq, **options)
+    assert torch.equal(want[0], whole)
+    normalize_rotate_qk(q, k, pos, freq, q_out=q, k_out=k, **options)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 9])
+@pytest.mark.parametrize("dim", [16, 64, 72, 128, 256])
+def test_appends_of_few_and_many_heads(heads, dim):
+    """Both forms of the append, 16-bit rows of every head count next to a wave's."""
+    gen = torch.Generator().manual_seed(heads * dim)
+    tokens = 133
+    k, v = (rows(gen, tokens, heads, dim, dtype=torch.bfloat16).cuda() for _ in range(2))
+    cache = DeviceKVCache(20, 8, heads, dim)
+    slots = torch.randperm(160, generator=gen)[:tokens].cuda()
+    slots[7], slots[132] = -1, 160
+    cache.append(k, v, slots)
+    ko, vo = cache.read(slots)
+    k[[7, 132]], v[[7, 132]] = 0, 0
+    assert torch.equal(ko, k) and torch.equal(vo, v)
+
+
 def test_replayed_graph_and_other_stream():
     gen = torch.Generator().manual_seed(11)
     fused = rows(gen, 5, 8, 64, dtype=torch.bfloat16).cuda()
