@@ -596,15 +596,16 @@ int32_t sa_run_resident_noalloc(const void* q, const void* k, const void* v, voi
  * gets scale NaN.
  *
  * K's and V's pages have the same strides, and so have their scales.  q and
- * q_out are NULL together; k goes to k_out or to k_pages (the other is
- * NULL); v and v_pages come with k_pages.  Strides in elements, unit in the
- * last dimension.  q, k, v, the outputs and 16-bit pages are 16-byte aligned
- * with strides in multiples of 8; int8 pages 8-byte aligned, strides in
- * multiples of 8.  head_dim is a multiple of 8 in [16, 256], axes at most 4,
- * num_pages * page_tokens below 2^31.  The rows of one call have distinct
- * slots.  Asynchronous on `stream`, a stream of `device`.
+ * q_out are NULL together; k goes to k_out or to k_pages (the other is NULL); v
+ * and v_pages come with k_pages.  Strides in elements, unit in the last
+ * dimension.  q, k, v, the outputs and 16-bit pages are 16-byte aligned with
+ * strides in multiples of 8; int8 pages 8-byte aligned, strides in multiples of
+ * 8.  head_dim is a multiple of 8 in [16, 256], axes at most 4, page_tokens at
+ * most SA_MAX_PAGE_TOKENS, num_pages * page_tokens below 2^31.  The rows of one
+ * call have distinct slots.  Asynchronous on `stream`, a stream of `device`.
  */
 #define SA_MAX_ROTARY_AXES 4
+#define SA_MAX_PAGE_TOKENS (1 << 20)
 typedef struct {
     const void *q, *k, *v;
     void *q_out, *k_out;

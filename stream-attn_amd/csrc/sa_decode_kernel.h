@@ -134,11 +134,15 @@ struct Reader {
   int32_t tile, page, row;
   int32_t ids, first_id;  // page numbers first_id + lane of the sequence
 
-  __device__ inline int32_t id_of(const DecodeParams& p, int32_t n, int lane) {
-    if (n - first_id >= 64) {
+  // Has pages n .. upto in `ids` (n never falls, upto - n < 64).
+  __device__ inline void hold(const DecodeParams& p, int32_t n, int32_t upto, int lane) {
+    if (upto - first_id >= 64) {
       first_id = n;
       ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
     }
+  }
+  __device__ inline int32_t id_of(const DecodeParams& p, int32_t n, int lane) {
+    hold(p, n, n, lane);
     return __builtin_amdgcn_readlane(ids, n - first_id);
   }
 
@@ -225,12 +229,13 @@ struct Step {
       }
     } else {
       seen = 0;
+      from.hold(p, page, page + uniform((int32_t)((uint64_t)(uint32_t)(row + kDecodeTile - 1) * p.page_magic >> p.page_shift)), lane);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        const int32_t key = key0 + 4 * t + j;
-        const int32_t n = (int32_t)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift);
-        const int32_t r = key - n * p.page_tokens;
-        int32_t id = n < p.max_pages ? x.table[n] : -1;
+        int32_t r = row + 4 * t + j;
+        const int32_t past = (int32_t)((uint64_t)(uint32_t)r * p.page_magic >> p.page_shift);
+        r -= past * p.page_tokens;
+        int32_t id = __shfl(from.ids, page + past - from.first_id);
         const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
         if (!ok) id = 0;
         seen |= (uint32_t)ok << t;

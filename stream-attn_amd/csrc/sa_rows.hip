@@ -604,8 +604,8 @@ int32_t check_sizes(const char* entry, int32_t dtype, int32_t head_dim, int32_t 
 }
 
 int32_t check_pool(const char* entry, int64_t num_pages, int32_t page_tokens) {
-  if (page_tokens < 1 || num_pages < 0 || num_pages > INT32_MAX / page_tokens)
-    return invalid(entry, "num_pages * page_tokens must be below 2^31");
+  if (page_tokens < 1 || page_tokens > SA_MAX_PAGE_TOKENS || num_pages < 0 || num_pages > INT32_MAX / page_tokens)
+    return invalid(entry, "page_tokens must be at most 2^20 and num_pages * page_tokens below 2^31");
   return 0;
 }
 

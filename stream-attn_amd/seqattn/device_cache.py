@@ -12,7 +12,7 @@ import torch
 
 from . import _native
 from .kernels.decode import paged_decode_attention
-from .kernels.rows import append_kv, normalize_rotate_append, read_kv
+from .kernels.rows import MAX_PAGE_TOKENS, append_kv, normalize_rotate_append, read_kv
 
 
 class DeviceKVCache:
@@ -38,8 +38,8 @@ class DeviceKVCache:
         _native.dtype_code(dtype)
         if min(num_pages, page_tokens, kv_heads) < 1:
             raise ValueError("num_pages, page_tokens and kv_heads must be positive")
-        if num_pages * page_tokens > 2**31 - 1:
-            raise ValueError("the cache must have fewer than 2^31 rows")
+        if page_tokens > MAX_PAGE_TOKENS or num_pages * page_tokens > 2**31 - 1:
+            raise ValueError(f"pages have at most {MAX_PAGE_TOKENS} rows, the cache fewer than 2^31")
         if head_dim % 8 or not 16 <= head_dim <= 256:
             raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {head_dim}")
         if storage_dtype not in (None, "int8", str(dtype).removeprefix("torch.")):

@@ -56,7 +56,9 @@ def paged_decode_attention(
     not seen, and what rows past a length hold does not matter.  A token that
     sees no key gets zeros, and LSE ``-inf``.
 
-    INT8 pages stand for ``value * scale``.  Logits, softmax and sums are FP32.
+    INT8 pages stand for ``value * scale``.  Logits, softmax and sums are FP32;
+    a weight enters the product with V as two 16-bit parts.  A seen value that is
+    not finite gives NaN.  ``out`` may be ``q``.
     Returns ``out`` (like ``q``), and with ``return_lse`` also the natural-log
     LSE ``[q_heads, sequences]``.
     """

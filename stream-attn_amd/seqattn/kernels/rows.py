@@ -28,6 +28,7 @@ import torch
 from .. import _native
 
 MAX_ROTARY_AXES = 4
+MAX_PAGE_TOKENS = 2**20
 # sa_rows_args: 14 pointers, 20 strides and counts, eps, 16 int32.
 _ROWS_ARGS = struct.Struct("=14Q20qd16i")
 # sa_read_args: 7 pointers, 8 strides and counts, 6 int32.
@@ -52,10 +53,10 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
         code = _native.dtype_code(rows.dtype)
         if dim % 8 or not 16 <= dim <= 256:
             raise ValueError(f"head_dim must be a multiple of 8 in [16, 256], got {dim}")
-        if heads < 1:
-            raise ValueError(f"{name} has no heads")
     elif rows.device != like.device or rows.dtype != like.dtype:
         raise ValueError(f"{name} must have the device and dtype of the other rows")
+    if heads < 1:
+        raise ValueError(f"{name} has no heads")
     if output:
         if (tokens > 1 and st < dim) or (heads > 1 and sh < dim) or (
                 tokens > 1 and heads > 1 and st < heads * sh and sh < tokens * st):
@@ -82,8 +83,8 @@ def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype:
         raise ValueError("pages must live on the device of the rows")
     if not k_pages.numel():
         raise ValueError("the cache has no pages")
-    if shape[0] * shape[1] > 2**31 - 1:
-        raise ValueError("the cache has 2^31 rows or more")
+    if shape[1] > MAX_PAGE_TOKENS or shape[0] * shape[1] > 2**31 - 1:
+        raise ValueError(f"pages have at most {MAX_PAGE_TOKENS} rows, the cache fewer than 2^31")
     if not int8:
         if k_scales is not None or v_scales is not None:
             raise ValueError("only INT8 pages have scales")

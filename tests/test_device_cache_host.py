@@ -43,7 +43,7 @@ def test_cache_pools_and_slots():
     int8 = DeviceKVCache(6, 4, 2, 16, dtype=torch.float16, storage_dtype="int8", device="cpu")
     assert int8.k_pages.dtype == torch.int8 and int8.k_scales.shape == (6, 4, 2)
     assert int8.bytes == 2 * 6 * 4 * 2 * 18
-    for bad in (dict(num_pages=0), dict(page_tokens=0), dict(head_dim=12), dict(head_dim=264), dict(num_pages=2**30),
+    for bad in (dict(num_pages=0), dict(page_tokens=0), dict(head_dim=12), dict(head_dim=264), dict(num_pages=2**30), dict(num_pages=1, page_tokens=2**20 + 1),
                 dict(storage_dtype="float16"), dict(storage_dtype="fp8")):
         with pytest.raises(ValueError):
             DeviceKVCache(**{**dict(num_pages=6, page_tokens=4, kv_heads=2, head_dim=16, device="cpu"), **bad})
@@ -89,7 +89,7 @@ def test_rows_entry_point_rejects_bad_arguments_without_a_gpu():
         (dict(pairs=33), -1, b"pairs"), (dict(pairs=32), -1, b"positions"), (dict(turned, axes=5), -1, b"axes"),
         (dict(turned, s0=31), -1, b"add up"), (dict(turned, s0=33), -1, b"add up"), (dict(turned, axes=2), -1, b"add up"),
         (dict(turned, frequencies=4), -1, b"positions"),
-        (dict(paged, page_tokens=0), -1, b"2^31"), (dict(paged, num_pages=2**30), -1, b"2^31"),
+        (dict(paged, page_tokens=0), -1, b"2^31"), (dict(paged, num_pages=1, page_tokens=2**20 + 1), -1, b"2^20"), (dict(paged, num_pages=2**30), -1, b"2^31"),
         (dict(paged, int8=1), -1, b"scales"), (dict(paged, pp=4), -1, b"aligned"), (dict(paged, slots=4), -1, b"aligned"),
     ):
         assert lib.sa_normalize_rotate_store(rows_args(**fields), 0, None) == status, fields
@@ -132,6 +132,7 @@ def test_decode_entry_point_rejects_bad_arguments_without_a_gpu():
 
     for fields, status in ((dict(dtype=2), -2), (dict(dim=12), -3), (dict(dim=264), -3), (dict(q_heads=3), -1),
                            (dict(kv_heads=0), -1), (dict(sequences=-1), -1), (dict(page=0), -1), (dict(num_pages=2**30), -1),
+                           (dict(num_pages=1, page=2**20 + 1), -1),
                            (dict(max_pages=2**30), -1), (dict(q=0), -1), (dict(out=8), -1), (dict(qt=4), -1),
                            (dict(pt=4), -1), (dict(int8=1), -1), (dict(table=0), -1), (dict(lengths=2), -1)):
         assert lib.sa_paged_decode(args(**fields), 0, None) == status, fields

@@ -114,6 +114,22 @@ def test_a_long_sequence_beside_short_ones():
     check(*make(gen, [5, 9000, 0, 1, 130], 8, 2, 64, 16, torch.bfloat16))
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page,dtype,int8,count", [
+    (8, 4, 64, 16, torch.bfloat16, False, 170),   # more items than workgroups, parts found by workgroup
+    (8, 4, 64, 24, torch.bfloat16, True, 300),
+    (12, 4, 128, 16, torch.float16, False, 150),
+    (36, 2, 128, 10, torch.bfloat16, False, 140),  # 18 query heads: two items per K/V head
+    (4, 2, 256, 32, torch.bfloat16, True, 150),
+    (2, 1, 40, 16, torch.bfloat16, False, 700),    # several sequences per thread of the scan
+])
+def test_many_sequences_of_very_different_lengths(q_heads, kv_heads, dim, page, dtype, int8, count):
+    gen = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 70, (count,), generator=gen)
+    lengths[torch.rand(count, generator=gen) < 0.2] = 0
+    lengths[3], lengths[count // 2], lengths[-1] = 3000, 700, 1500
+    check(*make(gen, lengths.tolist(), q_heads, kv_heads, dim, page, dtype, int8))
+
+
 def test_lengths_past_the_table_and_below_zero():
     gen = torch.Generator().manual_seed(3)
     q, pools, scales, table, lengths, dev, dev_scales = make(gen, [64, 32, 48], 4, 2, 64, 16, torch.bfloat16)

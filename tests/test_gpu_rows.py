@@ -327,6 +327,8 @@ def test_refusals():
     refused("both positions and frequencies", q, k, None, freq)
     refused("same tokens and head_dim", q, k[:3], pos, freq)
     refused("device and dtype", q, k.half(), pos, freq)
+    refused("no heads", q, k[:, :0], pos, freq)
+    refused("no heads", q[:, :0], k, pos, freq)
     refused("float16 or bfloat16", q.float(), k.float(), pos, freq)
     refused("multiple of 8", q[..., :12], k[..., :12], pos, freq[:6])
     refused("unit stride", q.transpose(1, 2), k, pos, freq)
