@@ -134,9 +134,12 @@ __device__ inline __attribute__((always_inline)) Raw<F, W> load_raw(const uint16
 #pragma unroll
     for (int i = 0; i < W; ++i) r.w[i] = row[u.at_lo(i)] | (uint32_t)row[u.at_hi(i)] << 16;
   } else if constexpr (F == kAdjacent) {
-    const Words<W> x = load_words<W, kOnce>(row + u.lo);
 #pragma unroll
-    for (int i = 0; i < W; ++i) r.w[i] = x.w[i];
+    for (int n = 0; n < W; n += 4) {
+      const Words<4> x = load_words<4, kOnce>(row + u.lo + 2 * n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[n + i] = x.w[i];
+    }
   } else {
     const Words<W / 2> x = load_words<W / 2, kOnce>(row + u.lo), y = load_words<W / 2, kOnce>(row + u.hi);
 #pragma unroll
@@ -186,10 +189,13 @@ __device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const flo
       row[u.at_hi(i)] = (uint16_t)T::pack(b[i], 0.f);
     }
   } else if constexpr (F == kAdjacent) {
-    Words<W> x;
 #pragma unroll
-    for (int i = 0; i < W; ++i) x.w[i] = T::pack(a[i], b[i]);
-    store_words<W, kOnce>(row + u.lo, x);
+    for (int n = 0; n < W; n += 4) {
+      Words<4> x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] = T::pack(a[n + i], b[n + i]);
+      store_words<4, kOnce>(row + u.lo + 2 * n, x);
+    }
   } else {
     Words<W / 2> x, y;
 #pragma unroll
@@ -216,8 +222,10 @@ __device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (
       row[u.at_hi(i)] = (char)(int32_t)b[i];
     }
   } else if constexpr (F == kAdjacent) {
-    static_assert(W == 4, "one 8-byte run");
-    store_words<2, kOnce>(row + u.lo, Words<2>{{pack_codes(a[0], b[0], a[1], b[1]), pack_codes(a[2], b[2], a[3], b[3])}});
+#pragma unroll
+    for (int n = 0; n < W; n += 4)
+      store_words<2, kOnce>(row + u.lo + 2 * n, Words<2>{{pack_codes(a[n], b[n], a[n + 1], b[n + 1]),
+                                                          pack_codes(a[n + 2], b[n + 2], a[n + 3], b[n + 3])}});
   } else {
     Words<W / 4> x, y;
 #pragma unroll
@@ -630,8 +638,9 @@ int32_t launch_rows(RowsParams p, bool adjacent, hipStream_t stream) {
   // elements.
   const int32_t rest = (p.head_dim - 2 * p.pairs) / 2;
   const auto fits = [&](int w) { return p.pairs % w == 0 && rest % w == 0; };
-  const int form = p.pairs > 0 ? (adjacent ? 0 : fits(8) ? 1 : fits(4) ? 2 : 3) : fits(8) ? 1 : 0;
-  p.lane_log2 = lanes_log2(p.head_dim, form == 1 ? 16 : 8);
+  const bool sixteen = p.head_dim % 16 == 0;  // elements of a lane
+  const int form = p.pairs > 0 && !adjacent ? (fits(8) ? 1 : fits(4) ? 2 : 3) : sixteen ? 4 : 0;
+  p.lane_log2 = lanes_log2(p.head_dim, form == 1 || form == 4 ? 16 : 8);
   const int32_t per_step = rows_per_step(p.lane_log2), steps = (p.heads + per_step - 1) / per_step;
   const int64_t waves = std::min<int64_t>(steps, (kWavesToFill + p.tokens - 1) / p.tokens);
   p.beside = steps >= kFourBeside ? 2 : steps >= kTwoBeside ? 1 : 0;
@@ -641,6 +650,8 @@ int32_t launch_rows(RowsParams p, bool adjacent, hipStream_t stream) {
     const dim3 grid((uint32_t)((count + tokens - 1) / tokens), (uint32_t)((waves + (1 << p.beside) - 1) >> p.beside));
     if (form == 0)
       rows_kernel<T, kAdjacent, 4, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
+    else if (form == 4)
+      rows_kernel<T, kAdjacent, 8, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else if (form == 1)
       rows_kernel<T, kHalves, 8, kInt8, kOnce><<<grid, 256, 0, stream>>>(p);
     else if (form == 2)
