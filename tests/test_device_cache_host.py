@@ -43,8 +43,8 @@ def test_cache_pools_and_slots():
     int8 = DeviceKVCache(6, 4, 2, 16, dtype=torch.float16, storage_dtype="int8", device="cpu")
     assert int8.k_pages.dtype == torch.int8 and int8.k_scales.shape == (6, 4, 2)
     assert int8.bytes == 2 * 6 * 4 * 2 * 18
-    for bad in (dict(num_pages=0), dict(page_tokens=0), dict(head_dim=12), dict(head_dim=264), dict(num_pages=2**30), dict(num_pages=1, page_tokens=2**20 + 1),
-                dict(storage_dtype="float16"), dict(storage_dtype="fp8")):
+    for bad in (dict(num_pages=0), dict(page_tokens=0), dict(head_dim=12), dict(head_dim=264), dict(num_pages=2**30),
+                dict(num_pages=1, page_tokens=2**20 + 1), dict(storage_dtype="float16"), dict(storage_dtype="fp8")):
         with pytest.raises(ValueError):
             DeviceKVCache(**{**dict(num_pages=6, page_tokens=4, kv_heads=2, head_dim=16, device="cpu"), **bad})
     with pytest.raises(ValueError, match="float16 or bfloat16"):
@@ -87,10 +87,12 @@ def test_rows_entry_point_rejects_bad_arguments_without_a_gpu():
         (dict(paged, v=0), -1, b"q with q_out"), (dict(paged, slots=0), -1, b"q with q_out"),
         (dict(qt=4), -1, b"multiples of 8"), (dict(q=24), -1, b"aligned"), (dict(q_weight=2), -1, b"aligned"),
         (dict(pairs=33), -1, b"pairs"), (dict(pairs=32), -1, b"positions"), (dict(turned, axes=5), -1, b"axes"),
-        (dict(turned, s0=31), -1, b"add up"), (dict(turned, s0=33), -1, b"add up"), (dict(turned, axes=2), -1, b"add up"),
+        (dict(turned, s0=31), -1, b"add up"), (dict(turned, s0=33), -1, b"add up"),
+        (dict(turned, axes=2), -1, b"add up"),
         (dict(turned, frequencies=4), -1, b"positions"),
-        (dict(paged, page_tokens=0), -1, b"2^31"), (dict(paged, num_pages=1, page_tokens=2**20 + 1), -1, b"2^20"), (dict(paged, num_pages=2**30), -1, b"2^31"),
-        (dict(paged, int8=1), -1, b"scales"), (dict(paged, pp=4), -1, b"aligned"), (dict(paged, slots=4), -1, b"aligned"),
+        (dict(paged, page_tokens=0), -1, b"2^31"), (dict(paged, num_pages=1, page_tokens=2**20 + 1), -1, b"2^20"),
+        (dict(paged, num_pages=2**30), -1, b"2^31"), (dict(paged, int8=1), -1, b"scales"),
+        (dict(paged, pp=4), -1, b"aligned"), (dict(paged, slots=4), -1, b"aligned"),
     ):
         assert lib.sa_normalize_rotate_store(rows_args(**fields), 0, None) == status, fields
         assert word in lib.sa_last_error(), (fields, lib.sa_last_error())
