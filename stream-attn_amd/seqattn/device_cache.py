@@ -46,15 +46,15 @@ class DeviceKVCache:
             raise ValueError("storage_dtype must be 'int8' or the cache's dtype")
         self.dtype = dtype
         self.page_tokens = page_tokens
-        self.device = torch.device(device)
         self.int8 = storage_dtype == "int8"
 
         def pool(shape, pool_dtype):
-            return torch.zeros(shape, dtype=pool_dtype, device=self.device).transpose(1, 2)
+            return torch.zeros(shape, dtype=pool_dtype, device=device).transpose(1, 2)
 
         shape = (num_pages, kv_heads, page_tokens, head_dim)
         stored = torch.int8 if self.int8 else dtype
         self.k_pages, self.v_pages = pool(shape, stored), pool(shape, stored)
+        self.device = self.k_pages.device
         self.k_scales = pool(shape[:3], torch.float16) if self.int8 else None
         self.v_scales = pool(shape[:3], torch.float16) if self.int8 else None
 

@@ -57,8 +57,10 @@ def paged_decode_attention(
     sees no key gets zeros, and LSE ``-inf``.
 
     INT8 pages stand for ``value * scale``.  Logits, softmax and sums are FP32;
-    a weight enters the product with V as two 16-bit parts.  A seen value that is
-    not finite gives NaN.  ``out`` may be ``q``.
+    a weight enters the product with V as two 16-bit parts.  A logit of NaN or
+    ``+inf`` makes its head NaN, one of ``-inf`` is a key without weight; an element
+    of a seen V that is not finite makes its element of ``out`` not finite.
+    ``out`` may be ``q``.
     Returns ``out`` (like ``q``), and with ``return_lse`` also the natural-log
     LSE ``[q_heads, sequences]``.
     """

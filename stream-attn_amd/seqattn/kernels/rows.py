@@ -36,6 +36,11 @@ _READ_ARGS = struct.Struct("=7Q8q6i")
 NO_STRIDES = (0, 0, 0)
 
 
+def _refuse_gradients() -> None:
+    if torch.is_grad_enabled():
+        raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+
+
 def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, *, output: bool = False) -> int:
     """[tokens, heads, head_dim] rows that the kernels can address; their dtype code (0 where ``like`` has it)."""
     if rows.ndim != 3:
@@ -61,12 +66,20 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
         if (tokens > 1 and st < dim) or (heads > 1 and sh < dim) or (
                 tokens > 1 and heads > 1 and st < heads * sh and sh < tokens * st):
             raise ValueError(f"{name} has rows that overlap")
-    elif rows.requires_grad and torch.is_grad_enabled():
-        raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+    elif rows.requires_grad:
+        _refuse_gradients()
     return code
 
 
-def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype) -> bool:
+def _repeats(tensor: torch.Tensor) -> bool:
+    """Whether an expanded dimension has several elements in one place."""
+    strides = tensor.stride()
+    return 0 in strides and any(n > 1 and s == 0 for n, s in zip(tensor.shape, strides))
+
+
+def check_pools(
+    k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype, *, written: bool = False
+) -> bool:
     """Both pools of a cache, on ``like``'s device; whether they hold INT8."""
     shape, strides, stored = k_pages.shape, k_pages.stride(), k_pages.dtype
     if len(shape) != 4:
@@ -85,6 +98,10 @@ def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype:
         raise ValueError("the cache has no pages")
     if shape[1] > MAX_PAGE_TOKENS or shape[0] * shape[1] > 2**31 - 1:
         raise ValueError(f"pages have at most {MAX_PAGE_TOKENS} rows, the cache fewer than 2^31")
+    if k_pages.requires_grad or v_pages.requires_grad:
+        _refuse_gradients()
+    if written and _repeats(k_pages):
+        raise ValueError("rows of written pages must not share memory")
     if not int8:
         if k_scales is not None or v_scales is not None:
             raise ValueError("only INT8 pages have scales")
@@ -98,6 +115,10 @@ def check_pools(k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype:
             raise ValueError("INT8 scales must be float16 [num_pages, page_tokens, kv_heads] on the pages' device")
     if k_scales.stride() != v_scales.stride():
         raise ValueError("k_scales and v_scales must have the same strides")
+    if k_scales.requires_grad or v_scales.requires_grad:
+        _refuse_gradients()
+    if written and _repeats(k_scales):
+        raise ValueError("scales of written pages must not share memory")
     return True
 
 
@@ -122,8 +143,8 @@ def _weight(name: str, weight: torch.Tensor | None, rows: torch.Tensor) -> int:
         raise ValueError(f"{name} must have the rows' dtype or float32")
     if weight.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned")
-    if weight.requires_grad and torch.is_grad_enabled():
-        raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+    if weight.requires_grad:
+        _refuse_gradients()
     return weight.data_ptr()
 
 
@@ -141,6 +162,8 @@ def _rotation(positions, frequencies, sections, pairing, rows: torch.Tensor):
     device = rows.device
     if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or frequencies.device != device:
         raise ValueError("frequencies must be a float64 [pairs] tensor on the rows' device")
+    if frequencies.requires_grad:
+        _refuse_gradients()
     pairs = frequencies.shape[0]
     if not 1 <= pairs <= dim // 2 or (pairs > 1 and frequencies.stride(0) != 1):
         raise ValueError("frequencies must be contiguous, for 1 to head_dim / 2 pairs")
@@ -258,7 +281,7 @@ def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots):
     check_rows("v", v, k)
     if v.shape != k.shape:
         raise ValueError(f"k and v must have identical shapes, got {k.shape} and {v.shape}")
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype)
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype, written=True)
     if k_pages.shape[2:] != k.shape[1:]:
         raise ValueError("the pages' kv_heads and head_dim must be the rows'")
     _check_slots(slots, k.shape[0], k.device)

@@ -374,3 +374,27 @@ def test_refusals():
         read_kv(k8, v8, slots, k_scales=s8, v_scales=t8, dtype=torch.float32)
     with pytest.raises(ValueError, match="needs a weight|both positions"):
         normalize_rotate_append(q, k, k, kp, vp, slots, pos)
+
+
+def test_gradients_and_shared_memory_are_refused():
+    k = torch.zeros((4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    freq, slots = rotary_frequencies(32), torch.arange(4, device="cuda")
+    kp, vp, _, _ = pools(2, 4, 2, 64, torch.bfloat16, "heads", False)
+    k8, v8, s8, t8 = pools(2, 4, 2, 64, torch.bfloat16, "heads", True)
+    learned = freq.clone().requires_grad_()
+    with pytest.raises(ValueError, match="inference-only"):
+        normalize_rotate_qk(k, k, slots, learned)
+    with torch.no_grad():
+        normalize_rotate_qk(k, k, slots, learned)
+    with pytest.raises(ValueError, match="inference-only"):
+        append_kv(k, k, kp, vp.clone().requires_grad_(), slots)
+    with pytest.raises(ValueError, match="inference-only"):
+        read_kv(kp.detach().requires_grad_(), vp, slots)
+    with pytest.raises(ValueError, match="inference-only"):
+        read_kv(k8, v8, slots, k_scales=s8, v_scales=t8.detach().requires_grad_())
+    with pytest.raises(ValueError, match="share memory"):
+        append_kv(k, k, kp[:1].expand(2, 4, 2, 64), vp[:1].expand(2, 4, 2, 64), slots)
+    with pytest.raises(ValueError, match="share memory"):
+        append_kv(k, k, k8, v8, slots, k_scales=s8[..., :1].expand(2, 4, 2), v_scales=t8[..., :1].expand(2, 4, 2))
+    read_kv(kp, kp, slots)
+    read_kv(kp[:1].expand(2, 4, 2, 64), vp[:1].expand(2, 4, 2, 64), slots)
