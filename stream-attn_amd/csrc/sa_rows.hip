@@ -209,18 +209,19 @@ __device__ inline void store_pairs(uint16_t* row, const Unit<F, W>& u, const flo
   }
 }
 
-__device__ inline uint32_t pack_codes(float a, float b, float c, float d) {
-  return ((uint32_t)(int32_t)a & 0xffu) | ((uint32_t)(int32_t)b & 0xffu) << 8 | ((uint32_t)(int32_t)c & 0xffu) << 16 |
-         (uint32_t)(int32_t)d << 24;
+// The low bytes of four words.
+__device__ inline uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
 }
 
 template <Form F, int W, bool kOnce>
-__device__ inline void store_codes(char* row, const Unit<F, W>& u, const float (&a)[W], const float (&b)[W]) {
+__device__ inline void store_codes(char* row, const Unit<F, W>& u, const uint32_t (&a)[W],
+                                   const uint32_t (&b)[W]) {
   if constexpr (F == kScalar) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      row[u.at_lo(i)] = (char)(int32_t)a[i];
-      row[u.at_hi(i)] = (char)(int32_t)b[i];
+      row[u.at_lo(i)] = (char)a[i];
+      row[u.at_hi(i)] = (char)b[i];
     }
   } else if constexpr (F == kAdjacent) {
 #pragma unroll
@@ -276,25 +277,26 @@ __device__ inline uint16_t scale_of(float amax, float step) {
   return (uint16_t)Fp16::pack(amax <= FLT_MAX ? step : NAN, 0.f);
 }
 
-// rint(x / step), with the quotient rounded as a division rounds it: only next to
-// a half do the quotient and the product with the reciprocal (off by less than
-// 127 * 2^-22) round apart.
+// rint(x / step) in the low byte, with the quotient rounded as a division rounds
+// it: only next to a half do the quotient and the product with the reciprocal (off
+// by less than 127 * 2^-22) round apart.  Adding 1.5 * 2^23 rounds to an integer
+// and leaves its two's complement in the low bits.  A finite row's are within 127
+// (its largest magnitude is 127 steps); another's scale is NaN, and that of steps
+// below float16's is 0, whatever the codes.
 template <int N>
-__device__ inline void codes(float (&x)[N], float step, float reciprocal) {
-  float q[N];
-  bool near = false;
+__device__ inline void codes(const float (&x)[N], float step, float reciprocal, uint32_t (&code)[N]) {
+  constexpr float kRound = 12582912.f;
+  float off = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float y = x[i] * reciprocal;
-    q[i] = rintf(y);
-    near = near || fabsf(y - q[i]) > 0.5f - 1.f / 32768;
+    const float y = fmaf(x[i], reciprocal, kRound);
+    code[i] = __builtin_bit_cast(uint32_t, y);
+    off = fmaxf(off, fabsf(fmaf(x[i], reciprocal, kRound - y)));
   }
-  if (__any(near)) {
+  if (__any(off > 0.5f - 1.f / 32768)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = rintf(x[i] / step);
+    for (int i = 0; i < N; ++i) code[i] = __builtin_bit_cast(uint32_t, x[i] / step + kRound);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = fminf(fmaxf(q[i], -127.f), 127.f);
 }
 
 // A wave takes rows of one token (Q's heads, then K's, then V's), 64 >>
@@ -431,9 +433,10 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
       if (active && !is_q && stored) {
         const float step = amax / 127.f > 0.f ? amax / 127.f : 1.f;
         const float reciprocal = 1.f / step;
-        codes(a, step, reciprocal);
-        codes(b, step, reciprocal);
-        store_codes<F, W, kOnce>(pages + at + head * p.kp.sh, u, a, b);
+        uint32_t code_a[W], code_b[W];
+        codes(a, step, reciprocal, code_a);
+        codes(b, step, reciprocal, code_b);
+        store_codes<F, W, kOnce>(pages + at + head * p.kp.sh, u, code_a, code_b);
         if (unit_lane == 0)
           reinterpret_cast<uint16_t*>(choose(mask_v, v_scales, k_scales))[scale_at + head * p.kp.ss_h] =
               scale_of(amax, step);
@@ -513,10 +516,11 @@ __global__ __launch_bounds__(256) void store_kernel(const StoreParams p) {
         const float amax = over_lanes(live ? __builtin_bit_cast(float, min(top, 0x7f800000u)) : 0.f, p.lane_log2,
                                       [](float a, float b) { return fmaxf(a, b); });
         const float step = amax / 127.f > 0.f ? amax / 127.f : 1.f;
-        codes(y, step, 1.f / step);
+        uint32_t code[8];
+        codes(y, step, 1.f / step, code);
         if (!stored) continue;
         *reinterpret_cast<u32x2*>(pages + at) =
-            u32x2{pack_codes(y[0], y[1], y[2], y[3]), pack_codes(y[4], y[5], y[6], y[7])};
+            u32x2{pack_codes(code[0], code[1], code[2], code[3]), pack_codes(code[4], code[5], code[6], code[7])};
         if (g == 0)
           reinterpret_cast<uint16_t*>(choose(is_v[i], (int64_t)p.vp.scale, (int64_t)p.kp.scale))
               [page * p.kp.ss_p + row * p.kp.ss_t + head[i] * p.kp.ss_h] = scale_of(amax, step);
