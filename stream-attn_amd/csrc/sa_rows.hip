@@ -469,7 +469,7 @@ struct StoreParams {
 // leave lanes of a wave without one (rows_kernel), a workgroup has the rows of
 // `each` tokens, four of a thread under way together.  A row's granules (8
 // elements) are on 2^lane_log2 lanes.  60,000 rows of 128, with one K/V head
-// 44 -> 30 us (INT8 66 -> 40), two 28 -> 24; four and more as fast in rows_kernel,
+// 44 -> 30 us (INT8 66 -> 38), two 28 -> 24; four and more as fast in rows_kernel,
 // 56 slower here (186 and 177).
 template <typename T, bool kInt8>
 __global__ __launch_bounds__(256) void store_kernel(const StoreParams p) {
