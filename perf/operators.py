@@ -22,7 +22,6 @@ and benchmark; pages lie in the pool in random order.
 
 from __future__ import annotations
 
-import functools
 import itertools
 import math
 import random
@@ -229,7 +228,6 @@ def prepare(case, seed):
 # ---- the framework's entry points -------------------------------------------
 
 
-@functools.lru_cache
 def _kernels():
     package = str(Path(__file__).resolve().parents[1] / "stream-attn_amd")
     if package not in sys.path:
