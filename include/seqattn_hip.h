@@ -632,8 +632,8 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* args, int32_t device, void
 /*
  * Rows of a page pool as packed K and V: k_out, v_out [tokens, kv_heads,
  * head_dim] (bf16/fp16, contiguous) row t = the pages' row of slots[t], INT8
- * values times their scale; zeros for a slot outside the pool.  16-bit pages
- * have the outputs' type.  Limits as above.
+ * values times their scale; zeros for a slot outside the pool, which has at
+ * least one page.  16-bit pages have the outputs' type.  Limits as above.
  */
 typedef struct {
     const void *k_pages, *v_pages, *k_scales, *v_scales;
@@ -658,9 +658,9 @@ int32_t sa_read_kv(const sa_read_args* args, int32_t device, void* stream);
  *
  * Key j of sequence s is row j % page_tokens of page page_table[s, j /
  * page_tokens].  A length below 0 counts as 0, one past the table's row as the
- * row's keys; keys of a page outside [0, num_pages) are not seen.  A token
- * that sees no key gets output 0 and LSE -inf.  Nothing in rows past a
- * length is used, whatever they hold.
+ * row's keys; keys of a page outside [0, num_pages) are not seen; num_pages is
+ * at least 1.  A token that sees no key gets output 0 and LSE -inf.  Nothing in
+ * rows past a length is used, whatever they hold.
  *
  * `workspace` (sa_paged_decode_workspace_bytes, 16-byte aligned) is the call's
  * own until it has run.  Token strides of the pages are in [0, 2^26).

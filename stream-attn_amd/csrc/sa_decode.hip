@@ -71,6 +71,7 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   const int32_t rc = check(a);
   if (rc != 0) return rc;
   if (a->sequences == 0) return 0;
+  if (a->num_pages < 1) return invalid("the pool must have at least one page");  // the kernel reads page 0 for bad pages
   const int64_t strides[] = {a->stride_qt, a->stride_qh, a->stride_ot, a->stride_oh, a->stride_pp, a->stride_pt,
                              a->stride_ph};
   for (int64_t s : strides)

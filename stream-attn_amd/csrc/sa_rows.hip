@@ -799,6 +799,7 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
       !aligned(a->k_out, 16) || !aligned(a->v_out, 16))
     return invalid(entry, "slots or outputs are missing or not aligned");
   if (a->tokens == 0) return 0;
+  if (a->num_pages < 1) return invalid(entry, "the pool must have at least one page");  // row 0 is read for bad slots
   p.k_out = static_cast<uint16_t*>(a->k_out), p.v_out = static_cast<uint16_t*>(a->v_out);
   p.slots = a->slots, p.tokens = a->tokens;
   p.num_slots = (uint32_t)(a->num_pages * a->page_tokens), p.page_tokens = (uint32_t)a->page_tokens;

@@ -147,3 +147,42 @@ def test_decode_entry_point_rejects_bad_arguments_without_a_gpu():
     # Its sizes alone decide, and calls of one size need the same.
     assert lib.sa_paged_decode_workspace_bytes(args(q=0, k=0, lengths=0), 0, ctypes.byref(needed)) == 0
     assert needed.value >= 0 and needed.value % 16 == 0
+
+
+DECODE_FIELDS = (
+    "q k v ks vs table lengths out lse workspace workspace_bytes qt qh ot oh pp pt ph sp st sh "
+    "table_stride lse_stride num_pages scale sequences max_pages q_heads kv_heads dim page dtype int8").split()
+
+
+def decode_args(**fields):
+    """Arguments of which every refusal but the one asked for is out of the way: the workspace is there and large."""
+    values = dict.fromkeys(DECODE_FIELDS, 0)
+    values.update(q=16, k=16, v=16, table=4, lengths=4, out=16, workspace=16, workspace_bytes=2**40, num_pages=2,
+                  scale=0.1, sequences=1, max_pages=2, q_heads=4, kv_heads=2, dim=64, page=16)
+    values.update(fields)
+    return _DECODE_ARGS.pack(*(values[n] for n in DECODE_FIELDS))
+
+
+READ_FIELDS = "k v ks vs slots ko vo pp pt ph sp st sh tokens pages heads dim page dtype int8 _".split()
+
+
+def read_args(**fields):
+    values = dict.fromkeys(READ_FIELDS, 0)
+    values.update(k=16, v=16, slots=8, ko=16, vo=16, tokens=4, pages=2, heads=2, dim=64, page=4)
+    values.update(fields)
+    return _READ_ARGS.pack(*(values[n] for n in READ_FIELDS))
+
+
+@built
+def test_pools_without_pages_are_refused_where_rows_are_read():
+    """Pages and slots out of range are replaced by row 0 of page 0, which an empty pool does not have."""
+    lib = _native.lib()
+    assert lib.sa_paged_decode(decode_args(num_pages=0), 0, None) == -1
+    assert b"at least one page" in lib.sa_last_error()
+    assert lib.sa_paged_decode(decode_args(num_pages=0, sequences=0), 0, None) == 0
+    assert lib.sa_read_kv(read_args(pages=0), 0, None) == -1
+    assert b"at least one page" in lib.sa_last_error()
+    assert lib.sa_read_kv(read_args(pages=0, tokens=0), 0, None) == 0
+    # The workspace's size does not depend on the pool.
+    needed = ctypes.c_int64()
+    assert lib.sa_paged_decode_workspace_bytes(decode_args(num_pages=0), 0, ctypes.byref(needed)) == 0 < needed.value
