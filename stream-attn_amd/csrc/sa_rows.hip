@@ -377,8 +377,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     for (int i = 0; i < W; ++i) {
       const int pair = u.first + i;
       const float c = angles[wave][0][min(pair, p.pairs - 1)], s = angles[wave][1][min(pair, p.pairs - 1)];
-      cos_t[i] = pair < p.pairs ? c : 1.f;
-      sin_t[i] = pair < p.pairs ? s : 0.f;
+      cos_t[i] = c, sin_t[i] = s;
     }
   }
 
@@ -408,13 +407,21 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
         b[i] *= r * choose(mask_q, wqb[i], choose(mask_v, 1.f, wkb[i]));
       }
     }
-    if (p.pairs > 0 && !is_v) {
+    // Elements past the pairs are passed over, not turned by an angle of zero:
+    // an infinity or NaN there times that angle's sine is NaN in its neighbour.
+    const int turned = p.pairs - u.first;  // of the unit's pairs
+    if (turned > 0 && !is_v) {
+      const auto turn = [&](bool all) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float x = a[i] * cos_t[i] - b[i] * sin_t[i];
-        b[i] = b[i] * cos_t[i] + a[i] * sin_t[i];
-        a[i] = x;
-      }
+        for (int i = 0; i < W; ++i) {
+          const float x = a[i] * cos_t[i] - b[i] * sin_t[i], y = b[i] * cos_t[i] + a[i] * sin_t[i];
+          a[i] = all || i < turned ? x : a[i], b[i] = all || i < turned ? y : b[i];
+        }
+      };
+      if (F == kHalves || p.pairs % W == 0)
+        turn(true);
+      else
+        turn(false);
     }
     if (is_q || p.slots == nullptr) {
       uint16_t* out = reinterpret_cast<uint16_t*>(choose(mask_q, out_q, out_k)) + head * choose(mask_q, sqo_h, sko_h);

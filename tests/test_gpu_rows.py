@@ -398,3 +398,39 @@ def test_gradients_and_shared_memory_are_refused():
         append_kv(k, k, k8, v8, slots, k_scales=s8[..., :1].expand(2, 4, 2), v_scales=t8[..., :1].expand(2, 4, 2))
     read_kv(kp, kp, slots)
     read_kv(kp[:1].expand(2, 4, 2, 64), vp[:1].expand(2, 4, 2, 64), slots)
+
+
+@pytest.mark.parametrize("dim,sections,pairing,dtype", [
+    (128, (32,), "halves", torch.bfloat16),      # 16 elements of a lane
+    (80, (20,), "halves", torch.float16),        # 8
+    (96, (11, 6), "halves", torch.bfloat16),     # element by element
+    (128, (32,), "adjacent", torch.bfloat16),    # 16
+    (24, (5,), "adjacent", torch.float16),       # 8, an odd number of pairs: rotated and other pairs on one lane
+])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan"), -0.0])
+def test_elements_past_the_pairs_stay_as_they_are(dim, sections, pairing, dtype, bad):
+    """Without a norm their bits go through, also next to infinities and NaN, into rows and into pages."""
+    gen = torch.Generator().manual_seed(dim)
+    turned = 2 * sum(sections)
+    fused = rows(gen, dim, 6, dim, dtype=dtype)
+    for t in range(turned, dim):  # token t has one such element in every head
+        fused[t, :, t] = bad
+    freq, pos = rotary_frequencies(sections, device="cpu"), torch.arange(len(sections) * dim).view(len(sections), dim)
+    clean = torch.where(torch.isfinite(fused), fused, torch.zeros_like(fused))
+    q, k, v = fused.cuda().split([3, 2, 1], dim=1)
+    qo, ko = normalize_rotate_qk(q, k, pos.cuda(), freq.cuda(), sections=sections, pairing=pairing)
+    cache = DeviceKVCache(dim // 8, 8, 2, dim, dtype=dtype)
+    slots = torch.arange(dim, device="cuda")
+    v2 = torch.cat([v, v], dim=1)
+    q2 = cache.normalize_rotate_append(q, k, v2, slots, pos.cuda(), freq.cuda(), sections=sections, pairing=pairing)
+    k2, v_back = cache.read(slots)
+    for got, x in ((qo, fused[:, :3]), (q2, fused[:, :3]), (ko, fused[:, 3:5]), (k2, fused[:, 3:5])):
+        past, want = got.cpu()[..., turned:], x[..., turned:]
+        assert torch.equal(torch.isnan(past), torch.isnan(want))
+        assert torch.equal(past.contiguous().view(torch.int16)[~torch.isnan(want)],
+                           want.contiguous().view(torch.int16)[~torch.isnan(want)])
+    for got, start, heads in ((qo, 0, 3), (ko, 3, 2)):
+        ref, size = rotated(clean[:, start : start + heads].double(), pos, freq, sections, pairing)
+        close(got[..., :turned], ref[..., :turned], size[..., :turned], dtype)
+    assert torch.equal(torch.isnan(v_back), torch.isnan(v2))
+    assert torch.equal(v_back.nan_to_num(7.0), v2.nan_to_num(7.0))
