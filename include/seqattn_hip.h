@@ -663,7 +663,8 @@ int32_t sa_read_kv(const sa_read_args* args, int32_t device, void* stream);
  * rows past a length is used, whatever they hold.
  *
  * `workspace` (sa_paged_decode_workspace_bytes, 16-byte aligned) is the call's
- * own until it has run.  Token strides of the pages are in [0, 2^26).
+ * own until it has run.  Token strides of the pages are in [0, 2^26), sequences
+ * at most 2^30.
  */
 typedef struct {
     const void *q, *k_pages, *v_pages, *k_scales, *v_scales;

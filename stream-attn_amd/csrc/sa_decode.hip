@@ -29,6 +29,7 @@ int32_t check(const sa_decode_args* a) {
   }
   if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads > (1 << 16) || a->q_heads % a->kv_heads)
     return invalid("q_heads must be a multiple of kv_heads");
+  if (a->sequences > (1 << 30)) return invalid("at most 2^30 sequences");
   if (a->sequences < 0 || a->max_pages < 0 || a->page_tokens < 1 || a->page_tokens > SA_MAX_PAGE_TOKENS ||
       a->num_pages < 0 || a->num_pages > INT32_MAX / a->page_tokens || a->max_pages > INT32_MAX / a->page_tokens)
     return invalid("page_tokens must be at most 2^20 and pages * page_tokens below 2^31");

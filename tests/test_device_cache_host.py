@@ -186,3 +186,12 @@ def test_pools_without_pages_are_refused_where_rows_are_read():
     # The workspace's size does not depend on the pool.
     needed = ctypes.c_int64()
     assert lib.sa_paged_decode_workspace_bytes(decode_args(num_pages=0), 0, ctypes.byref(needed)) == 0 < needed.value
+
+
+@built
+def test_decode_refuses_more_sequences_than_its_indexes_hold():
+    """A thread's and a workgroup's steps through the sequences would pass 2^31."""
+    lib = _native.lib()
+    for sequences in (2**30 + 1, 2**31 - 1):
+        assert lib.sa_paged_decode(decode_args(sequences=sequences), 0, None) == -1
+        assert b"at most 2^30 sequences" in lib.sa_last_error()
