@@ -350,3 +350,37 @@ def test_refusals():
     refused("device", q, k, v, table, n.cpu())
     refused("inference-only", q.clone().requires_grad_(), k, v, table, n)
     refused("unit stride", q, k.transpose(2, 3), v, table, n)
+
+
+# Every form of the kernel: type, kind of pages, padded head_dim (64, 128, 256), 8 or 16 query heads per item, pages
+# that do and do not end inside 16 keys.  Sequences that a wave has whole, that are split over a workgroup's waves and
+# over workgroups.
+@pytest.mark.parametrize("page", [64, 16, 24])
+@pytest.mark.parametrize("group", [3, 12, 17])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_form(dtype, int8, dim, group, page):
+    gen = torch.Generator().manual_seed(dim + group + page)
+    layout = "tokens" if group == 17 else "heads"
+    check(*make(gen, [1700, 0, 37, 260], group, 1, dim, page, dtype, int8, layout))
+
+
+@pytest.mark.parametrize("group,dim,page,dtype,int8", [
+    (12, 200, 16, torch.bfloat16, False),
+    (16, 248, 40, torch.float16, False),
+    (10, 136, 32, torch.float16, True),
+    (16, 256, 12, torch.bfloat16, True),
+    (12, 96, 16, torch.float16, False),
+    (16, 128, 64, torch.bfloat16, True),
+    (9, 104, 20, torch.float16, True),
+    (16, 56, 16, torch.bfloat16, True),
+    (11, 24, 6, torch.float16, False),
+])
+def test_many_sequences_of_groups_past_eight_heads(group, dim, page, dtype, int8):
+    """More items than workgroups, most of them whole in a wave's run of several tiles, some split."""
+    gen = torch.Generator().manual_seed(group * dim)
+    lengths = torch.randint(0, 90, (700,), generator=gen)
+    lengths[torch.rand(700, generator=gen) < 0.2] = 0
+    lengths[3], lengths[350], lengths[-1] = 3000, 700, 1500
+    check(*make(gen, lengths.tolist(), 2 * group, 2, dim, page, dtype, int8))
