@@ -82,7 +82,8 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
       (a->page_table == nullptr && a->max_pages > 0) ||
       (a->pages_int8 && (a->k_scales == nullptr || a->v_scales == nullptr)) || !aligned(a->q, 16) ||
       !aligned(a->out, 16) || !aligned(a->k_pages, page_align) || !aligned(a->v_pages, page_align) ||
-      !aligned(a->page_table, 4) || !aligned(a->lengths, 4))
+      !aligned(a->page_table, 4) || !aligned(a->lengths, 4) || !aligned(a->lse, 4) || !aligned(a->k_scales, 2) ||
+      !aligned(a->v_scales, 2))
     return invalid("an operand is missing or not aligned");
   if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
     return invalid("the workspace is missing, too small or not aligned");

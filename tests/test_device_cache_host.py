@@ -195,3 +195,11 @@ def test_decode_refuses_more_sequences_than_its_indexes_hold():
     for sequences in (2**30 + 1, 2**31 - 1):
         assert lib.sa_paged_decode(decode_args(sequences=sequences), 0, None) == -1
         assert b"at most 2^30 sequences" in lib.sa_last_error()
+
+
+@built
+def test_decode_refuses_a_misaligned_lse_and_misaligned_scales():
+    lib = _native.lib()
+    for fields in (dict(lse=2), dict(int8=1, ks=2, vs=3), dict(int8=1, ks=5, vs=2)):
+        assert lib.sa_paged_decode(decode_args(**fields), 0, None) == -1
+        assert b"missing or not aligned" in lib.sa_last_error()
