@@ -203,3 +203,38 @@ def test_decode_refuses_a_misaligned_lse_and_misaligned_scales():
     for fields in (dict(lse=2), dict(int8=1, ks=2, vs=3), dict(int8=1, ks=5, vs=2)):
         assert lib.sa_paged_decode(decode_args(**fields), 0, None) == -1
         assert b"missing or not aligned" in lib.sa_last_error()
+
+
+@built
+@pytest.mark.parametrize("fields,status,words", [
+    (dict(dtype=2), -2, b"dtype code 2"),
+    (dict(dim=12), -3, b"head_dim"), (dict(dim=8), -3, b"head_dim"), (dict(dim=264), -3, b"head_dim"),
+    (dict(q_heads=3), -1, b"multiple of kv_heads"), (dict(q_heads=0), -1, b"multiple of kv_heads"),
+    (dict(kv_heads=0), -1, b"multiple of kv_heads"), (dict(q_heads=2**17), -1, b"multiple of kv_heads"),
+    (dict(sequences=-1), -1, b"below 2^31"), (dict(max_pages=-1), -1, b"below 2^31"), (dict(page=0), -1, b"below 2^31"),
+    (dict(num_pages=-1), -1, b"below 2^31"), (dict(num_pages=2**30), -1, b"below 2^31"),
+    (dict(max_pages=2**30), -1, b"below 2^31"), (dict(num_pages=1, max_pages=1, page=2**20 + 1), -1, b"2^20"),
+    *((dict([(s, 4)]), -1, b"strides must be multiples of 8") for s in ("qt", "qh", "ot", "oh", "pp", "pt", "ph")),
+    *((dict([(p, 0)]), -1, b"missing or not aligned") for p in ("q", "k", "v", "out", "lengths", "table")),
+    *((dict([(p, 8)]), -1, b"missing or not aligned") for p in ("q", "k", "v", "out")),
+    (dict(table=2), -1, b"missing or not aligned"), (dict(lengths=2), -1, b"missing or not aligned"),
+    (dict(int8=1), -1, b"missing or not aligned"), (dict(int8=1, ks=2), -1, b"missing or not aligned"),
+    (dict(int8=1, ks=2, vs=2, k=4), -1, b"missing or not aligned"),
+    (dict(workspace=0), -1, b"workspace"), (dict(workspace=8), -1, b"workspace"),
+    (dict(pt=2**26), -1, b"token stride"), (dict(pt=-8), -1, b"token stride"),
+])
+def test_decode_entry_point_names_what_it_refuses(fields, status, words):
+    lib = _native.lib()
+    assert lib.sa_paged_decode(decode_args(**fields), 0, None) == status
+    assert words in lib.sa_last_error() and b"sa_paged_decode" in lib.sa_last_error()
+
+
+@built
+def test_decode_workspace_size_is_checked():
+    lib = _native.lib()
+    for sizes in (dict(), dict(q_heads=32, kv_heads=2), dict(dim=256), dict(int8=1, ks=2, vs=2)):
+        needed = ctypes.c_int64(-1)
+        assert lib.sa_paged_decode_workspace_bytes(decode_args(**sizes), 0, ctypes.byref(needed)) == 0
+        assert needed.value > 0 and needed.value % 16 == 0
+        assert lib.sa_paged_decode(decode_args(workspace_bytes=needed.value - 1, **sizes), 0, None) == -1
+        assert b"workspace" in lib.sa_last_error()
