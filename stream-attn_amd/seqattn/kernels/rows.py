@@ -41,6 +41,16 @@ def _refuse_gradients() -> None:
         raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
 
 
+def _overlap(counts: Sequence[int], strides: Sequence[int], extent: int) -> bool:
+    """Whether pieces of ``extent`` elements can lie over each other: a dimension steps past all that shorter steps span."""
+    for stride, n in sorted(zip(strides, counts)):
+        if n > 1:
+            if stride < extent:
+                return True
+            extent += (n - 1) * stride
+    return False
+
+
 def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, *, output: bool = False) -> int:
     """[tokens, heads, head_dim] rows that the kernels can address; their dtype code (0 where ``like`` has it)."""
     if rows.ndim != 3:
@@ -63,8 +73,7 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
     if heads < 1:
         raise ValueError(f"{name} has no heads")
     if output:
-        if (tokens > 1 and st < dim) or (heads > 1 and sh < dim) or (
-                tokens > 1 and heads > 1 and st < heads * sh and sh < tokens * st):
+        if _overlap((tokens, heads), (st, sh), dim):
             raise ValueError(f"{name} has rows that overlap")
     elif rows.requires_grad:
         _refuse_gradients()

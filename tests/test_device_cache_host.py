@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 
 import pytest
@@ -11,7 +12,7 @@ import torch
 from seqattn import DeviceKVCache, _native, rotary_frequencies
 from seqattn.kernels import append_kv, normalize_rotate_qk, paged_decode_attention, read_kv
 from seqattn.kernels.decode import _DECODE_ARGS
-from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS
+from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS, _overlap
 
 built = pytest.mark.skipif(not _native.library_is_built(), reason="native library not built")
 
@@ -238,3 +239,23 @@ def test_decode_workspace_size_is_checked():
         assert needed.value > 0 and needed.value % 16 == 0
         assert lib.sa_paged_decode(decode_args(workspace_bytes=needed.value - 1, **sizes), 0, None) == -1
         assert b"workspace" in lib.sa_last_error()
+
+
+def test_overlapping_layouts_are_told_from_disjoint_ones():
+    """The rows of a layout, counted element by element."""
+    def shared(counts, strides, extent):
+        places = torch.zeros(4000, dtype=torch.int64)
+        for index in itertools.product(*(range(n) for n in counts)):
+            at = sum(i * s for i, s in zip(index, strides))
+            places[at : at + extent] += 1
+        return bool((places > 1).any())
+
+    disjoint = [((4, 8), (15 * 16, 32), 16),   # every other one of 15 heads
+                ((4, 3), (16, 64), 16), ((4, 3), (48, 16), 16), ((1, 3), (0, 16), 16), ((5, 1), (16, 0), 16),
+                ((0, 3), (0, 16), 16), ((3, 4, 2), (256, 16, 64), 16), ((3, 4, 2), (8, 2, 1), 1)]
+    over = [((4, 8), (14 * 16, 32), 16), ((4, 3), (0, 16), 16), ((4, 3), (16, 0), 16), ((2, 2), (8, 64), 16),
+            ((3, 4, 2), (128, 16, 32), 16), ((3, 4, 2), (192, 16, 48), 16), ((3, 4, 2), (8, 2, 0), 1), ((2, 2, 2), (2, 1, 1), 1)]
+    for layout in disjoint:
+        assert not _overlap(*layout) and not shared(*layout), layout
+    for layout in over:
+        assert _overlap(*layout) and shared(*layout), layout

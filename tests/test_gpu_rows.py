@@ -434,3 +434,18 @@ def test_elements_past_the_pairs_stay_as_they_are(dim, sections, pairing, dtype,
         close(got[..., :turned], ref[..., :turned], size[..., :turned], dtype)
     assert torch.equal(torch.isnan(v_back), torch.isnan(v2))
     assert torch.equal(v_back.nan_to_num(7.0), v2.nan_to_num(7.0))
+
+
+def test_outputs_that_are_every_other_head_of_an_odd_count():
+    """Disjoint rows: the last head of a token ends where the next token starts."""
+    gen = torch.Generator().manual_seed(15)
+    q, k = rows(gen, 9, 8, 64, dtype=torch.bfloat16).cuda(), rows(gen, 9, 2, 64, dtype=torch.bfloat16).cuda()
+    freq, pos = rotary_frequencies(32), torch.arange(9, device="cuda")
+    want, _ = normalize_rotate_qk(q, k, pos, freq)
+    buffer = torch.full((9, 15, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    normalize_rotate_qk(q, k, pos, freq, q_out=buffer[:, ::2])
+    assert torch.equal(buffer[:, ::2], want) and bool((buffer[:, 1::2] == 5).all())
+    # One head fewer to a token: its last row is the next token's first.
+    shared = torch.empty(9 * 15 * 64, dtype=torch.bfloat16, device="cuda").as_strided((9, 8, 64), (14 * 64, 128, 1))
+    with pytest.raises(ValueError, match="overlap"):
+        normalize_rotate_qk(q, k, pos, freq, q_out=shared)
