@@ -20,6 +20,7 @@ into a graph.
 
 from __future__ import annotations
 
+import functools
 import struct
 from collections.abc import Sequence
 
@@ -80,10 +81,7 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
     return code
 
 
-def _repeats(tensor: torch.Tensor) -> bool:
-    """Whether an expanded dimension has several elements in one place."""
-    strides = tensor.stride()
-    return 0 in strides and any(n > 1 and s == 0 for n, s in zip(tensor.shape, strides))
+_layout_overlaps = functools.lru_cache(_overlap)  # of the few layouts of a program's pools
 
 
 def check_pools(
@@ -109,7 +107,7 @@ def check_pools(
         raise ValueError(f"pages have at most {MAX_PAGE_TOKENS} rows, the cache fewer than 2^31")
     if k_pages.requires_grad or v_pages.requires_grad:
         _refuse_gradients()
-    if written and _repeats(k_pages):
+    if written and _layout_overlaps(shape[:3], strides[:3], shape[3]):
         raise ValueError("rows of written pages must not share memory")
     if not int8:
         if k_scales is not None or v_scales is not None:
@@ -126,7 +124,7 @@ def check_pools(
         raise ValueError("k_scales and v_scales must have the same strides")
     if k_scales.requires_grad or v_scales.requires_grad:
         _refuse_gradients()
-    if written and _repeats(k_scales):
+    if written and _layout_overlaps(shape[:3], k_scales.stride(), 1):
         raise ValueError("scales of written pages must not share memory")
     return True
 

@@ -449,3 +449,24 @@ def test_outputs_that_are_every_other_head_of_an_odd_count():
     shared = torch.empty(9 * 15 * 64, dtype=torch.bfloat16, device="cuda").as_strided((9, 8, 64), (14 * 64, 128, 1))
     with pytest.raises(ValueError, match="overlap"):
         normalize_rotate_qk(q, k, pos, freq, q_out=shared)
+
+
+def test_written_pages_of_overlapping_strides_are_refused():
+    k = torch.zeros((4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(4, device="cuda")
+    memory = torch.zeros((2, 4096), dtype=torch.bfloat16, device="cuda")
+    for strides in ((256, 128, 64, 1), (512, 64, 64, 1), (512, 128, 32, 1)):
+        kp, vp = (m.as_strided((2, 4, 2, 64), strides) for m in memory)
+        with pytest.raises(ValueError, match="share memory"):
+            append_kv(k, k, kp, vp, slots)
+        read_kv(kp, vp, slots)
+    k8, v8, _, _ = pools(2, 4, 2, 64, torch.bfloat16, "heads", True)
+    ks, vs = (m.half().as_strided((2, 4, 2), (8, 1, 3)) for m in memory)
+    with pytest.raises(ValueError, match="share memory"):
+        append_kv(k, k, k8, v8, slots, k_scales=ks, v_scales=vs)
+    # Heads of a buffer that others have the rest of.
+    for strides in ((1024, 256, 128, 1), (1024, 64, 256, 1)):
+        kp, vp = (m.as_strided((2, 4, 2, 64), strides) for m in memory)
+        append_kv(k + 1, k + 2, kp, vp, slots)
+        ko, vo = read_kv(kp, vp, slots)
+        assert bool((ko == 1).all()) and bool((vo == 2).all())
