@@ -602,7 +602,8 @@ int32_t sa_run_resident_noalloc(const void* q, const void* k, const void* v, voi
  * strides in multiples of 8; int8 pages 8-byte aligned, strides in multiples of
  * 8.  head_dim is a multiple of 8 in [16, 256], axes at most 4, page_tokens at
  * most SA_MAX_PAGE_TOKENS, num_pages * page_tokens below 2^31.  The rows of one
- * call have distinct slots.  Asynchronous on `stream`, a stream of `device`.
+ * call have distinct slots, and K's and V's pages and scales share no memory.
+ * Asynchronous on `stream`, a stream of `device`.
  */
 #define SA_MAX_ROTARY_AXES 4
 #define SA_MAX_PAGE_TOKENS (1 << 20)

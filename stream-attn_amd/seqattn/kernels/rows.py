@@ -81,13 +81,41 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
     return code
 
 
-_layout_overlaps = functools.lru_cache(_overlap)  # of the few layouts of a program's pools
+def _meet(offset: int, steps: Sequence[tuple[int, int]], extent: int) -> bool:
+    """Whether pieces of two such layouts meet, one ``offset`` behind the other; ``steps``: (stride, count), long ones first."""
+    if not steps:
+        return offset < extent
+    (stride, n), *shorter = steps
+    behind, rest = divmod(offset, stride)
+    return (behind < n and _meet(rest, shorter, extent)) or (behind + 1 < n and _meet(stride - rest, shorter, extent))
+
+
+@functools.lru_cache  # the few layouts of a program's pools
+def _written_layout(offset: int, counts: Sequence[int], strides: Sequence[int], extent: int) -> tuple[bool, bool]:
+    """Whether pieces of a pool overlap, and whether they meet those of the other pool."""
+    if _overlap(counts, strides, extent):
+        return True, True
+    steps = sorted(((s, n) for s, n in zip(strides, counts) if n > 1), reverse=True)
+    return False, _meet(offset, steps, extent)
+
+
+def _check_written(name: str, k: torch.Tensor, v: torch.Tensor, counts, strides, extent: int, same_rows: bool) -> None:
+    offset = abs(v.data_ptr() - k.data_ptr()) // k.element_size()
+    overlap, meet = _written_layout(offset, counts, strides, extent)
+    if overlap:
+        raise ValueError(f"{name} of written pages must not share memory")
+    if meet and not (same_rows and offset == 0):
+        raise ValueError(f"{name} of K's and V's written pages must not share memory")
 
 
 def check_pools(
-    k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype, *, written: bool = False
+    k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype, *, written: bool = False,
+    same_rows: bool = False
 ) -> bool:
-    """Both pools of a cache, on ``like``'s device; whether they hold INT8."""
+    """Both pools of a cache, on ``like``'s device; whether they hold INT8.
+
+    ``written``: rows go into them, into both the same with ``same_rows``.
+    """
     shape, strides, stored = k_pages.shape, k_pages.stride(), k_pages.dtype
     if len(shape) != 4:
         raise ValueError("k_pages must use [num_pages, page_tokens, kv_heads, head_dim] layout")
@@ -107,8 +135,8 @@ def check_pools(
         raise ValueError(f"pages have at most {MAX_PAGE_TOKENS} rows, the cache fewer than 2^31")
     if k_pages.requires_grad or v_pages.requires_grad:
         _refuse_gradients()
-    if written and _layout_overlaps(shape[:3], strides[:3], shape[3]):
-        raise ValueError("rows of written pages must not share memory")
+    if written:
+        _check_written("rows", k_pages, v_pages, shape[:3], strides[:3], shape[3], same_rows)
     if not int8:
         if k_scales is not None or v_scales is not None:
             raise ValueError("only INT8 pages have scales")
@@ -124,8 +152,8 @@ def check_pools(
         raise ValueError("k_scales and v_scales must have the same strides")
     if k_scales.requires_grad or v_scales.requires_grad:
         _refuse_gradients()
-    if written and _layout_overlaps(shape[:3], k_scales.stride(), 1):
-        raise ValueError("scales of written pages must not share memory")
+    if written:
+        _check_written("scales", k_scales, v_scales, shape[:3], k_scales.stride(), 1, same_rows)
     return True
 
 
@@ -284,11 +312,11 @@ def normalize_rotate_qk(
     return q_out, k_out
 
 
-def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots):
+def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, same_rows):
     check_rows("v", v, k)
     if v.shape != k.shape:
         raise ValueError(f"k and v must have identical shapes, got {k.shape} and {v.shape}")
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype, written=True)
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype, written=True, same_rows=same_rows)
     if k_pages.shape[2:] != k.shape[1:]:
         raise ValueError("the pages' kv_heads and head_dim must be the rows'")
     _check_slots(slots, k.shape[0], k.device)
@@ -309,10 +337,12 @@ def append_kv(
 
     A row whose slot is negative (padding) or past the pool is not written.
     The slots of a call are distinct: of two rows with one slot either may
-    stay, in parts.  INT8 pages: a row that is not finite reads back as NaN.
+    stay, in parts.  K's and V's pages share no memory (one pool may be both
+    where ``k`` is ``v``).  INT8 pages: a row that is not finite reads back as NaN.
     """
     code = check_rows("k", k)
-    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    same_rows = k.data_ptr() == v.data_ptr() and k.stride() == v.stride()
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, same_rows)
     _run_rows(None, k, v, None, None, pools, slots, None, None, None, "adjacent", None, None, 0.0, code)
 
 
@@ -342,7 +372,7 @@ def normalize_rotate_append(
     is negative.
     """
     code = _check_qk(q, k)
-    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, False)
     q_out = _output("q_out", q_out, q)
     _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out

@@ -12,7 +12,7 @@ import torch
 from seqattn import DeviceKVCache, _native, rotary_frequencies
 from seqattn.kernels import append_kv, normalize_rotate_qk, paged_decode_attention, read_kv
 from seqattn.kernels.decode import _DECODE_ARGS
-from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS, _overlap
+from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS, _overlap, _written_layout
 
 built = pytest.mark.skipif(not _native.library_is_built(), reason="native library not built")
 
@@ -259,3 +259,20 @@ def test_overlapping_layouts_are_told_from_disjoint_ones():
         assert not _overlap(*layout) and not shared(*layout), layout
     for layout in over:
         assert _overlap(*layout) and shared(*layout), layout
+
+
+@pytest.mark.parametrize("counts,strides,extent", [
+    ((3, 4, 2), (128, 16, 64), 16),   # head by head in a page
+    ((3, 4, 2), (256, 64, 16), 16),   # room behind a token's heads
+    ((3, 4, 2), (256, 16, 128), 16),  # and between the heads
+    ((3, 1, 2), (64, 0, 24), 16),     # pieces with room between them
+    ((2, 3, 2), (10, 1, 5), 1),       # scales
+])
+def test_pools_that_meet_are_told_from_pools_that_do_not(counts, strides, extent):
+    def places(at):
+        starts = [sum(i * s for i, s in zip(index, strides)) for index in itertools.product(*(range(n) for n in counts))]
+        return {at + start + d for start in starts for d in range(extent)}
+
+    first, span = places(0), max(places(0)) + 1
+    for offset in range(0, span + 20):
+        assert _written_layout(offset, counts, strides, extent) == (False, bool(first & places(offset))), offset

@@ -470,3 +470,24 @@ def test_written_pages_of_overlapping_strides_are_refused():
         append_kv(k + 1, k + 2, kp, vp, slots)
         ko, vo = read_kv(kp, vp, slots)
         assert bool((ko == 1).all()) and bool((vo == 2).all())
+
+
+def test_one_pool_as_k_and_v_is_refused_for_different_rows():
+    k, v = (torch.full((4, 2, 64), x, dtype=torch.bfloat16, device="cuda") for x in (1.0, 2.0))
+    freq, slots = rotary_frequencies(32), torch.arange(4, device="cuda")
+    kp, vp, _, _ = pools(2, 4, 2, 64, torch.bfloat16, "heads", False)
+    k8, v8, ks, vs = pools(2, 4, 2, 64, torch.bfloat16, "heads", True)
+    both, wide = pools(3, 4, 2, 64, torch.bfloat16, "heads", False)[0], pools(2, 4, 4, 64, torch.bfloat16, "heads", False)[0]
+    for call in (lambda: append_kv(k, v, kp, kp, slots), lambda: append_kv(k, v, both[:2], both[1:], slots),
+                 lambda: append_kv(k, k, both[:2], both[1:], slots),
+                 lambda: append_kv(k, v, k8, v8, slots, k_scales=ks, v_scales=ks),
+                 lambda: append_kv(k, v, k8, k8, slots, k_scales=ks, v_scales=vs),
+                 lambda: normalize_rotate_append(k, k, k, kp, kp, slots, slots, freq)):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    assert bool((both == 3).all()) and bool((kp == 3).all())
+    # The same rows, and pools that are each other's neighbours.
+    append_kv(k, k, kp, kp, slots)
+    assert bool((kp[0] == 1).all()) and bool((kp[1] == 3).all())
+    append_kv(k, v, wide[:, :, :2], wide[:, :, 2:], slots)
+    assert bool((wide[0, :, :2] == 1).all()) and bool((wide[0, :, 2:] == 2).all()) and bool((wide[1] == 3).all())
