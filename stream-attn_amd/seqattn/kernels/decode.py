@@ -15,7 +15,7 @@ import struct
 import torch
 
 from .. import _native
-from .rows import NO_STRIDES, check_pools, check_rows, new_rows
+from .rows import NO_STRIDES, check_place, check_pools, check_rows, new_rows
 
 # sa_decode_args: 10 pointers, 14 sizes and strides, the scale, 8 int32.
 _DECODE_ARGS = struct.Struct("=10Q14qd8i")
@@ -60,7 +60,7 @@ def paged_decode_attention(
     a weight enters the product with V as two 16-bit parts.  A logit of NaN or
     ``+inf`` makes its head NaN, one of ``-inf`` is a key without weight; an element
     of a seen V that is not finite makes its element of ``out`` not finite.
-    ``out`` may be ``q``.
+    ``out`` may be ``q``, and shares no memory with the rest.
     Returns ``out`` (like ``q``), and with ``return_lse`` also the natural-log
     LSE ``[q_heads, sequences]``.
     """
@@ -88,6 +88,7 @@ def paged_decode_attention(
         check_rows("out", out, q, output=True)
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
+        check_place("out", out, q, (k_pages, v_pages))
     lse = None
     if return_lse:
         lse = torch.empty_strided((q_heads, sequences), (sequences, 1), dtype=torch.float32, device=device)

@@ -157,6 +157,16 @@ def check_pools(
     return True
 
 
+def check_place(name: str, out: torch.Tensor, rows: torch.Tensor, others: Sequence[torch.Tensor | None]) -> None:
+    """An output is apart from ``others``; where ``rows`` are, it is ``rows`` itself."""
+    where = out.data_ptr()
+    if where and any(t is not None and t.data_ptr() == where for t in others):
+        raise ValueError(f"{name} must not share memory with another operand")
+    if where and rows.data_ptr() == where:
+        if any(n > 1 and a != b for n, a, b in zip(out.shape, out.stride(), rows.stride())):
+            raise ValueError(f"{name} must not share memory with its input unless it is its input")
+
+
 def new_rows(tokens: int, heads: int, dim: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """Contiguous [tokens, heads, head_dim] memory (the strided form of torch.empty, which takes less host time)."""
     return torch.empty_strided((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=device)
@@ -266,12 +276,14 @@ def _check_qk(q: torch.Tensor, k: torch.Tensor) -> int:
     return code
 
 
-def _output(name: str, out: torch.Tensor | None, rows: torch.Tensor) -> torch.Tensor:
+def _output(name: str, out: torch.Tensor | None, rows: torch.Tensor, others: Sequence[torch.Tensor | None]) -> torch.Tensor:
+    """The output of ``rows``, which may be ``rows`` itself but none of ``others``."""
     if out is None:
         return new_rows(*rows.shape, rows.dtype, rows.device)
     check_rows(name, out, rows, output=True)
     if out.shape != rows.shape:
         raise ValueError(f"{name} must have the shape of its input")
+    check_place(name, out, rows, others)
     return out
 
 
@@ -302,12 +314,13 @@ def normalize_rotate_qk(
     frequencies).  Without positions and frequencies nothing is rotated.
 
     Returns ``(q_out, k_out)``, new tensors unless given.  An output may be
-    its input itself, but must not otherwise share memory with an input.
+    its input itself, but must not otherwise share memory with an input or the
+    other output.
     """
     code = _check_qk(q, k)
     if positions is None and frequencies is None and q_weight is None and k_weight is None:
         raise ValueError("normalize_rotate_qk needs a weight or a rotation")
-    q_out, k_out = _output("q_out", q_out, q), _output("k_out", k_out, k)
+    q_out, k_out = _output("q_out", q_out, q, (k, k_out)), _output("k_out", k_out, k, (q,))
     _run_rows(q, k, None, q_out, k_out, None, None, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out, k_out
 
@@ -369,11 +382,11 @@ def normalize_rotate_append(
 
     Returns the normalized and rotated Q.  INT8 pages take K before it is
     rounded to 16 bits.  Q is written for every token, also where a row's slot
-    is negative.
+    is negative; ``q_out`` may be ``q``, and shares no memory with the rest.
     """
     code = _check_qk(q, k)
     pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, False)
-    q_out = _output("q_out", q_out, q)
+    q_out = _output("q_out", q_out, q, (k, v))
     _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out
 

@@ -384,3 +384,12 @@ def test_many_sequences_of_groups_past_eight_heads(group, dim, page, dtype, int8
     lengths[torch.rand(700, generator=gen) < 0.2] = 0
     lengths[3], lengths[350], lengths[-1] = 3000, 700, 1500
     check(*make(gen, lengths.tolist(), 2 * group, 2, dim, page, dtype, int8))
+
+
+def test_an_output_in_the_place_of_other_operands_is_refused():
+    gen = torch.Generator().manual_seed(14)
+    q, _, _, table, n, (k, v), _ = make(gen, [20, 5, 3, 40], 4, 4, 64, 4, torch.bfloat16, layout="tokens")
+    q, table, n = q.cuda(), table.cuda(), n.cuda()
+    for out in (k[:4, 0], v[:4, 0], q.transpose(0, 1)):  # [pages, heads, head_dim] rows of the pools
+        with pytest.raises(ValueError, match="share memory"):
+            paged_decode_attention(q, k, v, table, n, out=out)

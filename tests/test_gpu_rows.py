@@ -491,3 +491,26 @@ def test_one_pool_as_k_and_v_is_refused_for_different_rows():
     assert bool((kp[0] == 1).all()) and bool((kp[1] == 3).all())
     append_kv(k, v, wide[:, :, :2], wide[:, :, 2:], slots)
     assert bool((wide[0, :, :2] == 1).all()) and bool((wide[0, :, 2:] == 2).all()) and bool((wide[1] == 3).all())
+
+
+def test_outputs_in_the_place_of_other_operands_are_refused():
+    gen = torch.Generator().manual_seed(16)
+    q, k, v = (rows(gen, 4, 4, 64, dtype=torch.bfloat16).cuda() for _ in range(3))
+    freq, pos = rotary_frequencies(32), torch.arange(4, device="cuda")
+    spare, held = torch.empty_like(q), q.clone()
+    kp, vp, _, _ = pools(1, 4, 4, 64, torch.bfloat16, "heads", False)
+    for outs in (dict(q_out=k), dict(k_out=q), dict(q_out=k, k_out=q), dict(q_out=spare, k_out=spare),
+                 dict(q_out=q.transpose(0, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            normalize_rotate_qk(q, k, pos, freq, **outs)
+    for out in (k, v):
+        with pytest.raises(ValueError, match="share memory"):
+            normalize_rotate_append(q, k, v, kp, vp, pos, pos, freq, q_out=out)
+    assert torch.equal(q, held)
+    want = normalize_rotate_qk(q, k, pos, freq)
+    normalize_rotate_append(q, k, v, kp, vp, pos, pos, freq, q_out=spare)
+    assert torch.equal(spare, want[0])
+    normalize_rotate_qk(q, k, pos, freq, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    # Nothing lies anywhere without tokens.
+    normalize_rotate_qk(q[:0], k[:0], pos[:0], freq, q_out=q[:0], k_out=q[:0])
