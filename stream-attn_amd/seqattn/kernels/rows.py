@@ -76,7 +76,7 @@ def check_rows(name: str, rows: torch.Tensor, like: torch.Tensor | None = None, 
     if output:
         if _overlap((tokens, heads), (st, sh), dim):
             raise ValueError(f"{name} has rows that overlap")
-    elif rows.requires_grad:
+    if rows.requires_grad:
         _refuse_gradients()
     return code
 

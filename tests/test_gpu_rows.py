@@ -16,7 +16,7 @@ import pytest
 import torch
 
 from seqattn import DeviceKVCache, rotary_frequencies
-from seqattn.kernels import append_kv, normalize_rotate_append, normalize_rotate_qk, read_kv
+from seqattn.kernels import append_kv, normalize_rotate_append, normalize_rotate_qk, paged_decode_attention, read_kv
 from paged_reference import HALF_STEP, normalized, quantized, rotated
 
 pytestmark = pytest.mark.gpu
@@ -514,3 +514,23 @@ def test_outputs_in_the_place_of_other_operands_are_refused():
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
     # Nothing lies anywhere without tokens.
     normalize_rotate_qk(q[:0], k[:0], pos[:0], freq, q_out=q[:0], k_out=q[:0])
+
+
+def test_outputs_that_require_gradients_are_refused():
+    q = torch.ones((4, 4, 64), dtype=torch.bfloat16, device="cuda")
+    freq, pos = rotary_frequencies(32), torch.arange(4, device="cuda")
+    learned = torch.zeros_like(q).requires_grad_()
+    kp, vp, _, _ = pools(1, 4, 4, 64, torch.bfloat16, "heads", False)
+    table, n = torch.zeros((4, 1), dtype=torch.int32, device="cuda"), torch.ones(4, dtype=torch.int32, device="cuda")
+    calls = (lambda: normalize_rotate_qk(q, q, pos, freq, q_out=learned),
+             lambda: normalize_rotate_qk(q, q, pos, freq, k_out=learned),
+             lambda: normalize_rotate_append(q, q, q, kp, vp, pos, pos, freq, q_out=learned),
+             lambda: paged_decode_attention(q, kp, vp, table, n, out=learned))
+    for call in calls:
+        with pytest.raises(ValueError, match="inference-only"):
+            call()
+        assert bool((learned == 0).all())
+        with torch.no_grad():
+            call()
+            assert not bool((learned == 0).all())
+            learned.zero_()
