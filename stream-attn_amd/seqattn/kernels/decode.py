@@ -15,7 +15,7 @@ import struct
 import torch
 
 from .. import _native
-from .rows import NO_STRIDES, check_place, check_pools, check_rows, new_rows
+from .rows import NO_STRIDES, check_place, check_pools, check_rows, new_rows, refuse_tangents
 
 # sa_decode_args: 10 pointers, 14 sizes and strides, the scale, 8 int32.
 _DECODE_ARGS = struct.Struct("=10Q14qd8i")
@@ -64,6 +64,7 @@ def paged_decode_attention(
     Returns ``out`` (like ``q``), and with ``return_lse`` also the natural-log
     LSE ``[q_heads, sequences]``.
     """
+    refuse_tangents(q, k_pages, v_pages, k_scales, v_scales, out)
     code = check_rows("q", q)
     int8 = check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
     sequences, q_heads, dim = q.shape

@@ -25,6 +25,7 @@ import struct
 from collections.abc import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -40,6 +41,13 @@ NO_STRIDES = (0, 0, 0)
 def _refuse_gradients() -> None:
     if torch.is_grad_enabled():
         raise ValueError("seqattn is inference-only: call it under torch.no_grad() or with detached tensors")
+
+
+def refuse_tangents(*operands: torch.Tensor | None) -> None:
+    """Forward-mode tangents would be lost (torch.no_grad() does not turn them off)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # -1: none can be there
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
+            raise ValueError("seqattn is inference-only: call it with detached tensors inside forward_ad.dual_level()")
 
 
 def _overlap(counts: Sequence[int], strides: Sequence[int], extent: int) -> bool:
@@ -317,6 +325,7 @@ def normalize_rotate_qk(
     its input itself, but must not otherwise share memory with an input or the
     other output.
     """
+    refuse_tangents(q, k, frequencies, q_weight, k_weight, q_out, k_out)
     code = _check_qk(q, k)
     if positions is None and frequencies is None and q_weight is None and k_weight is None:
         raise ValueError("normalize_rotate_qk needs a weight or a rotation")
@@ -353,6 +362,7 @@ def append_kv(
     stay, in parts.  K's and V's pages share no memory (one pool may be both
     where ``k`` is ``v``).  INT8 pages: a row that is not finite reads back as NaN.
     """
+    refuse_tangents(k, v, k_pages, v_pages, k_scales, v_scales)
     code = check_rows("k", k)
     same_rows = k.data_ptr() == v.data_ptr() and k.stride() == v.stride()
     pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, same_rows)
@@ -384,6 +394,7 @@ def normalize_rotate_append(
     rounded to 16 bits.  Q is written for every token, also where a row's slot
     is negative; ``q_out`` may be ``q``, and shares no memory with the rest.
     """
+    refuse_tangents(q, k, v, k_pages, v_pages, frequencies, q_weight, k_weight, k_scales, v_scales, q_out)
     code = _check_qk(q, k)
     pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, False)
     q_out = _output("q_out", q_out, q, (k, v))
@@ -405,6 +416,7 @@ def read_kv(
     INT8 rows come as ``value * scale`` in ``dtype`` (default bfloat16), others
     in the pages' own dtype.  A slot outside the pool gives zeros.
     """
+    refuse_tangents(k_pages, v_pages, k_scales, v_scales)
     if dtype is None:
         dtype = torch.bfloat16 if k_pages.dtype == torch.int8 else k_pages.dtype
     code = _native.dtype_code(dtype)

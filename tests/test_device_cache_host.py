@@ -8,9 +8,10 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from seqattn import DeviceKVCache, _native, rotary_frequencies
-from seqattn.kernels import append_kv, normalize_rotate_qk, paged_decode_attention, read_kv
+from seqattn.kernels import append_kv, normalize_rotate_append, normalize_rotate_qk, paged_decode_attention, read_kv
 from seqattn.kernels.decode import _DECODE_ARGS
 from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS, _overlap, _written_layout
 
@@ -276,3 +277,31 @@ def test_pools_that_meet_are_told_from_pools_that_do_not(counts, strides, extent
     first, span = places(0), max(places(0)) + 1
     for offset in range(0, span + 20):
         assert _written_layout(offset, counts, strides, extent) == (False, bool(first & places(offset))), offset
+
+
+def test_forward_mode_tangents_are_refused():
+    """Before any other check, so that host tensors show it."""
+    x, w = torch.zeros((2, 2, 16), dtype=torch.bfloat16), torch.zeros(16)
+    pool, scales = torch.zeros((2, 4, 2, 16), dtype=torch.bfloat16), torch.zeros((2, 4, 2), dtype=torch.float16)
+    i, n, freq = torch.zeros(2, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), rotary_frequencies(8, device="cpu")
+    calls = {
+        normalize_rotate_qk: dict(q=x, k=x, positions=i, frequencies=freq, q_weight=w, k_weight=w, q_out=x, k_out=x),
+        append_kv: dict(k=x, v=x, k_pages=pool, v_pages=pool, slots=i, k_scales=scales, v_scales=scales),
+        normalize_rotate_append: dict(q=x, k=x, v=x, k_pages=pool, v_pages=pool, slots=i, positions=i, frequencies=freq,
+                                      q_weight=w, k_weight=w, k_scales=scales, v_scales=scales, q_out=x),
+        read_kv: dict(k_pages=pool, v_pages=pool, slots=i, k_scales=scales, v_scales=scales),
+        paged_decode_attention: dict(q=x, k_pages=pool, v_pages=pool, page_table=n[:, None], lengths=n, k_scales=scales,
+                                     v_scales=scales, out=x),
+    }
+    with forward_ad.dual_level(), torch.no_grad():
+        for function, arguments in calls.items():
+            with pytest.raises(ValueError, match="device tensors"):
+                function(**arguments)
+            for name, t in arguments.items():
+                if not t.is_floating_point():
+                    continue
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(ValueError, match="inference-only"):
+                    function(**{**arguments, name: dual})
+                with pytest.raises(ValueError, match="device tensors"):
+                    function(**{**arguments, name: dual.detach()})
