@@ -15,6 +15,14 @@ from seqattn.kernels import append_kv, normalize_rotate_append, normalize_rotate
 from seqattn.kernels.decode import _DECODE_ARGS
 from seqattn.kernels.rows import _READ_ARGS, _ROWS_ARGS, _overlap, _written_layout
 
+@pytest.fixture(autouse=True)
+def no_error_left():
+    """A refusal's text stays until the next call of the library."""
+    yield
+    if _native.library_is_built():
+        assert _native.lib().sa_paged_decode(decode_args(sequences=0), 0, None) == 0
+
+
 built = pytest.mark.skipif(not _native.library_is_built(), reason="native library not built")
 
 
