@@ -43,7 +43,7 @@ struct RowsParams {
   int64_t pos_axis, pos_token, token0, tokens;
   float eps, inv_dim;
   uint32_t num_slots, page_tokens;
-  int32_t q_heads, kv_heads, head_dim, pairs, axes;
+  int32_t q_heads, kv_heads, head_dim, pairs;
   int32_t end0, end1, end2;  // first pair past axis 0, 1, 2
   int32_t heads;             // rows of a token: Q's, K's and V's
   int32_t lane_log2;         // log2 of the lanes of a head
@@ -240,8 +240,9 @@ __device__ inline void store_codes(char* row, const Unit<F, W>& u, const uint32_
   }
 }
 
-// A sum or maximum over the 2^n lanes of a head: exchanges within 4 lanes, then
-// mirrored halves of 8 and 16 (whose quarters hold one value by then).
+// A sum or maximum over the 2^n lanes of a head, at most 32 (256 elements, 8 or
+// more on a lane): exchanges within 4 lanes, then mirrored halves of 8 and 16
+// (whose quarters hold one value by then).
 template <int kControl>
 __device__ inline float exchanged(float x) {
   const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xf, 0xf, true);
@@ -254,7 +255,6 @@ __device__ inline float over_lanes(float x, int lane_log2, Join join) {
   if (lane_log2 > 2) x = join(x, exchanged<0x141>(x));
   if (lane_log2 > 3) x = join(x, exchanged<0x140>(x));
   if (lane_log2 > 4) x = join(x, __shfl_xor(x, 16));
-  if (lane_log2 > 5) x = join(x, __shfl_xor(x, 32));
   return x;
 }
 
@@ -769,7 +769,7 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* s
   p.eps = (float)a->eps, p.inv_dim = 1.f / (float)a->head_dim;
   p.q_heads = has_q ? a->q_heads : 0, p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
   p.heads = p.q_heads + p.kv_heads * (pages ? 2 : 1);
-  p.pairs = a->pairs, p.axes = a->axes;
+  p.pairs = a->pairs;
   p.end0 = ends[0], p.end1 = ends[1], p.end2 = ends[2];
   p.pos64 = a->positions_int64, p.qw32 = a->q_weight_fp32, p.kw32 = a->k_weight_fp32;
   DeviceGuard guard(device);
