@@ -534,3 +534,61 @@ def test_outputs_that_require_gradients_are_refused():
             call()
             assert not bool((learned == 0).all())
             learned.zero_()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_pools_past_32_bit_offsets_hold_k_and_v_apart(int8):
+    """K in the first, V in the last heads of one buffer of more than 2^32 elements: rows written, read and attended."""
+    pages, page, heads, dim = 32800, 64, 8, 128
+    both, _, scales, _ = pools(pages, page, 2 * heads, dim, torch.bfloat16, "heads", int8)
+    assert both.numel() > 2**32
+    kp, vp = both[:, :, :heads], both[:, :, heads:]
+    options = dict(k_scales=scales[:, :, :heads], v_scales=scales[:, :, heads:]) if int8 else {}
+    gen = torch.Generator().manual_seed(17)
+    k, v = (rows(gen, 130, heads, dim, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.tensor([[pages - 1, 2, pages - 2]], dtype=torch.int32)
+    at = torch.arange(130)
+    slots = (table[0, at // page].long() * page + at % page).cuda()
+    append_kv(k.cuda(), v.cuda(), kp, vp, slots, **options)
+    ko, vo = read_kv(kp, vp, slots, **options)
+    near = DeviceKVCache(3, page, heads, dim, storage_dtype="int8" if int8 else None)
+    near.append(k.cuda(), v.cuda(), at.cuda())
+    want_k, want_v = near.read(at.cuda())
+    assert torch.equal(ko, want_k) and torch.equal(vo, want_v)
+    if not int8:
+        assert torch.equal(ko.cpu(), k) and torch.equal(vo.cpu(), v)
+    page_of, row = slots // page, slots % page
+    assert torch.equal(both[page_of, row], torch.cat([near.k_pages, near.v_pages], dim=2)[at // page, at % page])
+    # The rows around them hold what they held.
+    assert bool((both[pages - 2, 2:] == 3).all()) and bool((both[1] == 3).all()) and bool((both[pages - 3] == 3).all())
+    q = rows(gen, 1, 4 * heads, dim, dtype=torch.bfloat16).cuda()
+    lengths = torch.tensor([130], dtype=torch.int32, device="cuda")
+    got = paged_decode_attention(q, kp, vp, table.cuda(), lengths, **options)
+    assert torch.equal(got, near.attend(q, torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda"), lengths))
+    del both, kp, vp, scales, options
+    torch.cuda.empty_cache()
+
+
+def test_launches_of_more_than_2_to_the_23_tokens_go_in_parts():
+    tokens, dim, page = 2**23 + 5, 16, 64
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    q, k, v = (torch.randn((tokens, 1, dim), generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3))
+    freq, pos = rotary_frequencies(8), torch.arange(tokens, device="cuda")
+    half = tokens // 2
+    parts = [normalize_rotate_qk(q[i], k[i], pos[i], freq) for i in (slice(0, half), slice(half, tokens))]
+    want_q, want_k = (torch.cat(x) for x in zip(*parts))
+    del parts
+    cache = DeviceKVCache(tokens // page + 1, page, 1, dim)
+    got_q = cache.normalize_rotate_append(q, k, v, pos, pos, freq)
+    assert torch.equal(got_q, want_q)
+    ko, vo = cache.read(pos)
+    assert torch.equal(ko, want_k) and torch.equal(vo, v)
+    got_q, got_k = normalize_rotate_qk(q, k, pos, freq)
+    assert torch.equal(got_q, want_q) and torch.equal(got_k, want_k)
+    cache.append(v, k, pos)
+    ko, vo = cache.read(pos)
+    assert torch.equal(ko, v) and torch.equal(vo, k)
+    last = cache.read(torch.arange(tokens, cache.num_pages * page, device="cuda"))
+    assert all(bool((x == 0).all()) for x in last)
+    del q, k, v, pos, want_q, want_k, cache, got_q, got_k, ko, vo
+    torch.cuda.empty_cache()
