@@ -409,13 +409,20 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams p) {
     }
     // Elements past the pairs are passed over, not turned by an angle of zero:
     // an infinity or NaN there times that angle's sine is NaN in its neighbour.
+    // Where a unit has both kinds, by the lanes that a pair's instructions run
+    // on (the asm keeps the compiler from selections, two more per pair: 40,000
+    // tokens of 32 heads of 80, half of each turned, 95 us, with them 101).
     const int turned = p.pairs - u.first;  // of the unit's pairs
     if (turned > 0 && !is_v) {
       const auto turn = [&](bool all) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const float x = a[i] * cos_t[i] - b[i] * sin_t[i], y = b[i] * cos_t[i] + a[i] * sin_t[i];
-          a[i] = all || i < turned ? x : a[i], b[i] = all || i < turned ? y : b[i];
+          if (all || i < turned) {
+            const float x = a[i] * cos_t[i] - b[i] * sin_t[i];
+            b[i] = b[i] * cos_t[i] + a[i] * sin_t[i];
+            a[i] = x;
+            if (!all) asm volatile("" : "+v"(a[i]), "+v"(b[i]));
+          }
         }
       };
       if (F == kHalves || p.pairs % W == 0)
