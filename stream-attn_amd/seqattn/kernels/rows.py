@@ -107,22 +107,25 @@ def _written_layout(offset: int, counts: Sequence[int], strides: Sequence[int], 
     return False, _meet(offset, steps, extent)
 
 
-def _check_written(name: str, k: torch.Tensor, v: torch.Tensor, counts, strides, extent: int, same_rows: bool) -> None:
+def _check_written(name: str, k: torch.Tensor, v: torch.Tensor, counts, strides, extent: int, rows) -> None:
     offset = abs(v.data_ptr() - k.data_ptr()) // k.element_size()
     overlap, meet = _written_layout(offset, counts, strides, extent)
     if overlap:
         raise ValueError(f"{name} of written pages must not share memory")
-    if meet and not (same_rows and offset == 0):
-        raise ValueError(f"{name} of K's and V's written pages must not share memory")
+    if meet:
+        # The same rows may go to one place.
+        same = rows is not None and rows[0].data_ptr() == rows[1].data_ptr() and rows[0].stride() == rows[1].stride()
+        if offset or not same:
+            raise ValueError(f"{name} of K's and V's written pages must not share memory")
 
 
 def check_pools(
     k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype, *, written: bool = False,
-    same_rows: bool = False
+    rows: tuple[torch.Tensor, torch.Tensor] | None = None
 ) -> bool:
     """Both pools of a cache, on ``like``'s device; whether they hold INT8.
 
-    ``written``: rows go into them, into both the same with ``same_rows``.
+    ``written``: rows go into them, those of ``rows`` as they are where it is given.
     """
     shape, strides, stored = k_pages.shape, k_pages.stride(), k_pages.dtype
     if len(shape) != 4:
@@ -144,7 +147,7 @@ def check_pools(
     if k_pages.requires_grad or v_pages.requires_grad:
         _refuse_gradients()
     if written:
-        _check_written("rows", k_pages, v_pages, shape[:3], strides[:3], shape[3], same_rows)
+        _check_written("rows", k_pages, v_pages, shape[:3], strides[:3], shape[3], rows)
     if not int8:
         if k_scales is not None or v_scales is not None:
             raise ValueError("only INT8 pages have scales")
@@ -161,7 +164,7 @@ def check_pools(
     if k_scales.requires_grad or v_scales.requires_grad:
         _refuse_gradients()
     if written:
-        _check_written("scales", k_scales, v_scales, shape[:3], k_scales.stride(), 1, same_rows)
+        _check_written("scales", k_scales, v_scales, shape[:3], k_scales.stride(), 1, rows)
     return True
 
 
@@ -334,11 +337,11 @@ def normalize_rotate_qk(
     return q_out, k_out
 
 
-def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, same_rows):
+def _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, rows):
     check_rows("v", v, k)
     if v.shape != k.shape:
         raise ValueError(f"k and v must have identical shapes, got {k.shape} and {v.shape}")
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype, written=True, same_rows=same_rows)
+    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, k, k.dtype, written=True, rows=rows)
     if k_pages.shape[2:] != k.shape[1:]:
         raise ValueError("the pages' kv_heads and head_dim must be the rows'")
     _check_slots(slots, k.shape[0], k.device)
@@ -364,8 +367,7 @@ def append_kv(
     """
     refuse_tangents(k, v, k_pages, v_pages, k_scales, v_scales)
     code = check_rows("k", k)
-    same_rows = k.data_ptr() == v.data_ptr() and k.stride() == v.stride()
-    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, same_rows)
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, (k, v))
     _run_rows(None, k, v, None, None, pools, slots, None, None, None, "adjacent", None, None, 0.0, code)
 
 
@@ -396,7 +398,7 @@ def normalize_rotate_append(
     """
     refuse_tangents(q, k, v, k_pages, v_pages, frequencies, q_weight, k_weight, k_scales, v_scales, q_out)
     code = _check_qk(q, k)
-    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, False)
+    pools = _check_append(k, v, k_pages, v_pages, k_scales, v_scales, slots, None)
     q_out = _output("q_out", q_out, q, (k, v))
     _run_rows(q, k, v, q_out, None, pools, slots, positions, frequencies, sections, pairing, q_weight, k_weight, eps, code)
     return q_out
