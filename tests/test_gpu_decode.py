@@ -393,3 +393,37 @@ def test_an_output_in_the_place_of_other_operands_is_refused():
     for out in (k[:4, 0], v[:4, 0], q.transpose(0, 1)):  # [pages, heads, head_dim] rows of the pools
         with pytest.raises(ValueError, match="share memory"):
             paged_decode_attention(q, k, v, table, n, out=out)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lengths,at", [([100, 40], 70), ([5000, 3], 70), ([5000, 3], 4999), ([33, 1], 32)])
+def test_logits_that_are_not_numbers_stay_in_their_head(int8, lengths, at):
+    """NaN or +inf: NaN for the head, split over waves and workgroups or not; -inf: a key without weight."""
+    gen = torch.Generator().manual_seed(at)
+    q, pools, scales, table, n, dev, dev_scales = make(gen, lengths, 8, 2, 64, 16, torch.bfloat16, int8)
+    page, row = int(table[0, at // 16]), at % 16
+    bad = (0, 1, 2, 3, 5)
+    if int8:  # a NaN scale: NaN logits of the K/V head's four query heads
+        scales[0][page, row, 0] = math.nan
+        dev_scales[0][page, row, 0] = math.nan
+    else:
+        pools[0][page, row, 0, 7] = math.inf
+        dev[0][page, row, 0, 7] = math.inf
+        q[0, :4, 7] = torch.tensor([1.0, -1.0, 0.0, 0.25])  # +inf, -inf, NaN, +inf
+        bad = (0, 2, 3, 5)
+    q[0, 5, 3] = math.nan
+    out, lse = paged_decode_attention(q.cuda(), *dev, table.cuda(), n.cuda(), k_scales=dev_scales[0],
+                                      v_scales=dev_scales[1], return_lse=True)
+    out, lse = out.cpu().double(), lse.cpu().double()
+    for h in range(8):
+        if h in bad:
+            assert bool(torch.isnan(out[0, h]).all()) and math.isnan(lse[h, 0])
+    good = [h for h in range(8) if h not in bad]
+    ref, ref_lse, size, _ = attention(q, *pools, table, n, 64**-0.5, *scales)
+    for s, heads in ((0, good), (1, range(8))):
+        for h in heads:
+            # Logits of at most 64 products of numbers below 8: e is below 68 * 2^-24 * 2^12 / 8.
+            e = 2.0**-9
+            bound = 2.0**-8 * ref[s, h].abs() + (1 + 2.0**-8) * (2 * e + 2.0**-15) * size[s, h] + 2.0**-25
+            assert bool(((out[s, h] - ref[s, h]).abs() <= bound).all())
+            assert abs(float(lse[h, s] - ref_lse[h, s])) <= e + 2.0**-19 * (1 + abs(float(ref_lse[h, s])))
