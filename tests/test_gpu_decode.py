@@ -427,3 +427,47 @@ def test_logits_that_are_not_numbers_stay_in_their_head(int8, lengths, at):
             bound = 2.0**-8 * ref[s, h].abs() + (1 + 2.0**-8) * (2 * e + 2.0**-15) * size[s, h] + 2.0**-25
             assert bool(((out[s, h] - ref[s, h]).abs() <= bound).all())
             assert abs(float(lse[h, s] - ref_lse[h, s])) <= e + 2.0**-19 * (1 + abs(float(ref_lse[h, s])))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_whole_step_captured_with_a_padded_sequence(int8):
+    """Slots, norm, rotation, append and attention in one graph, replayed while sequences grow, against the same calls
+    made eagerly on another cache; the last sequence is padding (no page, no key)."""
+    gen = torch.Generator().manual_seed(15)
+    q_heads, kv_heads, dim, page, count = 12, 2, 64, 8, 4
+    caches = [DeviceKVCache(24, page, kv_heads, dim, storage_dtype="int8" if int8 else None) for _ in range(2)]
+    table = torch.full((count, 6), -1, dtype=torch.int32, device="cuda")
+    free = torch.randperm(24, generator=gen).tolist()
+    lengths = torch.zeros(count, dtype=torch.int32, device="cuda")
+    positions, sequences = torch.zeros(count, dtype=torch.int64, device="cuda"), torch.arange(count, device="cuda")
+    freq, w = rotary_frequencies(32), torch.ones(dim, device="cuda")
+    fused = torch.zeros((count, q_heads + 2 * kv_heads, dim), dtype=torch.bfloat16, device="cuda")
+    q, k, v = fused.split([q_heads, kv_heads, kv_heads], dim=1)
+
+    def step(cache):
+        slots = cache.slots(table, sequences, positions)
+        turned = cache.normalize_rotate_append(q, k, v, slots, positions, freq, q_weight=w, k_weight=w)
+        return turned, *cache.attend(turned, table, lengths, return_lse=True)
+
+    stream, spare = torch.cuda.Stream(), DeviceKVCache(1, page, kv_heads, dim, storage_dtype="int8" if int8 else None)
+    with torch.cuda.stream(stream):
+        step(spare)  # nothing is in the table yet: nothing is written
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(caches[0])
+    for j in range(20):
+        fused.copy_(torch.randn(fused.shape, generator=gen))
+        for s in range(count - 1):
+            if j % page == 0:
+                table[s, j // page] = free.pop()
+            positions[s], lengths[s] = j, j + 1
+        positions[-1] = j
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(caches[1])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), j
+        assert bool((got[1][-1] == 0).all()) and bool((got[2][:, -1] == -math.inf).all())
+        assert bool(torch.isfinite(got[2][:, :-1]).all())
+    for a, b in ((caches[0].k_pages, caches[1].k_pages), (caches[0].v_pages, caches[1].v_pages)):
+        assert torch.equal(a, b)
