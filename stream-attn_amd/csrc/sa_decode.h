@@ -14,9 +14,11 @@ constexpr int kDecodeWaves = 4;  // wavefronts of a workgroup
 constexpr int kDecodeTile = 32;  // keys of a wave's step
 // Workgroups of a CU, by the registers that a wave takes (512 of a SIMD lane).
 // INT8 pages are half the bytes for more vector work per key, so that more
-// waves pay where they fit: head_dim 64, 1.5 M keys of 8 heads 453 us with two,
-// 292 with four; head_dim 128 with 16 query heads, 700,000 keys 433 with one,
-// 375 with two.  With spills they do not (16-bit pages there 443 and 522).
+// waves pay: head_dim 64, 1.5 M keys of 8 heads 453 us with two, 292 with four;
+// head_dim 128 with 16 query heads per K/V head, 700,000 keys of 8 heads 435 with
+// one, 383 with two, also though two leave it 3 to 5 registers short (16 to 24
+// bytes of scratch); with 9 query heads 433 and 369.  16-bit pages there, with more
+// to spill, 443 and 522.
 constexpr int decode_occupancy(int padded_dim, int blocks, bool int8) {
   if (padded_dim == 256 || (padded_dim == 128 && blocks == 2 && !int8)) return 1;
   return int8 && padded_dim == 64 && blocks == 1 ? 4 : 2;

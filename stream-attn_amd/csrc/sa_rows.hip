@@ -669,8 +669,11 @@ constexpr int64_t kWavesToFill = 4096;
 constexpr int64_t kCacheBytes = 256 << 20;
 // A token's steps (64 >> lane_log2 rows each) from which two or four waves of
 // a workgroup take them in turn, so that rows that lie together are read
-// together: 14 steps, 61,312 tokens 647 us with one wave, 606 with two, 586 (6.0 TB/s)
-// with four; 6 steps, 20,011 tokens 88.7, 87.2 and 99.
+// together.  Heads of 128, with one wave, two and four, us:
+//   61,312 tokens of 5 steps 217, 220, 264; of 6 266, 252, 295; of 8 362, 335, 351;
+//   of 11 512, 466, 456; of 12 562, 512, 492; of 14 683, 609, 586 (6.0 TB/s);
+//   20,011 tokens of 5 steps 78, 78, 94; of 6 94, 89, 102; of 12 188, 177, 170;
+//   20,011 tokens with the append, of 5 78, 77, 95; of 6 89, 87, 104; of 12 190, 175, 169.
 constexpr int32_t kTwoBeside = 6, kFourBeside = 12;
 
 template <typename T, bool kInt8, bool kOnce>
