@@ -23,7 +23,7 @@ QKVProjector = Callable[[torch.Tensor, int, int], tuple[torch.Tensor, torch.Tens
 OutputProjector = Callable[[torch.Tensor, int, int], torch.Tensor]
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)  # by identity: tensors have no truth value of their equality
 class QKRotation:
     """Norm and rotation of the projected Q and K (no counterpart in the reference).
 

@@ -55,3 +55,10 @@ def test_projected_stats_totals():
     stats.attention.d2h_bytes = 7
     totals = stats.as_dict()
     assert totals["total_h2d_bytes"] == 15 and totals["total_d2h_bytes"] == 37
+
+
+def test_rotations_are_compared_and_hashed_by_identity():
+    """Their tensors have no single truth value, and sections may be a list."""
+    make = lambda: seqattn.QKRotation(positions=torch.arange(3), frequencies=torch.ones(2), sections=[1, 1])  # noqa: E731
+    a, b = make(), make()
+    assert a == a and a != b and b in [a, b] and len({a, b, a}) == 2
