@@ -631,9 +631,51 @@ typedef struct {
 int32_t sa_normalize_rotate_store(const sa_rows_args* args, int32_t device, void* stream);
 
 /*
+ * What pages hold.  e4m3 pages (OCP, 8-byte aligned, strides in multiples of 8)
+ * have an E8M0 scale, the byte 127 + e for 2^e, per block of block_tokens rows
+ * and K/V head: [num_pages, page_tokens / block_tokens, kv_heads], strides in
+ * bytes.  block_tokens is a power of two from 16 on that divides page_tokens.
+ */
+#define SA_PAGES_ROWS 0 /* rows of the operands' type */
+#define SA_PAGES_INT8 1
+#define SA_PAGES_E4M3 2
+
+/*
+ * K and V rows quantised into e4m3 pages: the last rows of every sequence.
+ *
+ *   k, v [tokens, kv_heads, head_dim]   bf16/fp16, packed sequence by sequence
+ *   page_table [sequences, max_pages]   int32, page of rows page_tokens * i .. of a sequence
+ *   lengths [sequences]                 int32, the sequence's rows with the new ones
+ *   cu_tokens [sequences + 1]           int32, non-decreasing from 0: sequence s has rows
+ *                                       cu_tokens[s] .. of k and v; NULL: one row each
+ *
+ * The scale of a block and head is the smallest 2^e, e >= -126, of which 448
+ * reach the magnitude of every finite element that the call writes there, and
+ * at least the scale it has where the block has rows before the first new one;
+ * those are rounded again where it grows.  A value is rounded to nearest even
+ * in units of its scale; one that is not finite becomes NaN.  Rows at positions
+ * below 0 or past the table, and those whose page is outside the pool, are not
+ * written; rows of k and v past cu_tokens[sequences] are not read.  A page that
+ * a call writes to belongs to one sequence, and K's and V's pages and scales
+ * share no memory.
+ */
+typedef struct {
+    const void *k, *v;
+    void *k_pages, *v_pages, *k_scales, *v_scales;
+    const int32_t *page_table, *lengths, *cu_tokens;
+    int64_t stride_kt, stride_kh, stride_vt, stride_vh;
+    int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
+    int64_t stride_sp, stride_sb, stride_sh; /* of their scales */
+    int64_t stride_table, tokens, num_pages;
+    int32_t sequences, max_pages, kv_heads, head_dim, page_tokens, block_tokens, dtype, reserved;
+} sa_append_blocks_args;
+
+int32_t sa_append_kv_blocks(const sa_append_blocks_args* args, int32_t device, void* stream);
+
+/*
  * Rows of a page pool as packed K and V: k_out, v_out [tokens, kv_heads,
- * head_dim] (bf16/fp16, contiguous) row t = the pages' row of slots[t], INT8
- * values times their scale; zeros for a slot outside the pool, which has at
+ * head_dim] (bf16/fp16, contiguous) row t = the pages' row of slots[t], INT8 and
+ * e4m3 values times their scale; zeros for a slot outside the pool, which has at
  * least one page.  16-bit pages have the outputs' type.  Limits as above.
  */
 typedef struct {
@@ -641,9 +683,11 @@ typedef struct {
     const int64_t* slots;
     void *k_out, *v_out;
     int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
-    int64_t stride_sp, stride_st, stride_sh; /* of their scales */
+    int64_t stride_sp, stride_st, stride_sh; /* of their scales (e4m3: stride_st of a block) */
     int64_t tokens, num_pages;
-    int32_t kv_heads, head_dim, page_tokens, dtype, pages_int8, reserved;
+    int32_t kv_heads, head_dim, page_tokens, dtype;
+    int32_t pages_int8;   /* SA_PAGES_* */
+    int32_t block_tokens; /* e4m3 */
 } sa_read_args;
 
 int32_t sa_read_kv(const sa_read_args* args, int32_t device, void* stream);
@@ -688,6 +732,21 @@ int32_t sa_paged_decode(const sa_decode_args* args, int32_t device, void* stream
 
 /* Workspace bytes of a call (its sizes only; pointers and strides are not read). */
 int32_t sa_paged_decode_workspace_bytes(const sa_decode_args* args, int32_t device, int64_t* bytes);
+
+/*
+ * sa_paged_decode over pages of any kind (base.pages_int8: SA_PAGES_*), with a
+ * sliding window: the token at position p = length - 1 sees the keys j with
+ * p - j < window, and the first `sinks` keys of its sequence.  window 0: every
+ * key (sinks 0 then).  Pages whose keys are all hidden are not looked up.
+ */
+typedef struct {
+    sa_decode_args base;
+    int32_t window, sinks;
+    int32_t block_tokens; /* e4m3 */
+    int32_t reserved;
+} sa_window_decode_args;
+
+int32_t sa_paged_window_decode(const sa_window_decode_args* args, int32_t device, void* stream);
 
 /* hipStream_t of the pipeline's H2D (which == 0) or D2H (which == 1) copy stream. */
 void* sa_pipeline_stream(sa_pipeline* pipeline, int32_t which);

@@ -19,9 +19,9 @@ constexpr int kDecodeTile = 32;  // keys of a wave's step
 // one, 383 with two, also though two leave it 3 to 5 registers short (16 to 24
 // bytes of scratch); with 9 query heads 433 and 369.  16-bit pages there, with more
 // to spill, 443 and 522.
-constexpr int decode_occupancy(int padded_dim, int blocks, bool int8) {
-  if (padded_dim == 256 || (padded_dim == 128 && blocks == 2 && !int8)) return 1;
-  return int8 && padded_dim == 64 && blocks == 1 ? 4 : 2;
+constexpr int decode_occupancy(int padded_dim, int blocks, bool bytes) {
+  if (padded_dim == 256 || (padded_dim == 128 && blocks == 2 && !bytes)) return 1;
+  return bytes && padded_dim == 64 && blocks == 1 ? 4 : 2;
 }
 constexpr int kDecodeCUs = 256;
 constexpr int kMaxWorkgroups = 4 * kDecodeCUs;
@@ -48,6 +48,8 @@ struct DecodeParams {
   int32_t sequences, num_pages, max_pages, head_dim, page_tokens, room;  // room: keys of a table row
   int32_t by_item;
   int32_t kv_heads, group, blocks;  // blocks: items of a K/V head
+  int32_t window, sinks;            // every key: window INT32_MAX
+  int32_t block_log2;               // e4m3: rows of a block
   int32_t step_pages, step_rows;    // a tile in pages and rows
   uint32_t page_magic, page_shift;  // key / page_tokens = key * magic >> shift
 };
@@ -55,7 +57,8 @@ struct DecodeParams {
 struct DecodeLaunch {
   DecodeParams p;
   int32_t workgroups;
-  bool bf16, int8;
+  bool bf16;
+  PageKind kind;
   bool wide;      // 16 query heads per item instead of 8
   bool any_page;  // pages that end inside 16 keys
   hipStream_t stream;

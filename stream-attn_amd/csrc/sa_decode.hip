@@ -65,25 +65,31 @@ int32_t sa_paged_decode_workspace_bytes(const sa_decode_args* a, int32_t device,
   return rc;
 }
 
-int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) try {
-  using namespace sa;
-  clear_error();
-  if (a == nullptr) return invalid("null arguments");
+}  // extern "C"
+
+namespace sa {
+namespace {
+
+// window INT32_MAX: every key.
+int32_t run(const sa_decode_args* a, PageKind kind, int32_t window, int32_t sinks, int32_t block_tokens, int32_t device,
+            void* stream) {
   const int32_t rc = check(a);
   if (rc != 0) return rc;
+  const int32_t log2 = kind == kE4m3Pages ? block_log2(block_tokens, a->page_tokens) : 0;
+  if (log2 < 0) return invalid("block_tokens must be a power of two from 16 on that divides page_tokens");
   if (a->sequences == 0) return 0;
   if (a->num_pages < 1) return invalid("the pool must have at least one page");  // the kernel reads page 0 for bad pages
   const int64_t strides[] = {a->stride_qt, a->stride_qh, a->stride_ot, a->stride_oh, a->stride_pp, a->stride_pt,
                              a->stride_ph};
   for (int64_t s : strides)
     if (s % 8) return invalid("strides must be multiples of 8 elements");
-  const int64_t page_align = a->pages_int8 ? 8 : 16;
+  const int64_t page_align = kind != kRowPages ? 8 : 16;
   if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->lengths == nullptr ||
       (a->page_table == nullptr && a->max_pages > 0) ||
-      (a->pages_int8 && (a->k_scales == nullptr || a->v_scales == nullptr)) || !aligned(a->q, 16) ||
+      (kind != kRowPages && (a->k_scales == nullptr || a->v_scales == nullptr)) || !aligned(a->q, 16) ||
       !aligned(a->out, 16) || !aligned(a->k_pages, page_align) || !aligned(a->v_pages, page_align) ||
-      !aligned(a->page_table, 4) || !aligned(a->lengths, 4) || !aligned(a->lse, 4) || !aligned(a->k_scales, 2) ||
-      !aligned(a->v_scales, 2))
+      !aligned(a->page_table, 4) || !aligned(a->lengths, 4) || !aligned(a->lse, 4) ||
+      (kind != kE4m3Pages && (!aligned(a->k_scales, 2) || !aligned(a->v_scales, 2))))
     return invalid("an operand is missing or not aligned");
   if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
     return invalid("the workspace is missing, too small or not aligned");
@@ -117,7 +123,8 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + owned_bytes(a));
   launch.workgroups = workgroups(a);
   p.by_item = (int64_t)a->sequences * p.kv_heads * p.blocks <= launch.workgroups;
-  launch.bf16 = a->dtype == SA_DTYPE_BF16, launch.int8 = a->pages_int8 != 0;
+  p.window = window, p.sinks = sinks, p.block_log2 = log2;
+  launch.bf16 = a->dtype == SA_DTYPE_BF16, launch.kind = kind;
   launch.any_page = a->page_tokens % 16 != 0;
   launch.stream = static_cast<hipStream_t>(stream);
   DeviceGuard guard(device);
@@ -126,8 +133,32 @@ int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) t
   (width == 64 ? launch_decode_d64 : width == 128 ? launch_decode_d128 : launch_decode_d256)(launch);
   SA_HIP_RETURN(hipGetLastError());
   return 0;
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" {
+
+int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) try {
+  sa::clear_error();
+  if (a == nullptr) return sa::invalid("null arguments");
+  return sa::run(a, a->pages_int8 ? sa::kInt8Pages : sa::kRowPages, INT32_MAX, 0, 0, device, stream);
 } catch (const std::exception& error) {
   return sa::exception_status("sa_paged_decode", error);
+}
+
+int32_t sa_paged_window_decode(const sa_window_decode_args* a, int32_t device, void* stream) try {
+  sa::clear_error();
+  if (a == nullptr) return sa::invalid("null arguments");
+  const int32_t kind = a->base.pages_int8;
+  if (kind < sa::kRowPages || kind > sa::kE4m3Pages) return sa::invalid("unknown kind of pages");
+  if (a->window < 0 || a->sinks < 0 || (a->window == 0 && a->sinks > 0))
+    return sa::invalid("window and sinks must not be negative, and sinks need a window");
+  return sa::run(&a->base, (sa::PageKind)kind, a->window > 0 ? a->window : INT32_MAX, a->sinks, a->block_tokens, device,
+                 stream);
+} catch (const std::exception& error) {
+  return sa::exception_status("sa_paged_window_decode", error);
 }
 
 }  // extern "C"

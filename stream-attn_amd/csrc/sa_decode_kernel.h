@@ -109,17 +109,26 @@ __device__ inline float other_half(float x) {
 // 2^x of a running maximum's change: 0 from -inf, 1 where nothing changes.
 __device__ inline float ratio(float from, float to) { return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to); }
 
+// A sequence's tiles that hold a key that its token sees: all, or those up to
+// its sinks' last and those from its window's first, `skip` tiles later.
+struct Tiles {
+  int32_t count, sinks, skip;
+};
+
 // A wave's share of one item: tiles first .. last - 1 of the item's `tiles`.
 struct Piece {
   int64_t start;  // the launch's tile that is the item's first
   const int32_t* table;
   int32_t s, length, tiles, first, last;
+  int32_t jump, skip;  // tile t is the sequence's tile t + (t < jump ? 0 : skip)
   int32_t kv_head, block;  // query heads 8 NB block .. of the K/V head's group
 
   __device__ inline void bound(int64_t end) {  // as far as a run up to `end` goes
     const int64_t left = end - start;
     last = left < tiles ? (int32_t)left : tiles;
   }
+  __device__ inline void has(const Tiles& t) { tiles = t.count, jump = t.sinks, skip = t.skip; }
+  __device__ inline int32_t key_of(int32_t tile) const { return (tile + (tile < jump ? 0 : skip)) * kDecodeTile; }
 };
 
 // The kernel's arguments, read again where they are used: what only a piece's
@@ -136,7 +145,15 @@ __device__ inline int32_t length_of(Arguments a, int s) {
   const int32_t n = a->lengths[s];
   return n < a->room ? n : a->room;
 }
-__device__ inline int32_t tiles_of(int32_t length) { return length > 0 ? (length - 1) / kDecodeTile + 1 : 0; }
+__device__ inline Tiles tiles_of(Arguments a, int32_t length) {
+  if (length <= 0) return {0, 0, 0};
+  const int32_t all = (length - 1) / kDecodeTile + 1;
+  if (length <= a->window) return {all, 0, 0};
+  const int32_t low = length - a->window;  // the window's first key
+  const int32_t first = a->sinks < low ? a->sinks : low, sinks = first > 0 ? (first - 1) / kDecodeTile + 1 : 0;
+  const int32_t between = low / kDecodeTile - sinks;
+  return between > 0 ? Tiles{all - between, sinks, between} : Tiles{all, 0, 0};
+}
 
 // Where a wave's next load is: a tile of a piece, in row `row` of the
 // sequence's page number `page`.
@@ -159,14 +176,19 @@ struct Reader {
 
   __device__ inline void enter(const DecodeParams& p) {  // at the piece's first tile
     tile = x.first;
-    page = uniform((int32_t)((uint64_t)(uint32_t)(tile * kDecodeTile) * p.page_magic >> p.page_shift));
-    row = tile * kDecodeTile - page * p.page_tokens;
-    first_id = page - 64;
+    first_id = -64;
+    find(p);
+  }
+  __device__ inline void find(const DecodeParams& p) {
+    const int32_t key = x.key_of(tile);
+    page = uniform((int32_t)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift));
+    row = key - page * p.page_tokens;
   }
 
   // To the next tile of a run up to tile `end` of the launch, which has one.
   __device__ inline void advance(const DecodeParams& p, int64_t end) {
     if (++tile < x.last) {
+      if (tile == x.jump) return find(p);
       page += p.step_pages, row += p.step_rows;
       if (row >= p.page_tokens) ++page, row -= p.page_tokens;
       return;
@@ -180,7 +202,7 @@ struct Reader {
       x.kv_head = 0;
       do x.length = uniform(length_of(a, ++x.s));
       while (x.length <= 0);
-      x.tiles = tiles_of(x.length);
+      x.has(tiles_of(a, x.length));
       x.table = a->table + x.s * a->s_table;
     }
     x.bound(end);
@@ -189,13 +211,16 @@ struct Reader {
 };
 
 // A wave's loads of one step, in flight while the step before is computed.
-template <bool kInt8, int DP, bool kAnyPage>
+template <PageKind kKind, int DP, bool kAnyPage>
 struct Step {
+  static_assert(kKind != kE4m3Pages || !kAnyPage, "e4m3 pages are blocks of 16 keys and more");
   static constexpr int EL = Shape<DP>::EL, NP = Shape<DP>::NP;
-  static constexpr int RW = kInt8 ? EL / 4 : EL / 2;  // dwords of a granule
-  static constexpr int ES = kInt8 ? 1 : 2;            // bytes of an element
+  static constexpr int RW = kKind == kRowPages ? EL / 2 : EL / 4;  // dwords of a granule
+  static constexpr int ES = kKind == kRowPages ? 2 : 1;            // bytes of an element
   Dwords<RW> k[8][NP], v[8][NP];
-  uint32_t scale;  // INT8: lane g's of K (g < 8) or V, key 4 (g % 8) + j
+  // INT8: lane g's of K (g < 8) or V, key 4 (g % 8) + j.  e4m3: of K or V, keys
+  // 16 (g / 4 % 2) .. + 15.
+  uint32_t scale;
   uint32_t seen;   // bit t: key 4t + j has weight
   bool full;       // all 32 keys have
   Piece x;       // whose keys they are
@@ -204,7 +229,7 @@ struct Step {
   __device__ __attribute__((always_inline)) void load(const DecodeParams& p, Reader& from, int lane) {
     x = from.x, tile = from.tile;
     const int j = lane >> 4, g = lane & 15;
-    const int32_t key0 = tile * kDecodeTile;
+    const int32_t key0 = x.key_of(tile);
     int32_t page = from.page, row = from.row;
     const char *kh = p.k + x.kv_head * p.sh * ES, *vh = p.v + x.kv_head * p.sh * ES;
     uint32_t at[NP];
@@ -213,7 +238,7 @@ struct Step {
     const bool second = g >= 8;
     if constexpr (!kAnyPage) {
       // Two runs of 16 keys, each in one page.
-      full = x.length - key0 >= kDecodeTile;
+      full = within(p, key0);
       const uint32_t rows = j * (uint32_t)p.st * ES;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -231,9 +256,13 @@ struct Step {
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int c = 0; c < NP; ++c) v[4 * h + u][c] = load_dwords<RW>(vh + base + 4 * u * p.st * ES, rows + at[c]);
-        if constexpr (kInt8) {
+        if constexpr (kKind == kInt8Pages) {
           const uint16_t* s = (second ? p.vs : p.ks) + id * p.ssp + row * p.sst + x.kv_head * p.ssh;
           if ((g >> 2 & 1) == h) scale = s[(4 * (g & 3) + j) * p.sst];
+        }
+        if constexpr (kKind == kE4m3Pages) {
+          const uint8_t* s = reinterpret_cast<const uint8_t*>(second ? p.vs : p.ks);
+          if ((g >> 2 & 1) == h) scale = s[id * p.ssp + (row >> p.block_log2) * p.sst + x.kv_head * p.ssh];
         }
         const uint32_t mask = ok ? 15u : 0u;
         seen = h == 0 ? mask : seen | mask << 4;
@@ -255,16 +284,23 @@ struct Step {
 #pragma unroll
         for (int c = 0; c < NP; ++c)
           k[t][c] = load_dwords<RW>(kh + base, at[c]), v[t][c] = load_dwords<RW>(vh + base, at[c]);
-        if constexpr (kInt8)
+        if constexpr (kKind == kInt8Pages)
           if ((g & 7) == t) scale = (second ? p.vs : p.ks)[id * p.ssp + r * p.sst + x.kv_head * p.ssh];
       }
-      full = __all(seen == 255u) && x.length - key0 >= kDecodeTile;
+      full = __all(seen == 255u) && within(p, key0);
     }
-    if (x.length - key0 < kDecodeTile) {
+    if (!within(p, key0)) {
+      const int32_t low = x.length - p.window;
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
-        if (key0 + 4 * t + j >= x.length) seen &= ~(1u << t);
+      for (int t = 0; t < 8; ++t) {
+        const int32_t key = key0 + 4 * t + j;
+        if (key >= x.length || (key < low && key >= p.sinks)) seen &= ~(1u << t);
+      }
     }
+  }
+  // Whether all of a tile's keys are the sequence's and in its window, or sinks.
+  __device__ inline bool within(const DecodeParams& p, int32_t key0) const {
+    return x.length - key0 >= kDecodeTile && (key0 >= x.length - p.window || key0 + kDecodeTile <= p.sinks);
   }
 };
 
@@ -279,11 +315,13 @@ struct PartInfo {
 // Every wave has an equal run of the launch's tiles.  Items that lie whole in
 // it are done there; the others' parts meet in LDS, and those of items that
 // leave the workgroup's run in the workspace.
-template <typename T, bool kInt8, int DP, int NB, bool kAnyPage>
-__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8)) void decode_kernel(
+template <typename T, PageKind kKind, int DP, int NB, bool kAnyPage>
+__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kKind != kRowPages)) void decode_kernel(
     const DecodeParams p) {
+  constexpr bool kInt8 = kKind == kInt8Pages, kE4m3 = kKind == kE4m3Pages;
   using S = Shape<DP>;
-  using PT = std::conditional_t<kInt8, Bf16, T>;  // INT8: weights times V's scales, beyond float16's range
+  // With scales: weights times V's, beyond float16's range.
+  using PT = std::conditional_t<kKind == kRowPages, T, Bf16>;
   constexpr int EL = S::EL, NP = S::NP, NI = S::NI, NC = S::NC;
   constexpr float bias = kBias<PT>;
   constexpr int kRow = 2 * DP;  // bytes of a key in LDS
@@ -308,7 +346,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
     const int run = (a->sequences + 64 * kDecodeWaves - 1) / (64 * kDecodeWaves);
     const int s_first = tid * run, s_last = s_first + run < a->sequences ? s_first + run : a->sequences;
     int64_t own = 0;
-    for (int s = s_first; s < s_last; ++s) own += tiles_of(length_of(a, s));
+    for (int s = s_first; s < s_last; ++s) own += tiles_of(a, length_of(a, s)).count;
     int64_t upto = own;  // inclusive
     for (int i = 1; i < 64; i <<= 1) {
       const int64_t x = __shfl_up(upto, i);
@@ -331,7 +369,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
       int64_t before = upto - own;
       int s = s_first;
       for (; s < s_last; ++s) {
-        const int64_t n = tiles_of(length_of(a, s));
+        const int64_t n = tiles_of(a, length_of(a, s)).count;
         if (at < (before + n) * items) break;
         before += n;
       }
@@ -358,13 +396,13 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
   float* scales = reinterpret_cast<float*>(mine + kDecodeTile * kRow);
   if (begin < end) {
     Reader reader;
-    Step<kInt8, DP, kAnyPage> step;
+    Step<kKind, DP, kAnyPage> step;
     {
       const Arguments a = arguments();
       Piece& x = reader.x;
       x.s = uniform((int)found[wave][0]);
       x.length = uniform(length_of(a, x.s));
-      x.tiles = tiles_of(x.length);
+      x.has(tiles_of(a, x.length));
       const int64_t into = begin - found[wave][1];
       const int item = uniform((int)(into / x.tiles));
       x.start = found[wave][1] + (int64_t)item * x.tiles;
@@ -424,6 +462,12 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
             for (int i = 0; i < EL / 2; ++i)
               x[i] = T::pack(byte_float(step.k[t][c].w[i / 2], 2 * (i & 1)),
                              byte_float(step.k[t][c].w[i / 2], 2 * (i & 1) + 1));
+          } else if constexpr (kE4m3) {
+#pragma unroll
+            for (int i = 0; i < EL / 2; i += 2) {
+              x[i] = T::template e4m3_pair<false>(step.k[t][c].w[i / 2], 1.f);
+              x[i + 1] = T::template e4m3_pair<true>(step.k[t][c].w[i / 2], 1.f);
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < EL / 2; ++i) x[i] = step.k[t][c].w[i];
@@ -436,6 +480,15 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
       }
       // K's scales with the softmax's.
       if constexpr (kInt8) scales[16 * j + g] = Fp16::lo(step.scale) * (g < 8 ? p.scale_log2 : 1.f);
+      f32x2 k_scales, v_scales;  // e4m3: of the two runs of 16 keys
+      if constexpr (kE4m3) {
+        const int held = __builtin_bit_cast(int, e8m0_value(step.scale));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          k_scales[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(held, 4 * h)) * p.scale_log2;
+          v_scales[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(held, 8 + 4 * h));
+        }
+      }
       const bool full = step.full;
       const uint32_t seen = step.seen;
       // Rows without weight may hold anything: 0 * NaN is not 0.
@@ -455,7 +508,14 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
         for (int i = 0; i < EL; ++i)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            if constexpr (kInt8)
+            if constexpr (kE4m3) {
+              // Elements i and i + 1 of both keys in one dword.
+              if (i & 1) continue;
+              const uint32_t both = __builtin_amdgcn_perm(step.v[2 * u + 1][c].w[i / 4], step.v[2 * u][c].w[i / 4],
+                                                          i & 2 ? 0x07030602u : 0x05010400u);
+              vt[EL * c + i][u] = PT::template e4m3_pair<false>(both, 1.f);
+              vt[EL * c + i + 1][u] = PT::template e4m3_pair<true>(both, 1.f);
+            } else if constexpr (kInt8)
               vt[EL * c + i][u] = PT::pack(byte_float(step.v[2 * u][c].w[i / 4], i & 3),
                                            byte_float(step.v[2 * u + 1][c].w[i / 4], i & 3));
             else
@@ -486,6 +546,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
         factors[0] = *reinterpret_cast<const f32x4*>(scales + 16 * j);
         factors[1] = *reinterpret_cast<const f32x4*>(scales + 16 * j + 4);
       }
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) factors[h] = f32x4{k_scales[h], k_scales[h], k_scales[h], k_scales[h]};
+      }
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float y[8], top = -INFINITY;
@@ -509,10 +573,13 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
           for (int i = 0; i < NI; ++i) acc[n][i] *= keep;
         }
         f32x4 vs[2];
-        if constexpr (kInt8) {
+        if constexpr (kKind != kRowPages) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            vs[b] = *reinterpret_cast<const f32x4*>(scales + 16 * j + 8 + 4 * b);
+            if constexpr (kInt8)
+              vs[b] = *reinterpret_cast<const f32x4*>(scales + 16 * j + 8 + 4 * b);
+            else
+              vs[b] = f32x4{v_scales[b], v_scales[b], v_scales[b], v_scales[b]};
             if (!full)
 #pragma unroll
               for (int e = 0; e < 4; ++e) vs[b][e] = seen >> (4 * b + e) & 1 ? vs[b][e] : 0.f;
@@ -525,7 +592,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kInt8))
         for (int u = 0; u < 4; ++u) {
           float a = __builtin_amdgcn_exp2f(y[2 * u] - base), b = __builtin_amdgcn_exp2f(y[2 * u + 1] - base);
           l[n] += a + b;
-          if constexpr (kInt8) a *= vs[u / 2][2 * (u & 1)], b *= vs[u / 2][2 * (u & 1) + 1];
+          if constexpr (kKind != kRowPages) a *= vs[u / 2][2 * (u & 1)], b *= vs[u / 2][2 * (u & 1) + 1];
           const uint32_t high = PT::pack(a, b);
           weights[u] = PT::pack(a - low * PT::lo(high), b - low * PT::hi(high));
         }
@@ -719,12 +786,14 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const DecodeParams p
     p.lse[head * p.lse_h + s] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
 }
 
-template <typename T, bool kInt8, int DP, int NB>
+template <typename T, PageKind kKind, int DP, int NB>
 void launch_decode(const DecodeLaunch& l) {
-  if (l.any_page)
-    decode_kernel<T, kInt8, DP, NB, true><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
+  if constexpr (kKind == kE4m3Pages)
+    decode_kernel<T, kKind, DP, NB, false><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
+  else if (l.any_page)
+    decode_kernel<T, kKind, DP, NB, true><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
   else
-    decode_kernel<T, kInt8, DP, NB, false><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
+    decode_kernel<T, kKind, DP, NB, false><<<l.workgroups, 64 * kDecodeWaves, 0, l.stream>>>(l.p);
   const int heads = l.p.group < 8 * NB ? l.p.group : 8 * NB;
   const int entries = l.p.by_item ? l.p.sequences * l.p.kv_heads * l.p.blocks : l.workgroups;
   join_kernel<T, DP, NB><<<dim3(entries, heads), kJoinThreads, 0, l.stream>>>(l.p);
@@ -732,10 +801,12 @@ void launch_decode(const DecodeLaunch& l) {
 
 template <typename T, int DP>
 void launch_decode(const DecodeLaunch& l) {
-  if (l.int8)
-    l.wide ? launch_decode<T, true, DP, 2>(l) : launch_decode<T, true, DP, 1>(l);
+  if (l.kind == kE4m3Pages)
+    l.wide ? launch_decode<T, kE4m3Pages, DP, 2>(l) : launch_decode<T, kE4m3Pages, DP, 1>(l);
+  else if (l.kind == kInt8Pages)
+    l.wide ? launch_decode<T, kInt8Pages, DP, 2>(l) : launch_decode<T, kInt8Pages, DP, 1>(l);
   else
-    l.wide ? launch_decode<T, false, DP, 2>(l) : launch_decode<T, false, DP, 1>(l);
+    l.wide ? launch_decode<T, kRowPages, DP, 2>(l) : launch_decode<T, kRowPages, DP, 1>(l);
 }
 
 }  // namespace

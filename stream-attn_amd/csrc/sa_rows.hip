@@ -567,14 +567,14 @@ struct ReadParams {
   uint16_t *k_out, *v_out;
   int64_t token0, tokens;
   uint32_t num_slots, page_tokens;
-  int32_t kv_heads, head_dim;
+  int32_t kv_heads, head_dim, block_log2;
 };
 
 // Thread i of a workgroup moves granule (8 elements) i, i + 256, ... of K and
 // V rows of kReadTokens tokens, whose loads are under way together.
 constexpr int kReadTokens = 4;
 
-template <typename T, bool kInt8>
+template <typename T, PageKind kKind>
 __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
   const int64_t token = p.token0 + (int64_t)blockIdx.x * kReadTokens;
   int64_t at[kReadTokens], scale_at[kReadTokens];
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
     const uint32_t page = held[t] ? (uint32_t)slot / p.page_tokens : 0;
     const uint32_t row = held[t] ? (uint32_t)slot - page * p.page_tokens : 0;  // row 0 is there to be read
     at[t] = page * p.kp.sp + row * p.kp.st;
-    scale_at[t] = page * p.kp.ss_p + row * p.kp.ss_t;
+    scale_at[t] = page * p.kp.ss_p + (kKind == kE4m3Pages ? row >> p.block_log2 : row) * p.kp.ss_t;
   }
   const int granules = p.head_dim / 8, each = p.kv_heads * granules;
   for (int i = threadIdx.x; i < 2 * each; i += 256) {
@@ -594,7 +594,26 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
     const int g = is_v ? i - each : i, head = g / granules, d = 8 * (g - head * granules);
     const char* base = is_v ? p.vp.base : p.kp.base;
     u32x4 w[kReadTokens];
-    if constexpr (kInt8) {
+    if constexpr (kKind == kE4m3Pages) {
+      const uint8_t* scales = reinterpret_cast<const uint8_t*>(is_v ? p.vp.scale : p.kp.scale);
+      u32x2 c[kReadTokens];
+      uint8_t scale[kReadTokens];
+#pragma unroll
+      for (int t = 0; t < kReadTokens; ++t) {
+        c[t] = *reinterpret_cast<const u32x2*>(base + at[t] + head * p.kp.sh + d);
+        scale[t] = scales[scale_at[t] + head * p.kp.ss_h];
+      }
+#pragma unroll
+      for (int t = 0; t < kReadTokens; ++t) {
+        const float power = e8m0_value(scale[t]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x2 x = e4m3_floats<false>(c[t][j]), y = e4m3_floats<true>(c[t][j]);
+          w[t][2 * j] = T::pack(x[0] * power, x[1] * power);
+          w[t][2 * j + 1] = T::pack(y[0] * power, y[1] * power);
+        }
+      }
+    } else if constexpr (kKind == kInt8Pages) {
       const uint16_t* scales = is_v ? p.vp.scale : p.kp.scale;
       u32x2 c[kReadTokens];
       uint16_t scale[kReadTokens];
@@ -624,13 +643,14 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// scale_align: bytes of a scale.
 template <typename Args>
-bool page_rows(PageRows& r, const void* base, const void* scale, const Args* a) {
+bool page_rows(PageRows& r, const void* base, const void* scale, const Args* a, int64_t scale_align = 2) {
   const bool int8 = a->pages_int8;
   r = {static_cast<char*>(const_cast<void*>(base)), int8 ? static_cast<uint16_t*>(const_cast<void*>(scale)) : nullptr,
        a->stride_pp, a->stride_pt, a->stride_ph, a->stride_sp, a->stride_st, a->stride_sh};
   return base != nullptr && aligned(base, int8 ? 8 : 16) && r.sp % 8 == 0 && r.st % 8 == 0 && r.sh % 8 == 0 &&
-         (!int8 || (scale != nullptr && aligned(scale, 2)));
+         (!int8 || (scale != nullptr && aligned(scale, scale_align)));
 }
 
 int32_t invalid(const char* entry, const char* what) {
@@ -810,8 +830,12 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
   if (rc == 0) rc = check_pool(entry, a->num_pages, a->page_tokens);
   if (rc != 0) return rc;
   ReadParams p{};
-  if (!page_rows(p.kp, a->k_pages, a->k_scales, a) || !page_rows(p.vp, a->v_pages, a->v_scales, a))
+  const bool e4m3 = a->pages_int8 == SA_PAGES_E4M3;
+  const int64_t scale_align = e4m3 ? 1 : 2;
+  if (!page_rows(p.kp, a->k_pages, a->k_scales, a, scale_align) || !page_rows(p.vp, a->v_pages, a->v_scales, a, scale_align))
     return invalid(entry, "pages or scales are missing or not aligned");
+  if (e4m3 && (p.block_log2 = block_log2(a->block_tokens, a->page_tokens)) < 0)
+    return invalid(entry, "block_tokens must be a power of two from 16 on that divides page_tokens");
   if (a->slots == nullptr || !aligned(a->slots, 8) || a->k_out == nullptr || a->v_out == nullptr ||
       !aligned(a->k_out, 16) || !aligned(a->v_out, 16))
     return invalid(entry, "slots or outputs are missing or not aligned");
@@ -827,10 +851,12 @@ int32_t sa_read_kv(const sa_read_args* a, int32_t device, void* stream) try {
   const bool bf16 = a->dtype == SA_DTYPE_BF16;
   for (p.token0 = 0; p.token0 < a->tokens; p.token0 += kTokensPerLaunch) {
     const dim3 grid((uint32_t)((std::min(a->tokens - p.token0, kTokensPerLaunch) + kReadTokens - 1) / kReadTokens));
-    if (a->pages_int8)
-      bf16 ? read_kernel<Bf16, true><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, true><<<grid, 256, 0, hs>>>(p);
+    if (e4m3)
+      bf16 ? read_kernel<Bf16, kE4m3Pages><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, kE4m3Pages><<<grid, 256, 0, hs>>>(p);
+    else if (a->pages_int8)
+      bf16 ? read_kernel<Bf16, kInt8Pages><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, kInt8Pages><<<grid, 256, 0, hs>>>(p);
     else
-      bf16 ? read_kernel<Bf16, false><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, false><<<grid, 256, 0, hs>>>(p);
+      bf16 ? read_kernel<Bf16, kRowPages><<<grid, 256, 0, hs>>>(p) : read_kernel<Fp16, kRowPages><<<grid, 256, 0, hs>>>(p);
     SA_HIP_RETURN(hipGetLastError());
   }
   return 0;

@@ -5,6 +5,7 @@ library through its C ABI; ``triton_is_available`` is kept as an alias of
 ``hip_is_available`` so capability checks in caller code keep working.
 """
 
+from .blocks import append_kv_blocks
 from .decode import paged_decode_attention
 from .rows import append_kv, normalize_rotate_append, normalize_rotate_qk, read_kv
 from .streaming import (
@@ -17,6 +18,7 @@ from .streaming import (
 
 __all__ = [
     "append_kv",
+    "append_kv_blocks",
     "finalize_attention",
     "hip_is_available",
     "normalize_rotate_append",

@@ -10,21 +10,36 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import struct
 
 import torch
 
 from .. import _native
-from .rows import NO_STRIDES, check_place, check_pools, check_rows, new_rows, refuse_tangents
+from .rows import E4M3_PAGES, NO_STRIDES, check_place, check_pools, check_rows, check_sequences, new_rows, refuse_tangents
 
 # sa_decode_args: 10 pointers, 14 sizes and strides, the scale, 8 int32.
 _DECODE_ARGS = struct.Struct("=10Q14qd8i")
+# What sa_window_decode_args has behind them.
+_WINDOW_ARGS = struct.Struct("=4i")
+
+
+def check_window(window: int | None, sinks: int) -> tuple[int, int]:
+    """(window, sinks) as the entry points take them, a window of 0 for none."""
+    if window is None:
+        if sinks != 0:
+            raise ValueError("sinks need a window")
+        return 0, 0
+    window, sinks = operator.index(window), operator.index(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be positive and sinks must not be negative")
+    return min(window, 2**31 - 1), min(sinks, 2**31 - 1)
 
 
 @functools.lru_cache
-def _workspace_bytes(device_index: int, q_heads: int, kv_heads: int, head_dim: int, int8: bool) -> int:
+def _workspace_bytes(device_index: int, q_heads: int, kv_heads: int, head_dim: int, kind: int) -> int:
     """Workspace of a call, which depends on its head counts, head_dim and kind of pages alone."""
-    args = _DECODE_ARGS.pack(*(0,) * 24, 0.0, 1, 0, q_heads, kv_heads, head_dim, 1, 0, int8)
+    args = _DECODE_ARGS.pack(*(0,) * 24, 0.0, 1, 0, q_heads, kv_heads, head_dim, 1, 0, kind)
     needed = ctypes.c_int64()
     status = _native.lib().sa_paged_decode_workspace_bytes(args, device_index, ctypes.byref(needed))
     _native.check(status, "sa_paged_decode_workspace_bytes")
@@ -39,6 +54,8 @@ def paged_decode_attention(
     lengths: torch.Tensor,
     *,
     softmax_scale: float | None = None,
+    window: int | None = None,
+    sinks: int = 0,
     k_scales: torch.Tensor | None = None,
     v_scales: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
@@ -56,7 +73,11 @@ def paged_decode_attention(
     not seen, and what rows past a length hold does not matter.  A token that
     sees no key gets zeros, and LSE ``-inf``.
 
-    INT8 pages stand for ``value * scale``.  Logits, softmax and sums are FP32;
+    With a ``window`` the token, at position ``p = lengths[s] - 1``, sees the last
+    ``window`` keys (``j > p - window``) and the first ``sinks`` keys of its
+    sequence; pages that hold none of these are not looked up.
+
+    INT8 and e4m3 pages (:mod:`.blocks`) stand for ``value * scale``.  Logits, softmax and sums are FP32;
     a weight enters the product with V as two 16-bit parts.  A logit of NaN or
     ``+inf`` makes its head NaN, one of ``-inf`` is a key without weight; an element
     of a seen V that is not finite makes its element of ``out`` not finite.
@@ -66,23 +87,15 @@ def paged_decode_attention(
     """
     refuse_tangents(q, k_pages, v_pages, k_scales, v_scales, out)
     code = check_rows("q", q)
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype)
+    kind = check_pools(k_pages, v_pages, k_scales, v_scales, q, q.dtype, e4m3=True)
+    window, sinks = check_window(window, sinks)
     sequences, q_heads, dim = q.shape
     num_pages, page_tokens, kv_heads, _ = k_pages.shape
     device = q.device
     if k_pages.shape[3] != dim or q_heads % kv_heads:
         raise ValueError("the pages must have q's head_dim and a divisor of its heads")
-    if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.device != device:
-        raise ValueError("page_table must be an int32 [sequences, max_pages] tensor on q's device")
-    if lengths.dtype != torch.int32 or lengths.ndim != 1 or lengths.device != device:
-        raise ValueError("lengths must be an int32 [sequences] tensor on q's device")
+    check_sequences(page_table, lengths, None, sequences, page_tokens, q, "q")
     max_pages = page_table.shape[1]
-    if page_table.shape[0] != sequences or lengths.shape[0] != sequences:
-        raise ValueError("page_table and lengths must have one row per sequence")
-    if (max_pages > 1 and page_table.stride(1) != 1) or (sequences > 1 and lengths.stride(0) != 1):
-        raise ValueError("page_table rows and lengths must be contiguous")
-    if max_pages * page_tokens > 2**31 - 1:
-        raise ValueError("page_table rows must hold fewer than 2^31 keys")
     if out is None:
         out = new_rows(sequences, q_heads, dim, q.dtype, device)
     else:
@@ -95,18 +108,19 @@ def paged_decode_attention(
         lse = torch.empty_strided((q_heads, sequences), (sequences, 1), dtype=torch.float32, device=device)
     if sequences:
         index = device.index
-        needed = _workspace_bytes(index, q_heads, kv_heads, dim, int8)
+        needed = _workspace_bytes(index, q_heads, kv_heads, dim, kind)
         workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=device)
         args = _DECODE_ARGS.pack(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0,
-            v_scales.data_ptr() if int8 else 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if kind else 0,
+            v_scales.data_ptr() if kind else 0, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
             0 if lse is None else lse.data_ptr(), workspace.data_ptr(), needed, *q.stride()[:2], *out.stride()[:2],
-            *k_pages.stride()[:3], *(k_scales.stride() if int8 else NO_STRIDES), page_table.stride(0),
+            *k_pages.stride()[:3], *(k_scales.stride() if kind else NO_STRIDES), page_table.stride(0),
             max(sequences, 1), num_pages, dim**-0.5 if softmax_scale is None else float(softmax_scale), sequences, max_pages,
-            q_heads, kv_heads, dim, page_tokens, code, int8)
-        status = _native.lib().sa_paged_decode(args, index, _native.current_stream_handle(device))
+            q_heads, kv_heads, dim, page_tokens, code, kind)
+        args += _WINDOW_ARGS.pack(window, sinks, page_tokens // k_scales.shape[1] if kind == E4M3_PAGES else 0, 0)
+        status = _native.lib().sa_paged_window_decode(args, index, _native.current_stream_handle(device))
         if status:
-            _native.check(status, "sa_paged_decode")
+            _native.check(status, "sa_paged_window_decode")
     return (out, lse) if return_lse else out
 
 

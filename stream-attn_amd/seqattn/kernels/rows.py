@@ -8,7 +8,7 @@ page), and ``read_kv`` returns pages as packed rows.  None of them has a
 counterpart in the reference.
 
 Pages are ``[num_pages, page_tokens, kv_heads, head_dim]`` tensors of any page,
-token and head strides (K's and V's the same), 16-bit or INT8.  INT8 pages hold the storage format of
+token and head strides (K's and V's the same), 16-bit, INT8 or e4m3 (:mod:`.blocks`).  INT8 pages hold the storage format of
 :mod:`seqattn.quantization` with one token per group: ``[num_pages,
 page_tokens, kv_heads]`` float16 scales.  Slot ``page * page_tokens + row``
 names a row of them.  :class:`seqattn.DeviceKVCache` keeps such pages.
@@ -36,6 +36,8 @@ _ROWS_ARGS = struct.Struct("=14Q20qd16i")
 # sa_read_args: 7 pointers, 8 strides and counts, 6 int32.
 _READ_ARGS = struct.Struct("=7Q8q6i")
 NO_STRIDES = (0, 0, 0)
+# What pages hold (SA_PAGES_*).
+ROW_PAGES, INT8_PAGES, E4M3_PAGES = range(3)
 
 
 def _refuse_gradients() -> None:
@@ -121,11 +123,11 @@ def _check_written(name: str, k: torch.Tensor, v: torch.Tensor, counts, strides,
 
 def check_pools(
     k_pages, v_pages, k_scales, v_scales, like: torch.Tensor, dtype: torch.dtype, *, written: bool = False,
-    rows: tuple[torch.Tensor, torch.Tensor] | None = None
-) -> bool:
-    """Both pools of a cache, on ``like``'s device; whether they hold INT8.
+    rows: tuple[torch.Tensor, torch.Tensor] | None = None, e4m3: bool = False
+) -> int:
+    """Both pools of a cache, on ``like``'s device; what they hold (ROW_PAGES, INT8_PAGES, E4M3_PAGES).
 
-    ``written``: rows go into them, those of ``rows`` as they are where it is given.
+    ``written``: rows go into them, those of ``rows`` as they are where it is given.  ``e4m3``: they may hold e4m3.
     """
     shape, strides, stored = k_pages.shape, k_pages.stride(), k_pages.dtype
     if len(shape) != 4:
@@ -134,8 +136,8 @@ def check_pools(
         raise ValueError("pages must have a unit stride in head_dim")
     if v_pages.shape != shape or v_pages.dtype != stored or v_pages.stride() != strides:
         raise ValueError("k_pages and v_pages must have the same shape and dtype, and the same strides")
-    int8 = stored == torch.int8
-    align = 8 if int8 else 16
+    kind = INT8_PAGES if stored == torch.int8 else E4M3_PAGES if e4m3 and stored == torch.float8_e4m3fn else ROW_PAGES
+    align = 8 if kind else 16
     if strides[0] % 8 or strides[1] % 8 or strides[2] % 8 or k_pages.data_ptr() % align or v_pages.data_ptr() % align:
         raise ValueError("pages must be aligned, with their other strides in multiples of 8 elements")
     if k_pages.device != like.device or v_pages.device != like.device:
@@ -148,24 +150,60 @@ def check_pools(
         _refuse_gradients()
     if written:
         _check_written("rows", k_pages, v_pages, shape[:3], strides[:3], shape[3], rows)
-    if not int8:
+    if kind == ROW_PAGES:
         if k_scales is not None or v_scales is not None:
-            raise ValueError("only INT8 pages have scales")
+            raise ValueError("only INT8 pages have scales" + (", and e4m3 pages" if e4m3 else ""))
         if stored != dtype:
             raise ValueError(f"pages of {stored} do not match rows of {dtype}")
-        return False
+        return kind
     if k_scales is None or v_scales is None:
-        raise ValueError("INT8 pages need their scales")
+        raise ValueError(f"{'INT8' if kind == INT8_PAGES else 'e4m3'} pages need their scales")
     for scales in (k_scales, v_scales):
-        if scales.dtype != torch.float16 or scales.shape != shape[:3] or scales.device != like.device:
+        if kind == E4M3_PAGES:
+            check_block_scales(scales, shape, like.device)
+        elif scales.dtype != torch.float16 or scales.shape != shape[:3] or scales.device != like.device:
             raise ValueError("INT8 scales must be float16 [num_pages, page_tokens, kv_heads] on the pages' device")
     if k_scales.stride() != v_scales.stride():
         raise ValueError("k_scales and v_scales must have the same strides")
     if k_scales.requires_grad or v_scales.requires_grad:
         _refuse_gradients()
     if written:
-        _check_written("scales", k_scales, v_scales, shape[:3], k_scales.stride(), 1, rows)
-    return True
+        _check_written("scales", k_scales, v_scales, k_scales.shape, k_scales.stride(), 1, rows)
+    return kind
+
+
+def check_block_scales(scales: torch.Tensor, pages: Sequence[int], device: torch.device) -> None:
+    if scales.dtype != torch.float8_e8m0fnu or scales.ndim != 3 or scales.device != device:
+        raise ValueError("e4m3 scales must be float8_e8m0fnu [num_pages, page_tokens / block_tokens, kv_heads] "
+                         "on the pages' device")
+    blocks, page_tokens = scales.shape[1], pages[1]
+    if scales.shape[0] != pages[0] or scales.shape[2] != pages[2] or not blocks or page_tokens % blocks:
+        raise ValueError("e4m3 scales must have a scale per block of every page and K/V head")
+    block_tokens = page_tokens // blocks
+    if block_tokens < 16 or block_tokens & (block_tokens - 1):
+        raise ValueError(f"blocks must have a power of two of rows from 16 on, got {block_tokens}")
+
+
+def check_sequences(page_table: torch.Tensor, lengths: torch.Tensor, cu_tokens: torch.Tensor | None, tokens: int,
+                    page_tokens: int, rows: torch.Tensor, name: str) -> None:
+    """The pages and lengths of sequences, and where each one's rows start among ``tokens`` ones (one each without)."""
+    device = rows.device
+    if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.device != device:
+        raise ValueError(f"page_table must be an int32 [sequences, max_pages] tensor on {name}'s device")
+    if lengths.dtype != torch.int32 or lengths.ndim != 1 or lengths.device != device:
+        raise ValueError(f"lengths must be an int32 [sequences] tensor on {name}'s device")
+    sequences, max_pages = page_table.shape
+    if lengths.shape[0] != sequences or (cu_tokens is None and tokens != sequences):
+        raise ValueError("page_table and lengths must have one row per sequence")
+    if (max_pages > 1 and page_table.stride(1) != 1) or (sequences > 1 and lengths.stride(0) != 1):
+        raise ValueError("page_table rows and lengths must be contiguous")
+    if max_pages * page_tokens > 2**31 - 1:
+        raise ValueError("page_table rows must hold fewer than 2^31 keys")
+    if cu_tokens is not None:
+        if cu_tokens.dtype != torch.int32 or cu_tokens.ndim != 1 or cu_tokens.device != device:
+            raise ValueError(f"cu_tokens must be an int32 [sequences + 1] tensor on {name}'s device")
+        if cu_tokens.shape[0] != sequences + 1 or (sequences and cu_tokens.stride(0) != 1):
+            raise ValueError("cu_tokens must hold one start per sequence and the end, contiguously")
 
 
 def check_place(name: str, out: torch.Tensor, rows: torch.Tensor, others: Sequence[torch.Tensor | None]) -> None:
@@ -415,18 +453,18 @@ def read_kv(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The pages' rows at ``slots`` as packed ``(k, v) [tokens, kv_heads, head_dim]``, the runners' layout.
 
-    INT8 rows come as ``value * scale`` in ``dtype`` (default bfloat16), others
-    in the pages' own dtype.  A slot outside the pool gives zeros.
+    INT8 and e4m3 rows come as ``value * scale`` in ``dtype`` (default bfloat16),
+    others in the pages' own dtype.  A slot outside the pool gives zeros.
     """
     refuse_tangents(k_pages, v_pages, k_scales, v_scales)
     if dtype is None:
-        dtype = torch.bfloat16 if k_pages.dtype == torch.int8 else k_pages.dtype
+        dtype = torch.bfloat16 if k_pages.dtype in (torch.int8, torch.float8_e4m3fn) else k_pages.dtype
     code = _native.dtype_code(dtype)
     if slots.ndim != 1:
         raise ValueError("slots must be a one-dimensional int64 tensor on the rows' device")
     if slots.device.type != "cuda":
         raise ValueError("kernel operands must be device tensors")
-    int8 = check_pools(k_pages, v_pages, k_scales, v_scales, slots, dtype)
+    kind = check_pools(k_pages, v_pages, k_scales, v_scales, slots, dtype, e4m3=True)
     tokens, (num_pages, page_tokens, heads, dim) = slots.shape[0], k_pages.shape
     _check_slots(slots, tokens, k_pages.device)
     if dim % 8 or not 16 <= dim <= 256:
@@ -435,10 +473,11 @@ def read_kv(
     if tokens == 0:
         return k_out, v_out
     args = _READ_ARGS.pack(
-        k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if int8 else 0, v_scales.data_ptr() if int8 else 0,
+        k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if kind else 0, v_scales.data_ptr() if kind else 0,
         slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *k_pages.stride()[:3],
-        *(k_scales.stride() if int8 else NO_STRIDES),
-        tokens, num_pages, heads, dim, page_tokens, code, int8, 0)
+        *(k_scales.stride() if kind else NO_STRIDES),
+        tokens, num_pages, heads, dim, page_tokens, code, kind,
+        page_tokens // k_scales.shape[1] if kind == E4M3_PAGES else 0)
     device = k_pages.device
     status = _native.lib().sa_read_kv(args, device.index, _native.current_stream_handle(device))
     if status:
