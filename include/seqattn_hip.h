@@ -748,6 +748,53 @@ typedef struct {
 
 int32_t sa_paged_window_decode(const sa_window_decode_args* args, int32_t device, void* stream);
 
+/*
+ * Attention of the last tokens of every sequence over a paged K/V cache that
+ * holds their keys already: prompts, chunks of them, drafted tokens.
+ *
+ *   q, out [tokens, q_heads, head_dim]  bf16/fp16, packed sequence by sequence
+ *   cu_tokens [sequences + 1]           int32, non-decreasing from 0: sequence s has rows cu_tokens[s] ..
+ *   lengths [sequences]                 int32, the sequence's keys, its new tokens' among them
+ *   lse [q_heads, tokens]               fp32, natural log; may be NULL
+ *
+ * Token i of a sequence's n is at position p = length - n + i and sees the keys
+ * j <= p, with a window only those with p - j < window and the first `sinks`.
+ * Pages, scales, page_table and lengths as for sa_paged_window_decode; a token
+ * that sees no key gets output 0 and LSE -inf, rows past
+ * cu_tokens[sequences] stay as they are.  INT8 values enter in q's type, and so do
+ * e4m3 ones of V (float16: at most its largest value).
+ *
+ * 8-bit pages: head_dim and strides are multiples of 16, pages 16-byte aligned.
+ * tokens * q_heads / kv_heads is below 2^31 - 4096.  `workspace`
+ * (sa_paged_prefill_workspace_bytes, 16-byte aligned) is the call's own until
+ * it has run.
+ */
+typedef struct {
+    const void *q, *k_pages, *v_pages, *k_scales, *v_scales;
+    const int32_t *page_table, *lengths, *cu_tokens;
+    void* out;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t stride_qt, stride_qh, stride_ot, stride_oh;
+    int64_t stride_pp, stride_pt, stride_ph; /* of both pools */
+    int64_t stride_sp, stride_st, stride_sh; /* of their scales (e4m3: stride_st of a block) */
+    int64_t stride_table, lse_stride_h;
+    int64_t tokens, num_pages;
+    double softmax_scale;
+    int32_t sequences, max_pages;
+    int32_t q_heads, kv_heads, head_dim, page_tokens, dtype;
+    int32_t pages_kind; /* SA_PAGES_* */
+    int32_t window, sinks;
+    int32_t block_tokens; /* e4m3 */
+    int32_t reserved;
+} sa_prefill_args;
+
+int32_t sa_paged_prefill(const sa_prefill_args* args, int32_t device, void* stream);
+
+/* Workspace bytes of a call (its sizes only; pointers and strides are not read). */
+int32_t sa_paged_prefill_workspace_bytes(const sa_prefill_args* args, int32_t device, int64_t* bytes);
+
 /* hipStream_t of the pipeline's H2D (which == 0) or D2H (which == 1) copy stream. */
 void* sa_pipeline_stream(sa_pipeline* pipeline, int32_t which);
 

@@ -26,7 +26,8 @@ PROBE_LIB_PATH = LIB_DIR / "libseqattn_probe.so"
 ARCH = "gfx950"
 
 SOURCES = ("sa_kernels.hip", "sa_rows.hip", "sa_blocks.hip", "sa_decode.hip", "sa_decode_d64.hip", "sa_decode_d128.hip",
-           "sa_decode_d256.hip", "sa_update_d32.hip", "sa_update_d64.hip", "sa_update_d128.hip",
+           "sa_decode_d256.hip", "sa_prefill.hip", "sa_prefill_d64.hip", "sa_prefill_d128.hip", "sa_prefill_d256.hip",
+           "sa_update_d32.hip", "sa_update_d64.hip", "sa_update_d128.hip",
            "sa_update_d256.hip", "sa_pipeline.cpp")
 PROBE_SOURCES = ("sa_probe.hip",)
 

@@ -1,0 +1,6 @@
+// The kernels of a prompt's attention over the paged cache for a padded head_dim of 128.
+#include "sa_prefill_kernel.h"
+
+namespace sa {
+hipError_t launch_prefill_d128(const PrefillLaunch& l) { return launch_prefill<128>(l); }
+}  // namespace sa

@@ -1,0 +1,619 @@
+// Device code of a prompt's attention over the paged cache; included by the
+// sources that compile one head size.
+//
+//   s_ij = scale * q_i . k_j over the keys j <= p_i with p_i - j < window or j < sinks
+//   out_i = sum_j e^(s_ij) v_j / sum_j e^(s_ij),  lse_i = log sum_j e^(s_ij)
+//
+// One pass over a row's keys with the running maximum and sum.
+#pragma once
+
+#include <cmath>
+#include <type_traits>
+
+#include "sa_prefill.h"
+#include "sa_update_kernel.h"
+
+namespace sa {
+namespace {
+
+template <typename T>
+__device__ inline __attribute__((always_inline)) T uniform(T x) {
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t v = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return __builtin_bit_cast(T, (uint64_t)lo | (uint64_t)hi << 32);
+  } else {
+    return __builtin_amdgcn_readfirstlane(x);
+  }
+}
+
+// 2^x of a running maximum's change: 0 from -inf, 1 where nothing changes.
+__device__ inline float prefill_ratio(float from, float to) { return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to); }
+
+// The halves of a dword that are infinite or NaN, as a mask.
+template <typename T>
+__device__ inline uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<T, Bf16> ? 0x7f80u : 0x7c00u;
+  return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
+template <typename T, int DP, int QB, PageKind kKind, int STAGES>
+__global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillParams p) {
+  using Geo = Geometry<DP>;
+  constexpr bool QUANT = kKind != kRowPages;
+  constexpr int CK = Geo::CK, DB = Geo::DB;
+  constexpr int KB = DP == 256 ? (QB == 1 ? 4 : 2) : CK;
+  constexpr int VB = DP == 256 ? (QB == 1 ? 8 : 4) : DP == 128 && QB > 1 ? 8 : 4;
+  constexpr int BLOCK_M = Geo::WAVES * 16 * QB;
+  constexpr int STAGE_BYTES = 2 * Geo::TILE_BYTES;
+  constexpr int RAW_BYTES = Geo::I8_TILE_BYTES;  // of K or V of a raw tile
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE_BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t raw[QUANT ? 4 * RAW_BYTES : 16];
+  // Of the tiles in flight: which keys are in a page of the pool, and the scales of
+  // K and V (INT8 by key, e4m3 by run of 16 keys).
+  __shared__ __attribute__((aligned(8))) uint16_t seen_lds[4][4];
+  __shared__ __attribute__((aligned(16))) float scale_lds[QUANT ? 4 : 1][2][kTileKeys];
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r16 = lane & 15, j = lane >> 4;
+  const bool issues = wave < 4;
+
+  // The run of tiles of this workgroup; neighbouring runs are on one XCD.
+  const int run = (blockIdx.x & 7) * (p.runs >> 3) + (blockIdx.x >> 3);
+  const int64_t tiles = uniform(p.plan->tiles);
+  const int blocks = uniform(p.plan->blocks);
+  const int64_t total = tiles * p.kv_heads, share = (total + p.runs - 1) / p.runs;
+  const int64_t begin = run * share, end = begin + share < total ? begin + share : total;
+  if (tid == 0) p.splits[run].block = -1;
+  if (begin >= end) return;
+
+  // Elements of K past head_dim are zeros that no tile writes.
+  if (p.head_dim < DP) {
+    for (int i = tid; i < STAGES * STAGE_BYTES / 16; i += kPrefillThreads)
+      reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+  }
+
+  // The block that the run starts in: 64 of them looked at at once.
+  int head = (int)(begin / tiles), block = 0;
+  {
+    const int64_t into = begin - head * tiles;
+    for (int left = blocks; left > 1;) {
+      const int step = (left + 63) >> 6, at = lane * step;
+      const bool before = at < left && p.blocks[block + (at < left ? at : 0)].before <= into;
+      const int skipped = (__popcll(__ballot(before)) - 1) * step;
+      block += skipped;
+      left = min(step, left - skipped);
+    }
+  }
+
+  const float cf = scale_factor(p.scale_log2);
+  for (int64_t at = begin; at < end;) {
+    // ---- a piece: tiles first .. last - 1 of an item ----
+    const int64_t before = uniform(p.blocks[block].before) + head * tiles;
+    const int s = uniform(p.blocks[block].sequence), row0 = uniform(p.blocks[block].row);
+    PrefillSequence seq = prefill_sequence(p, s);
+    seq.from = uniform(seq.from), seq.count = uniform(seq.count), seq.base = uniform(seq.base);
+    const int rows = min(seq.count * p.group, row0 + BLOCK_M);  // end of the block's rows
+    PrefillTiles span = prefill_tiles(p, seq, row0, rows);
+    span.count = uniform(span.count), span.sinks = uniform(span.sinks), span.skip = uniform(span.skip);
+    const int first = (int)(at - before);
+    const int last = (int)min((int64_t)span.count, end - before);
+    const int ntiles = last - first;
+    const int32_t* table = p.table + s * p.s_table;
+
+    // Rows of this wave, and the bounds of what they see: no key at or past
+    // wave_end, every (window's) key before wave_first; no key below low_first but
+    // the sinks, every key (before wave_first) from low_last on.
+    const int qw0 = row0 + wave * 16 * QB;
+    const bool has_rows = qw0 < rows;
+    int pos[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) pos[qb] = seq.base + prefill_query(p, min(qw0 + 16 * qb + r16, rows - 1));
+    const int pos_first = uniform(seq.base + prefill_query(p, min(qw0, rows - 1)));
+    const int pos_last = uniform(seq.base + prefill_query(p, min(qw0 + 16 * QB, rows) - 1));
+    const int wave_end = has_rows ? pos_last + 1 : 0, wave_first = pos_first + 1;
+    const int low_first = (int)max((int64_t)pos_first - p.window + 1, (int64_t)0);
+    const int low_last = (int)max((int64_t)pos_last - p.window + 1, (int64_t)0);
+
+    // ---- loads ----
+    // Issuing wave w has keys 16 w .. + 15 of every tile: one page's where pages are
+    // multiples of 16.  Lane l holds the page of tile ids_first + l.
+    int32_t ids = -1, ids_first = first - 64;
+    const auto page_of = [&](int key, int& row) {
+      const int number = (int)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift);
+      row = key - number * p.page_tokens;
+      return number;
+    };
+    const auto id_of = [&](int tile) {
+      if (tile - ids_first >= 64) {
+        ids_first = tile;
+        int row;
+        const int number = tile + lane < last ? page_of(span.key_of(tile + lane) + 16 * wave, row) : p.max_pages;
+        ids = number < p.max_pages ? table[number] : -1;
+      }
+      return __builtin_amdgcn_readlane(ids, tile - ids_first);
+    };
+    constexpr int ES = QUANT ? 1 : 2;
+    const char* k_head = p.k + head * p.sh * ES;
+    const char* v_head = p.v + head * p.sh * ES;
+    auto dma = [](const char* at, uint8_t* dst) __attribute__((always_inline)) {
+      __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)at, (SA_LDS void*)dst, 16, 0, 0);
+    };
+    float scale_next = 0.f;  // a scale of the raw tile in flight
+    // Tile `tile`: its 16-bit rows to the stage, or its bytes to the raw buffer.
+    auto issue_tile = [&](int tile, uint8_t* to) __attribute__((always_inline)) {
+      if (!issues) return;
+      const int key0 = span.key_of(tile) + 16 * wave;
+      // A lane's key: one of the run's 16.
+      const int lane_key = QUANT ? (lane * 16) / DP : lane >> 2;
+      constexpr int KEYS = QUANT ? 1024 / DP : 16;  // of a wave-wide load
+      uint32_t seen = 0;
+#pragma unroll
+      for (int x = 0; x < 16 / KEYS; ++x) {
+        int64_t offset;
+        int32_t id, row;
+        if (p.any_page) {
+          const int number = page_of(key0 + x * KEYS + lane_key, row);
+          id = number < p.max_pages ? table[number] : -1;
+        } else {
+          id = id_of(tile);
+          page_of(key0, row);
+          row += x * KEYS + lane_key;
+        }
+        const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
+        if (!ok) id = 0, row = 0;  // a row that exists, read and not used
+        offset = (id * p.sp + row * p.st) * ES;
+        const uint64_t held = __ballot(ok);
+        if constexpr (QUANT) {
+          constexpr int LANES = DP / 16;  // of a key
+          uint32_t bits = 0;
+#pragma unroll
+          for (int i = 0; i < KEYS; ++i) bits |= (uint32_t)(held >> (i * LANES) & 1) << i;
+          seen |= bits << (x * KEYS);
+          const int d = (lane * 16) % DP;
+          const int64_t src = offset + (d < p.head_dim ? d : 0);
+          dma(k_head + src, to + wave * 16 * DP + x * 1024);
+          dma(v_head + src, to + RAW_BYTES + wave * 16 * DP + x * 1024);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) seen |= (uint32_t)(held >> (4 * i) & 1) << i;
+          const int kd = 8 * Geo::k_granule((lane & 3) ^ (lane >> 4)), vd = 8 * ((lane & 3) ^ (2 * ((lane >> 4) & 1)));
+#pragma unroll
+          for (int c = 0; c < CK; ++c) {
+            if (32 * c + kd < p.head_dim) dma(k_head + offset + (32 * c + kd) * ES, to + (CK * wave + c) * 1024);
+            if (32 * c + vd < p.head_dim)
+              dma(v_head + offset + (32 * c + vd) * ES, to + Geo::TILE_BYTES + (4 * c + wave) * 1024);
+          }
+        }
+      }
+      if constexpr (kKind == kInt8Pages) {
+        // Lanes 0 - 15 K's, 16 - 31 V's of the run's keys.
+        int32_t id, row;
+        const int number = page_of(key0 + r16, row);
+        id = number < p.max_pages ? table[number] : -1;
+        if ((uint32_t)id >= (uint32_t)p.num_pages) id = 0, row = 0;
+        const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? p.vs : p.ks);
+        scale_next = Fp16::lo(from[id * p.ssp + row * p.sst + head * p.ssh]);
+      } else if constexpr (kKind == kE4m3Pages) {
+        int32_t id = id_of(tile), row;
+        page_of(key0, row);
+        if ((uint32_t)id >= (uint32_t)p.num_pages) id = 0, row = 0;
+        const uint8_t* from = static_cast<const uint8_t*>(j & 1 ? p.vs : p.ks);
+        scale_next = e8m0_value(from[id * p.ssp + (row >> p.block_log2) * p.sst + head * p.ssh]);
+      }
+      if (lane == 0) seen_lds[tile & 3][wave] = (uint16_t)seen;
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // The scales that came with raw tile `tile`, by the waves that loaded them.
+    auto put_scales = [&](int tile) __attribute__((always_inline)) {
+      if constexpr (QUANT) {
+        if (issues && lane < 32) scale_lds[tile & 3][j][16 * wave + r16] = scale_next;
+      }
+    };
+    // A raw tile to 16 bits.  INT8: value * scale, at most float16's largest.  e4m3: K's
+    // values as they are (the scale is in the logits), V's times their power of
+    // two, exact in bfloat16; float16 has steps of its own below 2^-14.
+    auto dequant = [&](int tile, const uint8_t* from, uint8_t* stage) __attribute__((always_inline)) {
+      constexpr int GR = Geo::I8_GR;
+#pragma unroll
+      for (int x = 0; x < (Geo::I8_GRANULES + kPrefillThreads - 1) / kPrefillThreads; ++x) {
+        const int i = tid + x * kPrefillThreads;
+        if (i >= Geo::I8_GRANULES) break;
+        const int row = i / GR, gr = i % GR;
+        if (16 * gr >= p.head_dim) continue;
+#pragma unroll
+        for (int tensor = 0; tensor < 2; ++tensor) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(from + tensor * RAW_BYTES + row * DP + gr * 16);
+          const float scale = scale_lds[tile & 3][tensor][row];
+          u32x4 o[2];
+          if constexpr (kKind == kInt8Pages) {
+            // med3 of NaN bounds is NaN.
+            const float most = std::is_same_v<T, Bf16> ? INFINITY : scale == scale ? 65504.f : NAN;
+            const auto value = [&](int e) {
+              const float y = byte_float(w[e / 4], e & 3) * scale;
+              return std::is_same_v<T, Bf16> ? y : __builtin_amdgcn_fmed3f(y, -most, most);
+            };
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = T::pack(value(2 * e), value(2 * e + 1));
+          } else {
+            const float power = tensor == 0 ? 1.f : scale;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[e / 2][2 * (e & 1)] = T::template e4m3_pair<false>(w[e], power);
+              o[e / 2][2 * (e & 1) + 1] = T::template e4m3_pair<true>(w[e], power);
+            }
+            if (std::is_same_v<T, Fp16> && tensor == 1 && !(power < 256.f)) {
+              // Values past float16's largest become that.
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const f32x2 y = e & 1 ? e4m3_floats<true>(w[e / 2]) : e4m3_floats<false>(w[e / 2]);
+                const float a = y[0] * power, b = y[1] * power;
+                o[e / 4][e % 4] = T::pack(a == a ? __builtin_amdgcn_fmed3f(a, -65504.f, 65504.f) : a,
+                                          b == b ? __builtin_amdgcn_fmed3f(b, -65504.f, 65504.f) : b);
+              }
+            }
+          }
+          uint8_t* to = stage + tensor * Geo::TILE_BYTES;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (16 * gr + 8 * h >= p.head_dim) continue;
+            *reinterpret_cast<u32x4*>(to + (tensor == 0 ? Geo::k_offset(row, 2 * gr + h) : Geo::v_offset(row, 2 * gr + h))) = o[h];
+          }
+        }
+      }
+    };
+
+    __syncthreads();  // the stages are free (and, at first, cleared)
+    if constexpr (!QUANT) {
+      for (int t = 0; t < min(ntiles, STAGES - 1); ++t) issue_tile(first + t, lds + t * STAGE_BYTES);
+    } else {
+      issue_tile(first, raw);
+    }
+
+    // Q fragments: row qw0 + 16 qb + r16, d = 32 c + 8 j .. + 7.
+    u32x4 qf[QB][CK];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int row = min(qw0 + 16 * qb + r16, rows - 1), query = prefill_query(p, row);
+      const uint16_t* from = p.q + (int64_t)(seq.from + query) * p.sq_t + (int64_t)(head * p.group + row - query * p.group) * p.sq_h;
+#pragma unroll
+      for (int c = 0; c < CK; ++c) {
+        const int d = 32 * c + 8 * j;
+        qf[qb][c] = *reinterpret_cast<const u32x4*>(from + (d < p.head_dim ? d : 0));
+      }
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int c = 0; c < CK; ++c)
+        qf[qb][c] = qw0 + 16 * qb + r16 < rows && 32 * c + 8 * j < p.head_dim ? qf[qb][c] ^ q_sign(p.scale_log2) : u32x4{0, 0, 0, 0};
+
+    float m_run[QB], l_part[QB];
+    f32x4 acc[DB][QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      m_run[qb] = -INFINITY, l_part[qb] = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int k_lane = 64 * r16 + ((Geo::k_slot(j) ^ (r16 >> 2)) << 4);
+    const int v_lane = 256 * j + 64 * (r16 >> 2) + 32 * (j & 1) + 8 * (r16 & 3);
+
+    // ---- a tile's products ----
+    auto compute = [&](int tile, const uint8_t* stage) __attribute__((always_inline)) {
+      const int kt = span.key_of(tile);
+      const uint32_t base = (uint32_t)(uintptr_t)(const SA_LDS uint8_t*)(stage);
+      const uint64_t seen = uniform(*reinterpret_cast<const uint64_t*>(seen_lds[tile & 3]));
+#pragma unroll
+      for (int sub = 0; sub < kTileKeys / kSubKeys; ++sub) {
+        const int rb = sub * kSubKeys, key0 = kt + rb;
+        if (key0 >= wave_end) break;
+        if (key0 + kSubKeys <= low_first && key0 >= p.sinks) continue;
+        const uint32_t held = (uint32_t)(seen >> rb);
+        const bool masked = key0 + kSubKeys > wave_first || (key0 < low_last && key0 + kSubKeys > p.sinks) || held != ~0u;
+        // Whether row r16 of query block qb sees key k of the step.
+        const auto sees = [&](int qb, int k) {
+          const int key = key0 + k;
+          return key <= pos[qb] && (pos[qb] - key < p.window || key < p.sinks) && (held >> k & 1);
+        };
+
+        f32x4 st[2][QB];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) st[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c0 = 0; c0 < CK; c0 += KB) {
+          u32x4 kf[2 * KB];
+          read_k(kf, base + k_lane, (rb / 16 * CK + c0) * 1024, CK * 1024);
+#pragma unroll
+          for (int c = 0; c < KB; ++c)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int i = 0; i < QB; ++i) {
+                const int qb = kb == 0 ? i : QB - 1 - i;
+                st[kb][qb] = T::mma(kf[kb * KB + c], qf[qb][c0 + c], st[kb][qb]);
+              }
+        }
+        // What a logit's FMA multiplies it by: e4m3's with the scale of its 16 keys.
+        float factor[2] = {cf, cf};
+        if constexpr (kKind == kE4m3Pages) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const float f = cf * scale_lds[tile & 3][0][rb + 16 * kb];
+            factor[kb] = f < 1.17549435e-38f ? 1.17549435e-38f : f;  // times -inf it is -inf; NaN stays
+          }
+        }
+        if (__builtin_expect(masked, 0)) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            // A scale of NaN is one for those that see its keys.
+            const bool none = kKind == kE4m3Pages && factor[kb] != factor[kb];
+            if (none) factor[kb] = cf;
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                st[kb][qb][i] = !sees(qb, 16 * kb + 4 * j + i) ? -INFINITY : none ? NAN : st[kb][qb][i];
+          }
+        }
+        auto exps = [&](int qb, float neg_m, u32x4& pq) -> float {
+          float sum = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e], factor[kb], neg_m));
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e + 1], factor[kb], neg_m));
+              sum = (kb == 0 && e == 0) ? p0 + p1 : sum + (p0 + p1);
+              pq[2 * kb + e] = T::pack(p0, p1);
+            }
+          return sum;
+        };
+        u32x4 pf[QB];
+        float psum[QB];
+        bool grow[QB], any = false;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          // Every p <= 2^8 whenever the lane's sum is; against m = -inf the sum is
+          // inf or NaN.
+          psum[qb] = exps(qb, -m_run[qb], pf[qb]);
+          grow[qb] = !(psum[qb] <= 256.f);
+          any = any || grow[qb];
+        }
+        if (__builtin_expect(__ballot(any) != 0, 0)) {
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) {
+            const uint64_t bal = __ballot(grow[qb]);
+            uint32_t fold = (uint32_t)bal | (uint32_t)(bal >> 32);
+            fold |= fold >> 16;
+            const bool mine = (fold >> r16) & 1u;
+            float full = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+              full = fmaxf(full, fmaxf(fmaxf(st[kb][qb][0], st[kb][qb][1]), fmaxf(st[kb][qb][2], st[kb][qb][3])) * factor[kb]);
+            full = fmaxf(full, __shfl_xor(full, 16));
+            full = fmaxf(full, __shfl_xor(full, 32));
+            const float m_new = (mine && full > m_run[qb] + kRescaleThreshold) ? full : m_run[qb];
+            const bool none = m_new == -INFINITY;
+            if (m_new != m_run[qb] || none) {
+              const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+              l_part[qb] *= alpha;
+#pragma unroll
+              for (int db = 0; db < DB; ++db) acc[db][qb] *= alpha;
+              m_run[qb] = m_new;
+              psum[qb] = exps(qb, none ? 0.f : -m_new, pf[qb]);
+            }
+          }
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) l_part[qb] += psum[qb];
+
+        const uint32_t v_addr = base + Geo::TILE_BYTES + v_lane, v_odd = base + Geo::TILE_BYTES + (v_lane ^ 32);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int d0 = 0; d0 < DB; d0 += VB) {
+          u32x4 vf[VB];
+          read_v(vf, v_addr, v_odd, d0 / 2 * 4096 + rb * 64);
+          // A key that not every row sees: 0 * NaN is not 0, so what is not finite stays
+          // out of the products.
+          if (__builtin_expect(masked, 0)) {
+#pragma unroll
+            for (int dd = 0; dd < VB; ++dd)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t off = not_finite<T>(vf[dd][i]);
+                bad |= off;
+                vf[dd][i] &= ~off;
+              }
+          }
+#pragma unroll
+          for (int dd = 0; dd < VB; ++dd)
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+              const int qb = dd % 2 == 0 ? i : QB - 1 - i;
+              acc[d0 + dd][qb] = T::mma(vf[dd], pf[qb], acc[d0 + dd][qb]);
+            }
+        }
+        if (__builtin_expect(masked && __any(bad != 0), 0)) {
+          // And makes the elements of those that see it not finite.
+          for (int k = 0; k < kSubKeys; ++k) {
+            for (int db = 0; db < DB; ++db) {
+              const int d = 16 * db + 4 * j;
+              const u32x2 w = *reinterpret_cast<const u32x2*>(stage + Geo::TILE_BYTES + Geo::v_offset(rb + k, d >> 3) + 2 * (d & 7));
+              const uint32_t off[2] = {not_finite<T>(w[0]), not_finite<T>(w[1])};
+              if (!__any((off[0] | off[1]) != 0)) continue;
+#pragma unroll
+              for (int x = 0; x < DB; ++x) {
+                if (x != db) continue;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if ((off[e >> 1] >> (16 * (e & 1)) & 1) && sees(qb, k)) acc[x][qb][e] = NAN;
+              }
+            }
+          }
+        }
+      }
+    };
+
+    // ---- the tiles ----
+    if constexpr (!QUANT) {
+      // Tile t is computed while the next STAGES - 1 are in flight; an issuing wave's
+      // loads complete in order.
+      // Tile t is there once no more than the later tiles' loads are outstanding; with
+      // a padded head_dim they are fewer than that.
+      constexpr int PER_TILE = 2 * CK;
+      for (int t = 0; t < ntiles; ++t) {
+        const int later = p.head_dim < DP ? 0 : min(ntiles - 1 - t, STAGES - 2);
+        if (later >= 2)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER_TILE) : "memory");
+        else if (later == 1)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER_TILE) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + STAGES - 1 < ntiles)
+          issue_tile(first + t + STAGES - 1, lds + (t + STAGES - 1) % STAGES * STAGE_BYTES);
+        compute(first + t, lds + t % STAGES * STAGE_BYTES);
+      }
+    } else if constexpr (STAGES == 1) {
+      // LDS holds one converted tile (head_dim 256).
+      for (int t = 0; t < ntiles; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        put_scales(first + t);
+        __syncthreads();
+        dequant(first + t, raw + t % 2 * 2 * RAW_BYTES, lds);
+        if (t + 1 < ntiles) issue_tile(first + t + 1, raw + (t + 1) % 2 * 2 * RAW_BYTES);
+        __syncthreads();
+        compute(first + t, lds);
+      }
+    } else {
+      static_assert(STAGES == 2, "stages of converted tiles");
+      // At tile t: its 16-bit form is in its stage, raw tile t + 1 has arrived.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      put_scales(first);
+      __syncthreads();
+      dequant(first, raw, lds);
+      if (ntiles > 1) issue_tile(first + 1, raw + 2 * RAW_BYTES);
+      for (int t = 0; t < ntiles; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t + 1 < ntiles) put_scales(first + t + 1);
+        __syncthreads();
+        // The first wave of a SIMD converts before its products and the second one
+        // after them, so that each one's vector work meets the other's matrix work.
+        auto next = [&]() __attribute__((always_inline)) {
+          if (t + 1 < ntiles) dequant(first + t + 1, raw + (t + 1) % 2 * 2 * RAW_BYTES, lds + (t + 1) % 2 * STAGE_BYTES);
+        };
+        if (issues) {
+          next();
+          if (t + 2 < ntiles) issue_tile(first + t + 2, raw + t % 2 * 2 * RAW_BYTES);
+        }
+        compute(first + t, lds + t % 2 * STAGE_BYTES);
+        if (!issues) next();
+      }
+    }
+
+    // ---- the piece's end ----
+    const bool whole = first == 0 && last == span.count;
+    float* part = p.parts + ((int64_t)run * 2 + (first == 0)) * prefill_part_floats(BLOCK_M, DP);
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      float l = l_part[qb] + __shfl_xor(l_part[qb], 16);
+      l += __shfl_xor(l, 32);
+      const int row = qw0 + 16 * qb + r16;
+      if (whole) {
+        if (row >= rows) continue;
+        const int query = prefill_query(p, row), q_head = head * p.group + row - query * p.group;
+        uint16_t* to = p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + 4 * j;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          if (16 * db + 4 * j >= p.head_dim) continue;
+          const f32x4& a = acc[db][qb];
+          u32x2 o = {0, 0};
+          if (!(l == 0.f)) o[0] = T::pack(a[0] / l, a[1] / l), o[1] = T::pack(a[2] / l, a[3] / l);
+          *reinterpret_cast<u32x2*>(to + 16 * db) = o;
+        }
+        if (p.lse != nullptr && j == 0)
+          p.lse[q_head * p.lse_h + seq.from + query] = l == 0.f ? -INFINITY : (m_run[qb] + log2f(l)) * 0.69314718055994530942f;
+      } else if (has_rows) {
+        // In the order of the lanes.
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          *reinterpret_cast<f32x4*>(part + ((wave * QB + qb) * DB + db) * 256 + 4 * lane) = acc[db][qb];
+        if (j == 0) {
+          float* stats = part + BLOCK_M * DP + 2 * (row - row0);
+          stats[0] = m_run[qb], stats[1] = l;
+        }
+      }
+    }
+    if (!whole && first == 0 && tid == 0) p.splits[run] = {block, head, (int32_t)((before + span.count - 1) / share), 0};
+    at = before + last;
+    if (++block == blocks) block = 0, ++head;
+  }
+}
+
+// The parts of a split item joined: a thread has four elements of a row.
+constexpr int kPrefillJoinThreads = 256;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kPrefillJoinThreads) void prefill_join_kernel(const PrefillParams p) {
+  constexpr int DB = DP / 16;
+  const int run = blockIdx.x;
+  const PrefillSplit split = p.splits[run];
+  if (split.block < 0) return;
+  const PrefillBlock b = p.blocks[split.block];
+  const PrefillSequence seq = prefill_sequence(p, b.sequence);
+  const int chunk = blockIdx.y * kPrefillJoinThreads + threadIdx.x;  // 4 elements, in the parts' order
+  const int lane = chunk & 63, d = 16 * ((chunk >> 6) % DB) + 4 * (lane >> 4);
+  const int local = (chunk >> 6) / DB * 16 + (lane & 15), row = b.row + local;
+  if (row >= seq.count * p.group || d >= p.head_dim) return;
+  const int64_t size = prefill_part_floats(p.rows, DP);
+  const auto part = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == run)) * size; };
+  float top = -INFINITY;
+  for (int i = run; i <= split.last; ++i) top = fmaxf(top, part(i)[p.rows * DP + 2 * local]);
+  float weight = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = run; i <= split.last; ++i) {
+    const float* x = part(i);
+    const float f = prefill_ratio(x[p.rows * DP + 2 * local], top);
+    weight += x[p.rows * DP + 2 * local + 1] * f;
+    sum += *reinterpret_cast<const f32x4*>(x + 4 * chunk) * f;
+  }
+  const int query = prefill_query(p, row), q_head = split.head * p.group + row - query * p.group;
+  u32x2 o = {0, 0};
+  if (!(weight == 0.f)) o[0] = T::pack(sum[0] / weight, sum[1] / weight), o[1] = T::pack(sum[2] / weight, sum[3] / weight);
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + d) = o;
+  if (p.lse != nullptr && d == 0)
+    p.lse[q_head * p.lse_h + seq.from + query] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.69314718055994530942f;
+}
+
+template <typename T, int DP, int QB, PageKind kKind>
+hipError_t launch_prefill(const PrefillLaunch& l) {
+  constexpr int stages = kKind == kRowPages ? (QB == 1 && DP <= 128 ? 4 : 2) : DP == 256 ? 1 : 2;
+  prefill_kernel<T, DP, QB, kKind, stages><<<l.p.runs, kPrefillThreads, 0, l.stream>>>(l.p);
+  const hipError_t status = hipGetLastError();
+  if (status != hipSuccess) return status;
+  constexpr int chunks = 128 * QB * DP / 4;
+  prefill_join_kernel<T, DP><<<dim3(l.p.runs, chunks / kPrefillJoinThreads), kPrefillJoinThreads, 0, l.stream>>>(l.p);
+  return hipGetLastError();
+}
+
+template <typename T, int DP, int QB>
+hipError_t launch_prefill(const PrefillLaunch& l) {
+  return l.kind == kE4m3Pages ? launch_prefill<T, DP, QB, kE4m3Pages>(l)
+         : l.kind == kInt8Pages ? launch_prefill<T, DP, QB, kInt8Pages>(l)
+                                : launch_prefill<T, DP, QB, kRowPages>(l);
+}
+
+template <int DP>
+hipError_t launch_prefill(const PrefillLaunch& l) {
+  constexpr int many = prefill_rows(DP, true) / 128;
+  if (l.p.rows == 128) return l.bf16 ? launch_prefill<Bf16, DP, 1>(l) : launch_prefill<Fp16, DP, 1>(l);
+  return l.bf16 ? launch_prefill<Bf16, DP, many>(l) : launch_prefill<Fp16, DP, many>(l);
+}
+
+}  // namespace
+}  // namespace sa

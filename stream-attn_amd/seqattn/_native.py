@@ -159,13 +159,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sa_pipeline_kernel_busy": (
         c_int32, [c_void_p, ctypes.POINTER(c_double), ctypes.POINTER(c_double), ctypes.POINTER(c_int64)]
     ),
-    # Their argument structs are packed bytes (seqattn.kernels.rows, .blocks, .decode).
+    # Their argument structs are packed bytes (seqattn.kernels.rows, .blocks, .decode, .prefill).
     "sa_normalize_rotate_store": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
     "sa_read_kv": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
     "sa_append_kv_blocks": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
     "sa_paged_decode": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
     "sa_paged_window_decode": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
     "sa_paged_decode_workspace_bytes": (c_int32, [ctypes.c_char_p, c_int32, ctypes.POINTER(c_int64)]),
+    "sa_paged_prefill": (c_int32, [ctypes.c_char_p, c_int32, c_void_p]),
+    "sa_paged_prefill_workspace_bytes": (c_int32, [ctypes.c_char_p, c_int32, ctypes.POINTER(c_int64)]),
     "sa_pipeline_stream": (c_void_p, [c_void_p, c_int32]),
     "sa_pipeline_output_slot": (c_void_p, [c_void_p, c_int32]),
     "sa_pipeline_q_buffer": (c_void_p, [c_void_p]),

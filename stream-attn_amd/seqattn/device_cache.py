@@ -13,6 +13,7 @@ import torch
 from . import _native
 from .kernels.blocks import append_kv_blocks
 from .kernels.decode import paged_decode_attention
+from .kernels.prefill import paged_prefill_attention
 from .kernels.rows import MAX_PAGE_TOKENS, append_kv, check_sequences, normalize_rotate_append, read_kv
 
 
@@ -136,9 +137,13 @@ class DeviceKVCache:
         return read_kv(self.k_pages, self.v_pages, slots, k_scales=self.k_scales, v_scales=self.v_scales,
                        dtype=self.dtype)
 
-    def attend(self, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, **options):
-        return paged_decode_attention(q, self.k_pages, self.v_pages, page_table, lengths, k_scales=self.k_scales,
-                                      v_scales=self.v_scales, **options)
+    def attend(self, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+               cu_tokens: torch.Tensor | None = None, **options):
+        """One token per sequence (:func:`paged_decode_attention`), or with ``cu_tokens`` several."""
+        scales = dict(k_scales=self.k_scales, v_scales=self.v_scales)
+        if cu_tokens is None:
+            return paged_decode_attention(q, self.k_pages, self.v_pages, page_table, lengths, **scales, **options)
+        return paged_prefill_attention(q, self.k_pages, self.v_pages, page_table, lengths, cu_tokens, **scales, **options)
 
 
 __all__ = ["DeviceKVCache"]

@@ -7,6 +7,7 @@ library through its C ABI; ``triton_is_available`` is kept as an alias of
 
 from .blocks import append_kv_blocks
 from .decode import paged_decode_attention
+from .prefill import paged_prefill_attention
 from .rows import append_kv, normalize_rotate_append, normalize_rotate_qk, read_kv
 from .streaming import (
     finalize_attention,
@@ -24,6 +25,7 @@ __all__ = [
     "normalize_rotate_append",
     "normalize_rotate_qk",
     "paged_decode_attention",
+    "paged_prefill_attention",
     "read_kv",
     "triton_is_available",
     "update_attention_state",

@@ -144,3 +144,46 @@ def test_window_decode_entry_point_rejects_bad_arguments_without_a_gpu():
     assert call(dim=12) == -3 and call(dtype=5) == -2
     assert lib.sa_paged_window_decode(None, 0, None) == -1
     assert call(sequences=0, window=5, sinks=2, kind=2, block=32) == 0
+
+
+@built
+def test_prefill_entry_point_rejects_bad_arguments_without_a_gpu():
+    import ctypes
+
+    from seqattn.kernels.prefill import _PREFILL_ARGS
+
+    lib = _native.lib()
+    names = ("q k v ks vs table lengths cu out lse workspace workspace_bytes qt qh ot oh pp pt ph sp st sh table_stride "
+             "lse_stride tokens num_pages scale sequences max_pages q_heads kv_heads dim page dtype kind window sinks block _"
+             ).split()
+
+    def args(**fields):
+        values = dict.fromkeys(names, 0)
+        values.update(q=16, k=16, v=16, table=4, lengths=4, cu=4, out=16, workspace=16, tokens=5, num_pages=2, scale=0.1,
+                      sequences=2, max_pages=2, q_heads=4, kv_heads=2, dim=64, page=32)
+        values.update(fields)
+        return _PREFILL_ARGS.pack(*(values[n] for n in names))
+
+    for fields, status, word in (
+        (dict(dtype=7), -2, b"dtype"), (dict(dim=12), -3, b"head_dim"), (dict(dim=264), -3, b"head_dim"),
+        (dict(kind=1, dim=72), -3, b"multiple of 16"), (dict(kind=3), -1, b"kind"), (dict(kind=-1), -1, b"kind"),
+        (dict(q_heads=5), -1, b"multiple of kv_heads"), (dict(kv_heads=0), -1, b"multiple of kv_heads"),
+        (dict(tokens=-1), -1, b"2^31"), (dict(tokens=2**30), -1, b"2^31"), (dict(sequences=2**30 + 1), -1, b"2^30"),
+        (dict(page=0), -1, b"2^20"), (dict(num_pages=2**27), -1, b"2^31"), (dict(max_pages=2**27), -1, b"2^31"),
+        (dict(window=-1), -1, b"window"), (dict(sinks=2), -1, b"window"), (dict(window=1, sinks=-1), -1, b"window"),
+        (dict(kind=2, block=24), -1, b"power of two"), (dict(num_pages=0), -1, b"at least one page"),
+        (dict(qt=4), -1, b"multiples of 8"), (dict(pp=4), -1, b"16 bytes"), (dict(kind=1, ph=8), -1, b"16 bytes"),
+        (dict(q=8), -1, b"aligned"), (dict(cu=0), -1, b"missing"), (dict(cu=2), -1, b"aligned"), (dict(table=0), -1, b"missing"),
+        (dict(kind=1), -1, b"missing"), (dict(kind=1, ks=1, vs=2), -1, b"aligned"), (dict(kind=2, ks=1, vs=1, k=8, block=16), -1, b"aligned"),
+        (dict(workspace=0), -1, b"workspace"), (dict(workspace_bytes=1000), -1, b"workspace"),
+    ):
+        assert lib.sa_paged_prefill(args(**fields), 0, None) == status, fields
+        assert word in lib.sa_last_error(), (fields, lib.sa_last_error())
+    assert lib.sa_paged_prefill(None, 0, None) == -1
+    for nothing in (dict(tokens=0), dict(sequences=0)):
+        assert lib.sa_paged_prefill(args(**nothing), 0, None) == 0
+    needed = ctypes.c_int64()
+    assert lib.sa_paged_prefill_workspace_bytes(args(), 0, ctypes.byref(needed)) == 0 and needed.value > 0
+    assert lib.sa_paged_prefill_workspace_bytes(args(tokens=0), 0, ctypes.byref(needed)) == 0 and needed.value == 0
+    assert lib.sa_paged_prefill_workspace_bytes(args(dim=12), 0, ctypes.byref(needed)) == -3
+    assert lib.sa_paged_prefill_workspace_bytes(None, 0, ctypes.byref(needed)) == -1
