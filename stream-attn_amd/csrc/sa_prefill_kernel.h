@@ -30,17 +30,32 @@ __device__ inline __attribute__((always_inline)) T uniform(T x) {
 // 2^x of a running maximum's change: 0 from -inf, 1 where nothing changes.
 __device__ inline float prefill_ratio(float from, float to) { return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to); }
 
-// The halves of a dword that are infinite or NaN, as a mask.
+// Bits 15 and 31: the halves of a dword that are infinite or NaN (all ones in the
+// exponent, which one more carries over).
 template <typename T>
 __device__ inline uint32_t not_finite(uint32_t w) {
-  constexpr uint32_t e = std::is_same_v<T, Bf16> ? 0x7f80u : 0x7c00u;
-  return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+  constexpr bool bf16 = std::is_same_v<T, Bf16>;
+  return ((w & (bf16 ? 0x7f807f80u : 0x7c007c00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+// Halves of ones where those bits are.
+__device__ inline uint32_t halves(uint32_t m) { return (m - (m >> 15)) | m; }
+
+// The kernel's arguments, read again where they are used: what only a piece's ends
+// and masked steps need would otherwise sit in scalar registers, and those that do
+// not fit in lanes of vector registers, all through the loop over the tiles.
+typedef const PrefillParams SA_CONSTANT* PrefillArguments;
+__device__ inline PrefillArguments prefill_arguments() {
+  PrefillArguments a = (PrefillArguments)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
 }
 
 template <typename T, int DP, int QB, PageKind kKind, int STAGES>
 __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillParams p) {
   using Geo = Geometry<DP>;
   constexpr bool QUANT = kKind != kRowPages;
+  // INT8 in bfloat16: V's values as they are, weights times V's scales.
+  constexpr bool SCALED_P = kKind == kInt8Pages && std::is_same_v<T, Bf16>;
   constexpr int CK = Geo::CK, DB = Geo::DB;
   constexpr int KB = DP == 256 ? (QB == 1 ? 4 : 2) : CK;
   constexpr int VB = DP == 256 ? (QB == 1 ? 8 : 4) : DP == 128 && QB > 1 ? 8 : 4;
@@ -106,9 +121,6 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     // the sinks, every key (before wave_first) from low_last on.
     const int qw0 = row0 + wave * 16 * QB;
     const bool has_rows = qw0 < rows;
-    int pos[QB];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) pos[qb] = seq.base + prefill_query(p, min(qw0 + 16 * qb + r16, rows - 1));
     const int pos_first = uniform(seq.base + prefill_query(p, min(qw0, rows - 1)));
     const int pos_last = uniform(seq.base + prefill_query(p, min(qw0 + 16 * QB, rows) - 1));
     const int wave_end = has_rows ? pos_last + 1 : 0, wave_first = pos_first + 1;
@@ -116,90 +128,129 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     const int low_last = (int)max((int64_t)pos_last - p.window + 1, (int64_t)0);
 
     // ---- loads ----
-    // Issuing wave w has keys 16 w .. + 15 of every tile: one page's where pages are
-    // multiples of 16.  Lane l holds the page of tile ids_first + l.
-    int32_t ids = -1, ids_first = first - 64;
-    const auto page_of = [&](int key, int& row) {
-      const int number = (int)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift);
-      row = key - number * p.page_tokens;
-      return number;
-    };
-    const auto id_of = [&](int tile) {
-      if (tile - ids_first >= 64) {
-        ids_first = tile;
-        int row;
-        const int number = tile + lane < last ? page_of(span.key_of(tile + lane) + 16 * wave, row) : p.max_pages;
-        ids = number < p.max_pages ? table[number] : -1;
-      }
-      return __builtin_amdgcn_readlane(ids, tile - ids_first);
-    };
+    // Issuing wave w has keys 16 w .. + 15 of every tile, in one page where pages are
+    // multiples of 16.  Lane l then holds where those of tile held_first + l are, and
+    // their block's scales.
     constexpr int ES = QUANT ? 1 : 2;
     const char* k_head = p.k + head * p.sh * ES;
     const char* v_head = p.v + head * p.sh * ES;
-    auto dma = [](const char* at, uint8_t* dst) __attribute__((always_inline)) {
-      __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)at, (SA_LDS void*)dst, 16, 0, 0);
+    int held_first = first - 64;
+    uint32_t at_lo = 0, at_hi = 0;
+    uint64_t in_pool = 0;  // of the tiles held
+    float k_scale = 0.f, v_scale = 0.f;
+    const auto page_of = [](const auto& a, int key, int& row) {
+      const int number = (int)((uint64_t)(uint32_t)key * a.page_magic >> a.page_shift);
+      row = key - number * a.page_tokens;
+      return number;
     };
-    float scale_next = 0.f;  // a scale of the raw tile in flight
+    // The page and row of a key; a row that exists, read and not used, where there is no page.
+    const auto find = [&](const auto& a, int key, int& row, bool& ok) {
+      const int number = page_of(a, key, row);
+      int id = number < a.max_pages ? table[number] : -1;
+      ok = (uint32_t)id < (uint32_t)a.num_pages;
+      if (!ok) id = row = 0;
+      return id;
+    };
+    const auto hold = [&](int tile) {
+      const auto& a = *prefill_arguments();
+      held_first = tile;
+      int row;
+      bool ok;
+      const int id = find(a, span.key_of(min(tile + lane, last - 1)) + 16 * wave, row, ok);
+      const int64_t at = id * a.sp + row * a.st;
+      at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
+      in_pool = __ballot(ok);
+      if constexpr (kKind == kE4m3Pages) {
+        const int64_t scale = id * a.ssp + (row >> a.block_log2) * a.sst + head * a.ssh;
+        k_scale = e8m0_value(static_cast<const uint8_t*>(a.ks)[scale]);
+        v_scale = e8m0_value(static_cast<const uint8_t*>(a.vs)[scale]);
+      }
+    };
+    // A wave-uniform address plus 32 bits per lane.
+    auto dma = [](const char* base, uint32_t offset, uint8_t* dst) __attribute__((always_inline)) {
+      asm volatile("" : "+s"(base));
+      __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)(base + offset), (SA_LDS void*)dst, 16, 0, 0);
+    };
+    // Scales of the raw tile in flight: INT8 lane l's of key l % 16, K's (l < 16) or V's.
+    float scale_next = 0.f;
     // Tile `tile`: its 16-bit rows to the stage, or its bytes to the raw buffer.
     auto issue_tile = [&](int tile, uint8_t* to) __attribute__((always_inline)) {
       if (!issues) return;
-      const int key0 = span.key_of(tile) + 16 * wave;
-      // A lane's key: one of the run's 16.
-      const int lane_key = QUANT ? (lane * 16) / DP : lane >> 2;
-      constexpr int KEYS = QUANT ? 1024 / DP : 16;  // of a wave-wide load
-      uint32_t seen = 0;
-#pragma unroll
-      for (int x = 0; x < 16 / KEYS; ++x) {
-        int64_t offset;
-        int32_t id, row;
-        if (p.any_page) {
-          const int number = page_of(key0 + x * KEYS + lane_key, row);
-          id = number < p.max_pages ? table[number] : -1;
-        } else {
-          id = id_of(tile);
-          page_of(key0, row);
-          row += x * KEYS + lane_key;
-        }
-        const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
-        if (!ok) id = 0, row = 0;  // a row that exists, read and not used
-        offset = (id * p.sp + row * p.st) * ES;
-        const uint64_t held = __ballot(ok);
+      int l = lane;
+      if constexpr (QB > 1 && DP >= 128) asm volatile("" : "+v"(l));  // lane offsets anew: registers are short
+      const int key = QUANT ? l * 16 / DP : l >> 2;  // a lane's of a wave-wide load's
+      constexpr int KEYS = QUANT ? 1024 / DP : 16;
+      uint32_t seen;
+      if (__builtin_expect(!p.any_page, 1)) {
+        if (tile - held_first >= 64) hold(tile);
+        const int x = tile - held_first;
+        const uint32_t lo = __builtin_amdgcn_readlane(at_lo, x), hi = __builtin_amdgcn_readlane(at_hi, x);
+        const int64_t at = (int64_t)((uint64_t)hi << 32 | lo) * ES;
+        seen = in_pool >> x & 1 ? 0xffffu : 0u;
+        // Without a page every lane reads row 0 of one that exists.
+        const uint32_t step = seen ? (uint32_t)p.st * ES : 0u;
         if constexpr (QUANT) {
-          constexpr int LANES = DP / 16;  // of a key
-          uint32_t bits = 0;
+          const int d = l * 16 % DP;
+          const uint32_t offset = key * step + (d < p.head_dim ? d : 0);
 #pragma unroll
-          for (int i = 0; i < KEYS; ++i) bits |= (uint32_t)(held >> (i * LANES) & 1) << i;
-          seen |= bits << (x * KEYS);
-          const int d = (lane * 16) % DP;
-          const int64_t src = offset + (d < p.head_dim ? d : 0);
-          dma(k_head + src, to + wave * 16 * DP + x * 1024);
-          dma(v_head + src, to + RAW_BYTES + wave * 16 * DP + x * 1024);
+          for (int i = 0; i < 16 / KEYS; ++i) {
+            dma(k_head + at + (int64_t)i * KEYS * step, offset, to + wave * 16 * DP + i * 1024);
+            dma(v_head + at + (int64_t)i * KEYS * step, offset, to + RAW_BYTES + wave * 16 * DP + i * 1024);
+          }
+          if constexpr (kKind == kE4m3Pages)
+            scale_next = __builtin_bit_cast(float, j & 1 ? __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), x)
+                                                         : __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), x));
         } else {
+          const int kd = 8 * Geo::k_granule((l & 3) ^ (l >> 4)), vd = 8 * ((l & 3) ^ (2 * ((l >> 4) & 1)));
+          const uint32_t k_offset = key * step + kd * ES, v_offset = key * step + vd * ES;
+          if (__builtin_expect(p.head_dim == DP, 1)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) seen |= (uint32_t)(held >> (4 * i) & 1) << i;
-          const int kd = 8 * Geo::k_granule((lane & 3) ^ (lane >> 4)), vd = 8 * ((lane & 3) ^ (2 * ((lane >> 4) & 1)));
-#pragma unroll
-          for (int c = 0; c < CK; ++c) {
-            if (32 * c + kd < p.head_dim) dma(k_head + offset + (32 * c + kd) * ES, to + (CK * wave + c) * 1024);
-            if (32 * c + vd < p.head_dim)
-              dma(v_head + offset + (32 * c + vd) * ES, to + Geo::TILE_BYTES + (4 * c + wave) * 1024);
+            for (int c = 0; c < CK; ++c) {
+              dma(k_head + at + 32 * c * ES, k_offset, to + (CK * wave + c) * 1024);
+              dma(v_head + at + 32 * c * ES, v_offset, to + Geo::TILE_BYTES + (4 * c + wave) * 1024);
+            }
+          } else {
+            for (int c = 0; c < CK; ++c) {
+              if (32 * c + kd < p.head_dim) dma(k_head + at + 32 * c * ES, k_offset, to + (CK * wave + c) * 1024);
+              if (32 * c + vd < p.head_dim)
+                dma(v_head + at + 32 * c * ES, v_offset, to + Geo::TILE_BYTES + (4 * c + wave) * 1024);
+            }
+          }
+        }
+      } else {
+        // Pages that end anywhere: every lane looks for its key.
+        const auto& a = *prefill_arguments();
+        seen = 0;
+        for (int i = 0; i < 16 / KEYS; ++i) {
+          int row;
+          bool ok;
+          const int id = find(a, span.key_of(tile) + 16 * wave + i * KEYS + key, row, ok);
+          const char *k_row = k_head + (id * a.sp + row * a.st) * ES, *v_row = v_head + (id * a.sp + row * a.st) * ES;
+          const uint64_t held = __ballot(ok);
+          const auto dma_lane = [](const char* at, uint8_t* dst) {
+            __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)at, (SA_LDS void*)dst, 16, 0, 0);
+          };
+          for (int k = 0; k < KEYS; ++k) seen |= (uint32_t)(held >> (k * (64 / KEYS)) & 1) << (i * KEYS + k);
+          if constexpr (QUANT) {
+            const int d = l * 16 % DP < a.head_dim ? l * 16 % DP : 0;
+            dma_lane(k_row + d, to + wave * 16 * DP + i * 1024);
+            dma_lane(v_row + d, to + RAW_BYTES + wave * 16 * DP + i * 1024);
+          } else {
+            const int kd = 8 * Geo::k_granule((l & 3) ^ (l >> 4)), vd = 8 * ((l & 3) ^ (2 * ((l >> 4) & 1)));
+            for (int c = 0; c < CK; ++c) {
+              if (32 * c + kd < a.head_dim) dma_lane(k_row + (32 * c + kd) * ES, to + (CK * wave + c) * 1024);
+              if (32 * c + vd < a.head_dim) dma_lane(v_row + (32 * c + vd) * ES, to + Geo::TILE_BYTES + (4 * c + wave) * 1024);
+            }
           }
         }
       }
       if constexpr (kKind == kInt8Pages) {
-        // Lanes 0 - 15 K's, 16 - 31 V's of the run's keys.
-        int32_t id, row;
-        const int number = page_of(key0 + r16, row);
-        id = number < p.max_pages ? table[number] : -1;
-        if ((uint32_t)id >= (uint32_t)p.num_pages) id = 0, row = 0;
-        const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? p.vs : p.ks);
-        scale_next = Fp16::lo(from[id * p.ssp + row * p.sst + head * p.ssh]);
-      } else if constexpr (kKind == kE4m3Pages) {
-        int32_t id = id_of(tile), row;
-        page_of(key0, row);
-        if ((uint32_t)id >= (uint32_t)p.num_pages) id = 0, row = 0;
-        const uint8_t* from = static_cast<const uint8_t*>(j & 1 ? p.vs : p.ks);
-        scale_next = e8m0_value(from[id * p.ssp + (row >> p.block_log2) * p.sst + head * p.ssh]);
+        const auto& a = *prefill_arguments();
+        int row;
+        bool ok;
+        const int id = find(a, span.key_of(tile) + 16 * wave + r16, row, ok);
+        const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? a.vs : a.ks);
+        scale_next = Fp16::lo(from[id * a.ssp + row * a.sst + head * a.ssh]);
       }
       if (lane == 0) seen_lds[tile & 3][wave] = (uint16_t)seen;
       __builtin_amdgcn_sched_barrier(0);
@@ -210,9 +261,11 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         if (issues && lane < 32) scale_lds[tile & 3][j][16 * wave + r16] = scale_next;
       }
     };
-    // A raw tile to 16 bits.  INT8: value * scale, at most float16's largest.  e4m3: K's
-    // values as they are (the scale is in the logits), V's times their power of
-    // two, exact in bfloat16; float16 has steps of its own below 2^-14.
+    // A raw tile to 16 bits.  K's values as they are, exact: their scales are in the
+    // logits.  V's INT8 too where the weights take the scales; in float16, where
+    // weights times a scale could leave the type's range, value * scale, at most the
+    // type's largest.  V's e4m3 times their power of two: exact in bfloat16, float16
+    // has steps of its own below 2^-14.
     auto dequant = [&](int tile, const uint8_t* from, uint8_t* stage) __attribute__((always_inline)) {
       constexpr int GR = Geo::I8_GR;
 #pragma unroll
@@ -228,10 +281,11 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
           u32x4 o[2];
           if constexpr (kKind == kInt8Pages) {
             // med3 of NaN bounds is NaN.
-            const float most = std::is_same_v<T, Bf16> ? INFINITY : scale == scale ? 65504.f : NAN;
+            const bool as_is = tensor == 0 || SCALED_P;
+            const float most = scale == scale ? 65504.f : NAN;
             const auto value = [&](int e) {
-              const float y = byte_float(w[e / 4], e & 3) * scale;
-              return std::is_same_v<T, Bf16> ? y : __builtin_amdgcn_fmed3f(y, -most, most);
+              const float y = byte_float(w[e / 4], e & 3);
+              return as_is ? y : __builtin_amdgcn_fmed3f(y * scale, -most, most);
             };
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = T::pack(value(2 * e), value(2 * e + 1));
@@ -311,12 +365,6 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         if (key0 + kSubKeys <= low_first && key0 >= p.sinks) continue;
         const uint32_t held = (uint32_t)(seen >> rb);
         const bool masked = key0 + kSubKeys > wave_first || (key0 < low_last && key0 + kSubKeys > p.sinks) || held != ~0u;
-        // Whether row r16 of query block qb sees key k of the step.
-        const auto sees = [&](int qb, int k) {
-          const int key = key0 + k;
-          return key <= pos[qb] && (pos[qb] - key < p.window || key < p.sinks) && (held >> k & 1);
-        };
-
         f32x4 st[2][QB];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -345,7 +393,36 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
             factor[kb] = f < 1.17549435e-38f ? 1.17549435e-38f : f;  // times -inf it is -inf; NaN stays
           }
         }
+        f32x4 v_factor[2];
+        if constexpr (kKind == kInt8Pages) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const f32x4 f = *reinterpret_cast<const f32x4*>(&scale_lds[tile & 3][0][rb + 16 * kb + 4 * j]);
+            if constexpr (SCALED_P) v_factor[kb] = *reinterpret_cast<const f32x4*>(&scale_lds[tile & 3][1][rb + 16 * kb + 4 * j]);
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) st[kb][qb] *= f;
+          }
+        }
+        // Bit 4 kb + i: row r16 of the query block sees the lane's key 16 kb + 4 j + i.
+        uint32_t sees[QB];
         if (__builtin_expect(masked, 0)) {
+          const auto& a = *prefill_arguments();
+          int l = r16;
+          asm volatile("" : "+v"(l));
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) {
+            // Keys behind the row's position: from behind -> 0 on are seen, in a window's reach.
+            const int behind = seq.base + prefill_query(a, min(qw0 + 16 * qb + l, rows - 1)) - key0 - 4 * j;
+            const int sinks = a.sinks - key0 - 4 * j;
+            sees[qb] = 0;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int k = x / 4 * 16 + x % 4;
+              const bool near = (uint32_t)(behind - k) < (uint32_t)a.window, sink = (behind >= k) & (k < sinks);
+              sees[qb] |= (uint32_t)(near | sink) << x;
+            }
+            sees[qb] &= (held >> (4 * j) & 15) | (held >> (16 + 4 * j) & 15) << 4;
+          }
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             // A scale of NaN is one for those that see its keys.
@@ -355,7 +432,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                st[kb][qb][i] = !sees(qb, 16 * kb + 4 * j + i) ? -INFINITY : none ? NAN : st[kb][qb][i];
+                st[kb][qb][i] = !(sees[qb] >> (4 * kb + i) & 1) ? -INFINITY : none ? NAN : st[kb][qb][i];
           }
         }
         auto exps = [&](int qb, float neg_m, u32x4& pq) -> float {
@@ -367,7 +444,16 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
               const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e], factor[kb], neg_m));
               const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e + 1], factor[kb], neg_m));
               sum = (kb == 0 && e == 0) ? p0 + p1 : sum + (p0 + p1);
-              pq[2 * kb + e] = T::pack(p0, p1);
+              if constexpr (SCALED_P) {
+                float a = p0 * v_factor[kb][2 * e], b = p1 * v_factor[kb][2 * e + 1];
+                if (masked) {  // 0 * NaN is not 0
+                  a = sees[qb] >> (4 * kb + 2 * e) & 1 ? a : 0.f;
+                  b = sees[qb] >> (4 * kb + 2 * e + 1) & 1 ? b : 0.f;
+                }
+                pq[2 * kb + e] = T::pack(a, b);
+              } else {
+                pq[2 * kb + e] = T::pack(p0, p1);
+              }
             }
           return sum;
         };
@@ -411,22 +497,26 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         for (int qb = 0; qb < QB; ++qb) l_part[qb] += psum[qb];
 
         const uint32_t v_addr = base + Geo::TILE_BYTES + v_lane, v_odd = base + Geo::TILE_BYTES + (v_lane ^ 32);
-        uint32_t bad = 0;
 #pragma unroll
         for (int d0 = 0; d0 < DB; d0 += VB) {
           u32x4 vf[VB];
           read_v(vf, v_addr, v_odd, d0 / 2 * 4096 + rb * 64);
           // A key that not every row sees: 0 * NaN is not 0, so what is not finite stays
           // out of the products.
+          bool odd = false;
           if (__builtin_expect(masked, 0)) {
+            uint32_t bad = 0;
 #pragma unroll
             for (int dd = 0; dd < VB; ++dd)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t off = not_finite<T>(vf[dd][i]);
-                bad |= off;
-                vf[dd][i] &= ~off;
-              }
+              for (int i = 0; i < 4; ++i) bad |= not_finite<T>(vf[dd][i]);
+            odd = __any(bad != 0);
+            if (__builtin_expect(odd, 0)) {
+#pragma unroll
+              for (int dd = 0; dd < VB; ++dd)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vf[dd][i] &= ~halves(not_finite<T>(vf[dd][i]));
+            }
           }
 #pragma unroll
           for (int dd = 0; dd < VB; ++dd)
@@ -435,23 +525,25 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
               const int qb = dd % 2 == 0 ? i : QB - 1 - i;
               acc[d0 + dd][qb] = T::mma(vf[dd], pf[qb], acc[d0 + dd][qb]);
             }
-        }
-        if (__builtin_expect(masked && __any(bad != 0), 0)) {
-          // And makes the elements of those that see it not finite.
-          for (int k = 0; k < kSubKeys; ++k) {
-            for (int db = 0; db < DB; ++db) {
-              const int d = 16 * db + 4 * j;
-              const u32x2 w = *reinterpret_cast<const u32x2*>(stage + Geo::TILE_BYTES + Geo::v_offset(rb + k, d >> 3) + 2 * (d & 7));
-              const uint32_t off[2] = {not_finite<T>(w[0]), not_finite<T>(w[1])};
-              if (!__any((off[0] | off[1]) != 0)) continue;
+          if (__builtin_expect(odd, 0)) {
+            // The elements of the rows that see one: their number, as a product of ones.
+            constexpr uint32_t kOnes = std::is_same_v<T, Bf16> ? 0x3f803f80u : 0x3c003c00u;
+            read_v(vf, v_addr, v_odd, d0 / 2 * 4096 + rb * 64);
 #pragma unroll
-              for (int x = 0; x < DB; ++x) {
-                if (x != db) continue;
+            for (int qb = 0; qb < QB; ++qb) {
+              u32x4 seers;
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb)
+              for (int x = 0; x < 4; ++x)
+                seers[x] = kOnes & ((sees[qb] >> (2 * x) & 1 ? 0xffffu : 0u) | (sees[qb] >> (2 * x + 1) & 1 ? 0xffff0000u : 0u));
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if ((off[e >> 1] >> (16 * (e & 1)) & 1) && sees(qb, k)) acc[x][qb][e] = NAN;
+              for (int dd = 0; dd < VB; ++dd) {
+                u32x4 ones;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ones[i] = halves(not_finite<T>(vf[dd][i])) & kOnes;
+                const f32x4 count = T::mma(ones, seers, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (count[e] > 0.f) acc[d0 + dd][qb][e] = NAN;
               }
             }
           }
@@ -517,8 +609,9 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     }
 
     // ---- the piece's end ----
+    const auto& a = *prefill_arguments();
     const bool whole = first == 0 && last == span.count;
-    float* part = p.parts + ((int64_t)run * 2 + (first == 0)) * prefill_part_floats(BLOCK_M, DP);
+    float* part = a.parts + ((int64_t)run * 2 + (first == 0)) * prefill_part_floats(BLOCK_M, DP);
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       float l = l_part[qb] + __shfl_xor(l_part[qb], 16);
@@ -526,18 +619,18 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
       const int row = qw0 + 16 * qb + r16;
       if (whole) {
         if (row >= rows) continue;
-        const int query = prefill_query(p, row), q_head = head * p.group + row - query * p.group;
-        uint16_t* to = p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + 4 * j;
+        const int query = prefill_query(a, row), q_head = head * a.group + row - query * a.group;
+        uint16_t* to = a.out + (int64_t)(seq.from + query) * a.so_t + (int64_t)q_head * a.so_h + 4 * j;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          if (16 * db + 4 * j >= p.head_dim) continue;
-          const f32x4& a = acc[db][qb];
+          if (16 * db + 4 * j >= a.head_dim) continue;
+          const f32x4& x = acc[db][qb];
           u32x2 o = {0, 0};
-          if (!(l == 0.f)) o[0] = T::pack(a[0] / l, a[1] / l), o[1] = T::pack(a[2] / l, a[3] / l);
+          if (!(l == 0.f)) o[0] = T::pack(x[0] / l, x[1] / l), o[1] = T::pack(x[2] / l, x[3] / l);
           *reinterpret_cast<u32x2*>(to + 16 * db) = o;
         }
-        if (p.lse != nullptr && j == 0)
-          p.lse[q_head * p.lse_h + seq.from + query] = l == 0.f ? -INFINITY : (m_run[qb] + log2f(l)) * 0.69314718055994530942f;
+        if (a.lse != nullptr && j == 0)
+          a.lse[q_head * a.lse_h + seq.from + query] = l == 0.f ? -INFINITY : (m_run[qb] + log2f(l)) * 0.69314718055994530942f;
       } else if (has_rows) {
         // In the order of the lanes.
 #pragma unroll
@@ -549,7 +642,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         }
       }
     }
-    if (!whole && first == 0 && tid == 0) p.splits[run] = {block, head, (int32_t)((before + span.count - 1) / share), 0};
+    if (!whole && first == 0 && tid == 0) a.splits[run] = {block, head, (int32_t)((before + span.count - 1) / share), 0};
     at = before + last;
     if (++block == blocks) block = 0, ++head;
   }
