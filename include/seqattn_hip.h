@@ -761,8 +761,8 @@ int32_t sa_paged_window_decode(const sa_window_decode_args* args, int32_t device
  * j <= p, with a window only those with p - j < window and the first `sinks`.
  * Pages, scales, page_table and lengths as for sa_paged_window_decode; a token
  * that sees no key gets output 0 and LSE -inf, rows past
- * cu_tokens[sequences] stay as they are.  INT8 values enter in q's type, and so do
- * e4m3 ones of V (float16: at most its largest value).
+ * cu_tokens[sequences] stay as they are.  V's 8-bit values times their scale enter
+ * in q's type (float16: at most its largest value).
  *
  * 8-bit pages: head_dim and strides are multiples of 16, pages 16-byte aligned.
  * tokens * q_heads / kv_heads is below 2^31 - 4096.  `workspace`

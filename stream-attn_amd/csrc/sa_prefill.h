@@ -25,7 +25,9 @@ struct PrefillBlock {
 };
 struct PrefillPlan {
   int64_t tiles;  // of all blocks
-  int32_t blocks, pad;
+  int32_t blocks;
+  int32_t whole;    // items are not split, each XCD's workgroups take its items in turn
+  int32_t next[8];  // of every XCD
 };
 // An item (a K/V head's block) that is split over runs first .. last.
 struct PrefillSplit {
@@ -62,6 +64,9 @@ struct PrefillLaunch {
 
 // Rows of a workgroup: 128 or, with many rows, what the registers hold.
 constexpr int prefill_rows(int padded_dim, bool many) { return !many ? 128 : padded_dim == 128 ? 384 : 256; }
+
+// Workgroups of a CU.
+constexpr int prefill_occupancy(int padded_dim) { return padded_dim == 64 ? 2 : 1; }
 
 // One padded head_dim each.
 hipError_t launch_prefill_d64(const PrefillLaunch& l);

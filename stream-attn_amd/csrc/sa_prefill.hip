@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefill_plan_kernel(const Prefil
     if (i < blocks) p.blocks[i] = {tiles + upto - count, s, row};
     tiles += of_all;
   }
-  if (tid == 0) *p.plan = {tiles, blocks, 0};
+  if (tid == 0) *p.plan = {tiles, blocks, (int64_t)blocks * p.kv_heads >= 4 * p.runs, {}};
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -130,7 +130,7 @@ Workspace workspace(const sa_prefill_args* a) {
   const int64_t rows = a->tokens * (a->q_heads / a->kv_heads);
   const int many = prefill_rows(dim, true);
   w.rows = rows >= (int64_t)a->sequences * many * 2 ? many : 128;
-  w.runs = kPrefillCUs;
+  w.runs = kPrefillCUs * prefill_occupancy(dim);
   w.max_blocks = std::min(rows, rows / w.rows + a->sequences);
   const auto next = [](int64_t at) { return (at + 255) & ~(int64_t)255; };
   w.blocks = next(sizeof(PrefillPlan));

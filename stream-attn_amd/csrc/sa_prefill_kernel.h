@@ -51,11 +51,9 @@ __device__ inline PrefillArguments prefill_arguments() {
 }
 
 template <typename T, int DP, int QB, PageKind kKind, int STAGES>
-__global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillParams p) {
+__global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void prefill_kernel(const PrefillParams p) {
   using Geo = Geometry<DP>;
   constexpr bool QUANT = kKind != kRowPages;
-  // INT8 in bfloat16: V's values as they are, weights times V's scales.
-  constexpr bool SCALED_P = kKind == kInt8Pages && std::is_same_v<T, Bf16>;
   constexpr int CK = Geo::CK, DB = Geo::DB;
   constexpr int KB = DP == 256 ? (QB == 1 ? 4 : 2) : CK;
   constexpr int VB = DP == 256 ? (QB == 1 ? 8 : 4) : DP == 128 && QB > 1 ? 8 : 4;
@@ -64,10 +62,10 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
   constexpr int RAW_BYTES = Geo::I8_TILE_BYTES;  // of K or V of a raw tile
   __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE_BYTES];
   __shared__ __attribute__((aligned(1024))) uint8_t raw[QUANT ? 4 * RAW_BYTES : 16];
-  // Of the tiles in flight: which keys are in a page of the pool, and the scales of
-  // K and V (INT8 by key, e4m3 by run of 16 keys).
+  // Of the tiles in flight: which keys are in a page of the pool; by key what a logit's
+  // FMA multiplies it by, and what K's and V's values are converted with.
   __shared__ __attribute__((aligned(8))) uint16_t seen_lds[4][4];
-  __shared__ __attribute__((aligned(16))) float scale_lds[QUANT ? 4 : 1][2][kTileKeys];
+  __shared__ __attribute__((aligned(16))) float scale_lds[QUANT ? 4 : 1][3][kTileKeys];
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r16 = lane & 15, j = lane >> 4;
@@ -80,7 +78,8 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
   const int64_t total = tiles * p.kv_heads, share = (total + p.runs - 1) / p.runs;
   const int64_t begin = run * share, end = begin + share < total ? begin + share : total;
   if (tid == 0) p.splits[run].block = -1;
-  if (begin >= end) return;
+  const bool whole_items = uniform(p.plan->whole);
+  if (total == 0 || (!whole_items && begin >= end)) return;
 
   // Elements of K past head_dim are zeros that no tile writes.
   if (p.head_dim < DP) {
@@ -89,8 +88,9 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
   }
 
   // The block that the run starts in: 64 of them looked at at once.
-  int head = (int)(begin / tiles), block = 0;
-  {
+  int head = 0, block = 0;
+  if (!whole_items) {
+    head = (int)(begin / tiles);
     const int64_t into = begin - head * tiles;
     for (int left = blocks; left > 1;) {
       const int step = (left + 63) >> 6, at = lane * step;
@@ -101,8 +101,22 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     }
   }
 
+  // Whole items: the next of this XCD's.
+  __shared__ int32_t next_lds;
+  constexpr int kFetcher = kPrefillThreads - 64;  // a wave that issues no loads
+  const int xcd = blockIdx.x & 7;
+  int fetched = 0;
+  if (whole_items && tid == kFetcher) next_lds = atomicAdd(&p.plan->next[xcd], 1);
+
   const float cf = scale_factor(p.scale_log2);
-  for (int64_t at = begin; at < end;) {
+  for (int64_t at = begin; whole_items || at < end;) {
+    __syncthreads();  // the stages are free (and, at first, cleared)
+    if (whole_items) {
+      const int item = 8 * uniform(next_lds) + xcd;
+      if (item >= blocks * p.kv_heads) break;
+      block = blocks - 1 - item / p.kv_heads, head = item % p.kv_heads;
+      if (tid == kFetcher) fetched = atomicAdd(&p.plan->next[xcd], 1);
+    }
     // ---- a piece: tiles first .. last - 1 of an item ----
     const int64_t before = uniform(p.blocks[block].before) + head * tiles;
     const int s = uniform(p.blocks[block].sequence), row0 = uniform(p.blocks[block].row);
@@ -111,8 +125,8 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     const int rows = min(seq.count * p.group, row0 + BLOCK_M);  // end of the block's rows
     PrefillTiles span = prefill_tiles(p, seq, row0, rows);
     span.count = uniform(span.count), span.sinks = uniform(span.sinks), span.skip = uniform(span.skip);
-    const int first = (int)(at - before);
-    const int last = (int)min((int64_t)span.count, end - before);
+    const int first = whole_items ? 0 : (int)(at - before);
+    const int last = whole_items ? span.count : (int)min((int64_t)span.count, end - before);
     const int ntiles = last - first;
     const int32_t* table = p.table + s * p.s_table;
 
@@ -135,7 +149,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
     const char* k_head = p.k + head * p.sh * ES;
     const char* v_head = p.v + head * p.sh * ES;
     int held_first = first - 64;
-    uint32_t at_lo = 0, at_hi = 0;
+    uint32_t at_lo = 0, at_hi = 0, scale_lo = 0, scale_hi = 0;
     uint64_t in_pool = 0;  // of the tiles held
     float k_scale = 0.f, v_scale = 0.f;
     const auto page_of = [](const auto& a, int key, int& row) {
@@ -165,6 +179,10 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         k_scale = e8m0_value(static_cast<const uint8_t*>(a.ks)[scale]);
         v_scale = e8m0_value(static_cast<const uint8_t*>(a.vs)[scale]);
       }
+      if constexpr (kKind == kInt8Pages) {
+        const int64_t scale = id * a.ssp + row * a.sst + head * a.ssh;
+        scale_lo = (uint32_t)scale, scale_hi = (uint32_t)(scale >> 32);
+      }
     };
     // A wave-uniform address plus 32 bits per lane.
     auto dma = [](const char* base, uint32_t offset, uint8_t* dst) __attribute__((always_inline)) {
@@ -172,7 +190,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
       __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)(base + offset), (SA_LDS void*)dst, 16, 0, 0);
     };
     // Scales of the raw tile in flight: INT8 lane l's of key l % 16, K's (l < 16) or V's.
-    float scale_next = 0.f;
+    std::conditional_t<kKind == kInt8Pages, uint16_t, float> scale_next = 0;
     // Tile `tile`: its 16-bit rows to the stage, or its bytes to the raw buffer.
     auto issue_tile = [&](int tile, uint8_t* to) __attribute__((always_inline)) {
       if (!issues) return;
@@ -245,27 +263,51 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
         }
       }
       if constexpr (kKind == kInt8Pages) {
-        const auto& a = *prefill_arguments();
-        int row;
-        bool ok;
-        const int id = find(a, span.key_of(tile) + 16 * wave + r16, row, ok);
-        const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? a.vs : a.ks);
-        scale_next = Fp16::lo(from[id * a.ssp + row * a.sst + head * a.ssh]);
+        const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? p.vs : p.ks);
+        if (__builtin_expect(!p.any_page, 1)) {
+          const int x = tile - held_first;
+          const uint32_t lo = __builtin_amdgcn_readlane(scale_lo, x), hi = __builtin_amdgcn_readlane(scale_hi, x);
+          from += (int64_t)((uint64_t)hi << 32 | lo) + (seen ? r16 * p.sst : 0);
+        } else {
+          const auto& a = *prefill_arguments();
+          int row;
+          bool ok;
+          const int id = find(a, span.key_of(tile) + 16 * wave + r16, row, ok);
+          from += id * a.ssp + row * a.sst + head * a.ssh;
+        }
+        scale_next = *from;
       }
       if (lane == 0) seen_lds[tile & 3][wave] = (uint16_t)seen;
       __builtin_amdgcn_sched_barrier(0);
     };
-    // The scales that came with raw tile `tile`, by the waves that loaded them.
+    // The scales that came with raw tile `tile`, by the waves that loaded them.  K's go
+    // into the logits, their sign (and NaN) into the values; a factor of at least the
+    // smallest normal keeps a masked logit at -inf.
     auto put_scales = [&](int tile) __attribute__((always_inline)) {
       if constexpr (QUANT) {
-        if (issues && lane < 32) scale_lds[tile & 3][j][16 * wave + r16] = scale_next;
+        float scale;
+        if constexpr (kKind == kInt8Pages)
+          scale = Fp16::lo(scale_next);
+        else
+          scale = scale_next;
+        if (!issues || lane >= 32) return;
+        float(&to)[3][kTileKeys] = scale_lds[tile & 3];
+        const int key = 16 * wave + r16;
+        if (j == 0) {
+          to[0][key] = scale == scale ? fmaxf(fabsf(scale) * cf, 1.17549435e-38f) : cf;
+          to[1][key] = scale == scale ? (scale < 0.f ? -1.f : 1.f) : NAN;
+        } else {
+          to[2][key] = scale;
+        }
       }
     };
     // A raw tile to 16 bits.  K's values as they are, exact: their scales are in the
-    // logits.  V's INT8 too where the weights take the scales; in float16, where
-    // weights times a scale could leave the type's range, value * scale, at most the
-    // type's largest.  V's e4m3 times their power of two: exact in bfloat16, float16
-    // has steps of its own below 2^-14.
+    // logits.  V's times their scale: INT8 rounded once, e4m3 times a power of two,
+    // exact in bfloat16 (float16 has steps of its own below 2^-14).  In float16 at
+    // most the type's largest value, which the product of a row's largest can pass by a
+    // rounding.  (Weights times V's INT8 scales instead, values exact: one rounding
+    // less, 0.0023 instead of 0.0027 of the output's norm, and registers short, 950
+    // instead of 1,000 TFLOP/s at head_dim 128 and an eighth at 256.)
     auto dequant = [&](int tile, const uint8_t* from, uint8_t* stage) __attribute__((always_inline)) {
       constexpr int GR = Geo::I8_GR;
 #pragma unroll
@@ -277,20 +319,19 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
 #pragma unroll
         for (int tensor = 0; tensor < 2; ++tensor) {
           const u32x4 w = *reinterpret_cast<const u32x4*>(from + tensor * RAW_BYTES + row * DP + gr * 16);
-          const float scale = scale_lds[tile & 3][tensor][row];
+          const float scale = scale_lds[tile & 3][1 + tensor][row];
           u32x4 o[2];
           if constexpr (kKind == kInt8Pages) {
             // med3 of NaN bounds is NaN.
-            const bool as_is = tensor == 0 || SCALED_P;
             const float most = scale == scale ? 65504.f : NAN;
             const auto value = [&](int e) {
-              const float y = byte_float(w[e / 4], e & 3);
-              return as_is ? y : __builtin_amdgcn_fmed3f(y * scale, -most, most);
+              const float y = byte_float(w[e / 4], e & 3) * scale;
+              return tensor == 0 || std::is_same_v<T, Bf16> ? y : __builtin_amdgcn_fmed3f(y, -most, most);
             };
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = T::pack(value(2 * e), value(2 * e + 1));
           } else {
-            const float power = tensor == 0 ? 1.f : scale;
+            const float power = scale;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               o[e / 2][2 * (e & 1)] = T::template e4m3_pair<false>(w[e], power);
@@ -317,7 +358,6 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
       }
     };
 
-    __syncthreads();  // the stages are free (and, at first, cleared)
     if constexpr (!QUANT) {
       for (int t = 0; t < min(ntiles, STAGES - 1); ++t) issue_tile(first + t, lds + t * STAGE_BYTES);
     } else {
@@ -384,24 +424,14 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
                 st[kb][qb] = T::mma(kf[kb * KB + c], qf[qb][c0 + c], st[kb][qb]);
               }
         }
-        // What a logit's FMA multiplies it by: e4m3's with the scale of its 16 keys.
-        float factor[2] = {cf, cf};
-        if constexpr (kKind == kE4m3Pages) {
+        // By what a logit's FMA multiplies it: of all keys, e4m3's of 16 keys, INT8's of each.
+        constexpr bool BY_KEY = kKind == kInt8Pages;
+        f32x4 factor[2];
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const float f = cf * scale_lds[tile & 3][0][rb + 16 * kb];
-            factor[kb] = f < 1.17549435e-38f ? 1.17549435e-38f : f;  // times -inf it is -inf; NaN stays
-          }
-        }
-        f32x4 v_factor[2];
-        if constexpr (kKind == kInt8Pages) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 f = *reinterpret_cast<const f32x4*>(&scale_lds[tile & 3][0][rb + 16 * kb + 4 * j]);
-            if constexpr (SCALED_P) v_factor[kb] = *reinterpret_cast<const f32x4*>(&scale_lds[tile & 3][1][rb + 16 * kb + 4 * j]);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) st[kb][qb] *= f;
-          }
+        for (int kb = 0; kb < 2; ++kb) {
+          const float* at = &scale_lds[QUANT ? tile & 3 : 0][0][rb + 16 * kb];
+          const float f = QUANT ? at[0] : cf;
+          factor[kb] = BY_KEY ? *reinterpret_cast<const f32x4*>(at + 4 * j) : f32x4{f, f, f, f};
         }
         // Bit 4 kb + i: row r16 of the query block sees the lane's key 16 kb + 4 j + i.
         uint32_t sees[QB];
@@ -424,16 +454,11 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
             sees[qb] &= (held >> (4 * j) & 15) | (held >> (16 + 4 * j) & 15) << 4;
           }
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            // A scale of NaN is one for those that see its keys.
-            const bool none = kKind == kE4m3Pages && factor[kb] != factor[kb];
-            if (none) factor[kb] = cf;
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                st[kb][qb][i] = !(sees[qb] >> (4 * kb + i) & 1) ? -INFINITY : none ? NAN : st[kb][qb][i];
-          }
+              for (int i = 0; i < 4; ++i) st[kb][qb][i] = sees[qb] >> (4 * kb + i) & 1 ? st[kb][qb][i] : -INFINITY;
         }
         auto exps = [&](int qb, float neg_m, u32x4& pq) -> float {
           float sum = 0.f;
@@ -441,19 +466,10 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e], factor[kb], neg_m));
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e + 1], factor[kb], neg_m));
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e], factor[kb][2 * e], neg_m));
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e + 1], factor[kb][2 * e + 1], neg_m));
               sum = (kb == 0 && e == 0) ? p0 + p1 : sum + (p0 + p1);
-              if constexpr (SCALED_P) {
-                float a = p0 * v_factor[kb][2 * e], b = p1 * v_factor[kb][2 * e + 1];
-                if (masked) {  // 0 * NaN is not 0
-                  a = sees[qb] >> (4 * kb + 2 * e) & 1 ? a : 0.f;
-                  b = sees[qb] >> (4 * kb + 2 * e + 1) & 1 ? b : 0.f;
-                }
-                pq[2 * kb + e] = T::pack(a, b);
-              } else {
-                pq[2 * kb + e] = T::pack(p0, p1);
-              }
+              pq[2 * kb + e] = T::pack(p0, p1);
             }
           return sum;
         };
@@ -477,8 +493,13 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
             const bool mine = (fold >> r16) & 1u;
             float full = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-              full = fmaxf(full, fmaxf(fmaxf(st[kb][qb][0], st[kb][qb][1]), fmaxf(st[kb][qb][2], st[kb][qb][3])) * factor[kb]);
+            for (int kb = 0; kb < 2; ++kb) {
+              if constexpr (BY_KEY)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) full = fmaxf(full, st[kb][qb][i] * factor[kb][i]);
+              else
+                full = fmaxf(full, fmaxf(fmaxf(st[kb][qb][0], st[kb][qb][1]), fmaxf(st[kb][qb][2], st[kb][qb][3])) * factor[kb][0]);
+            }
             full = fmaxf(full, __shfl_xor(full, 16));
             full = fmaxf(full, __shfl_xor(full, 32));
             const float m_new = (mine && full > m_run[qb] + kRescaleThreshold) ? full : m_run[qb];
@@ -643,6 +664,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(const PrefillP
       }
     }
     if (!whole && first == 0 && tid == 0) a.splits[run] = {block, head, (int32_t)((before + span.count - 1) / share), 0};
+    if (whole_items && tid == kFetcher) next_lds = fetched;
     at = before + last;
     if (++block == blocks) block = 0, ++head;
   }

@@ -62,9 +62,8 @@ def paged_prefill_attention(
     ``-inf``.  Rows of ``out`` past ``cu_tokens[-1]`` are not written.
 
     Logits, softmax and sums are FP32, a weight enters the product with V in
-    ``q``'s dtype.  INT8 values times their scale enter in ``q``'s dtype, and so do
-    e4m3 ones of V (exact in bfloat16; float16: at most its largest value); 8-bit
-    pages need a head_dim and strides in multiples of 16.  A logit of NaN or ``+inf``
+    ``q``'s dtype.  V's 8-bit values times their scale enter in ``q``'s dtype (e4m3
+    ones are exact in bfloat16; float16: at most its largest value); 8-bit pages need a head_dim and strides in multiples of 16.  A logit of NaN or ``+inf``
     makes its row NaN, one of ``-inf`` is a key without weight; an element of a seen V
     that is not finite makes its element of ``out`` not finite.  ``out`` may be ``q``,
     and shares no memory with the rest.  Returns ``out`` (like ``q``), and with

@@ -6,10 +6,10 @@ the product with V rounded to q's type (h = 2^-8 or 2^-11 of it; in float16, who
 steps end at 2^-24, also by 2^-25 of the row's largest weight), everything else
 is FP32 (2^-15 covers the exponential and sums of thousands of keys).  So the
 output is off by (2 e + h + 2^-15) times the sum of weight * |v|, with float16 also
-keys 2^-25 max |v|, plus its rounding, and the LSE by e + 2^-19 (1 + |lse|).  INT8 values
-times their scale are rounded to q's type: h more of the sums of |q k| in e and
-of the weighted |v|.  e4m3 values are exact but for V in float16, whose steps
-end at 2^-24.
+keys 2^-25 max |v|, plus its rounding, and the LSE by e + 2^-19 (1 + |lse|).  K's 8-bit
+values are exact, their scales a rounding more of the logits (in the 4); V's INT8
+values times their scale are rounded to q's type, h more; e4m3 ones are exact but
+for float16, whose steps end at 2^-24.
 """
 
 from __future__ import annotations
@@ -111,7 +111,7 @@ def check(data, page, window=None, sinks=0, scale=None, out=None, padding=0, kin
     ref, ref_lse, size, products, most = reference(q, stand, table, lengths, cu, page, scale, window, sinks)
     half = HALF_STEP[q.dtype]
     rounded = half if kind == "int8" else 0.0
-    e = ((q.shape[2] + 4) * 2.0**-24 + 2 * rounded) * products
+    e = (q.shape[2] + 4) * 2.0**-24 * products
     bound = half * ref.abs() + (1 + half) * (2 * e.t()[..., None] + half + rounded + 2.0**-15) * size + 2.0**-24
     if q.dtype == torch.float16:
         bound += most * 2.0**-25 * float(size.max())
