@@ -19,9 +19,9 @@ constexpr int kDecodeTile = 32;  // keys of a wave's step
 // one, 383 with two, also though two leave it 3 to 5 registers short (16 to 24
 // bytes of scratch); with 9 query heads 433 and 369.  16-bit pages there, with more
 // to spill, 443 and 522.
-constexpr int decode_occupancy(int padded_dim, int blocks, bool bytes) {
-  if (padded_dim == 256 || (padded_dim == 128 && blocks == 2 && !bytes)) return 1;
-  return bytes && padded_dim == 64 && blocks == 1 ? 4 : 2;
+constexpr int decode_occupancy(int padded_dim, int blocks, PageKind kind) {
+  if (padded_dim == 256 || (padded_dim == 128 && blocks == 2 && kind == kRowPages)) return 1;
+  return kind != kRowPages && padded_dim == 64 && blocks == 1 ? 4 : 2;
 }
 constexpr int kDecodeCUs = 256;
 constexpr int kMaxWorkgroups = 4 * kDecodeCUs;

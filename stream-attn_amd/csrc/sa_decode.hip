@@ -41,14 +41,17 @@ int padded(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 12
 // Workgroups of a launch: what the chip holds at once.  A launch over fewer
 // tiles leaves some without work.
 bool wide(const sa_decode_args* a) { return a->q_heads / a->kv_heads > 8; }
-int workgroups(const sa_decode_args* a) {
-  return kDecodeCUs * decode_occupancy(padded(a->head_dim), wide(a) ? 2 : 1, a->pages_int8 != 0);
+PageKind kind_of(const sa_decode_args* a) {
+  return a->pages_int8 == SA_PAGES_E4M3 ? kE4m3Pages : a->pages_int8 ? kInt8Pages : kRowPages;
+}
+int workgroups(const sa_decode_args* a, PageKind kind) {
+  return kDecodeCUs * decode_occupancy(padded(a->head_dim), wide(a) ? 2 : 1, kind);
 }
 
 // owned, then parts.
-int64_t owned_bytes(const sa_decode_args* a) { return (int64_t)workgroups(a) * 16; }
-int64_t workspace_bytes(const sa_decode_args* a) {
-  return owned_bytes(a) + (int64_t)workgroups(a) * 2 * (wide(a) ? 16 : 8) * (padded(a->head_dim) + 2) * 4;
+int64_t owned_bytes(const sa_decode_args* a, PageKind kind) { return (int64_t)workgroups(a, kind) * 16; }
+int64_t workspace_bytes(const sa_decode_args* a, PageKind kind) {
+  return owned_bytes(a, kind) + (int64_t)workgroups(a, kind) * 2 * (wide(a) ? 16 : 8) * (padded(a->head_dim) + 2) * 4;
 }
 
 }  // namespace
@@ -61,7 +64,7 @@ int32_t sa_paged_decode_workspace_bytes(const sa_decode_args* a, int32_t device,
   sa::clear_error();
   if (a == nullptr || bytes == nullptr) return sa::invalid("null arguments");
   const int32_t rc = sa::check(a);
-  *bytes = rc == 0 && a->sequences > 0 ? sa::workspace_bytes(a) : 0;
+  *bytes = rc == 0 && a->sequences > 0 ? sa::workspace_bytes(a, sa::kind_of(a)) : 0;
   return rc;
 }
 
@@ -91,7 +94,7 @@ int32_t run(const sa_decode_args* a, PageKind kind, int32_t window, int32_t sink
       !aligned(a->page_table, 4) || !aligned(a->lengths, 4) || !aligned(a->lse, 4) ||
       (kind != kE4m3Pages && (!aligned(a->k_scales, 2) || !aligned(a->v_scales, 2))))
     return invalid("an operand is missing or not aligned");
-  if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a))
+  if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < workspace_bytes(a, kind))
     return invalid("the workspace is missing, too small or not aligned");
   if (a->stride_pt < 0 || a->stride_pt >= (1 << 26))
     return invalid("the pages' token stride must be below 2^26 elements");
@@ -120,8 +123,8 @@ int32_t run(const sa_decode_args* a, PageKind kind, int32_t window, int32_t sink
   p.page_shift = 31 + n;
   p.page_magic = (uint32_t)(((uint64_t)1 << p.page_shift) / (uint32_t)p.page_tokens + 1);
   p.owned = static_cast<int32_t*>(a->workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + owned_bytes(a));
-  launch.workgroups = workgroups(a);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + owned_bytes(a, kind));
+  launch.workgroups = workgroups(a, kind);
   p.by_item = (int64_t)a->sequences * p.kv_heads * p.blocks <= launch.workgroups;
   p.window = window, p.sinks = sinks, p.block_log2 = log2;
   launch.bf16 = a->dtype == SA_DTYPE_BF16, launch.kind = kind;

@@ -167,6 +167,10 @@ struct Reader {
     if (upto - first_id >= 64) {
       first_id = n;
       ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
+      // Waited for here: behind the branch the wait would be for every load in flight,
+      // in each step (96 sequences over 1,048,576 keys, e4m3 447 us, here 353; INT8 362 and
+      // 353, with heads of 256 over 500,000 keys 443 and 368).
+      asm volatile("" : "+v"(ids));
     }
   }
   __device__ inline int32_t id_of(const DecodeParams& p, int32_t n, int lane) {
@@ -240,6 +244,20 @@ struct Step {
       // Two runs of 16 keys, each in one page.
       full = within(p, key0);
       const uint32_t rows = j * (uint32_t)p.st * ES;
+      // Loads return in their order, and the scales are needed before the next step's
+      // loads are issued, V's rows are not: the scales go first.
+      if constexpr (kKind == kE4m3Pages) {
+        const uint8_t* s = reinterpret_cast<const uint8_t*>(second ? p.vs : p.ks) + x.kv_head * p.ssh;
+        int32_t n = page, r = row;
+        int64_t at[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && (r += 16) >= p.page_tokens) ++n, r -= p.page_tokens;
+          const int32_t id = from.id_of(p, n, lane);
+          at[h] = ((uint32_t)id < (uint32_t)p.num_pages ? id : 0) * p.ssp + (r >> p.block_log2) * p.sst;
+        }
+        scale = s[g & 4 ? at[1] : at[0]];
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (h == 1 && (row += 16) >= p.page_tokens) ++page, row -= p.page_tokens;
@@ -259,10 +277,6 @@ struct Step {
         if constexpr (kKind == kInt8Pages) {
           const uint16_t* s = (second ? p.vs : p.ks) + id * p.ssp + row * p.sst + x.kv_head * p.ssh;
           if ((g >> 2 & 1) == h) scale = s[(4 * (g & 3) + j) * p.sst];
-        }
-        if constexpr (kKind == kE4m3Pages) {
-          const uint8_t* s = reinterpret_cast<const uint8_t*>(second ? p.vs : p.ks);
-          if ((g >> 2 & 1) == h) scale = s[id * p.ssp + (row >> p.block_log2) * p.sst + x.kv_head * p.ssh];
         }
         const uint32_t mask = ok ? 15u : 0u;
         seen = h == 0 ? mask : seen | mask << 4;
@@ -316,7 +330,7 @@ struct PartInfo {
 // it are done there; the others' parts meet in LDS, and those of items that
 // leave the workgroup's run in the workspace.
 template <typename T, PageKind kKind, int DP, int NB, bool kAnyPage>
-__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kKind != kRowPages)) void decode_kernel(
+__global__ __launch_bounds__(64 * kDecodeWaves, decode_occupancy(DP, NB, kKind)) void decode_kernel(
     const DecodeParams p) {
   constexpr bool kInt8 = kKind == kInt8Pages, kE4m3 = kKind == kE4m3Pages;
   using S = Shape<DP>;
