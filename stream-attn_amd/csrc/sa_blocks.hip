@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "sa_common.h"
 #include "sa_types.h"
@@ -26,9 +27,10 @@ namespace {
 constexpr int kAppendWaves = 4;
 // Workgroups over the blocks of a launch; every one looks at all sequences.
 constexpr int64_t kMaxBlockGroups = 4096;
-// Rows (of one granule per lane) that a wave holds between the block's largest
-// magnitude and its codes.
-constexpr int kHeldRows = 16;
+// Loads of a wave (a granule of a row per lane each) that it holds between the
+// block's largest magnitude and its codes; and about as many of a block's rows as
+// a wave takes, so that there are waves enough.
+constexpr int kHeldLoads = 4, kWaveLoads = 4;
 
 struct AppendParams {
   const uint16_t *k, *v;
@@ -36,6 +38,7 @@ struct AppendParams {
   const int32_t *table, *lengths, *cu;
   int64_t sk_t, sk_h, sv_t, sv_h, sp, st, sh, ssp, ssb, ssh, s_table, tokens;
   int32_t sequences, num_pages, room, kv_heads, head_dim, page_tokens, block_log2, lane_log2;
+  int32_t unit_log2;  // log2 of the waves of a block, K/V head and one of K and V
 };
 
 // The new rows of a sequence: positions start .. end - 1, rows row0 .. of k and v.
@@ -69,13 +72,33 @@ __device__ inline int32_t scale_byte(float x) {
   return byte < 1 ? 1 : byte;
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The halves of a dword that are infinite or NaN, as halves of ones.
 template <typename T>
-__device__ inline void floats_of(u32x4 x, float (&y)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[2 * i] = T::lo(x[i]), y[2 * i + 1] = T::hi(x[i]);
+__device__ inline uint32_t not_finite(uint32_t w) {
+  return ((w & T::kInfinity) == T::kInfinity ? 0xffffu : 0u) |
+         ((w >> 16 & T::kInfinity) == T::kInfinity ? 0xffff0000u : 0u);
 }
 
-__device__ inline bool finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) != 0x7f800000u; }
+// A lane's largest magnitudes, as the bits of 16-bit floats (which are in their
+// order); with kFinite of the finite ones.
+template <bool kFinite, typename T>
+__device__ inline u16x2 largest(u32x4 x, u16x2 top) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = x[i] & 0x7fff7fffu;
+    if (kFinite) w &= ~not_finite<T>(w);
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w));
+  }
+  return top;
+}
+
+__device__ inline uint32_t over_wave(u16x2 x) {
+  uint32_t top = x[0] > x[1] ? x[0] : x[1];
+  for (int i = 1; i < 64; i <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, i));
+  return top;
+}
 
 // Row `first` + step * i of this lane, or the last row (one of the same block, so
 // that the largest magnitude is the same): a load under a condition would wait for
@@ -89,89 +112,93 @@ struct RowReader {
   }
 };
 
+// A unit is the rows of one block, one K/V head and one of K and V, on 2^unit_log2
+// waves; a granule (8 elements) of a row is on each of 2^lane_log2 lanes.
+//
+// Measured: WWW
 template <typename T>
-__device__ inline float largest(u32x4 x, float top) {
-  float y[8];
-  floats_of<T>(x, y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = finite(y[i]) ? fmaxf(top, fabsf(y[i])) : top;
-  return top;
-}
-
-template <typename T>
-__device__ inline u32x2 codes_of(u32x4 x, int32_t shift) {
-  float y[8];
-  floats_of<T>(x, y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = finite(y[i]) ? __builtin_ldexpf(y[i], shift) : NAN;
-  return u32x2{e4m3_pack(y[0], y[1], y[2], y[3]), e4m3_pack(y[4], y[5], y[6], y[7])};
-}
-
-// A wave takes the rows of one block, one K/V head and one of K and V, a granule
-// (8 elements) of a row on each of 2^lane_log2 lanes.
-template <typename T>
-__global__ __launch_bounds__(64 * kAppendWaves) void append_blocks_kernel(const AppendParams p) {
+__global__ __launch_bounds__(64 * kAppendWaves, 6) void append_blocks_kernel(const AppendParams p) {
   __shared__ int64_t sums[kAppendWaves];
   __shared__ int64_t found[2];
+  __shared__ uint32_t tops[2][2 * kAppendWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int run = (p.sequences + 64 * kAppendWaves - 1) / (64 * kAppendWaves);
-  const int s_first = min(tid * run, p.sequences), s_last = min(s_first + run, p.sequences);
-  int64_t own = 0;
-  for (int s = s_first; s < s_last; ++s) own += new_rows(p, s).blocks(p.block_log2);
-  int64_t upto = own;  // inclusive
-  for (int i = 1; i < 64; i <<= 1) {
-    const int64_t x = __shfl_up(upto, i);
-    if (lane >= i) upto += x;
-  }
-  if (lane == 63) sums[wave] = upto;
-  __syncthreads();
-  int64_t total = 0;
-  for (int i = 0; i < kAppendWaves; ++i) {
-    if (i < wave) upto += sums[i];
-    total += sums[i];
-  }
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = blockIdx.x * share, end = min(begin + share, total);
-  if (begin >= upto - own && begin < upto) {
-    int64_t before = upto - own;
-    int s = s_first;
-    for (; s < s_last; ++s) {
-      const int64_t n = new_rows(p, s).blocks(p.block_log2);
-      if (begin < before + n) break;
-      before += n;
+  // Items are blocks that take rows, numbered sequence by sequence; with one row
+  // each, sequences.
+  int64_t begin, end, before;
+  int s;
+  if (p.cu == nullptr) {
+    const int64_t share = (p.sequences + gridDim.y - 1) / gridDim.y;
+    begin = before = blockIdx.y * share, end = min(begin + share, (int64_t)p.sequences);
+    s = (int)begin;
+    if (begin >= end) return;
+  } else {
+    const int run = (p.sequences + 64 * kAppendWaves - 1) / (64 * kAppendWaves);
+    const int s_first = min(tid * run, p.sequences), s_last = min(s_first + run, p.sequences);
+    int64_t own = 0;
+    for (int x = s_first; x < s_last; ++x) own += new_rows(p, x).blocks(p.block_log2);
+    int64_t upto = own;  // inclusive
+    for (int i = 1; i < 64; i <<= 1) {
+      const int64_t x = __shfl_up(upto, i);
+      if (lane >= i) upto += x;
     }
-    found[0] = s, found[1] = before;
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int64_t total = 0;
+    for (int i = 0; i < kAppendWaves; ++i) {
+      if (i < wave) upto += sums[i];
+      total += sums[i];
+    }
+    const int64_t share = (total + gridDim.y - 1) / gridDim.y;
+    begin = blockIdx.y * share, end = min(begin + share, total);
+    if (begin >= upto - own && begin < upto) {
+      int64_t ahead = upto - own;
+      int x = s_first;
+      for (; x < s_last; ++x) {
+        const int64_t n = new_rows(p, x).blocks(p.block_log2);
+        if (begin < ahead + n) break;
+        ahead += n;
+      }
+      found[0] = x, found[1] = ahead;
+    }
+    __syncthreads();
+    if (begin >= end) return;
+    s = __builtin_amdgcn_readfirstlane((int)found[0]);
+    before = found[1];
   }
-  __syncthreads();
-  const int unit = blockIdx.y * kAppendWaves + wave;
-  if (begin >= total || unit >= 2 * p.kv_heads) return;
-
+  // Waves past the last unit take it along: the workgroup's waves meet at barriers.
+  const int waves = 1 << p.unit_log2, part = wave & (waves - 1);
+  const int wanted = blockIdx.x * (kAppendWaves >> p.unit_log2) + (wave >> p.unit_log2);
+  const bool writes = wanted < 2 * p.kv_heads;
+  const int unit = min(wanted, 2 * p.kv_heads - 1);
   const bool is_v = unit >= p.kv_heads;
   const int head = is_v ? unit - p.kv_heads : unit;
-  const int g = lane & ((1 << p.lane_log2) - 1), r = lane >> p.lane_log2, step = 64 >> p.lane_log2;
+  const int g = lane & ((1 << p.lane_log2) - 1), per_load = 64 >> p.lane_log2;
+  const int r = part * per_load + (lane >> p.lane_log2), step = waves * per_load;
   const bool live = 8 * g < p.head_dim;
   const uint16_t* rows = is_v ? p.v + head * p.sv_h : p.k + head * p.sk_h;
   const int64_t stride = is_v ? p.sv_t : p.sk_t;
   uint8_t* pages = (is_v ? p.vp : p.kp) + head * p.sh;
   uint8_t* scales = (is_v ? p.vs : p.ks) + head * p.ssh;
-  int s = __builtin_amdgcn_readfirstlane((int)found[0]);
-  int64_t before = found[1];
   NewRows n = new_rows(p, s);
+  int turn = 0;
   for (int64_t at = begin; at < end; ++at) {
-    while (at >= before + n.blocks(p.block_log2)) before += n.blocks(p.block_log2), n = new_rows(p, ++s);
+    if (p.cu == nullptr) {
+      n = new_rows(p, (int)at), s = (int)at, before = at;
+      if (n.end <= n.start) continue;
+    } else {
+      while (at >= before + n.blocks(p.block_log2)) before += n.blocks(p.block_log2), n = new_rows(p, ++s);
+    }
     const int32_t block = (n.start >> p.block_log2) + (int32_t)(at - before), low = block << p.block_log2;
     const int32_t first = max(n.start, low), last = min(n.end, low + (1 << p.block_log2));
     const int32_t page = low / p.page_tokens, in_page = low - page * p.page_tokens;
     const int32_t id = p.table[s * p.s_table + page];
-    if ((uint32_t)id >= (uint32_t)p.num_pages) continue;
     const RowReader read{rows + (n.row0 + (first - n.start)) * stride + (live ? 8 * g : 0), stride, r, step, last - first};
-    const int32_t passes = (last - first + step - 1) / step;
+    const int32_t loads = (last - first + step - 1) / step;
 
-    u32x4 held[kHeldRows];
-    float top = 0.f;
+    u32x4 held[kHeldLoads];
 #pragma unroll
-    for (int i = 0; i < kHeldRows; i += 4) {
-      if (i < passes) {
+    for (int i = 0; i < kHeldLoads; i += 4) {
+      if (i < loads) {
 #pragma unroll
         for (int x = i; x < i + 4; ++x) held[x] = read(x);
       } else {
@@ -179,21 +206,36 @@ __global__ __launch_bounds__(64 * kAppendWaves) void append_blocks_kernel(const 
         for (int x = i; x < i + 4; ++x) held[x] = u32x4{0, 0, 0, 0};
       }
     }
+    if ((uint32_t)id >= (uint32_t)p.num_pages) continue;  // of all waves alike
     uint8_t* scale = scales + id * p.ssp + (in_page >> p.block_log2) * p.ssb;
     const int32_t old = *scale;
+    // What is not finite is rare: only where it comes up is it left out.
+    const auto top_of = [&](auto finite) {
+      u16x2 x = {0, 0};
 #pragma unroll
-    for (int i = 0; i < kHeldRows; ++i) top = largest<T>(held[i], top);
-    for (int i = kHeldRows; i < passes; ++i) top = largest<T>(read(i), top);
-    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
-    int32_t byte = scale_byte(top);
+      for (int i = 0; i < kHeldLoads; ++i) x = largest<decltype(finite)::value, T>(held[i], x);
+      for (int i = kHeldLoads; i < loads; ++i) x = largest<decltype(finite)::value, T>(read(i), x);
+      return over_wave(x);
+    };
+    uint32_t any = top_of(std::false_type()), top = any;
+    if (any >= T::kInfinity) top = top_of(std::true_type());
+    if (waves > 1) {
+      // A place is written again two barriers later.
+      if (lane == 0) tops[turn][2 * wave] = any, tops[turn][2 * wave + 1] = top;
+      __syncthreads();
+      for (int i = wave - part; i < wave - part + waves; ++i)
+        any = max(any, tops[turn][2 * i]), top = max(top, tops[turn][2 * i + 1]);
+      turn ^= 1;
+    }
+    int32_t byte = scale_byte(T::lo(top));
     if (first > low) byte = max(byte, old);
+    const float power = e8m0_value(byte);
 
     uint8_t* to = pages + id * p.sp + in_page * p.st + 8 * g;
-    if (first > low && byte != old) {
+    if (first > low && byte != old && live && writes) {
       // Rows of earlier calls, in the scale that is theirs now.
       const int32_t shift = old - byte;
       for (int32_t x = r; x < first - low; x += step) {
-        if (!live) continue;
         u32x2* row = reinterpret_cast<u32x2*>(to + x * p.st);
         u32x2 c = *row;
 #pragma unroll
@@ -207,13 +249,22 @@ __global__ __launch_bounds__(64 * kAppendWaves) void append_blocks_kernel(const 
     }
     to += (first - low + r) * p.st;
     const auto store = [&](int i, u32x4 x) __attribute__((always_inline)) {
-      if (live && r + step * i < last - first) *reinterpret_cast<u32x2*>(to + step * i * p.st) = codes_of<T>(x, 127 - byte);
+      u32x2 codes = {T::to_e4m3(x[0], x[1], power), T::to_e4m3(x[2], x[3], power)};
+      if (any >= T::kInfinity) {
+        // Infinities are NaN too.
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t off = not_finite<T>(x[w]), bytes = (off & 0x7f) | (off >> 16 & 0x7f) << 8;
+          codes[w / 2] |= bytes << (16 * (w & 1));
+        }
+      }
+      if (live && writes && r + step * i < last - first) *reinterpret_cast<u32x2*>(to + step * i * p.st) = codes;
     };
 #pragma unroll
-    for (int i = 0; i < kHeldRows; ++i)
-      if (i < passes) store(i, held[i]);
-    for (int i = kHeldRows; i < passes; ++i) store(i, read(i));
-    if (lane == 0) *scale = (uint8_t)byte;
+    for (int i = 0; i < kHeldLoads; ++i)
+      if (i < loads) store(i, held[i]);
+    for (int i = kHeldLoads; i < loads; ++i) store(i, read(i));
+    if (lane == 0 && part == 0 && writes) *scale = (uint8_t)byte;
   }
 }
 
@@ -274,7 +325,11 @@ extern "C" int32_t sa_append_kv_blocks(const sa_append_blocks_args* a, int32_t d
   // A sequence's rows are in at most two blocks more than they fill, and in no
   // more than there are rows.
   const int64_t blocks = std::min(a->tokens, (a->tokens >> p.block_log2) + 2 * (int64_t)a->sequences);
-  const dim3 grid((uint32_t)std::min(blocks, kMaxBlockGroups), (uint32_t)((2 * a->kv_heads + kAppendWaves - 1) / kAppendWaves));
+  const int64_t block_loads = (((int64_t)1 << p.block_log2) << p.lane_log2) / 64;  // of a wave alone
+  while ((1 << p.unit_log2) < kAppendWaves && (kWaveLoads << p.unit_log2) < block_loads && a->cu_tokens != nullptr) ++p.unit_log2;
+  const int64_t units = kAppendWaves >> p.unit_log2;  // of a workgroup
+  // Neighbouring workgroups have the heads of the same rows.
+  const dim3 grid((uint32_t)((2 * a->kv_heads + units - 1) / units), (uint32_t)std::min(blocks, kMaxBlockGroups));
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (a->dtype == SA_DTYPE_BF16)
     append_blocks_kernel<Bf16><<<grid, 64 * kAppendWaves, 0, hs>>>(p);

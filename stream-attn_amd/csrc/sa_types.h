@@ -31,6 +31,13 @@ struct Bf16 {
   __device__ static inline uint32_t e4m3_pair(uint32_t w, float power) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, kHalf));
   }
+  // The four values of two dwords over 2^e to e4m3, to nearest even; at most 448.
+  __device__ static inline uint32_t to_e4m3(uint32_t a, uint32_t b, float power) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const s16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(s16x2{0, 0}, __builtin_bit_cast(bf16x2, a), power, false);
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(bf16x2, b), power, true));
+  }
+  static constexpr uint32_t kInfinity = 0x7f80u;
   __device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -46,6 +53,12 @@ struct Fp16 {
   __device__ static inline uint32_t e4m3_pair(uint32_t w, float power) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, kHalf));
   }
+  __device__ static inline uint32_t to_e4m3(uint32_t a, uint32_t b, float power) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const s16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(s16x2{0, 0}, __builtin_bit_cast(f16x2, a), power, false);
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, __builtin_bit_cast(f16x2, b), power, true));
+  }
+  static constexpr uint32_t kInfinity = 0x7c00u;
   __device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
