@@ -37,6 +37,13 @@ __device__ inline uint32_t not_finite(uint32_t w) {
   constexpr bool bf16 = std::is_same_v<T, Bf16>;
   return ((w & (bf16 ? 0x7f807f80u : 0x7c007c00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
 }
+// The larger magnitudes of the halves, as bits.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ inline u16x2 larger(u16x2 top, uint32_t w) {
+  return __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+}
+// Bits 0 .. n - 1.
+__device__ inline uint32_t below(int n) { return n > 0 ? ~0u >> (32 - (n < 32 ? n : 32)) : 0u; }
 // Halves of ones where those bits are.
 __device__ inline uint32_t halves(uint32_t m) { return (m - (m >> 15)) | m; }
 
@@ -433,32 +440,28 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
           const float f = QUANT ? at[0] : cf;
           factor[kb] = BY_KEY ? *reinterpret_cast<const f32x4*>(at + 4 * j) : f32x4{f, f, f, f};
         }
-        // Bit 4 kb + i: row r16 of the query block sees the lane's key 16 kb + 4 j + i.
+        // Bit k: row r16 of the query block sees the lane's key 4 j + k of the step (k 0 - 3
+        // and 16 - 19 are its own).
         uint32_t sees[QB];
         if (__builtin_expect(masked, 0)) {
           const auto& a = *prefill_arguments();
           int l = r16;
           asm volatile("" : "+v"(l));
+          const uint32_t here = held >> (4 * j);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) {
-            // Keys behind the row's position: from behind -> 0 on are seen, in a window's reach.
             const int behind = seq.base + prefill_query(a, min(qw0 + 16 * qb + l, rows - 1)) - key0 - 4 * j;
-            const int sinks = a.sinks - key0 - 4 * j;
-            sees[qb] = 0;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const int k = x / 4 * 16 + x % 4;
-              const bool near = (uint32_t)(behind - k) < (uint32_t)a.window, sink = (behind >= k) & (k < sinks);
-              sees[qb] |= (uint32_t)(near | sink) << x;
-            }
-            sees[qb] &= (held >> (4 * j) & 15) | (held >> (16 + 4 * j) & 15) << 4;
+            sees[qb] = below(behind + 1) & here;
+            uint32_t near = ~below((int)max((int64_t)behind - a.window + 1, (int64_t)0));
+            if (key0 < a.sinks) near |= below(a.sinks - key0 - 4 * j);
+            sees[qb] &= near;
           }
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) st[kb][qb][i] = sees[qb] >> (4 * kb + i) & 1 ? st[kb][qb][i] : -INFINITY;
+              for (int i = 0; i < 4; ++i) st[kb][qb][i] = sees[qb] >> (16 * kb + i) & 1 ? st[kb][qb][i] : -INFINITY;
         }
         auto exps = [&](int qb, float neg_m, u32x4& pq) -> float {
           float sum = 0.f;
@@ -526,12 +529,12 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
           // out of the products.
           bool odd = false;
           if (__builtin_expect(masked, 0)) {
-            uint32_t bad = 0;
+            u16x2 top = {0, 0};
 #pragma unroll
             for (int dd = 0; dd < VB; ++dd)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) bad |= not_finite<T>(vf[dd][i]);
-            odd = __any(bad != 0);
+              for (int i = 0; i < 4; ++i) top = larger(top, vf[dd][i]);
+            odd = __any(top[0] >= T::kInfinity || top[1] >= T::kInfinity);
             if (__builtin_expect(odd, 0)) {
 #pragma unroll
               for (int dd = 0; dd < VB; ++dd)
@@ -555,7 +558,8 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
               u32x4 seers;
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                seers[x] = kOnes & ((sees[qb] >> (2 * x) & 1 ? 0xffffu : 0u) | (sees[qb] >> (2 * x + 1) & 1 ? 0xffff0000u : 0u));
+                seers[x] = kOnes & ((sees[qb] >> (x / 2 * 16 + 2 * (x & 1)) & 1 ? 0xffffu : 0u) |
+                                    (sees[qb] >> (x / 2 * 16 + 2 * (x & 1) + 1) & 1 ? 0xffff0000u : 0u));
 #pragma unroll
               for (int dd = 0; dd < VB; ++dd) {
                 u32x4 ones;
