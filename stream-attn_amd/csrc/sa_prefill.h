@@ -45,6 +45,7 @@ struct PrefillParams {
   PrefillPlan* plan;
   PrefillBlock* blocks;
   int32_t* first_block;  // of every sequence, the plan's
+  int32_t* order;        // whole items: the blocks, long ones first
   PrefillSplit* splits;  // by the run that an item starts in
   float* parts;          // two per run
   int64_t sq_t, sq_h, so_t, so_h, sp, st, sh, ssp, sst, ssh, s_table, lse_h, tokens;

@@ -15,6 +15,9 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSequences = 4096;  // whose first blocks LDS holds
+constexpr int kClasses = 8;           // of blocks, by their tiles
+// What splitting items costs a workgroup, in tiles: writing and joining the parts.
+constexpr int kSplitTiles = 10;
 
 // Inclusive sum over a workgroup's threads; `sums` has a place per wave and one more.
 __device__ inline int64_t scan(int64_t x, int64_t* sums, int64_t& total) {
@@ -39,6 +42,7 @@ __device__ inline int64_t scan(int64_t x, int64_t* sums, int64_t& total) {
 __global__ __launch_bounds__(kPlanThreads) void prefill_plan_kernel(const PrefillParams p) {
   __shared__ int64_t sums[kPlanThreads / 64];
   __shared__ int32_t first_lds[kPlanSequences];
+  __shared__ int32_t most, of_class[kClasses], done[kClasses], of_wave[kPlanThreads / 64][kClasses];
   const int tid = threadIdx.x;
   const bool in_lds = p.sequences <= kPlanSequences;
   const int run = (p.sequences + kPlanThreads - 1) / kPlanThreads;
@@ -57,12 +61,16 @@ __global__ __launch_bounds__(kPlanThreads) void prefill_plan_kernel(const Prefil
       p.first_block[s] = first;
     before += blocks_of(s);
   }
+  if (tid < kClasses) of_class[tid] = 0;
+  if (tid == 0) most = 1;
   __syncthreads();
   const int blocks = (int)min(all, (int64_t)p.max_blocks);  // more only if the starts are in disorder
   int64_t tiles = 0;
+  int count = 0;  // of the thread's last block
   for (int base = 0; base < blocks; base += kPlanThreads) {
     const int i = base + tid;
-    int s = 0, row = 0, count = 0;
+    int s = 0, row = 0;
+    count = 0;
     if (i < blocks) {
       // The last sequence whose first block is not past i.
       for (int left = p.sequences; left > 1;) {
@@ -76,10 +84,55 @@ __global__ __launch_bounds__(kPlanThreads) void prefill_plan_kernel(const Prefil
     }
     int64_t of_all;
     const int64_t upto = scan(count, sums, of_all);
-    if (i < blocks) p.blocks[i] = {tiles + upto - count, s, row};
+    if (i < blocks) p.blocks[i] = {tiles + upto - count, s, row}, atomicMax(&most, count);
     tiles += of_all;
   }
-  if (tid == 0) *p.plan = {tiles, blocks, (int64_t)blocks * p.kv_heads >= 4 * p.runs, {}};
+  __syncthreads();
+  // Whole items, long ones first, where their longest workgroup has hardly more than an
+  // equal share and splitting costs more.  A block's class: 0 has the longest.
+  const float class_tiles = (float)kClasses / (float)most;
+  const auto class_of = [&](int i) {
+    int tiles_of = count;
+    if (blocks > kPlanThreads) tiles_of = (int)((i + 1 < blocks ? p.blocks[i + 1].before : tiles) - p.blocks[i].before);
+    return max(0, kClasses - 1 - (int)((float)(tiles_of - 1) * class_tiles));
+  };
+  for (int i = tid; i < blocks; i += kPlanThreads) atomicAdd(&of_class[class_of(i)], 1);
+  __syncthreads();
+  float items = 0.f, longest = 0.f;
+  for (int c = 0; c < kClasses; ++c) {
+    items += (float)of_class[c] * (float)p.kv_heads;
+    longest = fmaxf(longest, ceilf(items / (float)p.runs) * ((float)(kClasses - c) - 0.5f) / class_tiles);
+  }
+  const bool whole = longest <= (float)tiles * (float)p.kv_heads / (float)p.runs + kSplitTiles;
+  if (whole) {
+    // The last blocks first, stable, so that neighbours stay together.
+    const int lane = tid & 63, wave = tid >> 6;
+    for (int chunk = 0; chunk < blocks; chunk += kPlanThreads) {
+      const int base = (blocks - 1 - chunk) / kPlanThreads * kPlanThreads, i = base + tid;  // whole chunks from the last on
+      const int mine = i < blocks ? class_of(i) : -1;
+      int behind = 0;  // of the class, on later lanes
+      for (int c = 0; c < kClasses; ++c) {
+        const uint64_t same = __ballot(mine == c);
+        if (mine == c) behind = __popcll(same >> 1 >> lane);
+        if (lane == 0) of_wave[wave][c] = __popcll(same);
+      }
+      __syncthreads();
+      if (mine >= 0) {
+        int at = behind;
+        for (int c = 0; c < mine; ++c) at += of_class[c];
+        for (int w = wave + 1; w < kPlanThreads / 64; ++w) at += of_wave[w][mine];
+        p.order[at + (chunk > 0 ? done[mine] : 0)] = i;
+      }
+      __syncthreads();
+      if (tid < kClasses) {
+        int sum = chunk > 0 ? done[tid] : 0;
+        for (int w = 0; w < kPlanThreads / 64; ++w) sum += of_wave[w][tid];
+        done[tid] = sum;
+      }
+      __syncthreads();
+    }
+  }
+  if (tid == 0) *p.plan = {tiles, blocks, whole, {}};
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -121,7 +174,7 @@ int padded(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 12
 // Where the parts of the workspace start.
 struct Workspace {
   int32_t rows, runs;
-  int64_t max_blocks, blocks, first_block, splits, parts, bytes;
+  int64_t max_blocks, blocks, order, first_block, splits, parts, bytes;
 };
 
 Workspace workspace(const sa_prefill_args* a) {
@@ -134,7 +187,8 @@ Workspace workspace(const sa_prefill_args* a) {
   w.max_blocks = std::min(rows, rows / w.rows + a->sequences);
   const auto next = [](int64_t at) { return (at + 255) & ~(int64_t)255; };
   w.blocks = next(sizeof(PrefillPlan));
-  w.first_block = next(w.blocks + w.max_blocks * (int64_t)sizeof(PrefillBlock));
+  w.order = next(w.blocks + w.max_blocks * (int64_t)sizeof(PrefillBlock));
+  w.first_block = next(w.order + w.max_blocks * 4);
   w.splits = next(w.first_block + (a->sequences > kPlanSequences ? a->sequences * (int64_t)4 : 0));
   w.parts = next(w.splits + w.runs * (int64_t)sizeof(PrefillSplit));
   w.bytes = w.parts + w.runs * 2 * prefill_part_floats(w.rows, dim) * 4;
@@ -188,7 +242,7 @@ int32_t sa_paged_prefill(const sa_prefill_args* a, int32_t device, void* stream)
   const Workspace w = workspace(a);
   if (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < w.bytes)
     return invalid("the workspace is missing, too small or not aligned");
-  if (w.max_blocks > INT32_MAX) return invalid("too many tokens and sequences");
+  if (w.max_blocks > INT32_MAX / a->kv_heads) return invalid("too many tokens and sequences");
   PrefillLaunch launch{};
   PrefillParams& p = launch.p;
   p.q = static_cast<const uint16_t*>(a->q), p.out = static_cast<uint16_t*>(a->out), p.lse = a->lse;
@@ -198,6 +252,7 @@ int32_t sa_paged_prefill(const sa_prefill_args* a, int32_t device, void* stream)
   char* base = static_cast<char*>(a->workspace);
   p.plan = reinterpret_cast<PrefillPlan*>(base);
   p.blocks = reinterpret_cast<PrefillBlock*>(base + w.blocks);
+  p.order = reinterpret_cast<int32_t*>(base + w.order);
   p.first_block = reinterpret_cast<int32_t*>(base + w.first_block);
   p.splits = reinterpret_cast<PrefillSplit*>(base + w.splits);
   p.parts = reinterpret_cast<float*>(base + w.parts);

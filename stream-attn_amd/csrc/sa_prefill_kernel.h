@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
     if (whole_items) {
       const int item = 8 * uniform(next_lds) + xcd;
       if (item >= blocks * p.kv_heads) break;
-      block = blocks - 1 - item / p.kv_heads, head = item % p.kv_heads;
+      block = uniform(p.order[item / p.kv_heads]), head = item % p.kv_heads;
       if (tid == kFetcher) fetched = atomicAdd(&p.plan->next[xcd], 1);
     }
     // ---- a piece: tiles first .. last - 1 of an item ----
@@ -674,8 +674,9 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
   }
 }
 
-// The parts of a split item joined: a thread has four elements of a row.
-constexpr int kPrefillJoinThreads = 256;
+// The parts of a split item joined: a thread has four elements of a row, a workgroup
+// every kPrefillJoiners'th of a block's runs of threads.
+constexpr int kPrefillJoinThreads = 256, kPrefillJoiners = 16;
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kPrefillJoinThreads) void prefill_join_kernel(const PrefillParams p) {
@@ -685,28 +686,46 @@ __global__ __launch_bounds__(kPrefillJoinThreads) void prefill_join_kernel(const
   if (split.block < 0) return;
   const PrefillBlock b = p.blocks[split.block];
   const PrefillSequence seq = prefill_sequence(p, b.sequence);
-  const int chunk = blockIdx.y * kPrefillJoinThreads + threadIdx.x;  // 4 elements, in the parts' order
-  const int lane = chunk & 63, d = 16 * ((chunk >> 6) % DB) + 4 * (lane >> 4);
-  const int local = (chunk >> 6) / DB * 16 + (lane & 15), row = b.row + local;
-  if (row >= seq.count * p.group || d >= p.head_dim) return;
   const int64_t size = prefill_part_floats(p.rows, DP);
   const auto part = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == run)) * size; };
-  float top = -INFINITY;
-  for (int i = run; i <= split.last; ++i) top = fmaxf(top, part(i)[p.rows * DP + 2 * local]);
-  float weight = 0.f;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = run; i <= split.last; ++i) {
-    const float* x = part(i);
-    const float f = prefill_ratio(x[p.rows * DP + 2 * local], top);
-    weight += x[p.rows * DP + 2 * local + 1] * f;
-    sum += *reinterpret_cast<const f32x4*>(x + 4 * chunk) * f;
+  const int rows = min(seq.count * p.group - b.row, p.rows);
+  // In the parts' order: 16 rows of the block after the other.
+  for (int chunk = blockIdx.y * kPrefillJoinThreads + threadIdx.x; chunk < (rows + 15) / 16 * 4 * DP;
+       chunk += kPrefillJoiners * kPrefillJoinThreads) {
+    const int lane = chunk & 63, d = 16 * ((chunk >> 6) % DB) + 4 * (lane >> 4);
+    const int local = (chunk >> 6) / DB * 16 + (lane & 15);
+    if (local >= rows || d >= p.head_dim) continue;
+    float top = -INFINITY, weight = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    // Four parts' loads under way together.
+    for (int first = run; first <= split.last; first += 4) {
+      float m[4], l[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* from = part(min(first + i, split.last));
+        m[i] = from[p.rows * DP + 2 * local], l[i] = from[p.rows * DP + 2 * local + 1];
+        x[i] = *reinterpret_cast<const f32x4*>(from + 4 * chunk);
+      }
+      float to = top;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to = fmaxf(to, first + i <= split.last ? m[i] : -INFINITY);
+      const float keep = prefill_ratio(top, to);
+      weight *= keep, sum *= keep, top = to;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (first + i > split.last) continue;
+        const float f = prefill_ratio(m[i], to);
+        weight += l[i] * f, sum += x[i] * f;
+      }
+    }
+    const int row = b.row + local, query = prefill_query(p, row), q_head = split.head * p.group + row - query * p.group;
+    u32x2 o = {0, 0};
+    if (!(weight == 0.f)) o[0] = T::pack(sum[0] / weight, sum[1] / weight), o[1] = T::pack(sum[2] / weight, sum[3] / weight);
+    *reinterpret_cast<u32x2*>(p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + d) = o;
+    if (p.lse != nullptr && d == 0)
+      p.lse[q_head * p.lse_h + seq.from + query] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.69314718055994530942f;
   }
-  const int query = prefill_query(p, row), q_head = split.head * p.group + row - query * p.group;
-  u32x2 o = {0, 0};
-  if (!(weight == 0.f)) o[0] = T::pack(sum[0] / weight, sum[1] / weight), o[1] = T::pack(sum[2] / weight, sum[3] / weight);
-  *reinterpret_cast<u32x2*>(p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + d) = o;
-  if (p.lse != nullptr && d == 0)
-    p.lse[q_head * p.lse_h + seq.from + query] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.69314718055994530942f;
 }
 
 template <typename T, int DP, int QB, PageKind kKind>
@@ -715,8 +734,7 @@ hipError_t launch_prefill(const PrefillLaunch& l) {
   prefill_kernel<T, DP, QB, kKind, stages><<<l.p.runs, kPrefillThreads, 0, l.stream>>>(l.p);
   const hipError_t status = hipGetLastError();
   if (status != hipSuccess) return status;
-  constexpr int chunks = 128 * QB * DP / 4;
-  prefill_join_kernel<T, DP><<<dim3(l.p.runs, chunks / kPrefillJoinThreads), kPrefillJoinThreads, 0, l.stream>>>(l.p);
+  prefill_join_kernel<T, DP><<<dim3(l.p.runs, kPrefillJoiners), kPrefillJoinThreads, 0, l.stream>>>(l.p);
   return hipGetLastError();
 }
 
