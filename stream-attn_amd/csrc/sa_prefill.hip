@@ -177,13 +177,32 @@ struct Workspace {
   int64_t max_blocks, blocks, order, first_block, splits, parts, bytes;
 };
 
+// Rows of a workgroup.  Wide ones take less time per row and tile (head_dim 128 2.0, 256
+// 1.4, 64 1.2 times less) and more to start, end, split and even out, so they need many
+// tiles for every workgroup, and sequences that fill them.  The tiles are guessed: of a
+// window, else of all keys that the table has room for before a middle token.
+// One sequence, wide and narrow in us, guessed tiles:
+//   head_dim 128, 32/8 heads: 2,048 tokens 104, 97 (11); 6,000 with a window of 512 102, 131
+//   (18); 128 behind 20,000 keys 108, 90 (13); 256 128, 141 (26); 2,048 587, 887;
+//   256, 16/16 heads: 6,000 tokens 425, 382 (70); with a window of 1,024 239, 170 (27);
+//   2,048 behind 20,000 keys 615, 755 (156); 512 250, 232 (39);
+//   64, 12/4 heads: 6,000 tokens 116, 128 (26); 512 behind 20,000 keys 68, 77 (15); 256 59,
+//   52 (7); 512 with a window of 1,024 44, 35 (1).
+int32_t rows_of(const sa_prefill_args* a, int dim, int64_t rows, int32_t runs) {
+  const int many = prefill_rows(dim, true);
+  if (rows < (int64_t)a->sequences * many * 2) return 128;
+  double keys = (double)a->max_pages * a->page_tokens - 0.5 * (double)a->tokens / a->sequences;
+  if (a->window > 0) keys = std::min(keys, (double)a->window + a->sinks);
+  const double tiles = (double)rows / many * a->kv_heads / runs * (keys / kPrefillTile + 1);
+  return tiles >= (dim == 128 ? 16 : dim == 256 ? 80 : 9) ? many : 128;
+}
+
 Workspace workspace(const sa_prefill_args* a) {
   Workspace w;
   const int dim = padded(a->head_dim);
   const int64_t rows = a->tokens * (a->q_heads / a->kv_heads);
-  const int many = prefill_rows(dim, true);
-  w.rows = rows >= (int64_t)a->sequences * many * 2 ? many : 128;
   w.runs = kPrefillCUs * prefill_occupancy(dim);
+  w.rows = rows_of(a, dim, rows, w.runs);
   w.max_blocks = std::min(rows, rows / w.rows + a->sequences);
   const auto next = [](int64_t at) { return (at + 255) & ~(int64_t)255; };
   w.blocks = next(sizeof(PrefillPlan));

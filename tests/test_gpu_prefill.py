@@ -63,25 +63,26 @@ def make(gen, new, before, q_heads, kv_heads, dim, page, kind="rows", dtype=torc
     return q, stand, table, torch.tensor(lengths, dtype=torch.int32), cu, pools, scales
 
 
-def reference(q, stand, table, lengths, cu, page, scale, window, sinks):
+def reference(q, stand, table, lengths, cu, page, scale, window, sinks, device="cpu"):
     """(out, lse, sum of weight * |v|, sum of |q k| * scale, keys) in 64 bits, per row; NaN where a row's logits have one."""
-    k_all, v_all = stand
+    q, table = q.to(device), table.to(device)
+    k_all, v_all = (x.to(device) for x in stand)
     tokens, q_heads, dim = q.shape
     kv_heads = k_all.shape[2]
     group = q_heads // kv_heads
-    out, size = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2))
-    lse = torch.full((q_heads, tokens), -math.inf, dtype=torch.float64)
-    products = torch.zeros((q_heads, tokens), dtype=torch.float64)
+    out, size = (torch.zeros(q.shape, dtype=torch.float64, device=device) for _ in range(2))
+    lse = torch.full((q_heads, tokens), -math.inf, dtype=torch.float64, device=device)
+    products = torch.zeros((q_heads, tokens), dtype=torch.float64, device=device)
     most = 1
     for s in range(len(lengths)):
         start, stop = int(cu[s]), int(cu[s + 1])
         length = max(0, min(int(lengths[s]), table.shape[1] * page))
-        keys = torch.arange(length)
+        keys = torch.arange(length, device=device)
         ids = table[s, keys // page].long()
         held = (ids >= 0) & (ids < k_all.shape[0])
         rows = (keys % page)[held]
         keys, ids = keys[held], ids[held]
-        p = torch.arange(start, stop) + length - stop
+        p = torch.arange(start, stop, device=device) + length - stop
         mask = keys[None] <= p[:, None]
         if window is not None:
             mask &= (p[:, None] - keys[None] < window) | (keys[None] < sinks)
@@ -98,17 +99,17 @@ def reference(q, stand, table, lengths, cu, page, scale, window, sinks):
             lse[h, start:stop] = torch.logsumexp(logits, 1)
             w = torch.softmax(logits, 1).masked_fill(torch.isneginf(logits).all(1, keepdim=True), 0)
             out[start:stop, h], size[start:stop, h] = w @ vh, w @ vh.abs()
-    return out, lse, size, products, most
+    return out.cpu(), lse.cpu(), size.cpu(), products.cpu(), most
 
 
-def check(data, page, window=None, sinks=0, scale=None, out=None, padding=0, kind="rows"):
+def check(data, page, window=None, sinks=0, scale=None, out=None, padding=0, kind="rows", device="cpu"):
     q, stand, table, lengths, cu, pools, scales = data
     scale = q.shape[2] ** -0.5 if scale is None else scale
     dq = torch.cat([q, torch.full((padding, *q.shape[1:]), math.nan, dtype=q.dtype)]).cuda()
     got, lse = paged_prefill_attention(dq, *pools, table.cuda(), lengths.cuda(), cu.cuda(), softmax_scale=scale,
                                        window=window, sinks=sinks, k_scales=scales[0], v_scales=scales[1], out=out,
                                        return_lse=True)
-    ref, ref_lse, size, products, most = reference(q, stand, table, lengths, cu, page, scale, window, sinks)
+    ref, ref_lse, size, products, most = reference(q, stand, table, lengths, cu, page, scale, window, sinks, device)
     half = HALF_STEP[q.dtype]
     rounded = half if kind == "int8" else 0.0
     e = (q.shape[2] + 4) * 2.0**-24 * products
@@ -171,12 +172,31 @@ def test_pages_that_end_anywhere(kind, page):
                                                   (256, 1, torch.float16, "int8"), (64, 2, torch.float16, "int8"),
                                                   (96, 2, torch.bfloat16, "rows"), (200, 1, torch.bfloat16, "rows")])
 def test_many_rows(dim, group, dtype, kind):
-    """The widest workgroups: items whole, split once and split often."""
+    """The widest workgroups, which many tiles or a table with room for many choose: items split often."""
     gen = torch.Generator().manual_seed(dim + group)
-    if kind != "rows" and dim % 16:
-        pytest.skip("8-bit pages take multiples of 16")
-    for new, before, window, sinks in (([1500], [0], None, 0), ([1100, 900], [700, 0], 300, 9)):
-        check(make(gen, new, before, group, 1, dim, 64, kind, dtype, window, sinks), 64, window, sinks, kind=kind)
+    for new, before in (([1500], [0]), ([1100, 900], [700, 0])):
+        q, stand, table, lengths, cu, pools, scales = make(gen, new, before, group, 1, dim, 64, kind, dtype)
+        room = torch.full((len(new), 2**17), -1, dtype=torch.int32)
+        room[:, : table.shape[1]] = table
+        check((q, stand, room, lengths, cu, pools, scales), 64, kind=kind)
+
+
+@pytest.mark.parametrize("dim,kv_heads,new,before,window,sinks,kind,dtype", [
+    (128, 32, [1700, 900], [300, 0], 500, 9, "rows", torch.bfloat16),
+    (128, 12, [1800], [0], None, 0, "rows", torch.float16),
+    (128, 24, [1700, 900], [300, 0], 500, 9, "e4m3", torch.float16),
+    (128, 24, [1700, 900], [300, 0], 500, 70, "int8", torch.bfloat16),
+    (256, 44, [1700, 900], [300, 0], 700, 9, "rows", torch.float16),
+    (256, 44, [1700, 900], [300, 0], 700, 9, "e4m3", torch.bfloat16),
+    (64, 24, [1700, 900], [300, 0], 400, 9, "rows", torch.bfloat16),
+    (64, 24, [1700, 900], [300, 0], 400, 9, "int8", torch.float16),
+    (80, 24, [1700, 900], [300, 0], 500, 65, "rows", torch.bfloat16),
+])
+def test_many_items(dim, kv_heads, new, before, window, sinks, kind, dtype):
+    """Wide workgroups with windows, more items than workgroups."""
+    gen = torch.Generator().manual_seed(dim + kv_heads)
+    data = make(gen, new, before, 4 * kv_heads, kv_heads, dim, 64, kind, dtype, window, sinks)
+    check(data, 64, window, sinks, kind=kind, device="cuda")
 
 
 def test_scales_of_every_kind():
