@@ -150,15 +150,17 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
 
     // ---- loads ----
     // Issuing wave w has keys 16 w .. + 15 of every tile, in one page where pages are
-    // multiples of 16.  Lane l then holds where those of tile held_first + l are, and
-    // their block's scales.
+    // multiples of 16.  Where those of tiles held_first .. + 63 are (-1: in no page), and
+    // their scales (INT8: where they are), it then looks up at once and keeps in LDS: in
+    // registers read across lanes they did not outlive what the compiler does with
+    // registers where only some lanes are on.
     constexpr int ES = QUANT ? 1 : 2;
     const char* k_head = p.k + head * p.sh * ES;
     const char* v_head = p.v + head * p.sh * ES;
     int held_first = first - 64;
-    uint32_t at_lo = 0, at_hi = 0, scale_lo = 0, scale_hi = 0;
-    uint64_t in_pool = 0;  // of the tiles held
-    float k_scale = 0.f, v_scale = 0.f;
+    __shared__ int64_t held_lds[4][64];
+    __shared__ int64_t held_scales_at[kKind == kInt8Pages ? 4 : 1][64];
+    __shared__ float held_scales[kKind == kE4m3Pages ? 4 : 1][2][64];
     const auto page_of = [](const auto& a, int key, int& row) {
       const int number = (int)((uint64_t)(uint32_t)key * a.page_magic >> a.page_shift);
       row = key - number * a.page_tokens;
@@ -179,25 +181,38 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
       bool ok;
       const int id = find(a, span.key_of(min(tile + lane, last - 1)) + 16 * wave, row, ok);
       const int64_t at = id * a.sp + row * a.st;
-      at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
-      in_pool = __ballot(ok);
+      held_lds[wave][lane] = ok ? at * ES : -1;
       if constexpr (kKind == kE4m3Pages) {
         const int64_t scale = id * a.ssp + (row >> a.block_log2) * a.sst + head * a.ssh;
-        k_scale = e8m0_value(static_cast<const uint8_t*>(a.ks)[scale]);
-        v_scale = e8m0_value(static_cast<const uint8_t*>(a.vs)[scale]);
+        held_scales[wave][0][lane] = e8m0_value(static_cast<const uint8_t*>(a.ks)[scale]);
+        held_scales[wave][1][lane] = e8m0_value(static_cast<const uint8_t*>(a.vs)[scale]);
       }
       if constexpr (kKind == kInt8Pages) {
-        const int64_t scale = id * a.ssp + row * a.sst + head * a.ssh;
-        scale_lo = (uint32_t)scale, scale_hi = (uint32_t)(scale >> 32);
+        held_scales_at[wave][lane] = id * a.ssp + row * a.sst + head * a.ssh;
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     };
     // A wave-uniform address plus 32 bits per lane.
     auto dma = [](const char* base, uint32_t offset, uint8_t* dst) __attribute__((always_inline)) {
       asm volatile("" : "+s"(base));
       __builtin_amdgcn_global_load_lds((const SA_GLOBAL void*)(base + offset), (SA_LDS void*)dst, 16, 0, 0);
     };
-    // Scales of the raw tile in flight: INT8 lane l's of key l % 16, K's (l < 16) or V's.
-    std::conditional_t<kKind == kInt8Pages, uint16_t, float> scale_next = 0;
+    // INT8 scales of the raw tile in flight: lane l's of key l % 16, K's (l < 16) or V's.
+    uint16_t scale_next = 0;
+    // K's scales go into the logits, their sign (and NaN) into the values; a factor of at
+    // least the smallest normal keeps a masked logit at -inf.
+    const auto put = [&](int tile, float scale) __attribute__((always_inline)) {
+      if (lane >= 32) return;
+      float(&to)[3][kTileKeys] = scale_lds[QUANT ? tile & 3 : 0];
+      const int key = 16 * wave + r16;
+      if (j == 0) {
+        to[0][key] = scale == scale ? fmaxf(fabsf(scale) * cf, 1.17549435e-38f) : cf;
+        to[1][key] = scale == scale ? (scale < 0.f ? -1.f : 1.f) : NAN;
+      } else {
+        to[2][key] = scale;
+      }
+    };
     // Tile `tile`: its 16-bit rows to the stage, or its bytes to the raw buffer.
     auto issue_tile = [&](int tile, uint8_t* to) __attribute__((always_inline)) {
       if (!issues) return;
@@ -209,9 +224,8 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
       if (__builtin_expect(!p.any_page, 1)) {
         if (tile - held_first >= 64) hold(tile);
         const int x = tile - held_first;
-        const uint32_t lo = __builtin_amdgcn_readlane(at_lo, x), hi = __builtin_amdgcn_readlane(at_hi, x);
-        const int64_t at = (int64_t)((uint64_t)hi << 32 | lo) * ES;
-        seen = in_pool >> x & 1 ? 0xffffu : 0u;
+        const int64_t held = uniform(held_lds[wave][x]), at = held < 0 ? 0 : held;
+        seen = held < 0 ? 0u : 0xffffu;
         // Without a page every lane reads row 0 of one that exists.
         const uint32_t step = seen ? (uint32_t)p.st * ES : 0u;
         if constexpr (QUANT) {
@@ -223,8 +237,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
             dma(v_head + at + (int64_t)i * KEYS * step, offset, to + RAW_BYTES + wave * 16 * DP + i * 1024);
           }
           if constexpr (kKind == kE4m3Pages)
-            scale_next = __builtin_bit_cast(float, j & 1 ? __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), x)
-                                                         : __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), x));
+            put(tile, held_scales[wave][j & 1][x]);
         } else {
           const int kd = 8 * Geo::k_granule((l & 3) ^ (l >> 4)), vd = 8 * ((l & 3) ^ (2 * ((l >> 4) & 1)));
           const uint32_t k_offset = key * step + kd * ES, v_offset = key * step + vd * ES;
@@ -273,8 +286,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
         const uint16_t* from = static_cast<const uint16_t*>(j & 1 ? p.vs : p.ks);
         if (__builtin_expect(!p.any_page, 1)) {
           const int x = tile - held_first;
-          const uint32_t lo = __builtin_amdgcn_readlane(scale_lo, x), hi = __builtin_amdgcn_readlane(scale_hi, x);
-          from += (int64_t)((uint64_t)hi << 32 | lo) + (seen ? r16 * p.sst : 0);
+          from += held_scales_at[wave][x] + (seen ? r16 * p.sst : 0);
         } else {
           const auto& a = *prefill_arguments();
           int row;
@@ -287,25 +299,10 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
       if (lane == 0) seen_lds[tile & 3][wave] = (uint16_t)seen;
       __builtin_amdgcn_sched_barrier(0);
     };
-    // The scales that came with raw tile `tile`, by the waves that loaded them.  K's go
-    // into the logits, their sign (and NaN) into the values; a factor of at least the
-    // smallest normal keeps a masked logit at -inf.
+    // The INT8 scales that came with raw tile `tile`, by the waves that loaded them.
     auto put_scales = [&](int tile) __attribute__((always_inline)) {
-      if constexpr (QUANT) {
-        float scale;
-        if constexpr (kKind == kInt8Pages)
-          scale = Fp16::lo(scale_next);
-        else
-          scale = scale_next;
-        if (!issues || lane >= 32) return;
-        float(&to)[3][kTileKeys] = scale_lds[tile & 3];
-        const int key = 16 * wave + r16;
-        if (j == 0) {
-          to[0][key] = scale == scale ? fmaxf(fabsf(scale) * cf, 1.17549435e-38f) : cf;
-          to[1][key] = scale == scale ? (scale < 0.f ? -1.f : 1.f) : NAN;
-        } else {
-          to[2][key] = scale;
-        }
+      if constexpr (kKind == kInt8Pages) {
+        if (issues) put(tile, Fp16::lo(scale_next));
       }
     };
     // A raw tile to 16 bits.  K's values as they are, exact: their scales are in the
@@ -644,15 +641,15 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
       const int row = qw0 + 16 * qb + r16;
       if (whole) {
         if (row >= rows) continue;
+        // One rounding more than a division, in FP32.
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const int query = prefill_query(a, row), q_head = head * a.group + row - query * a.group;
         uint16_t* to = a.out + (int64_t)(seq.from + query) * a.so_t + (int64_t)q_head * a.so_h + 4 * j;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           if (16 * db + 4 * j >= a.head_dim) continue;
-          const f32x4& x = acc[db][qb];
-          u32x2 o = {0, 0};
-          if (!(l == 0.f)) o[0] = T::pack(x[0] / l, x[1] / l), o[1] = T::pack(x[2] / l, x[3] / l);
-          *reinterpret_cast<u32x2*>(to + 16 * db) = o;
+          const f32x4 o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[db][qb] * inv;
+          *reinterpret_cast<u32x2*>(to + 16 * db) = u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
         }
         if (a.lse != nullptr && j == 0)
           a.lse[q_head * a.lse_h + seq.from + query] = l == 0.f ? -INFINITY : (m_run[qb] + log2f(l)) * 0.69314718055994530942f;
