@@ -66,8 +66,13 @@ struct PrefillLaunch {
 // Rows of a workgroup: 128 or, with many rows, what the registers hold.
 constexpr int prefill_rows(int padded_dim, bool many) { return !many ? 128 : padded_dim == 128 ? 384 : 256; }
 
-// Workgroups of a CU.
-constexpr int prefill_occupancy(int padded_dim) { return padded_dim == 64 ? 2 : 1; }
+// Workgroups of a CU: two where registers and LDS hold them.  One sequence, 32/8 heads of
+// 128, narrow, two of two stages against one of four, us: 2,048 tokens with a window of 512
+// 53 and 57, 512 behind 20,000 keys with one of 1,024 43 and 47, 2,048 tokens of 16/16
+// heads 58 and 63, with a window of 512 (fewer items than CUs) 43 and 40.
+constexpr int prefill_occupancy(int padded_dim, int rows, PageKind kind) {
+  return padded_dim == 64 || (padded_dim == 128 && rows == 128 && kind == kRowPages) ? 2 : 1;
+}
 
 // One padded head_dim each.
 hipError_t launch_prefill_d64(const PrefillLaunch& l);

@@ -201,8 +201,8 @@ Workspace workspace(const sa_prefill_args* a) {
   Workspace w;
   const int dim = padded(a->head_dim);
   const int64_t rows = a->tokens * (a->q_heads / a->kv_heads);
-  w.runs = kPrefillCUs * prefill_occupancy(dim);
-  w.rows = rows_of(a, dim, rows, w.runs);
+  w.rows = rows_of(a, dim, rows, kPrefillCUs * (dim == 64 ? 2 : 1));
+  w.runs = kPrefillCUs * prefill_occupancy(dim, w.rows, (PageKind)a->pages_kind);
   w.max_blocks = std::min(rows, rows / w.rows + a->sequences);
   const auto next = [](int64_t at) { return (at + 255) & ~(int64_t)255; };
   w.blocks = next(sizeof(PrefillPlan));

@@ -58,7 +58,7 @@ __device__ inline PrefillArguments prefill_arguments() {
 }
 
 template <typename T, int DP, int QB, PageKind kKind, int STAGES>
-__global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void prefill_kernel(const PrefillParams p) {
+__global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB, kKind)) void prefill_kernel(const PrefillParams p) {
   using Geo = Geometry<DP>;
   constexpr bool QUANT = kKind != kRowPages;
   constexpr int CK = Geo::CK, DB = Geo::DB;
@@ -671,63 +671,90 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP)) void pr
   }
 }
 
-// The parts of a split item joined: a thread has four elements of a row, a workgroup
-// every kPrefillJoiners'th of a block's runs of threads.
-constexpr int kPrefillJoinThreads = 256, kPrefillJoiners = 16;
+// The parts of a split item joined: a thread has four elements of a row.  With many
+// parts (few rows over long keys) a workgroup's waves share them, four by four: 16
+// tokens behind 40,000 keys, 64 parts an item, 17 us instead of 30.
+constexpr int kPrefillJoinThreads = 256, kPrefillJoiners = 16, kPrefillSharedParts = 8, kPrefillSharedChunks = 4096;
+
+struct PrefillJoin {
+  float top, weight;
+  f32x4 sum;
+  __device__ inline void rescale(float to) {
+    const float keep = prefill_ratio(top, to);
+    weight *= keep, sum *= keep, top = to;
+  }
+};
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kPrefillJoinThreads) void prefill_join_kernel(const PrefillParams p) {
-  constexpr int DB = DP / 16;
-  const int run = blockIdx.x;
+  constexpr int DB = DP / 16, kWaves = kPrefillJoinThreads / 64;
+  __shared__ PrefillJoin joins[kWaves][64];
+  const int run = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   const PrefillSplit split = p.splits[run];
   if (split.block < 0) return;
   const PrefillBlock b = p.blocks[split.block];
   const PrefillSequence seq = prefill_sequence(p, b.sequence);
   const int64_t size = prefill_part_floats(p.rows, DP);
   const auto part = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == run)) * size; };
-  const int rows = min(seq.count * p.group - b.row, p.rows);
+  const int rows = min(seq.count * p.group - b.row, p.rows), chunks = (rows + 15) / 16 * 4 * DP;
+  const bool shared = split.last - run >= kPrefillSharedParts && chunks <= kPrefillSharedChunks;
+  const int mine = shared ? wave : 0, step = shared ? kWaves : 1;         // parts run + mine, + step, ...
+  const int width = shared ? 64 : kPrefillJoinThreads, at = shared ? tid & 63 : tid;
   // In the parts' order: 16 rows of the block after the other.
-  for (int chunk = blockIdx.y * kPrefillJoinThreads + threadIdx.x; chunk < (rows + 15) / 16 * 4 * DP;
-       chunk += kPrefillJoiners * kPrefillJoinThreads) {
+  for (int first_chunk = blockIdx.y * width; first_chunk < chunks; first_chunk += kPrefillJoiners * width) {
+    const int chunk = first_chunk + at;
     const int lane = chunk & 63, d = 16 * ((chunk >> 6) % DB) + 4 * (lane >> 4);
     const int local = (chunk >> 6) / DB * 16 + (lane & 15);
-    if (local >= rows || d >= p.head_dim) continue;
-    float top = -INFINITY, weight = 0.f;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    // Four parts' loads under way together.
-    for (int first = run; first <= split.last; first += 4) {
-      float m[4], l[4];
-      f32x4 x[4];
+    const bool live = chunk < chunks && local < rows && d < p.head_dim;
+    PrefillJoin x{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    if (live) {
+      // Four parts' loads under way together.
+      for (int first = run + mine; first <= split.last; first += 4 * step) {
+        float m[4], l[4];
+        f32x4 y[4];
+        float to = x.top;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* from = part(min(first + i, split.last));
-        m[i] = from[p.rows * DP + 2 * local], l[i] = from[p.rows * DP + 2 * local + 1];
-        x[i] = *reinterpret_cast<const f32x4*>(from + 4 * chunk);
-      }
-      float to = top;
+        for (int i = 0; i < 4; ++i) {
+          const float* from = part(min(first + i * step, split.last));
+          m[i] = from[p.rows * DP + 2 * local], l[i] = from[p.rows * DP + 2 * local + 1];
+          y[i] = *reinterpret_cast<const f32x4*>(from + 4 * chunk);
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to = fmaxf(to, first + i <= split.last ? m[i] : -INFINITY);
-      const float keep = prefill_ratio(top, to);
-      weight *= keep, sum *= keep, top = to;
+        for (int i = 0; i < 4; ++i) to = fmaxf(to, first + i * step <= split.last ? m[i] : -INFINITY);
+        x.rescale(to);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (first + i > split.last) continue;
-        const float f = prefill_ratio(m[i], to);
-        weight += l[i] * f, sum += x[i] * f;
+        for (int i = 0; i < 4; ++i) {
+          if (first + i * step > split.last) continue;
+          const float f = prefill_ratio(m[i], to);
+          x.weight += l[i] * f, x.sum += y[i] * f;
+        }
       }
     }
+    if (shared) {
+      __syncthreads();  // the joins of the chunks before are read
+      joins[wave][at] = x;
+      __syncthreads();
+      if (wave > 0) continue;
+      for (int w = 1; w < kWaves; ++w) {
+        const PrefillJoin y = joins[w][at];
+        const float to = fmaxf(x.top, y.top), f = prefill_ratio(y.top, to);
+        x.rescale(to);
+        x.weight += y.weight * f, x.sum += y.sum * f;
+      }
+    }
+    if (!live) continue;
     const int row = b.row + local, query = prefill_query(p, row), q_head = split.head * p.group + row - query * p.group;
-    u32x2 o = {0, 0};
-    if (!(weight == 0.f)) o[0] = T::pack(sum[0] / weight, sum[1] / weight), o[1] = T::pack(sum[2] / weight, sum[3] / weight);
-    *reinterpret_cast<u32x2*>(p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + d) = o;
+    const f32x4 o = x.weight == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x.sum * (1.f / x.weight);
+    *reinterpret_cast<u32x2*>(p.out + (int64_t)(seq.from + query) * p.so_t + (int64_t)q_head * p.so_h + d) =
+        u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
     if (p.lse != nullptr && d == 0)
-      p.lse[q_head * p.lse_h + seq.from + query] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.69314718055994530942f;
+      p.lse[q_head * p.lse_h + seq.from + query] = x.weight == 0.f ? -INFINITY : (x.top + log2f(x.weight)) * 0.69314718055994530942f;
   }
 }
 
 template <typename T, int DP, int QB, PageKind kKind>
 hipError_t launch_prefill(const PrefillLaunch& l) {
-  constexpr int stages = kKind == kRowPages ? (QB == 1 && DP <= 128 ? 4 : 2) : DP == 256 ? 1 : 2;
+  constexpr int stages = kKind == kRowPages ? (QB == 1 && DP <= 64 ? 4 : 2) : DP == 256 ? 1 : 2;
   prefill_kernel<T, DP, QB, kKind, stages><<<l.p.runs, kPrefillThreads, 0, l.stream>>>(l.p);
   const hipError_t status = hipGetLastError();
   if (status != hipSuccess) return status;

@@ -24,10 +24,10 @@ _PREFILL_ARGS = struct.Struct("=11Q15qd12i")
 
 @functools.lru_cache
 def _workspace_bytes(device_index: int, tokens: int, sequences: int, max_pages: int, q_heads: int, kv_heads: int,
-                     head_dim: int, page_tokens: int, window: int, sinks: int) -> int:
+                     head_dim: int, page_tokens: int, kind: int, window: int, sinks: int) -> int:
     """Workspace of a call, which depends on its sizes alone."""
-    args = _PREFILL_ARGS.pack(*(0,) * 24, tokens, 0, 0.0, sequences, max_pages, q_heads, kv_heads, head_dim, page_tokens, 0, 0,
-                              window, sinks, 0, 0)
+    args = _PREFILL_ARGS.pack(*(0,) * 24, tokens, 0, 0.0, sequences, max_pages, q_heads, kv_heads, head_dim, page_tokens, 0, kind,
+                              window, sinks, 16, 0)
     needed = ctypes.c_int64()
     status = _native.lib().sa_paged_prefill_workspace_bytes(args, device_index, ctypes.byref(needed))
     _native.check(status, "sa_paged_prefill_workspace_bytes")
@@ -100,7 +100,7 @@ def paged_prefill_attention(
         lse = torch.empty_strided((q_heads, tokens), (tokens, 1), dtype=torch.float32, device=device)
     if tokens and sequences:
         index = device.index
-        needed = _workspace_bytes(index, tokens, sequences, max_pages, q_heads, kv_heads, dim, page_tokens, window, sinks)
+        needed = _workspace_bytes(index, tokens, sequences, max_pages, q_heads, kv_heads, dim, page_tokens, kind, window, sinks)
         workspace = torch.empty_strided((needed,), (1,), dtype=torch.uint8, device=device)
         args = _PREFILL_ARGS.pack(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if kind else 0,
