@@ -640,18 +640,23 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
       l += __shfl_xor(l, 32);
       const int row = qw0 + 16 * qb + r16;
       if (whole) {
-        if (row >= rows) continue;
         // One rounding more than a division, in FP32.
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int query = prefill_query(a, row), q_head = head * a.group + row - query * a.group;
-        uint16_t* to = a.out + (int64_t)(seq.from + query) * a.so_t + (int64_t)q_head * a.so_h + 4 * j;
+        const int at_row = min(row, rows - 1);  // lanes past the rows take part in the exchange
+        const int query = prefill_query(a, at_row), q_head = head * a.group + at_row - query * a.group;
+        // Two blocks of 16 elements: lanes of odd j hand their four of the first to j - 1 and
+        // take those of the second, so that a lane stores eight.
+        uint16_t* to = a.out + (int64_t)(seq.from + query) * a.so_t + (int64_t)q_head * a.so_h + 16 * (j & 1) + 8 * (j >> 1);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          if (16 * db + 4 * j >= a.head_dim) continue;
-          const f32x4 o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[db][qb] * inv;
-          *reinterpret_cast<u32x2*>(to + 16 * db) = u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+        for (int db = 0; db < DB; db += 2) {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 o = l == 0.f ? zero : acc[db][qb] * inv, next = l == 0.f ? zero : acc[db + 1][qb] * inv;
+          const auto x = __builtin_amdgcn_permlane16_swap(T::pack(o[0], o[1]), T::pack(next[0], next[1]), false, false);
+          const auto y = __builtin_amdgcn_permlane16_swap(T::pack(o[2], o[3]), T::pack(next[2], next[3]), false, false);
+          if (row < rows && 16 * (db + (j & 1)) + 8 * (j >> 1) < a.head_dim)
+            *reinterpret_cast<u32x4*>(to + 16 * db) = u32x4{x[0], y[0], x[1], y[1]};
         }
-        if (a.lse != nullptr && j == 0)
+        if (a.lse != nullptr && j == 0 && row < rows)
           a.lse[q_head * a.lse_h + seq.from + query] = l == 0.f ? -INFINITY : (m_run[qb] + log2f(l)) * 0.69314718055994530942f;
       } else if (has_rows) {
         // In the order of the lanes.
