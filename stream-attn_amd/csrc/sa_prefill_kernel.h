@@ -30,6 +30,13 @@ __device__ inline __attribute__((always_inline)) T uniform(T x) {
 // 2^x of a running maximum's change: 0 from -inf, 1 where nothing changes.
 __device__ inline float prefill_ratio(float from, float to) { return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to); }
 
+// A weight is held at most 2^kWeightTop; a new maximum's is 2^kWeightShift.  float16
+// weights lie high in their range, so that those of 2^-32 of the largest still count.
+template <typename W>
+constexpr int kWeightTop = std::is_same_v<W, Fp16> ? 15 : 8;
+template <typename W>
+constexpr int kWeightShift = std::is_same_v<W, Fp16> ? 7 : 0;
+
 // Bits 15 and 31: the halves of a dword that are infinite or NaN (all ones in the
 // exponent, which one more carries over).
 template <typename T>
@@ -44,6 +51,8 @@ __device__ inline u16x2 larger(u16x2 top, uint32_t w) {
 }
 // Bits 0 .. n - 1.
 __device__ inline uint32_t below(int n) { return n > 0 ? ~0u >> (32 - (n < 32 ? n : 32)) : 0u; }
+// Bits 15 and 31: bits n and n + 1.
+__device__ inline uint32_t two_bits(uint32_t bits, int n) { return (bits >> n & 1) << 15 | (bits >> n & 2) << 30; }
 // Halves of ones where those bits are.
 __device__ inline uint32_t halves(uint32_t m) { return (m - (m >> 15)) | m; }
 
@@ -61,6 +70,9 @@ template <typename T, int DP, int QB, PageKind kKind, int STAGES>
 __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB, kKind)) void prefill_kernel(const PrefillParams p) {
   using Geo = Geometry<DP>;
   constexpr bool QUANT = kKind != kRowPages;
+  // What weights and V enter their product as: INT8 times a float16 scale has three bits
+  // more in float16 than in bfloat16.
+  using W = std::conditional_t<kKind == kInt8Pages, Fp16, T>;
   constexpr int CK = Geo::CK, DB = Geo::DB;
   constexpr int KB = DP == 256 ? (QB == 1 ? 4 : 2) : CK;
   constexpr int VB = DP == 256 ? (QB == 1 ? 8 : 4) : DP == 128 && QB > 1 ? 8 : 4;
@@ -306,12 +318,13 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
       }
     };
     // A raw tile to 16 bits.  K's values as they are, exact: their scales are in the
-    // logits.  V's times their scale: INT8 rounded once, e4m3 times a power of two,
-    // exact in bfloat16 (float16 has steps of its own below 2^-14).  In float16 at
-    // most the type's largest value, which the product of a row's largest can pass by a
-    // rounding.  (Weights times V's INT8 scales instead, values exact: one rounding
-    // less, 0.0023 instead of 0.0027 of the output's norm, and registers short, 950
-    // instead of 1,000 TFLOP/s at head_dim 128 and an eighth at 256.)
+    // logits.  V's times their scale: INT8 rounded once, to float16 (to bfloat16 it was
+    // 0.0028 of the output's norm instead of 0.0018), e4m3 times a power of two, exact in
+    // bfloat16 (float16 has steps of its own below 2^-14).  In float16 at most the type's
+    // largest value, which the product of a row's largest can pass by a rounding.  (Weights
+    // times V's INT8 scales instead: registers short, 950 instead of 1,000 TFLOP/s at
+    // head_dim 128 and an eighth at 256.  So are they with a path of their own for scales
+    // past 512: a third of the rate.)
     auto dequant = [&](int tile, const uint8_t* from, uint8_t* stage) __attribute__((always_inline)) {
       constexpr int GR = Geo::I8_GR;
 #pragma unroll
@@ -326,14 +339,30 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
           const float scale = scale_lds[tile & 3][1 + tensor][row];
           u32x4 o[2];
           if constexpr (kKind == kInt8Pages) {
-            // med3 of NaN bounds is NaN.
-            const float most = scale == scale ? 65504.f : NAN;
-            const auto value = [&](int e) {
-              const float y = byte_float(w[e / 4], e & 3) * scale;
-              return tensor == 0 || std::is_same_v<T, Bf16> ? y : __builtin_amdgcn_fmed3f(y, -most, most);
-            };
+            if (tensor == 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = T::pack(value(2 * e), value(2 * e + 1));
+              for (int e = 0; e < 8; ++e)
+                o[e / 4][e % 4] = T::pack(byte_float(w[e / 2], 2 * (e & 1)) * scale, byte_float(w[e / 2], 2 * (e & 1) + 1) * scale);
+            } else {
+              // The bytes plus 128 behind the exponent of 1024, less 1152.
+              const _Float16 h = (_Float16)scale;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t bytes = __builtin_amdgcn_perm(w[e / 2] ^ 0x80808080u, 0x64646464u, e & 1 ? 0x00070006u : 0x00050004u);
+                const f16x2 x = (__builtin_bit_cast(f16x2, bytes) - f16x2{1152, 1152}) * f16x2{h, h};
+                o[e / 4][e % 4] = __builtin_bit_cast(uint32_t, x);
+              }
+              if (__builtin_expect(!(fabsf(scale) < 512.f), 0)) {
+                // NaN bounds leave NaN.
+                const _Float16 m = fabsf(scale) < INFINITY ? (_Float16)65504.f : (_Float16)NAN;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t bits = o[e / 4][e % 4];  // (a cast of the element itself takes the vector's first)
+                  const f16x2 x = __builtin_elementwise_min(__builtin_bit_cast(f16x2, bits), f16x2{m, m});
+                  o[e / 4][e % 4] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, f16x2{-m, -m}));
+                }
+              }
+            }
           } else {
             const float power = scale;
 #pragma unroll
@@ -469,7 +498,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
               const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e], factor[kb][2 * e], neg_m));
               const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][2 * e + 1], factor[kb][2 * e + 1], neg_m));
               sum = (kb == 0 && e == 0) ? p0 + p1 : sum + (p0 + p1);
-              pq[2 * kb + e] = T::pack(p0, p1);
+              pq[2 * kb + e] = W::pack(p0, p1);
             }
           return sum;
         };
@@ -478,10 +507,10 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
         bool grow[QB], any = false;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-          // Every p <= 2^8 whenever the lane's sum is; against m = -inf the sum is
+          // Every p is at most that wherever the lane's sum is; against m = -inf the sum is
           // inf or NaN.
           psum[qb] = exps(qb, -m_run[qb], pf[qb]);
-          grow[qb] = !(psum[qb] <= 256.f);
+          grow[qb] = !(psum[qb] <= (float)(1 << kWeightTop<W>));
           any = any || grow[qb];
         }
         if (__builtin_expect(__ballot(any) != 0, 0)) {
@@ -502,7 +531,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
             }
             full = fmaxf(full, __shfl_xor(full, 16));
             full = fmaxf(full, __shfl_xor(full, 32));
-            const float m_new = (mine && full > m_run[qb] + kRescaleThreshold) ? full : m_run[qb];
+            const float m_new = mine && full > m_run[qb] + kWeightTop<W> ? full - kWeightShift<W> : m_run[qb];
             const bool none = m_new == -INFINITY;
             if (m_new != m_run[qb] || none) {
               const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(m_run[qb] - m_new);
@@ -531,12 +560,12 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
             for (int dd = 0; dd < VB; ++dd)
 #pragma unroll
               for (int i = 0; i < 4; ++i) top = larger(top, vf[dd][i]);
-            odd = __any(top[0] >= T::kInfinity || top[1] >= T::kInfinity);
+            odd = __any(top[0] >= W::kInfinity || top[1] >= W::kInfinity);
             if (__builtin_expect(odd, 0)) {
 #pragma unroll
               for (int dd = 0; dd < VB; ++dd)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vf[dd][i] &= ~halves(not_finite<T>(vf[dd][i]));
+                for (int i = 0; i < 4; ++i) vf[dd][i] &= ~halves(not_finite<W>(vf[dd][i]));
             }
           }
 #pragma unroll
@@ -544,25 +573,23 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
 #pragma unroll
             for (int i = 0; i < QB; ++i) {
               const int qb = dd % 2 == 0 ? i : QB - 1 - i;
-              acc[d0 + dd][qb] = T::mma(vf[dd], pf[qb], acc[d0 + dd][qb]);
+              acc[d0 + dd][qb] = W::mma(vf[dd], pf[qb], acc[d0 + dd][qb]);
             }
           if (__builtin_expect(odd, 0)) {
             // The elements of the rows that see one: their number, as a product of ones.
-            constexpr uint32_t kOnes = std::is_same_v<T, Bf16> ? 0x3f803f80u : 0x3c003c00u;
+            constexpr uint32_t kOnes = std::is_same_v<W, Bf16> ? 0x3f803f80u : 0x3c003c00u;
             read_v(vf, v_addr, v_odd, d0 / 2 * 4096 + rb * 64);
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
               u32x4 seers;
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                seers[x] = kOnes & ((sees[qb] >> (x / 2 * 16 + 2 * (x & 1)) & 1 ? 0xffffu : 0u) |
-                                    (sees[qb] >> (x / 2 * 16 + 2 * (x & 1) + 1) & 1 ? 0xffff0000u : 0u));
+              for (int x = 0; x < 4; ++x) seers[x] = kOnes & halves(two_bits(sees[qb], x / 2 * 16 + 2 * (x & 1)));
 #pragma unroll
               for (int dd = 0; dd < VB; ++dd) {
                 u32x4 ones;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ones[i] = halves(not_finite<T>(vf[dd][i])) & kOnes;
-                const f32x4 count = T::mma(ones, seers, f32x4{0.f, 0.f, 0.f, 0.f});
+                for (int i = 0; i < 4; ++i) ones[i] = halves(not_finite<W>(vf[dd][i])) & kOnes;
+                const f32x4 count = W::mma(ones, seers, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   if (count[e] > 0.f) acc[d0 + dd][qb][e] = NAN;

@@ -111,9 +111,10 @@ def check(data, page, window=None, sinks=0, scale=None, out=None, padding=0, kin
                                        return_lse=True)
     ref, ref_lse, size, products, most = reference(q, stand, table, lengths, cu, page, scale, window, sinks, device)
     half = HALF_STEP[q.dtype]
-    rounded = half if kind == "int8" else 0.0
+    # Weights in q's dtype; with INT8 V in float16, as V's values times their scale are.
+    weight, rounded = (2.0**-12, 2.0**-12) if kind == "int8" else (half, 0.0)
     e = (q.shape[2] + 4) * 2.0**-24 * products
-    bound = half * ref.abs() + (1 + half) * (2 * e.t()[..., None] + half + rounded + 2.0**-15) * size + 2.0**-24
+    bound = half * ref.abs() + (1 + half) * (2 * e.t()[..., None] + weight + rounded + 2.0**-15) * size + 2.0**-24
     if q.dtype == torch.float16:
         bound += most * 2.0**-25 * float(size.max())
     tokens = len(q)
@@ -222,6 +223,27 @@ def test_e4m3_scales_of_every_size():
             codes = pools[i].view(torch.uint8).cpu()
             stand[i] = values(codes.view(torch.float8_e4m3fn), power.view(torch.float8_e8m0fnu))
         check((q, stand, table, lengths, cu, pools, scales), 16)
+
+
+@pytest.mark.parametrize("head_dim,group", [(64, 1), (64, 4), (128, 3), (256, 2)])
+def test_int8_values_past_float16s_largest(head_dim, group):
+    """Values times their scale are held in float16, whose largest stands for what is past it; a window hides some."""
+    gen = torch.Generator().manual_seed(head_dim)
+    data = make(gen, [150, 70], [41, 0], 2 * group, 2, head_dim, 16, "int8", torch.bfloat16)
+    q, stand, table, lengths, cu, pools, scales = data
+    for key, scale in ((3, 512.0), (40, 511.75), (64, 6e4), (65, -6e4), (130, 2000.0), (131, 65504.0), (180, 515.5)):
+        page, row = int(table[0, key // 16]), key % 16
+        scales[1][page, row] = scale
+        value = pools[1][page, row].cpu().double() * float(scales[1][page, row, 0])
+        stand[1][page, row] = value.clamp(-65504, 65504)
+    check(data, 16)
+    check(data, 16, 50, 4)
+    page, row = int(table[0, 4]), 0
+    scales[1][page, row, 0] = math.inf
+    out = paged_prefill_attention(q.cuda(), *pools, table.cuda(), lengths.cuda(), cu.cuda(), k_scales=scales[0],
+                                  v_scales=scales[1])
+    assert not bool(torch.isfinite(out[23:150, :group]).any()) and bool(torch.isfinite(out[:23]).all())
+    assert bool(torch.isfinite(out[:150, group:]).all()) and bool(torch.isfinite(out[150:]).all())
 
 
 def test_float16_takes_8_bit_values_up_to_its_largest():
