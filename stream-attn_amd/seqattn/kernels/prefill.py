@@ -63,13 +63,15 @@ def paged_prefill_attention(
     a length, whatever they hold.  A token that sees no key gets zeros, and LSE
     ``-inf``.  Rows of ``out`` past ``cu_tokens[-1]`` are not written.
 
-    Logits, softmax and sums are FP32, a weight enters the product with V in
-    ``q``'s dtype.  V's 8-bit values times their scale enter in ``q``'s dtype (e4m3
-    ones are exact in bfloat16; float16: at most its largest value); 8-bit pages need a head_dim and strides in multiples of 16.  A logit of NaN or ``+inf``
-    makes its row NaN, one of ``-inf`` is a key without weight; an element of a seen V
-    that is not finite makes its element of ``out`` not finite.  ``out`` may be ``q``,
-    and shares no memory with the rest.  Returns ``out`` (like ``q``), and with
-    ``return_lse`` also the natural-log LSE ``[q_heads, tokens]``.
+    Logits, softmax and sums are FP32.  A weight enters the product with V in ``q``'s
+    dtype, with INT8 pages in float16; V's 8-bit values times their scale enter in the
+    same, so with INT8 pages and for float16 ``q`` values past float16's largest count as
+    that (e4m3 ones are exact in bfloat16).  8-bit pages need a head_dim and strides in
+    multiples of 16.  A logit of NaN or ``+inf`` makes its row NaN, one of ``-inf`` is a
+    key without weight; an element of a seen V that is not finite makes its element of
+    ``out`` not finite.  ``out`` may be ``q``, and shares no memory with the rest.  Returns
+    ``out`` (like ``q``), and with ``return_lse`` also the natural-log LSE ``[q_heads,
+    tokens]``.
     """
     refuse_tangents(q, k_pages, v_pages, k_scales, v_scales, out)
     code = check_rows("q", q)
