@@ -762,10 +762,11 @@ int32_t sa_paged_window_decode(const sa_window_decode_args* args, int32_t device
  * Pages, scales, page_table and lengths as for sa_paged_window_decode; a token
  * that sees no key gets output 0 and LSE -inf, rows past
  * cu_tokens[sequences] stay as they are.  V's 8-bit values times their scale enter
- * in q's type (float16: at most its largest value).
+ * in q's type, INT8 ones in float16 (float16: at most its largest value).
  *
  * 8-bit pages: head_dim and strides are multiples of 16, pages 16-byte aligned.
- * tokens * q_heads / kv_heads is below 2^31 - 4096.  `workspace`
+ * Token strides of the pages are in [0, 2^26), tokens * q_heads / kv_heads is below
+ * 2^31 - 4096.  `workspace`
  * (sa_paged_prefill_workspace_bytes, 16-byte aligned) is the call's own until
  * it has run.
  */

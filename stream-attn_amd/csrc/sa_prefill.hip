@@ -251,6 +251,8 @@ int32_t sa_paged_prefill(const sa_prefill_args* a, int32_t device, void* stream)
     if (s % 8) return invalid("strides must be multiples of 8 elements");
   for (int64_t s : {a->stride_pp, a->stride_pt, a->stride_ph})
     if (s % page_step) return invalid("the pages' strides must be multiples of 16 bytes");
+  // An offset within 16 rows of a page has 32 bits.
+  if (a->stride_pt < 0 || a->stride_pt >= (1 << 26)) return invalid("the pages' token stride must be below 2^26 elements");
   if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->lengths == nullptr ||
       a->cu_tokens == nullptr || (a->page_table == nullptr && a->max_pages > 0) ||
       (kind != kRowPages && (a->k_scales == nullptr || a->v_scales == nullptr)) || !aligned(a->q, 16) ||

@@ -173,6 +173,7 @@ def test_prefill_entry_point_rejects_bad_arguments_without_a_gpu():
         (dict(window=-1), -1, b"window"), (dict(sinks=2), -1, b"window"), (dict(window=1, sinks=-1), -1, b"window"),
         (dict(kind=2, block=24), -1, b"power of two"), (dict(num_pages=0), -1, b"at least one page"),
         (dict(qt=4), -1, b"multiples of 8"), (dict(pp=4), -1, b"16 bytes"), (dict(kind=1, ph=8), -1, b"16 bytes"),
+        (dict(pt=2**26), -1, b"token stride"), (dict(pt=-16), -1, b"token stride"),
         (dict(q=8), -1, b"aligned"), (dict(cu=0), -1, b"missing"), (dict(cu=2), -1, b"aligned"), (dict(table=0), -1, b"missing"),
         (dict(kind=1), -1, b"missing"), (dict(kind=1, ks=1, vs=2), -1, b"aligned"), (dict(kind=2, ks=1, vs=1, k=8, block=16), -1, b"aligned"),
         (dict(workspace=0), -1, b"workspace"), (dict(workspace_bytes=1000), -1, b"workspace"),
