@@ -141,9 +141,15 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
   int fetched = 0;
   if (whole_items && tid == kFetcher) next_lds = atomicAdd(&p.plan->next[xcd], 1);
 
+  // What a wave wrote to LDS, and loaded and stored, is through before the others go on: the
+  // compiler leaves this wait out here, and which keys are in a page came too late for some.
+  const auto barrier = []() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
   const float cf = scale_factor(p.scale_log2);
   for (int64_t at = begin; whole_items || at < end;) {
-    __syncthreads();  // the stages are free (and, at first, cleared)
+    barrier();  // the stages are free (and, at first, cleared)
     if (whole_items) {
       const int item = 8 * uniform(next_lds) + xcd;
       if (item >= blocks * p.kv_heads) break;
@@ -629,6 +635,7 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER_TILE) : "memory");
         else
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __syncthreads();
         if (t + STAGES - 1 < ntiles)
           issue_tile(first + t + STAGES - 1, lds + (t + STAGES - 1) % STAGES * STAGE_BYTES);
@@ -639,10 +646,10 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
       for (int t = 0; t < ntiles; ++t) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         put_scales(first + t);
-        __syncthreads();
+        barrier();
         dequant(first + t, raw + t % 2 * 2 * RAW_BYTES, lds);
         if (t + 1 < ntiles) issue_tile(first + t + 1, raw + (t + 1) % 2 * 2 * RAW_BYTES);
-        __syncthreads();
+        barrier();
         compute(first + t, lds);
       }
     } else {
@@ -650,13 +657,13 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
       // At tile t: its 16-bit form is in its stage, raw tile t + 1 has arrived.
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       put_scales(first);
-      __syncthreads();
+      barrier();
       dequant(first, raw, lds);
       if (ntiles > 1) issue_tile(first + 1, raw + 2 * RAW_BYTES);
       for (int t = 0; t < ntiles; ++t) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (t + 1 < ntiles) put_scales(first + t + 1);
-        __syncthreads();
+        barrier();
         // The first wave of a SIMD converts before its products and the second one
         // after them, so that each one's vector work meets the other's matrix work.
         auto next = [&]() __attribute__((always_inline)) {

@@ -200,6 +200,17 @@ def test_many_items(dim, kv_heads, new, before, window, sinks, kind, dtype):
     check(data, 64, window, sinks, kind=kind, device="cuda")
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_calls_repeat_bit_for_bit(kind):
+    """Split and whole items, many times: what one wave hands to the others is there in time."""
+    gen = torch.Generator().manual_seed(8)
+    q, _, table, lengths, cu, pools, scales = make(gen, [1800], [0], 48, 12, 128, 64, kind)
+    q, table, lengths, cu = q.cuda(), table.cuda(), lengths.cuda(), cu.cuda()
+    run = lambda: paged_prefill_attention(q, *pools, table, lengths, cu, k_scales=scales[0], v_scales=scales[1])
+    first = run()
+    assert sum(int(not torch.equal(run(), first)) for _ in range(300)) == 0
+
+
 def test_scales_of_every_kind():
     gen = torch.Generator().manual_seed(1)
     data = make(gen, [150, 20], [33, 400], 8, 2, 128, 64)
