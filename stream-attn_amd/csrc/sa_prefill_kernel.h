@@ -649,7 +649,8 @@ __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB
         barrier();
         dequant(first + t, raw + t % 2 * 2 * RAW_BYTES, lds);
         if (t + 1 < ntiles) issue_tile(first + t + 1, raw + (t + 1) % 2 * 2 * RAW_BYTES);
-        barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile under way stays so
+        __syncthreads();
         compute(first + t, lds);
       }
     } else {
