@@ -162,7 +162,9 @@ struct Reader {
   int32_t tile, page, row;
   int32_t ids, first_id;  // page numbers first_id + lane of the sequence
 
-  // Has pages n .. upto in `ids` (n never falls, upto - n < 64).
+  // Has pages n .. upto in `ids`, a step's first and last (upto - n < 64).  No later step
+  // starts before n; within one, all numbers are asked for here, before any is read: what
+  // is held from a step's second page on has lost its first.
   __device__ inline void hold(const DecodeParams& p, int32_t n, int32_t upto, int lane) {
     if (upto - first_id >= 64) {
       first_id = n;
@@ -173,10 +175,7 @@ struct Reader {
       asm volatile("" : "+v"(ids));
     }
   }
-  __device__ inline int32_t id_of(const DecodeParams& p, int32_t n, int lane) {
-    hold(p, n, n, lane);
-    return __builtin_amdgcn_readlane(ids, n - first_id);
-  }
+  __device__ inline int32_t id_of(int32_t n) const { return __builtin_amdgcn_readlane(ids, n - first_id); }
 
   __device__ inline void enter(const DecodeParams& p) {  // at the piece's first tile
     tile = x.first;
@@ -234,7 +233,7 @@ struct Step {
     x = from.x, tile = from.tile;
     const int j = lane >> 4, g = lane & 15;
     const int32_t key0 = x.key_of(tile);
-    int32_t page = from.page, row = from.row;
+    const int32_t page = from.page, row = from.row;
     const char *kh = p.k + x.kv_head * p.sh * ES, *vh = p.v + x.kv_head * p.sh * ES;
     uint32_t at[NP];
 #pragma unroll
@@ -243,29 +242,30 @@ struct Step {
     if constexpr (!kAnyPage) {
       // Two runs of 16 keys, each in one page.
       full = within(p, key0);
+      const bool crosses = row + 16 >= p.page_tokens;
+      const int32_t in_page[2] = {row, row + 16 - (crosses ? p.page_tokens : 0)};
+      from.hold(p, page, page + crosses, lane);
+      int32_t ids[2] = {from.id_of(page), from.id_of(page + crosses)};
+      bool ok[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok[h] = (uint32_t)ids[h] < (uint32_t)p.num_pages;
+        if (!ok[h]) ids[h] = 0;  // rows of a page that exists, read and not used
+        full = full && ok[h];
+      }
       const uint32_t rows = j * (uint32_t)p.st * ES;
       // Loads return in their order, and the scales are needed before the next step's
       // loads are issued, V's rows are not: the scales go first.
       if constexpr (kKind == kE4m3Pages) {
         const uint8_t* s = reinterpret_cast<const uint8_t*>(second ? p.vs : p.ks) + x.kv_head * p.ssh;
-        int32_t n = page, r = row;
         int64_t at[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 1 && (r += 16) >= p.page_tokens) ++n, r -= p.page_tokens;
-          const int32_t id = from.id_of(p, n, lane);
-          at[h] = ((uint32_t)id < (uint32_t)p.num_pages ? id : 0) * p.ssp + (r >> p.block_log2) * p.sst;
-        }
+        for (int h = 0; h < 2; ++h) at[h] = ids[h] * p.ssp + (in_page[h] >> p.block_log2) * p.sst;
         scale = s[g & 4 ? at[1] : at[0]];
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (h == 1 && (row += 16) >= p.page_tokens) ++page, row -= p.page_tokens;
-        int32_t id = from.id_of(p, page, lane);
-        const bool ok = (uint32_t)id < (uint32_t)p.num_pages;
-        if (!ok) id = 0;  // rows of a page that exists, read and not used
-        full = full && ok;
-        const int64_t base = (id * p.sp + row * p.st) * ES;
+        const int64_t base = (ids[h] * p.sp + in_page[h] * p.st) * ES;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -275,10 +275,10 @@ struct Step {
 #pragma unroll
           for (int c = 0; c < NP; ++c) v[4 * h + u][c] = load_dwords<RW>(vh + base + 4 * u * p.st * ES, rows + at[c]);
         if constexpr (kKind == kInt8Pages) {
-          const uint16_t* s = (second ? p.vs : p.ks) + id * p.ssp + row * p.sst + x.kv_head * p.ssh;
+          const uint16_t* s = (second ? p.vs : p.ks) + ids[h] * p.ssp + in_page[h] * p.sst + x.kv_head * p.ssh;
           if ((g >> 2 & 1) == h) scale = s[(4 * (g & 3) + j) * p.sst];
         }
-        const uint32_t mask = ok ? 15u : 0u;
+        const uint32_t mask = ok[h] ? 15u : 0u;
         seen = h == 0 ? mask : seen | mask << 4;
       }
     } else {
