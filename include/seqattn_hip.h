@@ -625,7 +625,7 @@ typedef struct {
     int32_t q_heads, kv_heads, head_dim, page_tokens;
     int32_t pairs, adjacent, axes, sections[SA_MAX_ROTARY_AXES];
     int32_t positions_int64, q_weight_fp32, k_weight_fp32;
-    int32_t dtype, pages_int8;
+    int32_t dtype, pages_int8; /* 1: int8; not SA_PAGES_E4M3 */
 } sa_rows_args;
 
 int32_t sa_normalize_rotate_store(const sa_rows_args* args, int32_t device, void* stream);
@@ -725,7 +725,8 @@ typedef struct {
     int64_t num_pages;
     double softmax_scale;
     int32_t sequences, max_pages;
-    int32_t q_heads, kv_heads, head_dim, page_tokens, dtype, pages_int8;
+    int32_t q_heads, kv_heads, head_dim, page_tokens, dtype;
+    int32_t pages_int8; /* 1: int8 */
 } sa_decode_args;
 
 int32_t sa_paged_decode(const sa_decode_args* args, int32_t device, void* stream);

@@ -146,6 +146,7 @@ extern "C" {
 int32_t sa_paged_decode(const sa_decode_args* a, int32_t device, void* stream) try {
   sa::clear_error();
   if (a == nullptr) return sa::invalid("null arguments");
+  if (a->pages_int8 == SA_PAGES_E4M3) return sa::invalid("e4m3 pages are read by sa_paged_window_decode");
   return sa::run(a, a->pages_int8 ? sa::kInt8Pages : sa::kRowPages, INT32_MAX, 0, 0, device, stream);
 } catch (const std::exception& error) {
   return sa::exception_status("sa_paged_decode", error);

@@ -779,6 +779,7 @@ int32_t sa_normalize_rotate_store(const sa_rows_args* a, int32_t device, void* s
   if (pages) {
     rc = check_pool(entry, a->num_pages, a->page_tokens);
     if (rc != 0) return rc;
+    if (a->pages_int8 == SA_PAGES_E4M3) return invalid(entry, "rows go into e4m3 pages by sa_append_kv_blocks");
     if (!page_rows(p.kp, a->k_pages, a->k_scales, a) || !page_rows(p.vp, a->v_pages, a->v_scales, a) ||
         !aligned(a->slots, 8))
       return invalid(entry, "pages, scales or slots are missing or not aligned");
