@@ -31,7 +31,7 @@
 //
 // Measured (a kernel that only reads reaches 7.0 TB/s): 64 sequences of 16,384
 // keys, 32/8 heads of 128, 633 us, 6.8 TB/s; one of 524,288 keys 325 us, 6.6 TB/s; 96
-// over 1,048,576 INT8 or e4m3 keys, 40/8 heads, 353 us, 6.1 TB/s: there two waves per SIMD
+// over 1,048,576 keys, 40/8 heads, INT8 353 us, 6.2 TB/s, e4m3 343 us, 6.3: there two waves per SIMD
 // wait for each other's conversions (vector units half busy), and a third has no
 // registers.  64 sequences with a window of 4,096 keys 174 us, 6.2 TB/s.  200 short sequences, 60,013 keys of 4 heads of 96, 24 us and 4 for
 // the join: 13 us of bytes, the rest the scan of the lengths, the first loads
@@ -170,7 +170,7 @@ struct Reader {
       first_id = n;
       ids = n + lane < p.max_pages ? x.table[n + lane] : -1;
       // Waited for here: behind the branch the wait would be for every load in flight,
-      // in each step (96 sequences over 1,048,576 keys, e4m3 447 us, here 353; INT8 362 and
+      // in each step (96 sequences over 1,048,576 keys, e4m3 447 us, here 343; INT8 362 and
       // 353, with heads of 256 over 500,000 keys 443 and 368).
       asm volatile("" : "+v"(ids));
     }

@@ -70,6 +70,11 @@ constexpr int prefill_rows(int padded_dim, bool many) { return !many ? 128 : pad
 // 128, narrow, two of two stages against one of four, us: 2,048 tokens with a window of 512
 // 53 and 57, 512 behind 20,000 keys with one of 1,024 43 and 47, 2,048 tokens of 16/16
 // heads 58 and 63, with a window of 512 (fewer items than CUs) 43 and 40.
+//
+// Not all registers are there: scratch of a lane, bytes, by rows of a workgroup (16-bit
+// pages; 8-bit ones): head_dim 64, 256 rows 24; 36 to 76; 128, 128 rows 56; none, 384 rows
+// none; 20 to 32; 256, 256 rows 148; 236 to 252; 128 rows of 64 and 256 none.  All times
+// here and at rows_of() are with it.
 constexpr int prefill_occupancy(int padded_dim, int rows, PageKind kind) {
   return padded_dim == 64 || (padded_dim == 128 && rows == 128 && kind == kRowPages) ? 2 : 1;
 }

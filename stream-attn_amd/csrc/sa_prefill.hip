@@ -16,7 +16,11 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSequences = 4096;  // whose first blocks LDS holds
 constexpr int kClasses = 8;           // of blocks, by their tiles
-// What splitting items costs a workgroup, in tiles: writing and joining the parts.
+// What splitting items costs a workgroup, in tiles: writing and joining the parts.  With
+// 0, this and 20, us: one sequence of 32/8 heads of 128, 2,048 tokens with a window of 512
+// 70, 53, 54; 9,000 with one of 1,024 221, 192, 192; 4,000 without 197, 197, 215; 16/16 of
+// 256, 3,000 tokens 148, 160, 160 (5 tiles 148); 12/4 of 64, four sequences, 9,000 tokens with a window of
+// 2,048 87, 88, 93; nine, 2,700 behind 36,000 INT8 keys 70, 70, 99.
 constexpr int kSplitTiles = 10;
 
 // Inclusive sum over a workgroup's threads; `sums` has a place per wave and one more.
@@ -180,7 +184,8 @@ struct Workspace {
 // Rows of a workgroup.  Wide ones take less time per row and tile (head_dim 128 2.0, 256
 // 1.4, 64 1.2 times less) and more to start, end, split and even out, so they need many
 // tiles for every workgroup, and sequences that fill them.  The tiles are guessed: of a
-// window, else of all keys that the table has room for before a middle token.
+// window, else of all keys that the table has room for before a middle token.  (Lengths are
+// not known here: in a table with far more room a short prompt gets wide ones.)
 // One sequence, wide and narrow in us, guessed tiles:
 //   head_dim 128, 32/8 heads: 2,048 tokens 104, 97 (11); 6,000 with a window of 512 102, 131
 //   (18); 128 behind 20,000 keys 108, 90 (13); 256 128, 141 (26); 2,048 587, 887;

@@ -15,8 +15,9 @@
 // of a SIMD before its products and by the second one after them.
 //
 // Measured (a library product reaches 1,620 TFLOP/s): 61,312 tokens, 56/8 heads of 128,
-// window 4,096, 6.0 ms, 1,160 TFLOP/s; 2,000 tokens behind 129,072 e4m3 keys, 40/8 heads,
-// 5.0 ms, 1,064 TFLOP/s; 20,011 tokens of 7 sequences 0.56 ms, 1,010 TFLOP/s.  A tile of
+// window 4,096, 5.9 ms, 1,181 TFLOP/s; 2,000 tokens behind 129,072 e4m3 keys, 40/8 heads,
+// 5.0 ms, 1,056 TFLOP/s; 20,011 tokens of 7 sequences 0.56 ms, 1,024 TFLOP/s (a card whose
+// clock falls lower under load: 1,067, 1,031 and 955).  A tile of
 // 384 rows takes 2.4 us (1,300 TFLOP/s), matrix and vector units half busy each and meeting
 // only in part with two waves per SIMD; an item 13 us to start and end.
 #pragma once
@@ -84,8 +85,11 @@ template <typename T, int DP, int QB, PageKind kKind, int STAGES>
 __global__ __launch_bounds__(kPrefillThreads, 2 * prefill_occupancy(DP, 128 * QB, kKind)) void prefill_kernel(const PrefillParams p) {
   using Geo = Geometry<DP>;
   constexpr bool QUANT = kKind != kRowPages;
-  // What weights and V enter their product as: INT8 times a float16 scale has three bits
-  // more in float16 than in bfloat16.
+  // What weights and V enter their product as, each rounded once.  A second 16-bit part of
+  // the weights, which single tokens have, would double this product, half of the matrix
+  // work: so outputs in bfloat16 are 0.0020 to 0.0023 of their norm off, 0.0016 of it by
+  // their own rounding, as the update kernel's are; in float16 0.00026 and 0.0002.  INT8
+  // times a float16 scale has three bits more in float16 than in bfloat16: 0.0017.
   using W = std::conditional_t<kKind == kInt8Pages, Fp16, T>;
   constexpr int CK = Geo::CK, DB = Geo::DB;
   constexpr int KB = DP == 256 ? (QB == 1 ? 4 : 2) : CK;
